@@ -681,6 +681,77 @@ int lsk_moe_pp_skinny_rows(int rows);
  * only (thread-local). */
 int lsk_moe_mx_select(int variant);
 
+/* ---------------------------------------------------------------- MXFP4 activations and weights */
+
+/* No counterpart in the reference: rows brought to MXFP4 (the format lsk_dequant_mxfp4 reads).  x [M, K]
+ * of x_dtype (LSK_F32 / LSK_BF16 / LSK_F16, row stride ldx), K % 32 == 0; packed [M, K/2] uint8 (low
+ * nibble = even element) and scale [M, K/32] uint8, both contiguous, packed 4-byte aligned.  Per block
+ * of 32 along K with a = max |x|:
+ *   s = clamp(floor(log2 a) - 2 + 127, 0, 254), 0 when a == 0;
+ *   code = E2M1 of x * 2^(127 - s), round to nearest, ties to the even code, magnitudes above 6 to 6,
+ *   the sign kept (also of zeros).
+ * A block that holds an infinity or a NaN: s = 255, code 7 with the sign at those elements, 0 at the
+ * others (lsk_gemm_mxfp4 takes 255 as NaN; lsk_dequant_mxfp4, whose 255 is 2^128, gives infinities and
+ * NaNs). */
+int lsk_quantize_mxfp4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* packed, uint8_t* scale,
+                       void* stream);
+
+/* No counterpart in the reference (its MXFP4 linears take int8 rows, lsk_gemm_mx): both operands MXFP4,
+ *   out[m, n] = round(sum_b 2^(a_scale[m, b] + w_scale[n, b] - 254) sum_{j in b} a[m, j] w[n, j] + bias[n]),
+ * the sum in binary32 on the matrix core over ascending K, the bias added in binary32, one rounding to
+ * out_dtype (LSK_F32 / LSK_BF16 / LSK_F16).  A scale byte of 255 is a NaN and makes its row's (column's)
+ * outputs NaN.  a [M, K/2] and w [N, K/2] packed E2M1 codes, a_scale [M, K/32] and w_scale [N, K/32]
+ * E8M0 bytes, all contiguous, the codes 16-byte aligned; K % 32 == 0 (K = 0: the bias alone); bias [N] or
+ * NULL; out [M, N] (row stride ldo).  A row's results are the same bits whatever the other rows are and
+ * however many, and on every launch.  workspace: lsk_gemm_mxfp4_workspace(M, N, K) bytes, 256-byte
+ * aligned (none needed when that is 0). */
+int64_t lsk_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K);
+int lsk_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, int64_t M, int64_t K, const uint8_t* w,
+                   const uint8_t* w_scale, int64_t N, const float* bias, void* out, int out_dtype, int64_t ldo,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/* lsk_quantize_mxfp4 of x [M, K] and lsk_gemm_mxfp4 of the result in one call: the same bits.
+ * workspace: lsk_linear_mxfp4_workspace(M, N, K) bytes, 256-byte aligned. */
+int64_t lsk_linear_mxfp4_workspace(int64_t M, int64_t N, int64_t K);
+int lsk_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int64_t M, int64_t K, const uint8_t* w,
+                     const uint8_t* w_scale, int64_t N, const float* bias, void* out, int out_dtype, int64_t ldo,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* lsk_gemm_mxfp4 per expert over rows already sorted by expert (beside lsk_grouped_gemm_mx, whose rows
+ * are int8): rows offs[e] .. offs[e + 1] - 1 (offs [E + 1] int32 on the device) through w_ptrs[e]
+ * (packed codes [N, K/2], row stride ldw bytes, 16-byte aligned, ldw % 16 == 0), ws_ptrs[e] (E8M0 bytes
+ * [N, K/32], row stride lds) and b_ptrs[e] (f32 [N]; b_ptrs NULL for no bias).  Offsets that decrease or
+ * leave [0, R] are taken as min(R, max(0, offs[0..j])); rows of no expert are not written.  The same
+ * bits as lsk_gemm_mxfp4 of each expert's rows.  workspace: lsk_grouped_gemm_mxfp4_workspace bytes,
+ * 256-byte aligned. */
+int64_t lsk_grouped_gemm_mxfp4_workspace(int64_t R, int64_t E, int64_t N, int64_t K);
+int lsk_grouped_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, const int32_t* offs, int64_t E, int64_t R,
+                           const int64_t* w_ptrs, int64_t ldw, const int64_t* ws_ptrs, int64_t lds,
+                           const int64_t* b_ptrs, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- logits */
+
+/* No counterpart in the reference: what a sampler does to a head's logits [B, V] (dtype LSK_F32 /
+ * LSK_BF16 / LSK_F16, row stride ldl) before it draws.  Per row b and token v, with n = how often v
+ * stands in the row's output and seen = v stands in its prompt or output, each step one binary32
+ * operation:
+ *   l = logits + bias;  seen: l = l > 0 ? l / repetition : l * repetition;
+ *   l = l - frequency * n (the product rounded first);  n > 0: l = l - presence;
+ *   mask bit 0: l = -inf;  out = l rounded to dtype.
+ * prompt [B, Lp] (row stride ldp) and output [B, Lo] (row stride ldo_tok): tokens, NULL for none; the
+ * first prompt_lens[b] / output_lens[b] of a row count (NULL: all; lengths are taken inside [0, L]), and
+ * tokens outside [0, V) count for nothing.  wide: bit 0 prompt, 1 output, 2 prompt_lens, 3 output_lens
+ * hold int64 (int32 where the bit is 0).  repetition, frequency, presence: f32 [B] or NULL (left out).
+ * bias: f32, row b at bias + b * ldb (ldb 0: one row for all), or NULL.  mask: row b at mask + b * ldm
+ * (words; ldm 0: one for all), bit v % 32 of word v / 32 allows v, ceil(V / 32) words, or NULL.  out
+ * [B, V] (row stride ldo) may be logits itself. */
+int lsk_penalize_logits(const void* logits, int dtype, int64_t ldl, int64_t B, int64_t V, const void* prompt, int64_t ldp,
+                        int64_t Lp, const void* prompt_lens, const void* output, int64_t ldo_tok, int64_t Lo,
+                        const void* output_lens, int wide, const float* repetition, const float* frequency,
+                        const float* presence, const float* bias, int64_t ldb, const int32_t* mask, int64_t ldm,
+                        void* out, int64_t ldo, void* stream);
+
 /* ---------------------------------------------------------------- diagnostics */
 
 /* The part's int8 MFMA ceiling, no counterpart in the reference: `blocks` x 256 threads each run

@@ -107,6 +107,16 @@ SIGNATURES = {
     "lsk_mfma_probe": (_I, [_P, _I64, _I64, _I, _P, _P]),
     "lsk_bf16_cvt_check": (_I, [ctypes.c_uint64, ctypes.c_uint64, _P, _P, _P]),
     "lsk_moe_mx_select": (_I, [_I]),
+    "lsk_quantize_mxfp4": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P]),
+    "lsk_gemm_mxfp4_workspace": (_I64, [_I64, _I64, _I64]),
+    "lsk_gemm_mxfp4": (_I, [_P, _P, _I64, _I64, _P, _P, _I64, _P, _P, _I, _I64, _P, _I64, _P]),
+    "lsk_linear_mxfp4_workspace": (_I64, [_I64, _I64, _I64]),
+    "lsk_linear_mxfp4": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I, _I64, _P, _I64, _P]),
+    "lsk_grouped_gemm_mxfp4_workspace": (_I64, [_I64, _I64, _I64, _I64]),
+    "lsk_grouped_gemm_mxfp4": (_I, [_P, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I, _I64, _P, _I64,
+                                    _P]),
+    "lsk_penalize_logits": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _P, _P, _P, _P,
+                                 _I64, _P, _I64, _P, _I64, _P]),
 }
 
 
@@ -158,6 +168,15 @@ def call(name: str, *args):
     if rc != 0:
         raise LockstepError("%s failed (code %d): %s" % (name, rc, last_error()))
     return rc
+
+
+def call_on(t: torch.Tensor, name: str, *args):
+    """call() with t's device current: a launch goes to the current device, whose streams t's are not
+    when t lives on another."""
+    if t.get_device() == torch._C._cuda_getDevice():
+        return call(name, *args)
+    with torch.cuda.device(t.device):
+        return call(name, *args)
 
 
 def dtype_code(dt: torch.dtype) -> int:

@@ -1,0 +1,324 @@
+// MXFP4 activations and weights: the quantiser and the products on the block-scaled matrix core.
+//
+// A value of an MXFP4 row is fp4(code) * 2^(s - 127): sixteen E2M1 codes {0, 0.5, 1, 1.5, 2, 3, 4, 6}
+// with a sign, one E8M0 byte s per 32 values along K.  With both operands in that form
+//   y[m, n] = sum_b 2^(sa[m, b] + sw[n, b] - 254) sum_{j in b} fa[m, j] fw[n, j]
+// runs on v_mfma_scale_f32_16x16x128_f8f6f4 and v_mfma_scale_f32_32x32x64_f8f6f4 as it lies in
+// memory: a lane holds the 16 code bytes of one block of one row and that block's scale byte.
+//
+// Every output is one chain of such instructions over ascending K from +0.  Chained 32x32x64 and
+// 16x16x128 give the same bits (measured on MI355X: 245,760 sums of 128 to 1024 products, exponents
+// spread over up to 40 octaves, zero and nonzero accumulators), so a row's result depends neither on
+// the tile that computes it nor on the other rows of the call.
+#include <hip/hip_runtime.h>
+
+#include "lsk_common.h"
+#include "mfma_tile.h"
+
+namespace lsk {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+
+// ---------------------------------------------------------------- the quantiser
+// Eight values of a block (the block's other 24 in the three neighbouring lanes of a quad) to eight
+// codes; s = the block's scale byte.  The largest magnitude's exponent E (biased) comes from its
+// bits, so s = E - 2 puts it in [4, 8) of its scale; the conversion instruction divides by 2^(s -
+// 127), rounds to nearest with ties to the even code and takes magnitudes above 6 to 6 (checked on
+// MI355X against the definition over every bf16 pattern and as many random binary32 at each of 255
+// scales).  A block that holds an infinity or a NaN gets s = 255, which makes every product with it
+// NaN, and code 7 at those elements, 0 elsewhere.
+LSK_DEV uint32_t quantize8_mxfp4(const float (&v)[8], uint32_t& s) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = __float_as_uint(v[i]) & 0x7fffffffu;
+    top = top > u ? top : u;
+  }
+  uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xb1, 0xf, 0xf, false);  // quad [1,0,3,2]
+  top = top > o ? top : o;
+  o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4e, 0xf, 0xf, false);  // quad [2,3,0,1]
+  top = top > o ? top : o;
+  const uint32_t E = top >> 23;
+  if (E == 255) {
+    s = 255;
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t u = __float_as_uint(v[i]);
+      if ((u & 0x7f800000u) == 0x7f800000u) w |= (7u | ((u >> 28) & 8u)) << (4 * i);
+    }
+    return w;
+  }
+  s = E > 2 ? E - 2 : 0;
+  const float sc = __uint_as_float(s ? s << 23 : 0x00400000u);  // 2^(s - 127)
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], sc, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], sc, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], sc, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], sc, 3);
+  return w;
+}
+
+// Eight elements from element i on, in 16-byte loads (VEC: aligned for them) or one by one.
+template <int DT, bool VEC>
+LSK_DEV void load8(const void* x, int64_t i, float (&v)[8]) {
+  if constexpr (VEC) {
+    load8_as_f32<DT>((const char*)x + i * (DT == LSK_F32 ? 4 : 2), 0, v);
+  } else {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) v[t] = load_as_f32(x, DT, i + t);
+  }
+}
+
+// A thread per eight values, a quad of lanes per block: M * K / 8 threads' worth of work (a multiple
+// of 4), whole quads inside or outside it.  Bound by HBM: s_x bytes read and 17/32 written a value.
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const void* __restrict__ x, int64_t ldx, int64_t total,
+                                                             int K8, uint8_t* __restrict__ packed,
+                                                             uint8_t* __restrict__ scale) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / K8;
+    float v[8];
+    load8<DT, VEC>(x, row * ldx + 8 * (i - row * K8), v);
+    uint32_t s;
+    ((uint32_t*)packed)[i] = quantize8_mxfp4(v, s);
+    if ((i & 3) == 0) scale[i >> 2] = (uint8_t)s;
+  }
+}
+
+static int quantize_launch(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* packed,
+                           uint8_t* scale, hipStream_t s) {
+  const int64_t total = M * (K / 8);
+  const int64_t blocks = (total + 255) / 256;
+  const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536)), blk(256);
+  const int size = x_dtype == LSK_F32 ? 4 : 2;
+  const bool vec = (uintptr_t)x % 16 == 0 && (ldx * size) % 16 == 0;
+#define LSK_Q4(DT, V) \
+  hipLaunchKernelGGL((quantize_mxfp4_kernel<DT, V>), grid, blk, 0, s, x, ldx, total, (int)(K / 8), packed, scale)
+  if (x_dtype == LSK_F32) {
+    if (vec) LSK_Q4(LSK_F32, true);
+    else LSK_Q4(LSK_F32, false);
+  } else if (x_dtype == LSK_BF16) {
+    if (vec) LSK_Q4(LSK_BF16, true);
+    else LSK_Q4(LSK_BF16, false);
+  } else {
+    if (vec) LSK_Q4(LSK_F16, true);
+    else LSK_Q4(LSK_F16, false);
+  }
+#undef LSK_Q4
+  return check_launch("quantize_mxfp4_kernel");
+}
+
+// ---------------------------------------------------------------- the products
+struct Fp4Args {
+  const uint8_t* a;   // codes [M, K/2], row stride lda bytes
+  const uint8_t* sa;  // scales [M, K/32], row stride ldsa
+  const uint8_t* w;   // codes [N, K/2], row stride ldw
+  const uint8_t* sw;  // scales [N, K/32], row stride ldsw
+  int64_t lda, ldsa, ldw, ldsw;
+  int64_t M, N;
+  int K;
+  const float* bias;  // [N] or null
+  void* out;
+  int out_dtype;
+  int64_t ldo;
+  // one projection of every expert: rows offs[e] .. offs[e + 1] - 1 through w_ptrs[e], ws_ptrs[e] and
+  // b_ptrs[e] (or null)
+  const int32_t* offs;  // [E + 1]
+  int E;
+  const int64_t* w_ptrs;
+  const int64_t* ws_ptrs;
+  const int64_t* b_ptrs;
+};
+
+// Row tile t of expert-sorted rows: expert e, its first row m0 and the end m1 of the expert's rows,
+// tiles of bm rows counted over the experts in order; false past the last tile.  Offsets that
+// decrease or leave [0, R] are taken as min(R, max(0, offs[0..j])), so that experts come out empty
+// or shortened and no row outside [0, R) is touched.  Every wave looks its tile up itself, 64
+// experts a step: no table to build in a launch of its own.
+LSK_DEV bool expert_tile(const int32_t* __restrict__ offs, int E, int R, int bm, int t, int& e, int& m0, int& m1) {
+  const int lane = threadIdx.x & 63;
+  int carry = min(max(offs[0], 0), R);
+  for (int e0 = 0; e0 < E; e0 += 64) {
+    int hi = min(max(offs[min(e0 + lane + 1, E)], 0), R);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(hi, d, 64);
+      if (lane >= d) hi = max(hi, o);
+    }
+    hi = max(hi, carry);
+    int lo = __shfl_up(hi, 1, 64);
+    if (lane == 0) lo = carry;
+    const int n = (hi - lo + bm - 1) / bm;
+    int sum = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += o;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(sum > t);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      e = e0 + l;
+      m0 = __builtin_amdgcn_readlane(lo, l) + (t - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l))) * bm;
+      m1 = __builtin_amdgcn_readlane(hi, l);
+      return true;
+    }
+    t -= __builtin_amdgcn_readlane(sum, 63);
+    carry = __builtin_amdgcn_readlane(hi, 63);
+  }
+  return false;
+}
+inline int64_t expert_tiles_max(int64_t R, int64_t E, int64_t bm) { return R / bm + (E < R ? E : R); }
+
+LSK_DEV v8i fp4_operand(v4i x) { return v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0}; }
+
+// One 16 x 16 piece of the output per wave over all of K: 16 weight rows as the instruction's rows,
+// 16 activation rows as its columns, so that a lane ends with four consecutive outputs of one row.
+// Rows past the end and blocks past K read zeros through the buffer range.
+template <bool GROUPED>
+__global__ __launch_bounds__(64) void fp4_rows_kernel(Fp4Args p) {
+  const int lane = threadIdx.x, r = lane & 15, q = lane >> 4;
+  const int64_t ngroups = (p.N + 15) / 16;
+  const int64_t tile = blockIdx.x / ngroups, n0 = (blockIdx.x - tile * ngroups) * 16;
+  int64_t m0 = tile * 16, m1 = p.M;
+  if constexpr (GROUPED) {
+    int e, first, end;
+    if (!expert_tile(p.offs, p.E, (int)p.M, 16, (int)tile, e, first, end)) return;
+    m0 = first;
+    m1 = end;
+    p.w = (const uint8_t*)p.w_ptrs[e];
+    p.sw = (const uint8_t*)p.ws_ptrs[e];
+    p.bias = p.b_ptrs ? (const float*)p.b_ptrs[e] : nullptr;
+  }
+  const int rows_a = m1 - m0 < 16 ? (int)(m1 - m0) : 16, rows_w = p.N - n0 < 16 ? (int)(p.N - n0) : 16;
+  const int nb = p.K / 32;
+  const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.a + m0 * p.lda, (rows_a - 1) * p.lda + p.K / 2);
+  const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w + n0 * p.ldw, (rows_w - 1) * p.ldw + p.K / 2);
+  const __amdgpu_buffer_rsrc_t rsa = make_rsrc(p.sa + m0 * p.ldsa, (rows_a - 1) * p.ldsa + nb);
+  const __amdgpu_buffer_rsrc_t rsw = make_rsrc(p.sw + n0 * p.ldsw, (rows_w - 1) * p.ldsw + nb);
+  const uint32_t oa = (uint32_t)(r * p.lda), ow = (uint32_t)(r * p.ldw);
+  const uint32_t osa = (uint32_t)(r * p.ldsa), osw = (uint32_t)(r * p.ldsw);
+  v4f acc = {0, 0, 0, 0};
+  for (int b0 = 0; b0 < nb; b0 += 4) {
+    const int b = b0 + q;
+    const bool oka = b < nb && r < rows_a, okw = b < nb && r < rows_w;
+    const v4i xa = buf_load16(ra, oka ? oa + 16 * b : kOob), xw = buf_load16(rw, okw ? ow + 16 * b : kOob);
+    const int sa = __builtin_amdgcn_raw_buffer_load_b8(rsa, oka ? (int)(osa + b) : (int)kOob, 0, 0);
+    const int sw = __builtin_amdgcn_raw_buffer_load_b8(rsw, okw ? (int)(osw + b) : (int)kOob, 0, 0);
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(xw), fp4_operand(xa), acc, 4, 4, 0, sw, 0, sa);
+  }
+  if (r >= rows_a) return;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int64_t n = n0 + 4 * q + t;
+    if (n < p.N) store_out(p.out, p.out_dtype, (m0 + r) * p.ldo + n, p.bias ? f32_add(acc[t], p.bias[n]) : acc[t]);
+  }
+}
+
+static int fp4_product(const Fp4Args& p, hipStream_t s) {
+  const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16) : (p.M + 15) / 16;
+  const int64_t blocks = tiles * ((p.N + 15) / 16);
+  LSK_REQUIRE(blocks <= 0x7fffffff, "mxfp4 product: grid too large");
+  const dim3 grid((unsigned)blocks), blk(64);
+  if (p.offs) hipLaunchKernelGGL(fp4_rows_kernel<true>, grid, blk, 0, s, p);
+  else hipLaunchKernelGGL(fp4_rows_kernel<false>, grid, blk, 0, s, p);
+  return check_launch("fp4_rows_kernel");
+}
+
+static bool is_float_dtype(int d) { return d == LSK_F32 || d == LSK_BF16 || d == LSK_F16; }
+
+static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace lsk
+
+extern "C" int lsk_quantize_mxfp4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* packed,
+                                  uint8_t* scale, void* stream) {
+  LSK_REQUIRE(lsk::is_float_dtype(x_dtype), "lsk_quantize_mxfp4: x_dtype must be f32, bf16 or f16");
+  LSK_REQUIRE(M >= 0 && K >= 0 && K % 32 == 0 && K <= 0x7fffffff, "lsk_quantize_mxfp4: K=%lld not a multiple of 32",
+              (long long)K);
+  if (M == 0 || K == 0) return LSK_OK;
+  LSK_REQUIRE(M <= 0x7fffffffffLL / K * 32, "lsk_quantize_mxfp4: M=%lld too large", (long long)M);
+  LSK_REQUIRE(M == 1 || ldx >= K, "lsk_quantize_mxfp4: ldx below K");
+  LSK_REQUIRE(x && packed && scale, "lsk_quantize_mxfp4: null pointer");
+  LSK_REQUIRE((uintptr_t)packed % 4 == 0, "lsk_quantize_mxfp4: packed must be 4-byte aligned");
+  return lsk::quantize_launch(x, x_dtype, M, K, ldx, packed, scale, (hipStream_t)stream);
+}
+
+static int mxfp4_check(const char* who, int64_t M, int64_t N, int64_t K, int out_dtype, int64_t ldo) {
+  LSK_REQUIRE(M >= 0 && N >= 0 && K >= 0 && K % 32 == 0, "%s: bad sizes M=%lld N=%lld K=%lld (K a multiple of 32)", who,
+              (long long)M, (long long)N, (long long)K);
+  LSK_REQUIRE(M <= 0x7fffffff && N <= 0x7fffffff && K <= (1 << 25), "%s: sizes beyond 31 bits (K beyond 2^25)", who);
+  LSK_REQUIRE(lsk::is_float_dtype(out_dtype), "%s: out_dtype must be f32, bf16 or f16", who);
+  LSK_REQUIRE(ldo >= N, "%s: ldo below N", who);
+  return LSK_OK;
+}
+
+extern "C" int64_t lsk_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
+  (void)M, (void)N, (void)K;
+  return 0;
+}
+
+extern "C" int lsk_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, int64_t M, int64_t K, const uint8_t* w,
+                              const uint8_t* w_scale, int64_t N, const float* bias, void* out, int out_dtype,
+                              int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = mxfp4_check("lsk_gemm_mxfp4", M, N, K, out_dtype, ldo);
+  if (rc) return rc;
+  if (M == 0 || N == 0) return LSK_OK;
+  LSK_REQUIRE(out && (K == 0 || (a && a_scale && w && w_scale)), "lsk_gemm_mxfp4: null pointer");
+  LSK_REQUIRE((uintptr_t)a % 16 == 0 && (uintptr_t)w % 16 == 0, "lsk_gemm_mxfp4: codes must be 16-byte aligned");
+  lsk::Fp4Args p{};
+  p.a = a, p.sa = a_scale, p.w = w, p.sw = w_scale;
+  p.lda = p.ldw = K / 2, p.ldsa = p.ldsw = K / 32;
+  p.M = M, p.N = N, p.K = (int)K;
+  p.bias = bias, p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
+  return lsk::fp4_product(p, (hipStream_t)stream);
+}
+
+extern "C" int64_t lsk_linear_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
+  return lsk::up256(M * (K / 2)) + lsk::up256(M * (K / 32)) + lsk_gemm_mxfp4_workspace(M, N, K);
+}
+
+extern "C" int lsk_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int64_t M, int64_t K, const uint8_t* w,
+                                const uint8_t* w_scale, int64_t N, const float* bias, void* out, int out_dtype,
+                                int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = mxfp4_check("lsk_linear_mxfp4", M, N, K, out_dtype, ldo);
+  if (rc) return rc;
+  if (M == 0 || N == 0) return LSK_OK;
+  const int64_t need = lsk_linear_mxfp4_workspace(M, N, K);
+  LSK_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 256 == 0)),
+              "lsk_linear_mxfp4: workspace of %lld bytes (256-byte aligned) needed", (long long)need);
+  uint8_t* q = (uint8_t*)workspace;
+  uint8_t* qs = q + lsk::up256(M * (K / 2));
+  uint8_t* rest = qs + lsk::up256(M * (K / 32));
+  rc = lsk_quantize_mxfp4(x, x_dtype, M, K, ldx, q, qs, stream);
+  if (rc) return rc;
+  return lsk_gemm_mxfp4(q, qs, M, K, w, w_scale, N, bias, out, out_dtype, ldo, rest,
+                        workspace_bytes - (int64_t)(rest - (uint8_t*)workspace), stream);
+}
+
+extern "C" int64_t lsk_grouped_gemm_mxfp4_workspace(int64_t R, int64_t E, int64_t N, int64_t K) {
+  (void)R, (void)E, (void)N, (void)K;
+  return 0;
+}
+
+extern "C" int lsk_grouped_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, const int32_t* offs, int64_t E, int64_t R,
+                                      const int64_t* w_ptrs, int64_t ldw, const int64_t* ws_ptrs, int64_t lds,
+                                      const int64_t* b_ptrs, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo,
+                                      void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = mxfp4_check("lsk_grouped_gemm_mxfp4", R, N, K, out_dtype, ldo);
+  if (rc) return rc;
+  LSK_REQUIRE(E >= 1 && E <= (1 << 20), "lsk_grouped_gemm_mxfp4: E=%lld not in [1, 2^20]", (long long)E);
+  if (R == 0 || N == 0) return LSK_OK;
+  LSK_REQUIRE(out && offs && w_ptrs && ws_ptrs && (K == 0 || (a && a_scale)), "lsk_grouped_gemm_mxfp4: null pointer");
+  LSK_REQUIRE((uintptr_t)a % 16 == 0 && ldw >= K / 2 && ldw % 16 == 0 && lds >= K / 32,
+              "lsk_grouped_gemm_mxfp4: codes in rows of 16-byte multiples, strides that cover K");
+  LSK_REQUIRE(ldw <= (1 << 26) && lds <= (1 << 26), "lsk_grouped_gemm_mxfp4: row strides beyond 2^26 bytes");
+  lsk::Fp4Args p{};
+  p.a = a, p.sa = a_scale;
+  p.lda = K / 2, p.ldsa = K / 32, p.ldw = ldw, p.ldsw = lds;
+  p.M = R, p.N = N, p.K = (int)K;
+  p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
+  p.offs = offs, p.E = (int)E, p.w_ptrs = w_ptrs, p.ws_ptrs = ws_ptrs, p.b_ptrs = b_ptrs;
+  return lsk::fp4_product(p, (hipStream_t)stream);
+}

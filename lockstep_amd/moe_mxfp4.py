@@ -5,6 +5,12 @@
     dequant_mxfp4(packed, scale_e8m0, out_dtype, block)   moe_mxfp4.py:26-35
     self_test(device)                               moe_mxfp4.py:38-48
 
+and, with no counterpart there, tensors brought to that format and multiplied in it:
+
+    quantize_mxfp4(x)                               x -> packed codes, scales
+    mm_mxfp4(a, a_scale, w, w_scale, ...)           the product of quantised rows and weight rows
+    linear_mxfp4(x, w, w_scale, ...)                the rows quantised on the way
+
 Layout (the checkpoint's): packed uint8 [..., K/2], element 2i in the low nibble; scale uint8
 [..., K/32], one E8M0 exponent per block.  Every value fp4 * 2^(e - 127) is exact in bf16.
 """
@@ -44,6 +50,27 @@ def fp4_values(codes: torch.Tensor) -> torch.Tensor:
 def dequant_mxfp4(packed: torch.Tensor, scale_e8m0: torch.Tensor, out_dtype=torch.bfloat16, block: int = 32):
     """packed uint8 [..., K/2], scale uint8 [..., K/block] -> [..., K] in out_dtype, exact."""
     return ops.dequant_mxfp4(packed, scale_e8m0, out_dtype, block)
+
+
+def quantize_mxfp4(x: torch.Tensor):
+    """x [..., K] (f32 / bf16 / f16), K % 32 == 0 -> (packed uint8 [..., K/2], scale uint8 [..., K/32]).
+    Per block of 32: the scale 2^(scale - 127) puts the largest magnitude in [4, 8) (scale 0 where that is
+    below 2^-125), the codes are x / 2^(scale - 127) rounded to nearest, ties to the even code, magnitudes
+    above 6 to 6.  A block with an infinity or a NaN gets scale 255, code 7 at those elements and 0 at
+    the others: products with it are NaN."""
+    return ops.quantize_mxfp4(x)
+
+
+def mm_mxfp4(a, a_scale, w, w_scale, bias=None, out_dtype=torch.float32):
+    """a [M, K/2], a_scale [M, K/32] times w [N, K/2], w_scale [N, K/32] (+ bias [N]) -> [M, N], binary32
+    accumulation over ascending K, rounded once to out_dtype; a row's bits do not depend on the other
+    rows.  A scale byte of 255 is a NaN."""
+    return ops.mm_mxfp4(a, a_scale, w, w_scale, bias, out_dtype)
+
+
+def linear_mxfp4(x, w, w_scale, bias=None, out_dtype=None):
+    """mm_mxfp4(*quantize_mxfp4(x), w, w_scale, bias, out_dtype or x's dtype), in one call."""
+    return ops.linear_mxfp4(x, w, w_scale, bias, out_dtype)
 
 
 def self_test(device="cuda"):

@@ -604,6 +604,36 @@ def grouped_linear_mx(tables, which: str, a8, asc, offs):
     return out
 
 
+def grouped_linear_mxfp4(tables, which: str, a, a_scale, offs, out_dtype=BF):
+    """The form with MXFP4 rows (no counterpart in the reference): per expert
+    moe_mxfp4.mm_mxfp4(a[rows], a_scale[rows], codes_e, scales_e[, b_e]) over expert-sorted rows.
+    a uint8 [R, K/2], a_scale uint8 [R, K/32] as moe_mxfp4.quantize_mxfp4 gives them; out [R, N] of
+    out_dtype.  Rows past offs[E] belong to no expert and are not written."""
+    tables = expert_tables_mx(tables)
+    what = "grouped_linear_mxfp4"
+    if which not in ("w13", "w2"):
+        raise ValueError("%s: which must be 'w13' or 'w2'" % what)
+    L.require_cuda(a, a_scale, offs, tables.w13, what=what)
+    if offs.dtype != torch.int32 or offs.dim() != 1 or offs.numel() != tables.E + 1:
+        raise ValueError("%s: offs must be int32 [E + 1] = [%d]" % (what, tables.E + 1))
+    N, K = (2 * tables.I, tables.H) if which == "w13" else (tables.H, tables.I)
+    a, a_scale, R, Ka = ops._mxfp4_codes(a, a_scale, what)
+    if Ka != K:
+        raise ValueError("%s: rows of %d values for experts of %d" % (what, Ka, K))
+    code = ops._mxfp4_out(what, out_dtype)
+    w, ws, b = (tables.w13, tables.ws13, tables.b13) if which == "w13" else (tables.w2, tables.ws2, tables.b2)
+    ldw, lds = (tables.ldw13, tables.lds13) if which == "w13" else (tables.ldw2, tables.lds2)
+    offs = offs.contiguous()
+    out = torch.empty((R, N), dtype=out_dtype, device=a.device)
+    if R:
+        nbytes = L.load().lsk_grouped_gemm_mxfp4_workspace(R, tables.E, N, K)
+        work = torch.empty((nbytes,), dtype=torch.uint8, device=a.device) if nbytes else None
+        L.call_on(a, "lsk_grouped_gemm_mxfp4", L.ptr(a), L.ptr(a_scale), L.ptr(offs), tables.E, R,
+                  L.ptr(w), ldw, L.ptr(ws), lds, L.ptr(b), N, K, L.ptr(out), code, N, L.ptr(work), nbytes,
+                  L.stream_of(a))
+    return out
+
+
 def _moe_layer_mx(x, idx, w, t: ExpertTablesMX, act: int, wfmt: int = 1, route=None):
     what = "moe_forward_mx2" if wfmt == 2 else "moe_forward_mx"
     fields, keep = {}, None

@@ -672,3 +672,173 @@ def pack_m2(m2: torch.Tensor):
     if int(bad.item()):
         raise ValueError("m2 holds a value that is not 2 * an E2M1 value {0, +-1, +-2, +-3, +-4, +-6, +-8, +-12}")
     return packed
+
+
+# ---------------------------------------------------------------- MXFP4 activations and weights
+def quantize_mxfp4(x: torch.Tensor):
+    """x [..., K] (f32 / bf16 / f16; other float dtypes go through f32), K % 32 == 0, to MXFP4:
+    (packed E2M1 codes uint8 [..., K/2], low nibble first, E8M0 scales uint8 [..., K/32])."""
+    L.require_cuda(x, what="quantize_mxfp4")
+    if x.dim() == 0 or x.shape[-1] % 32:
+        raise ValueError("quantize_mxfp4: x must be [..., K] with K a multiple of 32, got %s" % (tuple(x.shape),))
+    if not x.is_floating_point():
+        raise TypeError("quantize_mxfp4: x must be floating point, got %s" % x.dtype)
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        x = x.to(torch.float32)
+    lead, K = x.shape[:-1], x.shape[-1]
+    packed = torch.empty((*lead, K // 2), dtype=torch.uint8, device=x.device)
+    scale = torch.empty((*lead, K // 32), dtype=torch.uint8, device=x.device)
+    if x.numel():
+        x2 = _rows(x)
+        M = x2.shape[0]
+        L.call_on(x, "lsk_quantize_mxfp4", L.ptr(x2), L.dtype_code(x2.dtype), M, K, x2.stride(0) if M > 1 else K,
+                  L.ptr(packed), L.ptr(scale), L.stream_of(x))
+    return packed, scale
+
+
+def _mxfp4_codes(packed: torch.Tensor, scale: torch.Tensor, what: str):
+    """packed uint8 [rows, K/2] and scale uint8 [rows, K/32] as the kernels read them: contiguous, codes
+    16-byte aligned (a copy where they are not).  Returns (packed, scale, rows, K)."""
+    if packed.dtype != torch.uint8 or scale.dtype != torch.uint8:
+        raise TypeError("%s: packed codes and scales must be uint8, got %s and %s" % (what, packed.dtype, scale.dtype))
+    if packed.dim() != 2 or scale.dim() != 2 or packed.shape[1] % 16 \
+            or tuple(scale.shape) != (packed.shape[0], packed.shape[1] // 16):
+        raise ValueError("%s: packed [rows, K/2] and scale [rows, K/32] with K a multiple of 32 expected, got %s and %s"
+                         % (what, tuple(packed.shape), tuple(scale.shape)))
+    if not packed.is_contiguous() or packed.data_ptr() % 16:
+        packed = packed.clone(memory_format=torch.contiguous_format)
+    return packed, scale.contiguous(), packed.shape[0], packed.shape[1] * 2
+
+
+def _mxfp4_out(what: str, out_dtype):
+    if out_dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError("%s: out_dtype %s not supported (float32, bfloat16, float16)" % (what, out_dtype))
+    return L.dtype_code(out_dtype)
+
+
+def _mxfp4_bias(bias, N: int, what: str):
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError("%s: bias must be [%d], got %s" % (what, N, tuple(bias.shape)))
+    return _f32(bias)
+
+
+def mm_mxfp4(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=None,
+             out_dtype=torch.float32) -> torch.Tensor:
+    """MXFP4 rows a [M, K/2], a_scale [M, K/32] times MXFP4 weight rows w [N, K/2], w_scale [N, K/32]
+    (+ bias [N]) -> [M, N] of out_dtype: binary32 accumulation over ascending K, one rounding at the
+    end.  A row's result is the same bits whatever the other rows are and however many."""
+    L.require_cuda(a, a_scale, w, w_scale, bias, what="mm_mxfp4")
+    a, a_scale, M, K = _mxfp4_codes(a, a_scale, "mm_mxfp4")
+    w, w_scale, N, K2 = _mxfp4_codes(w, w_scale, "mm_mxfp4")
+    if K != K2:
+        raise ValueError("mm_mxfp4: K mismatch %d vs %d" % (K, K2))
+    code = _mxfp4_out("mm_mxfp4", out_dtype)
+    bias = _mxfp4_bias(bias, N, "mm_mxfp4")
+    out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    if M and N:
+        nbytes = L.load().lsk_gemm_mxfp4_workspace(M, N, K)
+        work = torch.empty((nbytes,), dtype=torch.uint8, device=a.device) if nbytes else None
+        L.call_on(a, "lsk_gemm_mxfp4", L.ptr(a), L.ptr(a_scale), M, K, L.ptr(w), L.ptr(w_scale), N, L.ptr(bias),
+                  L.ptr(out), code, N, L.ptr(work), nbytes, L.stream_of(a))
+    return out
+
+
+def linear_mxfp4(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=None, out_dtype=None) -> torch.Tensor:
+    """x [..., K] (f32 / bf16 / f16) quantised to MXFP4 (quantize_mxfp4) and multiplied with MXFP4 weight
+    rows w [N, K/2], w_scale [N, K/32] (+ bias [N]) -> [..., N] of out_dtype (x's by default): mm_mxfp4 of
+    the quantised rows, the same bits, in one call."""
+    L.require_cuda(x, w, w_scale, bias, what="linear_mxfp4")
+    w, w_scale, N, K = _mxfp4_codes(w, w_scale, "linear_mxfp4")
+    if x.dim() == 0 or x.shape[-1] != K:
+        raise ValueError("linear_mxfp4: x must be [..., %d], got %s" % (K, tuple(x.shape)))
+    if not x.is_floating_point():
+        raise TypeError("linear_mxfp4: x must be floating point, got %s" % x.dtype)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    code = _mxfp4_out("linear_mxfp4", out_dtype)
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        x = x.to(torch.float32)
+    bias = _mxfp4_bias(bias, N, "linear_mxfp4")
+    out = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=x.device)
+    if out.numel():
+        x2 = _rows(x) if K else x.reshape(out.numel() // N, 0)
+        M = x2.shape[0]
+        nbytes = L.load().lsk_linear_mxfp4_workspace(M, N, K)
+        work = torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
+        L.call_on(x, "lsk_linear_mxfp4", L.ptr(x2), L.dtype_code(x2.dtype), x2.stride(0) if M > 1 else K, M, K, L.ptr(w),
+                  L.ptr(w_scale), N, L.ptr(bias), L.ptr(out), code, N, L.ptr(work), nbytes, L.stream_of(x))
+    return out
+
+
+# ---------------------------------------------------------------- logits
+def _history(tokens, lens, B: int, what: str):
+    """(tokens [B, L] with unit stride, lens [B] contiguous, wide flags) of one token history."""
+    if tokens is None:
+        if lens is not None:
+            raise ValueError("penalize_logits: %s_lens without %s" % (what, what))
+        return None, None, 0, 0
+    if tokens.dim() != 2 or tokens.shape[0] != B or tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("penalize_logits: %s must be int32 or int64 [%d, L], got %s %s"
+                         % (what, B, tokens.dtype, tuple(tokens.shape)))
+    if tokens.shape[1] > 1 and tokens.stride(1) != 1:
+        tokens = tokens.contiguous()
+    if lens is not None:
+        if tuple(lens.shape) != (B,) or lens.dtype not in (torch.int32, torch.int64):
+            raise ValueError("penalize_logits: %s_lens must be int32 or int64 [%d], got %s %s"
+                             % (what, B, lens.dtype, tuple(lens.shape)))
+        lens = lens.contiguous()
+    return (tokens, lens, 1 if tokens.dtype == torch.int64 else 0,
+            1 if lens is not None and lens.dtype == torch.int64 else 0)
+
+
+def penalize_logits(logits: torch.Tensor, prompt=None, prompt_lens=None, output=None, output_lens=None, repetition=None,
+                    frequency=None, presence=None, bias=None, mask=None, out=None) -> torch.Tensor:
+    """logits [B, V] (f32 / bf16 / f16) -> the same shape and type (into `out` when given; out=logits
+    works in place), per row b and token v, in binary32, each step one rounding:
+        l = logits + bias                                  bias f32 [V] or [B, V]
+        v in the row's prompt or output:  l = l / repetition if l > 0 else l * repetition
+        l = l - frequency * (times v stands in the output)
+        v in the output:  l = l - presence
+        v not allowed by mask:  l = -inf                   mask int32 [B, ceil(V / 32)] (or [1, ...] for
+                                                           all rows): bit v % 32 of word v // 32 allows v
+    prompt [B, Lp] and output [B, Lo] are int32 or int64 tokens of which prompt_lens / output_lens [B]
+    (all when None) count; tokens outside [0, V) (padding) count for nothing.  repetition, frequency and
+    presence are f32 [B]; what is None is left out.  A row whose mask allows nothing is -inf throughout."""
+    L.require_cuda(logits, prompt, prompt_lens, output, output_lens, repetition, frequency, presence, bias, mask, out,
+                   what="penalize_logits")
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError("penalize_logits: logits must be f32, bf16 or f16 [B, V], got %s %s"
+                         % (logits.dtype, tuple(logits.shape)))
+    B, V = logits.shape
+    prompt, prompt_lens, p64, pl64 = _history(prompt, prompt_lens, B, "prompt")
+    output, output_lens, o64, ol64 = _history(output, output_lens, B, "output")
+    for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+        if t is not None and (tuple(t.shape) != (B,) or t.dtype != torch.float32):
+            raise ValueError("penalize_logits: %s must be f32 [%d], got %s %s" % (name, B, t.dtype, tuple(t.shape)))
+    if bias is not None:
+        if bias.dtype != torch.float32 or tuple(bias.shape) not in ((V,), (B, V)):
+            raise ValueError("penalize_logits: bias must be f32 [%d] or [%d, %d], got %s %s"
+                             % (V, B, V, bias.dtype, tuple(bias.shape)))
+        bias = bias if V < 2 or bias.stride(-1) == 1 else bias.contiguous()
+    if mask is not None:
+        words = (V + 31) // 32
+        if mask.dtype != torch.int32 or tuple(mask.shape) not in ((B, words), (1, words)):
+            raise ValueError("penalize_logits: mask must be int32 [%d, %d] or [1, %d], got %s %s"
+                             % (B, words, words, mask.dtype, tuple(mask.shape)))
+        mask = mask if words < 2 or mask.stride(1) == 1 else mask.contiguous()
+    if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1)
+                            or (B > 1 and out.stride(0) < V)):
+        raise ValueError("penalize_logits: out must be %s [%d, %d] with rows of consecutive tokens" % (logits.dtype, B, V))
+    if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
+        logits = logits.contiguous()
+    if out is None:
+        out = torch.empty((B, V), dtype=logits.dtype, device=logits.device)
+    if B and V:
+        rep, freq, pres = (None if t is None else t.contiguous() for t in (repetition, frequency, presence))
+        row = lambda t: 0 if t is None else t.stride(0)  # noqa: E731
+        cols = lambda t: 0 if t is None else t.shape[1]  # noqa: E731
+        L.call_on(logits, "lsk_penalize_logits", L.ptr(logits), L.dtype_code(logits.dtype), row(logits), B, V,
+                  L.ptr(prompt), row(prompt), cols(prompt), L.ptr(prompt_lens), L.ptr(output), row(output), cols(output),
+                  L.ptr(output_lens), p64 | o64 << 1 | pl64 << 2 | ol64 << 3, L.ptr(rep), L.ptr(freq), L.ptr(pres),
+                  L.ptr(bias), row(bias) if bias is not None and bias.dim() == 2 else 0, L.ptr(mask),
+                  row(mask) if mask is not None and mask.shape[0] > 1 else 0, L.ptr(out), row(out), L.stream_of(logits))
+    return out

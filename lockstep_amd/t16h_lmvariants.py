@@ -12,6 +12,9 @@ arithmetic runs in the HIP kernels of liblockstep_amd.so):
     _mm_planes(x2, wplanes, ws, abits)   :115-125               planes combined exactly in int64
     Variant, build(spec), needs_calibration(specs)              :128-201
 
+and, with no counterpart there, the variant "mxfp4" (weight and rows in MXFP4, moe_mxfp4.linear_mxfp4)
+and penalize_logits(logits, ...): penalties for repeated tokens, biases and allowed-token masks.
+
 A <B>-bit value (B in 8, 11, 15) rides two int8 planes hi = a >> (B - 8), lo = a - (hi << (B - 8));
 the plane products are exact int32 GEMMs and the combine is exact in int64, so the result is
 fl32(fl32(fl32(s) * asc[m]) * ws[n]) of the exact integer s = sum_k a[m, k] * w[n, k].  On the
@@ -114,11 +117,15 @@ class Variant:
         self.name, self.kind = name, kind
         self.abits, self.wbits, self.alpha = abits, wbits, alpha
         self.wplanes = self.ws = self.sdiv = self.W_bf16 = None
+        self._w4 = None            # the MXFP4 variant's packed codes [N, K/2] (ws: its scales [N, K/32])
         self._w2 = None            # the stacked weight planes [P * N, K] the kernels read
 
     def prepare(self, W, act_amax=None):
         self.W_bf16 = W
         if self.kind == "bf16":
+            return self
+        if self.kind == "mxfp4":
+            self._w4, self.ws = ops.quantize_mxfp4(W.detach())
             return self
         if self.alpha is not None:
             if act_amax is None:
@@ -137,6 +144,8 @@ class Variant:
         """x2 : [rows, K] float32 -> [rows, N] float32."""
         if self.kind == "bf16":
             return torch.nn.functional.linear(x2.to(self.W_bf16.dtype), self.W_bf16).float()
+        if self.kind == "mxfp4":
+            return ops.linear_mxfp4(x2, self._w4, self.ws, out_dtype=torch.float32)
         rows = x2.numel() // max(1, x2.shape[-1])
         return ops.planes_linear(x2, self._w2, self.wbits, self.ws, self.abits, sdiv=self.sdiv,
                                  w_pairs=ops.planes_pairs(self._w2, rows, self.abits))
@@ -145,13 +154,15 @@ class Variant:
         return int(self.W_bf16.shape[0])
 
     def gemms(self):
-        """int8 GEMMs per call: activation planes x weight planes (0 for the float head)."""
-        if self.kind == "bf16":
+        """int8 GEMMs per call: activation planes x weight planes (0 for the float and MXFP4 heads)."""
+        if self.kind in ("bf16", "mxfp4"):
             return 0
         return (2 if self.abits > 8 else 1) * len(self.wplanes)
 
     def nbytes(self):
         """Bytes of the published constants: weight planes, smoothing vector, scales."""
+        if self.kind == "mxfp4":
+            return 0 if self._w4 is None else self._w4.numel() + self.ws.numel()
         parts = [p.numel() for _, p in (self.wplanes or [])]
         parts += [4 * t.numel() for t in (self.sdiv, self.ws) if t is not None]
         return sum(parts)
@@ -162,10 +173,10 @@ _AW = re.compile(r"(?:a(?P<a>\d+))?(?:w(?P<w>\d+))?")
 
 
 def build(spec: str) -> Variant:
-    """bf16 | [sq<AA>][a<A>][w<W>].  e.g. a8  a15  a15w15  sq50  sq50a15  sq80a15w15"""
+    """bf16 | mxfp4 | [sq<AA>][a<A>][w<W>].  e.g. a8  a15  a15w15  sq50  sq50a15  sq80a15w15"""
     s = spec.strip()
-    if s == "bf16":
-        return Variant(s, "bf16")
+    if s in ("bf16", "mxfp4"):
+        return Variant(s, s)
     head = _SPEC.fullmatch(s)
     alpha = None
     if s.startswith("sq"):
@@ -185,3 +196,12 @@ def build(spec: str) -> Variant:
 
 def needs_calibration(specs) -> bool:
     return any(sp.strip().startswith("sq") for sp in specs)
+
+
+def penalize_logits(logits, prompt=None, prompt_lens=None, output=None, output_lens=None, repetition=None, frequency=None,
+                    presence=None, bias=None, mask=None, out=None):
+    """What a sampler does to a head's logits [B, V] before it draws, in one pass (ops.penalize_logits):
+    bias, the repetition penalty over prompt and output tokens, the frequency and presence penalties
+    over output tokens, then -inf where the allowed-token bits of `mask` are 0."""
+    return ops.penalize_logits(logits, prompt, prompt_lens, output, output_lens, repetition, frequency, presence, bias,
+                               mask, out)

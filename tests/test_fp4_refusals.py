@@ -1,0 +1,99 @@
+"""What the MXFP4 and logits entry points refuse, at the C boundary and in Python, without a GPU."""
+import pytest
+import torch
+
+from lockstep_amd import _lib as L
+from lockstep_amd import moe_mxfp4, moe_ref, t16h_lmvariants
+
+P = 1 << 20      # a plausible, 256-byte aligned address: every call here is refused before it is used
+
+
+def _refused(rc, word):
+    lib = L.load()
+    assert rc == 1 and word in lib.lsk_last_error(), (rc, lib.lsk_last_error())
+
+
+def test_quantize_refusals():
+    q = L.load().lsk_quantize_mxfp4
+    _refused(q(P, L.LSK_I8, 1, 32, 32, P, P, None), b"x_dtype")
+    _refused(q(P, L.LSK_F32, 1, 33, 33, P, P, None), b"multiple of 32")
+    _refused(q(P, L.LSK_F32, -1, 32, 32, P, P, None), b"multiple of 32")
+    _refused(q(P, L.LSK_F32, 2, 64, 32, P, P, None), b"ldx")
+    _refused(q(None, L.LSK_F32, 2, 64, 64, P, P, None), b"null")
+    _refused(q(P, L.LSK_F32, 2, 64, 64, P + 2, P, None), b"aligned")
+    assert q(None, L.LSK_F32, 0, 64, 64, None, None, None) == 0
+    assert q(None, L.LSK_F32, 5, 0, 0, None, None, None) == 0
+
+
+def test_product_refusals():
+    lib = L.load()
+
+    def gemm(M=4, K=64, N=8, odt=L.LSK_F32, ldo=8, a=P, w=P, out=P):
+        return lib.lsk_gemm_mxfp4(a, P, M, K, w, P, N, None, out, odt, ldo, None, 0, None)
+    _refused(gemm(K=48), b"multiple of 32")
+    _refused(gemm(M=-1), b"bad sizes")
+    _refused(gemm(odt=L.LSK_I32), b"out_dtype")
+    _refused(gemm(ldo=7), b"ldo")
+    _refused(gemm(a=P + 8), b"16-byte")
+    _refused(gemm(w=P + 4), b"16-byte")
+    _refused(gemm(a=None), b"null")
+    _refused(gemm(out=None), b"null")
+    _refused(gemm(M=1 << 32), b"31 bits")
+    assert gemm(M=0, a=None, w=None, out=None) == 0
+    assert gemm(N=0, ldo=0, a=None, w=None, out=None) == 0
+    need = lib.lsk_linear_mxfp4_workspace(4, 8, 64)
+    assert need > 0
+    _refused(lib.lsk_linear_mxfp4(P, L.LSK_F32, 64, 4, 64, P, P, 8, None, P, L.LSK_F32, 8, P, need - 1, None), b"workspace")
+    _refused(lib.lsk_linear_mxfp4(P, L.LSK_F32, 64, 4, 64, P, P, 8, None, P, L.LSK_F32, 8, P + 16, need, None), b"workspace")
+    _refused(lib.lsk_linear_mxfp4(P, L.LSK_I32, 64, 4, 64, P, P, 8, None, P, L.LSK_F32, 8, P, need, None), b"x_dtype")
+
+
+def test_grouped_refusals():
+    lib = L.load()
+
+    def grouped(E=2, R=4, ldw=32, lds=2, N=8, K=64, ldo=8, offs=P, odt=L.LSK_BF16):
+        need = lib.lsk_grouped_gemm_mxfp4_workspace(R, E, N, K)
+        return lib.lsk_grouped_gemm_mxfp4(P, P, offs, E, R, P, ldw, P, lds, None, N, K, P, odt, ldo, P, need, None)
+    _refused(grouped(E=0), b"E=0")
+    _refused(grouped(ldw=24), b"strides")
+    _refused(grouped(ldw=40), b"strides")
+    _refused(grouped(lds=1), b"strides")
+    _refused(grouped(offs=None), b"null")
+    _refused(grouped(K=63), b"multiple of 32")
+    _refused(grouped(odt=L.LSK_I32), b"out_dtype")
+    assert grouped(R=0) == 0
+
+
+def test_logits_refusals():
+    lib = L.load()
+
+    def pen(dtype=L.LSK_F32, B=2, V=100, ldl=100, ldo=100, Lp=0, Lo=0, logits=P, out=P):
+        return lib.lsk_penalize_logits(logits, dtype, ldl, B, V, P, Lp, Lp, None, P, Lo, Lo, None, 0, None, None, None,
+                                       None, 0, None, 0, out, ldo, None)
+    _refused(pen(dtype=L.LSK_I32), b"dtype")
+    _refused(pen(B=-1), b"bad sizes")
+    _refused(pen(ldl=99), b"strides")
+    _refused(pen(ldo=99), b"strides")
+    _refused(pen(Lp=-1), b"history")
+    _refused(pen(logits=None), b"null")
+    assert pen(B=0, logits=None, out=None) == 0
+    assert pen(V=0, ldl=0, ldo=0, logits=None, out=None) == 0
+
+
+def test_cpu_tensors_are_refused():
+    x, u = torch.zeros(2, 64), torch.zeros(2, 32, dtype=torch.uint8)
+    s = torch.zeros(2, 2, dtype=torch.uint8)
+    for call in (lambda: moe_mxfp4.quantize_mxfp4(x), lambda: moe_mxfp4.mm_mxfp4(u, s, u, s),
+                 lambda: moe_mxfp4.linear_mxfp4(x, u, s), lambda: t16h_lmvariants.penalize_logits(x),
+                 lambda: t16h_lmvariants.build("mxfp4").prepare(x)):
+        with pytest.raises(ValueError, match="GPU tensor"):
+            call()
+    with pytest.raises(ValueError):
+        moe_ref.grouped_linear_mxfp4([], "w13", u, s, torch.zeros(3, dtype=torch.int32))
+
+
+def test_head_variant_names():
+    assert t16h_lmvariants.build(" mxfp4 ").kind == "mxfp4"
+    assert t16h_lmvariants.build("mxfp4").gemms() == 0 and t16h_lmvariants.build("mxfp4").nbytes() == 0
+    with pytest.raises(ValueError):
+        t16h_lmvariants.build("mxfp6")

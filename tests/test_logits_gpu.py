@@ -1,0 +1,125 @@
+"""t16h_lmvariants.penalize_logits against its declared steps, each one binary32 operation, bit for
+bit (fp4_util.penalize)."""
+import numpy as np
+import pytest
+import torch
+
+import fp4_util as U
+from gpu_util import bits, dev, say, to_dev
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    import lockstep_amd._lib as L
+    L.load()
+
+
+def _case(g, B, V, Lp, Lo, dtype, tok=np.int64):
+    l = torch.from_numpy((3 * g.standard_normal((B, V))).astype(np.float32)).to(dtype)
+    p = g.integers(-2, V + 3, (B, Lp)).astype(tok)
+    o = np.minimum(g.geometric(0.02, (B, Lo)), V + 1).astype(tok) - 1
+    c = dict(prompt=p, prompt_lens=g.integers(0, Lp + 1, B).astype(np.int32), output=o,
+             output_lens=g.integers(-1, Lo + 3, B).astype(np.int64), repetition=g.uniform(0.7, 1.6, B).astype(np.float32),
+             frequency=g.uniform(-0.5, 0.9, B).astype(np.float32), presence=g.uniform(-0.5, 0.9, B).astype(np.float32),
+             bias=g.standard_normal(V).astype(np.float32),
+             mask=g.integers(-2 ** 31, 2 ** 31, (B, (V + 31) // 32)).astype(np.int32))
+    return l, c
+
+
+def _run(l, c, **kw):
+    from lockstep_amd import t16h_lmvariants as TH
+    return TH.penalize_logits(l.to(dev()), **{k: to_dev(v) for k, v in c.items()}, **kw)
+
+
+def _check(l, c):
+    want = torch.from_numpy(U.penalize(l.float().numpy(), **c)).to(l.dtype)
+    assert np.array_equal(bits(_run(l, c)), bits(want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,V,Lp,Lo", [(1, 1, 1, 1), (1, 65536, 300, 100), (3, 1000, 40, 60), (2, 33, 5, 700),
+                                       (5, 16391, 1, 257), (17, 8193, 90, 30), (300, 77, 10, 10), (2, 152064, 2000, 900)])
+def test_all_steps(B, V, Lp, Lo, dtype):
+    say("logits", B, V, Lp, Lo, dtype)
+    l, c = _case(np.random.default_rng(B + V), B, V, Lp, Lo, dtype, np.int32 if V % 2 else np.int64)
+    _check(l, c)
+
+
+@pytest.mark.parametrize("left", [(), ("prompt", "prompt_lens"), ("output", "output_lens"), ("mask",), ("bias",),
+                                  ("repetition",), ("frequency", "presence"), ("prompt_lens", "output_lens"),
+                                  ("prompt", "prompt_lens", "output", "output_lens")])
+def test_each_part_may_be_left_out(left):
+    l, c = _case(np.random.default_rng(7), 4, 5003, 60, 50, torch.bfloat16)
+    _check(l, {k: v for k, v in c.items() if k not in left})
+    _check(l, {k: v for k, v in c.items() if k in left and k.replace("_lens", "") in left})   # (lengths need tokens)
+
+
+def test_special_values():
+    """Infinite and NaN logits, also in masked and penalised places, and a row whose mask allows nothing."""
+    g = np.random.default_rng(8)
+    l, c = _case(g, 4, 3000, 500, 400, torch.float32)
+    flat = l.view(-1)
+    for i, v in enumerate((float("inf"), float("-inf"), float("nan"), 0.0, -0.0, torch.finfo(torch.float32).min)):
+        flat[torch.from_numpy(g.integers(0, flat.numel(), 300))] = v
+    c["mask"][2] = 0
+    c["mask"][3] = -1
+    c["bias"][::7] = -np.inf
+    got = _run(l, c).cpu().numpy()
+    want = U.penalize(l.numpy(), **c)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(got[~np.isnan(got)].view(np.uint32), want[~np.isnan(want)].view(np.uint32))
+    assert np.isneginf(got[2]).all()
+
+
+def test_layouts_and_in_place():
+    from lockstep_amd import t16h_lmvariants as TH
+    g = np.random.default_rng(9)
+    B, V = 5, 2050
+    l, c = _case(g, B, V, 64, 64, torch.bfloat16)
+    want = bits(torch.from_numpy(U.penalize(l.float().numpy(), **c)).to(l.dtype))
+    d = {k: to_dev(v) for k, v in c.items()}
+    for off in (0, 1, 3, 8):
+        wide = torch.zeros((B, V + 11), dtype=l.dtype, device=dev())
+        wide[:, off:off + V] = l.to(dev())
+        view = wide[:, off:off + V]
+        assert np.array_equal(bits(TH.penalize_logits(view, **d)), want)
+        guard = wide.clone()
+        out = guard[:, off:off + V]
+        assert TH.penalize_logits(out, **d, out=out) is out
+        assert np.array_equal(bits(out), want)
+        assert torch.equal(guard[:, :off], wide[:, :off]) and torch.equal(guard[:, off + V:], wide[:, off + V:])
+    assert np.array_equal(bits(TH.penalize_logits(l.to(dev()).t().contiguous().t(), **d)), want)
+    assert np.array_equal(bits(TH.penalize_logits(l.to(dev()), **{**d, "bias": d["bias"].expand(B, V)})), want)
+    many = to_dev(g.standard_normal((B, V)).astype(np.float32))
+    one = torch.from_numpy(U.penalize(l.float().numpy(), **{**c, "bias": many.cpu().numpy(), "mask": c["mask"][1:2].repeat(B, 0)}))
+    got = TH.penalize_logits(l.to(dev()), **{**d, "bias": many, "mask": d["mask"][1:2]})
+    assert np.array_equal(bits(got), bits(one.to(l.dtype)))
+    got = TH.penalize_logits(l.to(dev()), **{**d, "prompt": d["prompt"].t().contiguous().t(), "mask": d["mask"].expand(B, -1)})
+    assert np.array_equal(bits(got), want)
+    assert TH.penalize_logits(torch.zeros((0, V), device=dev())).shape == (0, V)
+    assert TH.penalize_logits(torch.zeros((B, 0), device=dev())).shape == (B, 0)
+    z = torch.zeros((B, 0), dtype=torch.int64, device=dev())
+    assert np.array_equal(bits(TH.penalize_logits(l.to(dev()), prompt=z, output=z)), bits(l))
+
+
+def test_bad_arguments():
+    from lockstep_amd import t16h_lmvariants as TH
+    l, c = _case(np.random.default_rng(10), 3, 100, 8, 8, torch.float32)
+    d = {k: to_dev(v) for k, v in c.items()}
+    l = l.to(dev())
+    bad = [dict(prompt=d["prompt"].float()), dict(prompt=d["prompt"][:2]), dict(prompt_lens=d["prompt_lens"]),
+           dict(output=d["output"], output_lens=d["output_lens"].float()), dict(repetition=d["repetition"][:2]),
+           dict(frequency=d["frequency"].double()), dict(bias=d["bias"][:99]), dict(mask=d["mask"][:, :3]),
+           dict(mask=d["mask"].to(torch.int64)), dict(out=torch.empty((3, 101), device=dev())),
+           dict(out=l.to(torch.bfloat16)), dict(out=l[:1].expand(3, 100)), dict(presence=d["presence"].cpu())]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            TH.penalize_logits(l, **kw)
+    with pytest.raises(ValueError):
+        TH.penalize_logits(l[0])
+    with pytest.raises(ValueError):
+        TH.penalize_logits(l.to(torch.int32))
