@@ -13,11 +13,10 @@
 #include <hip/hip_runtime.h>
 
 #include "lsk_common.h"
+#include "fp4_tile.h"
 #include "mfma_tile.h"
 
 namespace lsk {
-
-typedef int v8i __attribute__((ext_vector_type(8)));
 
 // ---------------------------------------------------------------- the quantiser
 // Eight values of a block (the block's other 24 in the three neighbouring lanes of a quad) to eight
@@ -70,42 +69,62 @@ LSK_DEV void load8(const void* x, int64_t i, float (&v)[8]) {
   }
 }
 
-// A thread per eight values, a quad of lanes per block: M * K / 8 threads' worth of work (a multiple
-// of 4), whole quads inside or outside it.  Bound by HBM: s_x bytes read and 17/32 written a value.
-template <int DT, bool VEC>
-__global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const void* __restrict__ x, int64_t ldx, int64_t total,
-                                                             int K8, uint8_t* __restrict__ packed,
-                                                             uint8_t* __restrict__ scale) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+// Where block b of row r of `rows` keeps its scale byte in the transposed form the tiles read:
+// [b / 4][row] dwords, byte b % 4.  Bytes past the last block are 0 (a 255 there would make NaNs of
+// the zero codes beside it).
+LSK_DEV void store_scale_t(uint8_t* t, int64_t rows, int64_t r, int b, int nb, uint32_t s) {
+  uint8_t* d = t + ((b >> 2) * rows + r) * 4;
+  d[b & 3] = (uint8_t)s;
+  if (b == nb - 1)
+    for (int z = (b & 3) + 1; z < 4; ++z) d[z] = 0;
+}
+
+// A thread per eight values, a quad of lanes per block: total = M * K / 8 threads' worth of work (a
+// multiple of 4, so quads lie wholly inside or outside it).  Bound by HBM: s_x bytes read and 17/32
+// written a value.  TS: the scales transposed.
+template <int DT, bool VEC, bool TS>
+LSK_DEV void quantize_run(const void* __restrict__ x, int64_t ldx, int64_t M, int64_t total, int K8, int block,
+                          int blocks, uint8_t* __restrict__ packed, uint8_t* __restrict__ scale) {
+  for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < total; i += (int64_t)blocks * 256) {
     const int64_t row = i / K8;
+    const int c = (int)(i - row * K8);
     float v[8];
-    load8<DT, VEC>(x, row * ldx + 8 * (i - row * K8), v);
+    load8<DT, VEC>(x, row * ldx + 8 * c, v);
     uint32_t s;
     ((uint32_t*)packed)[i] = quantize8_mxfp4(v, s);
-    if ((i & 3) == 0) scale[i >> 2] = (uint8_t)s;
+    if ((i & 3) == 0) {
+      if constexpr (TS) store_scale_t(scale, M, row, c >> 2, K8 >> 2, s);
+      else scale[i >> 2] = (uint8_t)s;
+    }
   }
+}
+
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const void* __restrict__ x, int64_t ldx, int64_t M,
+                                                             int64_t total, int K8, uint8_t* __restrict__ packed,
+                                                             uint8_t* __restrict__ scale) {
+  quantize_run<DT, VEC, false>(x, ldx, M, total, K8, blockIdx.x, gridDim.x, packed, scale);
+}
+
+// f(dtype, vec) with the dtype and the alignment of x's rows as compile-time values.
+template <class F>
+static void by_input(const void* x, int x_dtype, int64_t ldx, F f) {
+  const int size = x_dtype == LSK_F32 ? 4 : 2;
+  const bool vec = (uintptr_t)x % 16 == 0 && (ldx * size) % 16 == 0;
+  auto with = [&](auto dt) { vec ? f(dt, std::true_type{}) : f(dt, std::false_type{}); };
+  if (x_dtype == LSK_F32) with(std::integral_constant<int, LSK_F32>{});
+  else if (x_dtype == LSK_BF16) with(std::integral_constant<int, LSK_BF16>{});
+  else with(std::integral_constant<int, LSK_F16>{});
 }
 
 static int quantize_launch(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* packed,
                            uint8_t* scale, hipStream_t s) {
-  const int64_t total = M * (K / 8);
-  const int64_t blocks = (total + 255) / 256;
+  const int64_t total = M * (K / 8), blocks = (total + 255) / 256;
   const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536)), blk(256);
-  const int size = x_dtype == LSK_F32 ? 4 : 2;
-  const bool vec = (uintptr_t)x % 16 == 0 && (ldx * size) % 16 == 0;
-#define LSK_Q4(DT, V) \
-  hipLaunchKernelGGL((quantize_mxfp4_kernel<DT, V>), grid, blk, 0, s, x, ldx, total, (int)(K / 8), packed, scale)
-  if (x_dtype == LSK_F32) {
-    if (vec) LSK_Q4(LSK_F32, true);
-    else LSK_Q4(LSK_F32, false);
-  } else if (x_dtype == LSK_BF16) {
-    if (vec) LSK_Q4(LSK_BF16, true);
-    else LSK_Q4(LSK_BF16, false);
-  } else {
-    if (vec) LSK_Q4(LSK_F16, true);
-    else LSK_Q4(LSK_F16, false);
-  }
-#undef LSK_Q4
+  by_input(x, x_dtype, ldx, [&](auto dt, auto vec) {
+    hipLaunchKernelGGL((quantize_mxfp4_kernel<decltype(dt)::value, decltype(vec)::value>), grid, blk, 0, s, x, ldx, M,
+                       total, (int)(K / 8), packed, scale);
+  });
   return check_launch("quantize_mxfp4_kernel");
 }
 
@@ -171,8 +190,6 @@ LSK_DEV bool expert_tile(const int32_t* __restrict__ offs, int E, int R, int bm,
 }
 inline int64_t expert_tiles_max(int64_t R, int64_t E, int64_t bm) { return R / bm + (E < R ? E : R); }
 
-LSK_DEV v8i fp4_operand(v4i x) { return v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0}; }
-
 // One 16 x 16 piece of the output per wave over all of K: 16 weight rows as the instruction's rows,
 // 16 activation rows as its columns, so that a lane ends with four consecutive outputs of one row.
 // Rows past the end and blocks past K read zeros through the buffer range.
@@ -216,7 +233,215 @@ __global__ __launch_bounds__(64) void fp4_rows_kernel(Fp4Args p) {
   }
 }
 
-static int fp4_product(const Fp4Args& p, hipStream_t s) {
+// ---------------------------------------------------------------- tiles
+// Scales [rows, nb] bytes (row stride lds) to the transposed form, 8 dwords of a row a thread.
+LSK_DEV void transpose_scales(const uint8_t* __restrict__ s, int64_t lds, int64_t rows, int nb, int64_t block,
+                              uint32_t* __restrict__ t) {
+  const int nst = (nb + 3) / 4;
+  const int64_t rblocks = (rows + 255) / 256;
+  const int64_t c = block / rblocks, r = (block - c * rblocks) * 256 + threadIdx.x;
+  if (r >= rows) return;
+  const uint8_t* p = s + r * lds;
+  for (int d = (int)c * 8; d < (int)c * 8 + 8 && d < nst; ++d) {
+    uint32_t w = 0;
+    if (4 * d + 4 <= nb) __builtin_memcpy(&w, p + 4 * d, 4);
+    else
+      for (int z = 0; 4 * d + z < nb; ++z) w |= (uint32_t)p[4 * d + z] << (8 * z);
+    t[d * rows + r] = w;
+  }
+}
+inline int64_t transpose_blocks(int64_t rows, int64_t K) { return ((rows + 255) / 256) * ((K / 32 + 31) / 32); }
+
+// What the tiles need beside the codes, in one launch: the rows quantised with transposed scales (DT an
+// input type) or their scales transposed (DT < 0), and the weights' scales transposed, every expert's
+// in turn.
+struct Fp4Prep {
+  const void* x;
+  int64_t ldx, M, total;
+  int K;
+  uint8_t* q;
+  const uint8_t* sa;
+  int64_t ldsa;
+  uint32_t* sat;
+  int64_t ablocks;
+  const uint8_t* sw;
+  const int64_t* ws_ptrs;
+  int64_t ldsw, N, wblocks;  // blocks of one weight
+  uint32_t* swt;
+};
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void fp4_prep_kernel(Fp4Prep p) {
+  if (blockIdx.x < p.ablocks) {
+    if constexpr (DT >= 0)
+      quantize_run<DT, VEC, true>(p.x, p.ldx, p.M, p.total, p.K / 8, blockIdx.x, (int)p.ablocks, p.q, (uint8_t*)p.sat);
+    else
+      transpose_scales(p.sa, p.ldsa, p.M, p.K / 32, blockIdx.x, p.sat);
+    return;
+  }
+  const int64_t b = blockIdx.x - p.ablocks, e = b / p.wblocks;
+  transpose_scales(p.ws_ptrs ? (const uint8_t*)p.ws_ptrs[e] : p.sw, p.ldsw, p.N, p.K / 32, b - e * p.wblocks,
+                   p.swt + e * p.N * ((p.K + 127) / 128));
+}
+
+// A BM x BN tile: tiles walk kGroupM row tiles down a column of weight tiles inside each XCD's run
+// of them, so the row tiles that share a weight tile run together on one L2.
+template <int BM, int BN, int WM, int WN, int RING, int BKB, bool GROUPED>
+__global__ __launch_bounds__(512) void fp4_tile_kernel(Fp4Args p, const uint32_t* __restrict__ sat,
+                                                       const uint32_t* __restrict__ swt, int64_t mtiles, int vec) {
+  using C = Fp4Cfg<BM, BN, WM, WN, RING, BKB>;
+  constexpr int kGroupM = 4;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int ntiles = (int)((p.N + BN - 1) / BN);
+  const int L = xcd_logical_id(blockIdx.x, (int)mtiles * ntiles);
+  const int first = L / (kGroupM * ntiles) * kGroupM;
+  const int gsize = (int)mtiles - first < kGroupM ? (int)mtiles - first : kGroupM;
+  const int in = L - first * ntiles;
+  const int n0 = in / gsize * BN;
+  int m0 = (first + in % gsize) * BM, m1 = (int)p.M;
+  const int nst = (p.K + 127) / 128;
+  if constexpr (GROUPED) {
+    int e, f, l;
+    if (!expert_tile(p.offs, p.E, (int)p.M, BM, first + in % gsize, e, f, l)) return;
+    m0 = f, m1 = l;
+    p.w = (const uint8_t*)wave_uniform64(p.w_ptrs[e]);
+    p.bias = p.b_ptrs ? (const float*)wave_uniform64(p.b_ptrs[e]) : nullptr;
+    swt += (int64_t)e * nst * p.N;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+  const int rows_a = m1 - m0 < BM ? m1 - m0 : BM, rows_w = (int)p.N - n0 < BN ? (int)p.N - n0 : BN;
+
+  Fp4Rows<C> t;
+  const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.a + (int64_t)m0 * p.lda, (int64_t)(rows_a - 1) * p.lda + p.K / 2);
+  const __amdgpu_buffer_rsrc_t rb = make_rsrc(p.w + (int64_t)n0 * p.ldw, (int64_t)(rows_w - 1) * p.ldw + p.K / 2);
+  t.sta = (uint32_t)(4 * p.M), t.stb = (uint32_t)(4 * p.N);
+  const __amdgpu_buffer_rsrc_t rsa = make_rsrc(sat + m0, 4 * ((int64_t)nst * p.M - m0));
+  const __amdgpu_buffer_rsrc_t rsb = make_rsrc(swt + n0, 4 * ((int64_t)nst * p.N - n0));
+#pragma unroll
+  for (int j = 0; j < C::kLA; ++j) {
+    int row, kb;
+    pp_slot<C::kThreads, C::kChunks>(tid, j, row, kb);
+    t.a[j] = row < rows_a ? (uint32_t)(row * p.lda) : kOob;
+  }
+#pragma unroll
+  for (int j = 0; j < C::kLB; ++j) {
+    int row, kb;
+    pp_slot<C::kThreads, C::kChunks>(tid, j, row, kb);
+    t.b[j] = row < rows_w ? (uint32_t)(row * p.ldw) : kOob;
+  }
+  t.s = tid < BM ? (tid < rows_a ? 4u * tid : kOob) : (tid - BM < rows_w ? 4u * (tid - BM) : kOob);
+
+  typename C::Acc acc;
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+#ifdef __HIP_DEVICE_COMPILE__  // (the host pass does not instantiate the main loop twice)
+  fp4_mainloop<BM, BN, WM, WN, RING, BKB>(acc, ra, rb, rsa, rsb, t, p.K, smem);
+#endif
+  __syncthreads();
+
+  // a 32-row strip at a time through the wave's part of LDS, out of it four consecutive columns a lane
+  const int wm = wave / C::kWN, wn = wave % C::kWN;
+  float* strip = (float*)(smem + wave * 32 * C::kLdc * 4);
+  constexpr int kLanes = C::WTN / 4, kRows = 64 / kLanes;  // lanes a row, rows an instruction
+  const int col = wn * C::WTN + lane % kLanes * 4;
+  float b[4] = {0, 0, 0, 0};
+  if (p.bias)
+#pragma unroll
+    for (int z = 0; z < 4; ++z)
+      if (col + z < rows_w) b[z] = p.bias[n0 + col + z];
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        *(v4f*)(strip + (lane & 31) * C::kLdc + j * 32 + 8 * h + 4 * (lane >> 5)) =
+            v4f{acc[i][j][4 * h], acc[i][j][4 * h + 1], acc[i][j][4 * h + 2], acc[i][j][4 * h + 3]};
+    // (a wave's own LDS operations run in order)
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += kRows) {
+      const int r = r0 + lane / kLanes, row = wm * C::WTM + i * 32 + r;
+      v4f v = *(const v4f*)(strip + r * C::kLdc + lane % kLanes * 4);
+      if (row >= rows_a || col >= rows_w) continue;
+      float y[4];
+#pragma unroll
+      for (int z = 0; z < 4; ++z) y[z] = p.bias ? f32_add(v[z], b[z]) : v[z];
+      const int64_t o = (int64_t)(m0 + row) * p.ldo + n0 + col;
+      if (vec && col + 4 <= rows_w) store4_out(p.out, LSK_EPI_V21, p.out_dtype, o, y, zero4());
+      else
+        for (int z = 0; z < 4 && col + z < rows_w; ++z) store_out(p.out, p.out_dtype, o + z, y[z]);
+    }
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int RING, int BKB>
+static int fp4_tile_launch(const Fp4Args& p, const uint32_t* sat, const uint32_t* swt, hipStream_t s) {
+  using C = Fp4Cfg<BM, BN, WM, WN, RING, BKB>;
+  const int64_t mtiles = p.offs ? expert_tiles_max(p.M, p.E, BM) : (p.M + BM - 1) / BM;
+  const int64_t blocks = mtiles * ((p.N + BN - 1) / BN);
+  LSK_REQUIRE(blocks <= 0x7fffffff, "mxfp4 product: grid too large");
+  const int vec = out_vec_ok(p.out, p.out_dtype, p.ldo);
+  auto run = [&](auto kern) {
+    if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes) != hipSuccess)
+      return set_error("fp4_tile_kernel: cannot reserve LDS"), LSK_ERR_HIP;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(C::kThreads), C::kSmemBytes, s, p, sat, swt, mtiles, vec);
+    return check_launch("fp4_tile_kernel");
+  };
+  return p.offs ? run(fp4_tile_kernel<BM, BN, WM, WN, RING, BKB, true>)
+                : run(fp4_tile_kernel<BM, BN, WM, WN, RING, BKB, false>);
+}
+
+// Whether the products of M rows (R over E experts) run on the tiles, which need the operands' offsets
+// inside 31 bits.
+static bool fp4_takes_tiles(int64_t M, int64_t N, int64_t K, int64_t E) {
+  const int64_t nst = (K + 127) / 128;
+  return K > 0 && M > 64 * E && 4 * nst * M < 0x7fffffff && 4 * nst * N < 0x7fffffff && 256 * (K / 2) < 0x7fffffff;
+}
+
+static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// Bytes of the transposed scales of M rows and of E weights of N rows.
+static int64_t fp4_prep_bytes(int64_t M, int64_t N, int64_t K, int64_t E) {
+  const int64_t nst = (K + 127) / 128;
+  return up256(4 * nst * M) + up256(4 * nst * N * E);
+}
+
+// The tiles' products: p.a / p.sa the rows (x null), or x to be quantised into q first.
+static int fp4_tiles(Fp4Args p, const void* x, int x_dtype, int64_t ldx, uint8_t* q, char* work, hipStream_t s) {
+  const int64_t nst = (p.K + 127) / 128, E = p.offs ? p.E : 1;
+  Fp4Prep r{};
+  r.M = p.M, r.K = p.K;
+  r.sat = (uint32_t*)work, r.swt = (uint32_t*)(work + up256(4 * nst * p.M));
+  r.sw = p.sw, r.ws_ptrs = p.offs ? p.ws_ptrs : nullptr, r.ldsw = p.ldsw, r.N = p.N;
+  r.wblocks = transpose_blocks(p.N, p.K);
+  if (x) {
+    r.x = x, r.ldx = ldx, r.total = p.M * (p.K / 8), r.q = q;
+    r.ablocks = (r.total + 255) / 256 < 65536 ? (r.total + 255) / 256 : 65536;
+    p.a = q;
+  } else {
+    r.sa = p.sa, r.ldsa = p.ldsa, r.ablocks = transpose_blocks(p.M, p.K);
+  }
+  LSK_REQUIRE(r.ablocks + r.wblocks * E <= 0x7fffffff, "mxfp4 product: grid too large");
+  const dim3 grid((unsigned)(r.ablocks + r.wblocks * E)), blk(256);
+  if (x)
+    by_input(x, x_dtype, ldx, [&](auto dt, auto vec) {
+      hipLaunchKernelGGL((fp4_prep_kernel<decltype(dt)::value, decltype(vec)::value>), grid, blk, 0, s, r);
+    });
+  else
+    hipLaunchKernelGGL((fp4_prep_kernel<-1, false>), grid, blk, 0, s, r);
+  const int rc = check_launch("fp4_prep_kernel");
+  if (rc) return rc;
+  const int64_t per = p.M / E;  // rows an expert, on average
+  const auto tiles = [&](int64_t bm, int64_t bn) { return ((per + bm - 1) / bm) * E * ((p.N + bn - 1) / bn); };
+  if (tiles(256, 256) >= 256) return fp4_tile_launch<256, 256, 2, 4, 4, 64>(p, r.sat, r.swt, s);
+  if (tiles(128, 128) >= 192) return fp4_tile_launch<128, 128, 4, 2, 4, 128>(p, r.sat, r.swt, s);
+  return fp4_tile_launch<64, 128, 2, 4, 5, 128>(p, r.sat, r.swt, s);
+}
+
+static int fp4_rows(const Fp4Args& p, hipStream_t s) {
   const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16) : (p.M + 15) / 16;
   const int64_t blocks = tiles * ((p.N + 15) / 16);
   LSK_REQUIRE(blocks <= 0x7fffffff, "mxfp4 product: grid too large");
@@ -228,7 +453,9 @@ static int fp4_product(const Fp4Args& p, hipStream_t s) {
 
 static bool is_float_dtype(int d) { return d == LSK_F32 || d == LSK_BF16 || d == LSK_F16; }
 
-static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+static bool work_ok(const void* w, int64_t have, int64_t need) {
+  return have >= need && (need == 0 || (w && (uintptr_t)w % 256 == 0));
+}
 
 }  // namespace lsk
 
@@ -255,9 +482,12 @@ static int mxfp4_check(const char* who, int64_t M, int64_t N, int64_t K, int out
 }
 
 extern "C" int64_t lsk_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
-  (void)M, (void)N, (void)K;
-  return 0;
+  return lsk::fp4_takes_tiles(M, N, K, 1) ? lsk::fp4_prep_bytes(M, N, K, 1) : 0;
 }
+
+#define LSK_REQUIRE_WORK(who, need)                                                                                  \
+  LSK_REQUIRE(lsk::work_ok(workspace, workspace_bytes, need), who ": workspace of %lld bytes (256-byte aligned) needed", \
+              (long long)(need))
 
 extern "C" int lsk_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, int64_t M, int64_t K, const uint8_t* w,
                               const uint8_t* w_scale, int64_t N, const float* bias, void* out, int out_dtype,
@@ -267,16 +497,20 @@ extern "C" int lsk_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, int64_t 
   if (M == 0 || N == 0) return LSK_OK;
   LSK_REQUIRE(out && (K == 0 || (a && a_scale && w && w_scale)), "lsk_gemm_mxfp4: null pointer");
   LSK_REQUIRE((uintptr_t)a % 16 == 0 && (uintptr_t)w % 16 == 0, "lsk_gemm_mxfp4: codes must be 16-byte aligned");
+  LSK_REQUIRE_WORK("lsk_gemm_mxfp4", lsk_gemm_mxfp4_workspace(M, N, K));
   lsk::Fp4Args p{};
   p.a = a, p.sa = a_scale, p.w = w, p.sw = w_scale;
   p.lda = p.ldw = K / 2, p.ldsa = p.ldsw = K / 32;
   p.M = M, p.N = N, p.K = (int)K;
   p.bias = bias, p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
-  return lsk::fp4_product(p, (hipStream_t)stream);
+  if (lsk::fp4_takes_tiles(M, N, K, 1)) return lsk::fp4_tiles(p, nullptr, 0, 0, nullptr, (char*)workspace, (hipStream_t)stream);
+  return lsk::fp4_rows(p, (hipStream_t)stream);
 }
 
+// The quantised rows come first in the workspace, then their scales (the row kernels) or the tiles' part.
 extern "C" int64_t lsk_linear_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
-  return lsk::up256(M * (K / 2)) + lsk::up256(M * (K / 32)) + lsk_gemm_mxfp4_workspace(M, N, K);
+  return lsk::up256(M * (K / 2)) +
+         (lsk::fp4_takes_tiles(M, N, K, 1) ? lsk::fp4_prep_bytes(M, N, K, 1) : lsk::up256(M * (K / 32)));
 }
 
 extern "C" int lsk_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int64_t M, int64_t K, const uint8_t* w,
@@ -284,22 +518,27 @@ extern "C" int lsk_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int64_t
                                 int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream) {
   int rc = mxfp4_check("lsk_linear_mxfp4", M, N, K, out_dtype, ldo);
   if (rc) return rc;
+  LSK_REQUIRE(lsk::is_float_dtype(x_dtype), "lsk_linear_mxfp4: x_dtype must be f32, bf16 or f16");
   if (M == 0 || N == 0) return LSK_OK;
-  const int64_t need = lsk_linear_mxfp4_workspace(M, N, K);
-  LSK_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 256 == 0)),
-              "lsk_linear_mxfp4: workspace of %lld bytes (256-byte aligned) needed", (long long)need);
+  LSK_REQUIRE(out && (K == 0 || (x && w && w_scale)), "lsk_linear_mxfp4: null pointer");
+  LSK_REQUIRE(M == 1 || ldx >= K, "lsk_linear_mxfp4: ldx below K");
+  LSK_REQUIRE((uintptr_t)w % 16 == 0, "lsk_linear_mxfp4: codes must be 16-byte aligned");
+  LSK_REQUIRE_WORK("lsk_linear_mxfp4", lsk_linear_mxfp4_workspace(M, N, K));
+  hipStream_t s = (hipStream_t)stream;
   uint8_t* q = (uint8_t*)workspace;
-  uint8_t* qs = q + lsk::up256(M * (K / 2));
-  uint8_t* rest = qs + lsk::up256(M * (K / 32));
-  rc = lsk_quantize_mxfp4(x, x_dtype, M, K, ldx, q, qs, stream);
-  if (rc) return rc;
-  return lsk_gemm_mxfp4(q, qs, M, K, w, w_scale, N, bias, out, out_dtype, ldo, rest,
-                        workspace_bytes - (int64_t)(rest - (uint8_t*)workspace), stream);
+  uint8_t* rest = q + lsk::up256(M * (K / 2));
+  lsk::Fp4Args p{};
+  p.a = q, p.sa = rest, p.w = w, p.sw = w_scale;
+  p.lda = p.ldw = K / 2, p.ldsa = p.ldsw = K / 32;
+  p.M = M, p.N = N, p.K = (int)K;
+  p.bias = bias, p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
+  if (lsk::fp4_takes_tiles(M, N, K, 1)) return lsk::fp4_tiles(p, x, x_dtype, ldx, q, (char*)rest, s);
+  if (K > 0 && (rc = lsk::quantize_launch(x, x_dtype, M, K, ldx, q, rest, s))) return rc;
+  return lsk::fp4_rows(p, s);
 }
 
 extern "C" int64_t lsk_grouped_gemm_mxfp4_workspace(int64_t R, int64_t E, int64_t N, int64_t K) {
-  (void)R, (void)E, (void)N, (void)K;
-  return 0;
+  return lsk::fp4_takes_tiles(R, N, K, E) ? lsk::fp4_prep_bytes(R, N, K, E) : 0;
 }
 
 extern "C" int lsk_grouped_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, const int32_t* offs, int64_t E, int64_t R,
@@ -314,11 +553,13 @@ extern "C" int lsk_grouped_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, 
   LSK_REQUIRE((uintptr_t)a % 16 == 0 && ldw >= K / 2 && ldw % 16 == 0 && lds >= K / 32,
               "lsk_grouped_gemm_mxfp4: codes in rows of 16-byte multiples, strides that cover K");
   LSK_REQUIRE(ldw <= (1 << 26) && lds <= (1 << 26), "lsk_grouped_gemm_mxfp4: row strides beyond 2^26 bytes");
+  LSK_REQUIRE_WORK("lsk_grouped_gemm_mxfp4", lsk_grouped_gemm_mxfp4_workspace(R, E, N, K));
   lsk::Fp4Args p{};
   p.a = a, p.sa = a_scale;
   p.lda = K / 2, p.ldsa = K / 32, p.ldw = ldw, p.ldsw = lds;
   p.M = R, p.N = N, p.K = (int)K;
   p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
   p.offs = offs, p.E = (int)E, p.w_ptrs = w_ptrs, p.ws_ptrs = ws_ptrs, p.b_ptrs = b_ptrs;
-  return lsk::fp4_product(p, (hipStream_t)stream);
+  if (lsk::fp4_takes_tiles(R, N, K, E)) return lsk::fp4_tiles(p, nullptr, 0, 0, nullptr, (char*)workspace, (hipStream_t)stream);
+  return lsk::fp4_rows(p, (hipStream_t)stream);
 }
