@@ -4,10 +4,14 @@
 // prompt or output:
 //   l = fl32(l + bias[v]);  seen: l = l > 0 ? fl32(l / r) : fl32(l * r);
 //   l = fl32(l - fl32(f * n));  n > 0: l = fl32(l - p);  mask bit 0: l = -inf;  out = round(l)
-// A block owns a run of one row's tokens: it counts the row's history into a table of that run in LDS
-// (a word per token: the output count, and the top bit for the prompt; integer atomics, so the order
-// of tokens changes nothing), then streams the logits past it.  Every block of a row reads the whole
-// history, which stays in the L2.
+// A block owns a run of one row's tokens.  It counts the row's history into a table of that run in LDS
+// (the output count, and the top bit for the prompt; integer atomics, so the order of tokens changes
+// nothing), streams the run once with bias and mask, leaving the counted tokens as they came, and then
+// walks the history again: the first thread to take a token's count out of the table computes that
+// token from its logit and stores it.  So the penalties cost their few tokens, not every token, and
+// the stream is a copy at the rate of HBM.  Every block of a row reads the whole history, which stays
+// in the L2: runs are as long as the LDS of two blocks a CU allows, and shorter where there are too
+// few rows to fill the part with them.
 #include <hip/hip_runtime.h>
 
 #include "lsk_common.h"
@@ -29,63 +33,171 @@ struct PenaltyArgs {
   int64_t ldm;
   void* out;
   int64_t ldo;
-  int chunk;                              // tokens of a block, a multiple of 8
+  int chunk;                              // tokens of a block
 };
-
-constexpr uint32_t kInPrompt = 0x80000000u;
 
 LSK_DEV int64_t int_at(const void* p, int wide, int64_t i) {
   return wide ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
 }
 
-template <int DT>
-LSK_DEV float logit_at(const void* p, int64_t i) { return load_as_f32(p, DT, i); }
+// The count table: 16-bit entries, two a word, while no count can reach the prompt's bit (Lo < 2^15),
+// else 32-bit ones.
+template <int BITS>
+struct CountTable {
+  uint32_t* w;
+  static constexpr uint32_t kPrompt = 1u << (BITS - 1), kAll = BITS == 32 ? 0xffffffffu : 0xffffu;
+  LSK_DEV int word(int i) const { return BITS == 32 ? i : i >> 1; }
+  LSK_DEV int shift(int i) const { return BITS == 32 ? 0 : (i & 1) * 16; }
+  LSK_DEV void mark_prompt(int i) { atomicOr(&w[word(i)], kPrompt << shift(i)); }
+  LSK_DEV void count(int i) { atomicAdd(&w[word(i)], 1u << shift(i)); }
+  LSK_DEV uint32_t at(int i) const { return (w[word(i)] >> shift(i)) & kAll; }
+  LSK_DEV uint32_t take(int i) { return (atomicAnd(&w[word(i)], ~(kAll << shift(i))) >> shift(i)) & kAll; }
+};
 
-template <int DT>
-__global__ __launch_bounds__(512) void penalize_logits_kernel(PenaltyArgs p) {
-  extern __shared__ uint32_t count[];
-  const int tid = threadIdx.x, chunks = (int)((p.V + p.chunk - 1) / p.chunk);
+// f(local token) for each token of a row's history that lies in the block's run [v0, v0 + n).
+template <class F>
+LSK_DEV void each_token(const void* tok, int wide, int64_t ld, int64_t L, const void* lens, int lwide, int64_t b,
+                        int64_t v0, int n, F f) {
+  if (!tok) return;
+  int64_t len = lens ? int_at(lens, lwide, b) : L;
+  len = len < L ? len : L;
+  for (int64_t i = threadIdx.x; i < len; i += blockDim.x) {
+    const int64_t t = int_at(tok, wide, b * ld + i) - v0;
+    if (t >= 0 && t < n) f((int)t);
+  }
+}
+
+template <int DT, int BITS>
+__global__ __launch_bounds__(1024) void penalize_logits_kernel(PenaltyArgs p) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t smem[];
+  constexpr int VEC = DT == LSK_F32 ? 4 : 8, SIZE = DT == LSK_F32 ? 4 : 2;
+  const int tid = threadIdx.x, nt = blockDim.x, chunks = (int)((p.V + p.chunk - 1) / p.chunk);
   const int64_t b = blockIdx.x / chunks, v0 = (int64_t)(blockIdx.x - b * chunks) * p.chunk;
   const int n = (int)(p.V - v0 < p.chunk ? p.V - v0 : p.chunk);
   const bool counted = p.prompt || p.output;
+  const char* in = (const char*)p.logits + (b * p.ldl + v0) * SIZE;
+  char* out = (char*)p.out + (b * p.ldo + v0) * SIZE;
+  const float* bias = p.bias ? p.bias + b * p.ldb + v0 : nullptr;
+  const uint32_t* mask = p.mask ? p.mask + b * p.ldm : nullptr;
+  // the run's first 16-byte boundary, where the vectors start (rows of in and out that differ modulo
+  // 16 bytes go token by token); the table starts `pad` entries in, so that vectors of it are whole too
+  const bool vec = ((uintptr_t)in & 15) == ((uintptr_t)out & 15) && (uintptr_t)in % SIZE == 0;
+  int head = vec ? (int)((16 - ((uintptr_t)in & 15)) & 15) / SIZE : n;
+  head = head < n ? head : n;
+  const int pad = (VEC - head % VEC) % VEC;
+  CountTable<BITS> table{smem};
+  auto prompt = [&](auto f) { each_token(p.prompt, p.p64, p.ldp, p.Lp, p.prompt_lens, p.pl64, b, v0, n, f); };
+  auto output = [&](auto f) { each_token(p.output, p.o64, p.ldo_tok, p.Lo, p.output_lens, p.ol64, b, v0, n, f); };
   if (counted) {
-    for (int i = tid; i < n; i += 512) count[i] = 0;
+    const int words = ((n + pad) * BITS + 31) / 32;
+    for (int i = tid; i < (words + 3) / 4; i += nt) ((uint4*)smem)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (p.prompt) {
-      int64_t len = p.prompt_lens ? int_at(p.prompt_lens, p.pl64, b) : p.Lp;
-      len = len < p.Lp ? len : p.Lp;
-      for (int64_t i = tid; i < len; i += 512) {
-        const int64_t t = int_at(p.prompt, p.p64, b * p.ldp + i) - v0;
-        if (t >= 0 && t < n) atomicOr(&count[t], kInPrompt);
-      }
-    }
-    if (p.output) {
-      int64_t len = p.output_lens ? int_at(p.output_lens, p.ol64, b) : p.Lo;
-      len = len < p.Lo ? len : p.Lo;
-      for (int64_t i = tid; i < len; i += 512) {
-        const int64_t t = int_at(p.output, p.o64, b * p.ldo_tok + i) - v0;
-        if (t >= 0 && t < n) atomicAdd(&count[t], 1u);
-      }
-    }
+    prompt([&](int t) { table.mark_prompt(t + pad); });
+    output([&](int t) { table.count(t + pad); });
     __syncthreads();
   }
-  const float rep = p.rep ? p.rep[b] : 1.0f, freq = p.freq ? p.freq[b] : 0.0f, pres = p.pres ? p.pres[b] : 0.0f;
-  for (int i = tid; i < n; i += 512) {
+
+  auto allowed = [&](int i) {
     const int64_t v = v0 + i;
-    float l = logit_at<DT>(p.logits, b * p.ldl + v);
-    if (p.bias) l = f32_add(l, p.bias[b * p.ldb + v]);
-    const uint32_t c = counted ? count[i] : 0;
-    if (c) {
-      if (p.rep) l = l > 0.0f ? f32_div(l, rep) : f32_mul(l, rep);
-      const uint32_t k = c & ~kInPrompt;
-      if (k) {
-        if (p.freq) l = l - f32_mul(freq, (float)k);
-        if (p.pres) l = l - pres;
+    return !mask || ((mask[v >> 5] >> (v & 31)) & 1u);
+  };
+  auto one = [&](int i) {
+    float l = load_as_f32(in, DT, i);
+    if (counted && table.at(i + pad)) {
+      if (in != out) store_out(out, DT, i, l);
+      return;
+    }
+    if (bias) l = f32_add(l, bias[i]);
+    store_out(out, DT, i, allowed(i) ? l : -__builtin_inff());
+  };
+  for (int i = tid; i < head; i += nt) one(i);
+  const int nvec = (n - head) / VEC;
+  for (int g = tid; g < nvec; g += nt) {
+    const int i = head + g * VEC;
+    const v4u32 raw = *(const v4u32*)(in + (int64_t)i * SIZE);
+    uint32_t live = 0;  // a bit per counted token
+    if (counted) {
+      const uint4* c = (const uint4*)((const char*)smem + (int64_t)(i + pad) * (BITS / 8));
+#pragma unroll
+      for (int q = 0; q < VEC * BITS / 128; ++q) {
+        const uint4 u = c[q];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          if constexpr (BITS == 32) {
+            live |= (w[z] ? 1u : 0u) << (4 * q + z);
+          } else {
+            live |= ((w[z] & 0xffffu) ? 1u : 0u) << (8 * q + 2 * z);
+            live |= ((w[z] >> 16) ? 1u : 0u) << (8 * q + 2 * z + 1);
+          }
+        }
       }
     }
-    if (p.mask && !((p.mask[b * p.ldm + (v >> 5)] >> (v & 31)) & 1u)) l = -__builtin_inff();
-    store_out(p.out, DT, b * p.ldo + v, l);
+    if (!bias && !mask) {  // nothing to do but copy
+      if (in != out) *(v4u32*)(out + (int64_t)i * SIZE) = raw;
+      continue;
+    }
+    float l[VEC], s[VEC];
+    const uint32_t rw[4] = {raw[0], raw[1], raw[2], raw[3]};
+#pragma unroll
+    for (int z = 0; z < VEC; ++z) {
+      if constexpr (DT == LSK_F32) l[z] = __uint_as_float(rw[z]);
+      else if constexpr (DT == LSK_BF16) l[z] = bf16_to_f32((uint16_t)(rw[z / 2] >> (z % 2 * 16)));
+      else l[z] = (float)__builtin_bit_cast(_Float16, (uint16_t)(rw[z / 2] >> (z % 2 * 16)));
+      s[z] = l[z];
+    }
+    if (bias) {
+      float bv[VEC];
+      __builtin_memcpy(bv, bias + i, VEC * 4);
+#pragma unroll
+      for (int z = 0; z < VEC; ++z) s[z] = f32_add(s[z], bv[z]);
+    }
+    if (mask) {
+      const int64_t v = v0 + i;
+      const uint64_t lo = mask[v >> 5], hi = mask[(v + VEC - 1) >> 5];
+      const uint32_t m = (uint32_t)(((hi << 32) | lo) >> (v & 31));  // (VEC bits at most: inside 64)
+#pragma unroll
+      for (int z = 0; z < VEC; ++z)
+        if (!((m >> z) & 1u)) s[z] = -__builtin_inff();
+    }
+    uint32_t o[4];
+#pragma unroll
+    for (int z = 0; z < VEC; ++z)
+      if ((live >> z) & 1u) s[z] = l[z];
+    if constexpr (DT == LSK_F32) {
+#pragma unroll
+      for (int z = 0; z < 4; ++z) o[z] = __float_as_uint(s[z]);
+    } else if constexpr (DT == LSK_BF16) {
+#pragma unroll
+      for (int z = 0; z < 4; ++z) o[z] = pack_bf16x2(s[2 * z], s[2 * z + 1]);
+    } else {
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+        o[z] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)s[2 * z]) |
+               ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)s[2 * z + 1]) << 16);
+    }
+    store16_split(out + (int64_t)i * SIZE, o[0], o[1], o[2], o[3]);
   }
+  for (int i = head + nvec * VEC + tid; i < n; i += nt) one(i);
+  if (!counted) return;
+
+  __syncthreads();
+  const float rep = p.rep ? p.rep[b] : 1.0f, freq = p.freq ? p.freq[b] : 0.0f, pres = p.pres ? p.pres[b] : 0.0f;
+  auto penalize = [&](int i) {
+    const uint32_t c = table.take(i + pad);
+    if (!c) return;  // another thread has it
+    float l = load_as_f32(in, DT, i);
+    if (bias) l = f32_add(l, bias[i]);
+    if (p.rep) l = l > 0.0f ? f32_div(l, rep) : f32_mul(l, rep);
+    const uint32_t k = c & (CountTable<BITS>::kPrompt - 1);
+    if (k) {
+      if (p.freq) l = l - f32_mul(freq, (float)k);
+      if (p.pres) l = l - pres;
+    }
+    store_out(out, DT, i, allowed(i) ? l : -__builtin_inff());
+  };
+  prompt(penalize);
+  output(penalize);
 }
 
 }  // namespace lsk
@@ -113,14 +225,29 @@ extern "C" int lsk_penalize_logits(const void* logits, int dtype, int64_t ldl, i
   p.rep = repetition, p.freq = frequency, p.pres = presence;
   p.bias = bias, p.ldb = ldb, p.mask = (const uint32_t*)mask, p.ldm = ldm;
   p.out = out, p.ldo = ldo;
-  p.chunk = 8192;
+  // 16-bit counts while they cannot reach the prompt's bit; runs of up to 76 KB of them (two blocks a
+  // CU), at least 512 blocks where runs of 1024 tokens give as many
+  const bool narrow = Lo < (1 << 15), counted = p.prompt || p.output;
+  const int64_t most = counted && !narrow ? 19456 : 38912;
+  int64_t chunks = (512 + B - 1) / B;
+  if (chunks > (V + 1023) / 1024) chunks = (V + 1023) / 1024;
+  if (chunks < (V + most - 1) / most) chunks = (V + most - 1) / most;
+  p.chunk = (int)(((V + chunks - 1) / chunks + 31) / 32 * 32);
   const int64_t blocks = B * ((V + p.chunk - 1) / p.chunk);
   LSK_REQUIRE(blocks <= 0x7fffffff, "lsk_penalize_logits: grid too large");
-  const size_t smem = p.prompt || p.output ? 4 * (size_t)p.chunk : 0;
-  const dim3 grid((unsigned)blocks), blk(512);
+  const size_t smem = counted ? ((size_t)p.chunk + 8) * (narrow ? 2 : 4) + 16 : 0;
+  const dim3 grid((unsigned)blocks), blk(p.chunk >= 8192 ? 1024 : 256);
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == LSK_F32) hipLaunchKernelGGL(lsk::penalize_logits_kernel<LSK_F32>, grid, blk, smem, s, p);
-  else if (dtype == LSK_BF16) hipLaunchKernelGGL(lsk::penalize_logits_kernel<LSK_BF16>, grid, blk, smem, s, p);
-  else hipLaunchKernelGGL(lsk::penalize_logits_kernel<LSK_F16>, grid, blk, smem, s, p);
-  return lsk::check_launch("penalize_logits_kernel");
+  auto run = [&](auto kern) {
+    if (smem > 65536 &&
+        hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != hipSuccess)
+      return lsk::set_error("lsk_penalize_logits: cannot reserve LDS"), LSK_ERR_HIP;
+    hipLaunchKernelGGL(kern, grid, blk, smem, s, p);
+    return lsk::check_launch("penalize_logits_kernel");
+  };
+  if (dtype == LSK_F32)
+    return narrow ? run(lsk::penalize_logits_kernel<LSK_F32, 16>) : run(lsk::penalize_logits_kernel<LSK_F32, 32>);
+  if (dtype == LSK_BF16)
+    return narrow ? run(lsk::penalize_logits_kernel<LSK_BF16, 16>) : run(lsk::penalize_logits_kernel<LSK_BF16, 32>);
+  return narrow ? run(lsk::penalize_logits_kernel<LSK_F16, 16>) : run(lsk::penalize_logits_kernel<LSK_F16, 32>);
 }
