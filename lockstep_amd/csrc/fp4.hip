@@ -190,46 +190,126 @@ LSK_DEV bool expert_tile(const int32_t* __restrict__ offs, int E, int R, int bm,
 }
 inline int64_t expert_tiles_max(int64_t R, int64_t E, int64_t bm) { return R / bm + (E < R ? E : R); }
 
-// One 16 x 16 piece of the output per wave over all of K: 16 weight rows as the instruction's rows,
-// 16 activation rows as its columns, so that a lane ends with four consecutive outputs of one row.
-// Rows past the end and blocks past K read zeros through the buffer range.
-template <bool GROUPED>
-__global__ __launch_bounds__(64) void fp4_rows_kernel(Fp4Args p) {
+// Four steps of 128 values of a wave's rows: 16 weight rows, MT x 16 activation rows.
+template <int MT>
+struct Fp4Unit {
+  v4i w[4], a[MT][4];  // a lane's block of each step: row lane % 16, block lane / 16
+  v4u32 sw, sa[MT];    // its rows' scale dwords of the four steps
+};
+
+// Few rows: a wave computes 16 output columns of MT x 16 rows over all of K, streaming its 16 weight
+// rows from HBM into the instruction (weight rows as its rows, activation rows as its columns, so a
+// lane ends with four consecutive outputs of a row).  Bound by HBM, that is by bytes in flight: P units
+// of four steps are kept in flight in registers, each reissued as soon as it has been multiplied (P
+// KB-sized loads of four a wave).  The main loop has no branch around a load; a last partial unit is
+// loaded first, block by block.  K is not split over waves: a row's bits would depend on the split.
+template <int MT, int P, bool GROUPED>
+__global__ __launch_bounds__(64, 1) void fp4_rows_kernel(Fp4Args p) {
   const int lane = threadIdx.x, r = lane & 15, q = lane >> 4;
-  const int64_t ngroups = (p.N + 15) / 16;
-  const int64_t tile = blockIdx.x / ngroups, n0 = (blockIdx.x - tile * ngroups) * 16;
-  int64_t m0 = tile * 16, m1 = p.M;
+  const int ngroups = (int)((p.N + 15) / 16);
+  const int tile = blockIdx.x / ngroups, n0 = (blockIdx.x - tile * ngroups) * 16;
+  int64_t m0 = (int64_t)tile * 16 * MT, m1 = p.M;
   if constexpr (GROUPED) {
     int e, first, end;
-    if (!expert_tile(p.offs, p.E, (int)p.M, 16, (int)tile, e, first, end)) return;
+    if (!expert_tile(p.offs, p.E, (int)p.M, 16 * MT, tile, e, first, end)) return;
     m0 = first;
     m1 = end;
-    p.w = (const uint8_t*)p.w_ptrs[e];
-    p.sw = (const uint8_t*)p.ws_ptrs[e];
-    p.bias = p.b_ptrs ? (const float*)p.b_ptrs[e] : nullptr;
+    p.w = (const uint8_t*)wave_uniform64(p.w_ptrs[e]);
+    p.sw = (const uint8_t*)wave_uniform64(p.ws_ptrs[e]);
+    p.bias = p.b_ptrs ? (const float*)wave_uniform64(p.b_ptrs[e]) : nullptr;
   }
-  const int rows_a = m1 - m0 < 16 ? (int)(m1 - m0) : 16, rows_w = p.N - n0 < 16 ? (int)(p.N - n0) : 16;
-  const int nb = p.K / 32;
-  const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.a + m0 * p.lda, (rows_a - 1) * p.lda + p.K / 2);
-  const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w + n0 * p.ldw, (rows_w - 1) * p.ldw + p.K / 2);
-  const __amdgpu_buffer_rsrc_t rsa = make_rsrc(p.sa + m0 * p.ldsa, (rows_a - 1) * p.ldsa + nb);
-  const __amdgpu_buffer_rsrc_t rsw = make_rsrc(p.sw + n0 * p.ldsw, (rows_w - 1) * p.ldsw + nb);
-  const uint32_t oa = (uint32_t)(r * p.lda), ow = (uint32_t)(r * p.ldw);
-  const uint32_t osa = (uint32_t)(r * p.ldsa), osw = (uint32_t)(r * p.ldsw);
-  v4f acc = {0, 0, 0, 0};
-  for (int b0 = 0; b0 < nb; b0 += 4) {
-    const int b = b0 + q;
-    const bool oka = b < nb && r < rows_a, okw = b < nb && r < rows_w;
-    const v4i xa = buf_load16(ra, oka ? oa + 16 * b : kOob), xw = buf_load16(rw, okw ? ow + 16 * b : kOob);
-    const int sa = __builtin_amdgcn_raw_buffer_load_b8(rsa, oka ? (int)(osa + b) : (int)kOob, 0, 0);
-    const int sw = __builtin_amdgcn_raw_buffer_load_b8(rsw, okw ? (int)(osw + b) : (int)kOob, 0, 0);
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(xw), fp4_operand(xa), acc, 4, 4, 0, sw, 0, sa);
-  }
-  if (r >= rows_a) return;
+  const int rows_a = m1 - m0 < 16 * MT ? (int)(m1 - m0) : 16 * MT, rows_w = p.N - n0 < 16 ? (int)(p.N - n0) : 16;
+  const int nb = p.K / 32, nfull = nb / 16;
+  // (rows past the end repeat the last one: their results are not stored)
+  const uint8_t* wr = p.w + (int64_t)(n0 + min(r, rows_w - 1)) * p.ldw + 16 * q;
+  const uint8_t* swr = p.sw + (int64_t)(n0 + min(r, rows_w - 1)) * p.ldsw;
+  const uint8_t *ar[MT], *sar[MT];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int64_t n = n0 + 4 * q + t;
-    if (n < p.N) store_out(p.out, p.out_dtype, (m0 + r) * p.ldo + n, p.bias ? f32_add(acc[t], p.bias[n]) : acc[t]);
+  for (int m = 0; m < MT; ++m) {
+    const int64_t row = m0 + min(16 * m + r, rows_a - 1);
+    ar[m] = p.a + row * p.lda + 16 * q;
+    sar[m] = p.sa + row * p.ldsa;
+  }
+  using U = Fp4Unit<MT>;
+  auto load = [&](U& u, int k) {  // unit k < nfull
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      u.w[s] = __builtin_nontemporal_load((const v4i*)(wr + 256 * k + 64 * s));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) u.a[m][s] = *(const v4i*)(ar[m] + 256 * k + 64 * s);
+    }
+    __builtin_memcpy(&u.sw, swr + 16 * k, 16);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) __builtin_memcpy(&u.sa[m], sar[m] + 16 * k, 16);
+  };
+  v4f acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = v4f{0, 0, 0, 0};
+  auto multiply = [&](const U& u) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(u.w[s]), fp4_operand(u.a[m][s]), acc[m], 4, 4,
+                                                                  0, (int)(u.sw[s] >> (8 * q)), 0,
+                                                                  (int)(u.sa[m][s] >> (8 * q)));
+  };
+  // the blocks past the last whole unit, zeros (codes and scales) past the last block
+  U last;
+  if (nb > 16 * nfull) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int b = 16 * nfull + 4 * s + q;
+      last.w[s] = v4i{0, 0, 0, 0};
+      last.sw[s] = 0;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        last.a[m][s] = v4i{0, 0, 0, 0};
+        last.sa[m][s] = 0;
+      }
+      if (b < nb) {
+        last.w[s] = *(const v4i*)(wr + 256 * nfull + 64 * s);
+        last.sw[s] = (uint32_t)swr[b] << (8 * q);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          last.a[m][s] = *(const v4i*)(ar[m] + 256 * nfull + 64 * s);
+          last.sa[m][s] = (uint32_t)sar[m][b] << (8 * q);
+        }
+      }
+    }
+  }
+  if (nfull > 0) {
+    U u[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) load(u[i], min(i, nfull - 1));
+    int k = 0;
+    for (; k + 2 * P <= nfull; k += P)
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        multiply(u[i]);
+        load(u[i], k + P + i);
+      }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      if (k + i < nfull) multiply(u[i]);
+      if (k + P + i < nfull) load(u[i], k + P + i);
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (k + P + i < nfull) multiply(u[i]);
+  }
+  if (nb > 16 * nfull) multiply(last);
+  float b[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) b[t] = p.bias && n0 + 4 * q + t < p.N ? p.bias[n0 + 4 * q + t] : 0.0f;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    if (16 * m + r >= rows_a) continue;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int64_t n = n0 + 4 * q + t;
+      if (n < p.N) store_out(p.out, p.out_dtype, (m0 + 16 * m + r) * p.ldo + n, p.bias ? f32_add(acc[m][t], b[t]) : acc[m][t]);
+    }
   }
 }
 
@@ -436,19 +516,27 @@ static int fp4_tiles(Fp4Args p, const void* x, int x_dtype, int64_t ldx, uint8_t
   if (rc) return rc;
   const int64_t per = p.M / E;  // rows an expert, on average
   const auto tiles = [&](int64_t bm, int64_t bn) { return ((per + bm - 1) / bm) * E * ((p.N + bn - 1) / bn); };
-  if (tiles(256, 256) >= 256) return fp4_tile_launch<256, 256, 2, 4, 4, 64>(p, r.sat, r.swt, s);
-  if (tiles(128, 128) >= 192) return fp4_tile_launch<128, 128, 4, 2, 4, 128>(p, r.sat, r.swt, s);
+  if (per > 192 && tiles(256, 256) >= 256) return fp4_tile_launch<256, 256, 2, 4, 4, 64>(p, r.sat, r.swt, s);
+  if (per > 64 && tiles(128, 128) >= 192) return fp4_tile_launch<128, 128, 4, 2, 4, 128>(p, r.sat, r.swt, s);
   return fp4_tile_launch<64, 128, 2, 4, 5, 128>(p, r.sat, r.swt, s);
 }
 
-static int fp4_rows(const Fp4Args& p, hipStream_t s) {
-  const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16) : (p.M + 15) / 16;
+template <int MT, int P>
+static int fp4_rows_launch(const Fp4Args& p, hipStream_t s) {
+  const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
   const int64_t blocks = tiles * ((p.N + 15) / 16);
   LSK_REQUIRE(blocks <= 0x7fffffff, "mxfp4 product: grid too large");
   const dim3 grid((unsigned)blocks), blk(64);
-  if (p.offs) hipLaunchKernelGGL(fp4_rows_kernel<true>, grid, blk, 0, s, p);
-  else hipLaunchKernelGGL(fp4_rows_kernel<false>, grid, blk, 0, s, p);
+  if (p.offs) hipLaunchKernelGGL((fp4_rows_kernel<MT, P, true>), grid, blk, 0, s, p);
+  else hipLaunchKernelGGL((fp4_rows_kernel<MT, P, false>), grid, blk, 0, s, p);
   return check_launch("fp4_rows_kernel");
+}
+
+static int fp4_rows(const Fp4Args& p, hipStream_t s) {
+  const int64_t per = p.offs ? 2 * p.M / p.E : p.M;
+  if (per <= 16) return fp4_rows_launch<1, 4>(p, s);
+  if (per <= 32) return fp4_rows_launch<2, 4>(p, s);
+  return fp4_rows_launch<4, 2>(p, s);
 }
 
 static bool is_float_dtype(int d) { return d == LSK_F32 || d == LSK_BF16 || d == LSK_F16; }
