@@ -16,6 +16,8 @@
 #include "fp4_tile.h"
 #include "mfma_tile.h"
 
+#define LSK_HD __host__ __device__ inline
+
 namespace lsk {
 
 // ---------------------------------------------------------------- the quantiser
@@ -188,26 +190,86 @@ LSK_DEV bool expert_tile(const int32_t* __restrict__ offs, int E, int R, int bm,
   }
   return false;
 }
+// How many such tiles there are in all.
+LSK_DEV int expert_tile_count(const int32_t* __restrict__ offs, int E, int R, int bm) {
+  const int lane = threadIdx.x & 63;
+  int carry = min(max(offs[0], 0), R), total = 0;
+  for (int e0 = 0; e0 < E; e0 += 64) {
+    int hi = min(max(offs[min(e0 + lane + 1, E)], 0), R);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(hi, d, 64);
+      if (lane >= d) hi = max(hi, o);
+    }
+    hi = max(hi, carry);
+    int lo = __shfl_up(hi, 1, 64);
+    if (lane == 0) lo = carry;
+    total += wave_sum_i32((hi - lo + bm - 1) / bm);
+    carry = __builtin_amdgcn_readlane(hi, 63);
+  }
+  return total;
+}
 inline int64_t expert_tiles_max(int64_t R, int64_t E, int64_t bm) { return R / bm + (E < R ? E : R); }
 
-// Four steps of 128 values of a wave's rows: 16 weight rows, MT x 16 activation rows.
-template <int MT>
-struct Fp4Unit {
-  v4i w[4], a[MT][4];  // a lane's block of each step: row lane % 16, block lane / 16
-  v4u32 sw, sa[MT];    // its rows' scale dwords of the four steps
+// Few rows: a block computes NG x 16 output columns of up to MT x 16 rows over all of K, streaming its
+// weight rows from HBM.  Four waves bring the codes in, 512 values (256 bytes of a row, whole lines) a
+// stage, by direct global -> LDS loads RING - 1 stages ahead; the first NG of them multiply, a group of
+// 16 weight rows each, on 16x16x128 instructions (weight rows as their rows, activation rows as their
+// columns, so a lane ends with four consecutive outputs of a row).  Bound by HBM, that is by bytes in
+// flight: with a few thousand weight rows there is a block of 16 of them a CU, which is why waves that
+// do not multiply load.  K is not split over waves or blocks: a row's bits would depend on the split.
+// The scale bytes of the block's rows lie together in memory and are copied into LDS whole.
+// DT >= 0: the rows of x (at most four, whole rows 16-byte aligned) are quantised by every block into
+// LDS itself, which saves a launch and the wait for it; x comes from the L2.
+template <int NG, int MT, bool FUSE>
+struct Fp4StreamCfg {
+  static constexpr int kStageW = NG * 16 * 256, kStageA = FUSE ? 0 : MT * 16 * 256, kStage = kStageW + kStageA;
+  static constexpr int kPer = NG + (FUSE ? 0 : MT);              // loads per thread per stage
+  static constexpr int kMW = NG * MT > 4 ? NG * MT / 4 : 1;      // row tiles of a wave
+  static_assert(NG * MT <= 4 || NG == 4, "a wave's row tiles share its weight rows");
 };
 
-// Few rows: a wave computes 16 output columns of MT x 16 rows over all of K, streaming its 16 weight
-// rows from HBM into the instruction (weight rows as its rows, activation rows as its columns, so a
-// lane ends with four consecutive outputs of a row).  Bound by HBM, that is by bytes in flight: P units
-// of four steps are kept in flight in registers, each reissued as soon as it has been multiplied (P
-// KB-sized loads of four a wave).  The main loop has no branch around a load; a last partial unit is
-// loaded first, block by block.  K is not split over waves: a row's bits would depend on the split.
-template <int MT, int P, bool GROUPED>
-__global__ __launch_bounds__(64, 1) void fp4_rows_kernel(Fp4Args p) {
-  const int lane = threadIdx.x, r = lane & 15, q = lane >> 4;
-  const int ngroups = (int)((p.N + 15) / 16);
-  const int tile = blockIdx.x / ngroups, n0 = (blockIdx.x - tile * ngroups) * 16;
+// Bytes from one row of scales to the next in LDS: whole 16-byte pieces, an odd number of them, so that
+// 16 rows read at once lie in 16 bank groups.
+LSK_HD int scale_pitch(int nb) { return (nb + 15) / 16 * 16 | 16; }
+
+// `rows` rows of nb scale bytes (row stride ld, any alignment) into LDS at d, zeros past nb.
+LSK_DEV void copy_scales(const uint8_t* __restrict__ p, int64_t ld, int rows, int nb, char* d) {
+  const int pieces = (nb + 15) / 16, pitch = scale_pitch(nb);
+  for (int i = threadIdx.x; i < rows * pieces; i += 256) {
+    const int row = i / pieces, c = i - row * pieces;
+    const uint8_t* src = p + row * ld;
+    if (nb >= 16) {  // the last piece from the 16 bytes that end the row, shifted down
+      const int at = min(16 * c, nb - 16), sh = 8 * (16 * c - at);
+      uint64_t v[2];
+      __builtin_memcpy(v, src + at, 16);
+      if (sh >= 64) v[0] = v[1] >> (sh - 64), v[1] = 0;
+      else if (sh > 0) v[0] = v[0] >> sh | v[1] << (64 - sh), v[1] >>= sh;
+      *(ulonglong2*)(d + row * pitch + 16 * c) = make_ulonglong2(v[0], v[1]);
+      continue;
+    }
+    v4u32 v = {0, 0, 0, 0};
+    for (int z = 0; z < nb; ++z) v[z >> 2] |= (uint32_t)src[z] << (8 * (z & 3));
+    *(v4u32*)(d + row * pitch + 16 * c) = v;
+  }
+}
+
+// Bytes of LDS of such a block: the ring, the rows' codes (FUSE: `rows` of them) and the scales.
+LSK_HD int fused_pitch(int K) { return (K + 511) / 512 * 256 + 16; }
+template <int NG, int MT, int RING, bool FUSE>
+static int64_t fp4_stream_lds(int K, int rows) {
+  return RING * Fp4StreamCfg<NG, MT, FUSE>::kStage + (FUSE ? (int64_t)rows * fused_pitch(K) : 0) +
+         (int64_t)(NG * 16 + (FUSE ? rows : MT * 16)) * scale_pitch(K / 32);
+}
+
+template <int NG, int MT, int RING, int DT, bool GROUPED>
+__global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* __restrict__ x, int64_t ldx) {
+  constexpr bool FUSE = DT >= 0;
+  using C = Fp4StreamCfg<NG, MT, FUSE>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), r = lane & 15, q = lane >> 4;
+  const int ngroups = (int)((p.N + 16 * NG - 1) / (16 * NG));
+  const int tile = blockIdx.x / ngroups, n0 = (blockIdx.x - tile * ngroups) * 16 * NG;
   int64_t m0 = (int64_t)tile * 16 * MT, m1 = p.M;
   if constexpr (GROUPED) {
     int e, first, end;
@@ -218,97 +280,115 @@ __global__ __launch_bounds__(64, 1) void fp4_rows_kernel(Fp4Args p) {
     p.sw = (const uint8_t*)wave_uniform64(p.ws_ptrs[e]);
     p.bias = p.b_ptrs ? (const float*)wave_uniform64(p.b_ptrs[e]) : nullptr;
   }
-  const int rows_a = m1 - m0 < 16 * MT ? (int)(m1 - m0) : 16 * MT, rows_w = p.N - n0 < 16 ? (int)(p.N - n0) : 16;
-  const int nb = p.K / 32, nfull = nb / 16;
-  // (rows past the end repeat the last one: their results are not stored)
-  const uint8_t* wr = p.w + (int64_t)(n0 + min(r, rows_w - 1)) * p.ldw + 16 * q;
-  const uint8_t* swr = p.sw + (int64_t)(n0 + min(r, rows_w - 1)) * p.ldsw;
-  const uint8_t *ar[MT], *sar[MT];
+  const int rows_a = m1 - m0 < 16 * MT ? (int)(m1 - m0) : 16 * MT;
+  const int rows_w = p.N - n0 < 16 * NG ? (int)p.N - n0 : 16 * NG;
+  const int nb = p.K / 32, Kb = p.K / 2, nk = (p.K + 511) / 512;
+  const int sp = scale_pitch(nb), fp = fused_pitch(p.K);
+  char* const fused = smem + RING * C::kStage;  // FUSE: the rows' codes
+  char* const scw = fused + (FUSE ? rows_a * fp : 0);
+  char* const sca = scw + NG * 16 * sp;
+
+  // scales first: their registers are then waited for without waiting for the stages
+  copy_scales(p.sw + n0 * p.ldsw, p.ldsw, rows_w, nb, scw);
+  if constexpr (!FUSE) copy_scales(p.sa + m0 * p.ldsa, p.ldsa, rows_a, nb, sca);
+
+  const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w + (int64_t)n0 * p.ldw, (int64_t)(rows_w - 1) * p.ldw + Kb);
+  const __amdgpu_buffer_rsrc_t ra = FUSE ? rw : make_rsrc(p.a + m0 * p.lda, (int64_t)(rows_a - 1) * p.lda + Kb);
+  // a thread's 16-byte slot j of a stage: row 16 j + tid / 16, chunk c of its 256 bytes in place c ^ row % 16
+  const int row = tid >> 4, kc = 16 * ((tid & 15) ^ row);
+  auto issue = [&](int s) {
+    char* base = smem + (s % RING) * C::kStage;
+    const int k = 256 * s + kc;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int64_t row = m0 + min(16 * m + r, rows_a - 1);
-    ar[m] = p.a + row * p.lda + 16 * q;
-    sar[m] = p.sa + row * p.ldsa;
-  }
-  using U = Fp4Unit<MT>;
-  auto load = [&](U& u, int k) {  // unit k < nfull
+    for (int j = 0; j < NG; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_void_t)(base + j * 4096 + wave * 1024), 16,
+                                               k < Kb && 16 * j + row < rows_w ? (uint32_t)((16 * j + row) * p.ldw + k) : kOob,
+                                               0, 0, 0);
+    if constexpr (!FUSE) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      u.w[s] = __builtin_nontemporal_load((const v4i*)(wr + 256 * k + 64 * s));
-#pragma unroll
-      for (int m = 0; m < MT; ++m) u.a[m][s] = *(const v4i*)(ar[m] + 256 * k + 64 * s);
+      for (int j = 0; j < MT; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            ra, (lds_void_t)(base + C::kStageW + j * 4096 + wave * 1024), 16,
+            k < Kb && 16 * j + row < rows_a ? (uint32_t)((16 * j + row) * p.lda + k) : kOob, 0, 0, 0);
     }
-    __builtin_memcpy(&u.sw, swr + 16 * k, 16);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) __builtin_memcpy(&u.sa[m], sar[m] + 16 * k, 16);
   };
-  v4f acc[MT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m] = v4f{0, 0, 0, 0};
-  auto multiply = [&](const U& u) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(u.w[s]), fp4_operand(u.a[m][s]), acc[m], 4, 4,
-                                                                  0, (int)(u.sw[s] >> (8 * q)), 0,
-                                                                  (int)(u.sa[m][s] >> (8 * q)));
-  };
-  // the blocks past the last whole unit, zeros (codes and scales) past the last block
-  U last;
-  if (nb > 16 * nfull) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int b = 16 * nfull + 4 * s + q;
-      last.w[s] = v4i{0, 0, 0, 0};
-      last.sw[s] = 0;
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        last.a[m][s] = v4i{0, 0, 0, 0};
-        last.sa[m][s] = 0;
+  for (int s = 0; s < RING - 1; ++s) issue(s);
+  if constexpr (FUSE) {
+    // (codes past K stay as they were: the weights beside them are zeros; scales past K are written 0)
+    const int K8 = p.K / 8;
+    for (int m = 0; m < rows_a; ++m)
+      for (int c = tid; c < K8; c += 256) {
+        float v[8];
+        load8<DT, true>(x, (m0 + m) * ldx + 8 * c, v);
+        uint32_t sc;
+        *(uint32_t*)(fused + m * fp + 4 * c) = quantize8_mxfp4(v, sc);
+        if ((c & 3) == 0) sca[m * sp + (c >> 2)] = (char)sc;
       }
-      if (b < nb) {
-        last.w[s] = *(const v4i*)(wr + 256 * nfull + 64 * s);
-        last.sw[s] = (uint32_t)swr[b] << (8 * q);
+    for (int i = tid; i < rows_a * 16; i += 256)
+      if (nb + (i & 15) < (nb + 15) / 16 * 16) sca[(i >> 4) * sp + nb + (i & 15)] = 0;
+  }
+
+  // wave w multiplies weight group w % NG with row tiles w / NG (and, NG * MT > 4, the next ones)
+  constexpr int MW = C::kMW;
+  const int g = wave % NG, mt = wave / NG * MW;
+  const bool multiplies = NG * MT >= 4 || wave < NG * MT;
+  v4f acc[MW];
+  const char *ars[MW], *arc[MW];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          last.a[m][s] = *(const v4i*)(ar[m] + 256 * nfull + 64 * s);
-          last.sa[m][s] = (uint32_t)sar[m][b] << (8 * q);
-        }
+  for (int m = 0; m < MW; ++m) {
+    acc[m] = v4f{0, 0, 0, 0};
+    // (rows past the end: whatever lies there, their results are not stored)
+    const int ar = FUSE ? min(r, rows_a - 1) : 16 * (mt + m) + r;
+    ars[m] = sca + ar * sp;
+    arc[m] = FUSE ? fused + ar * fp : smem + C::kStageW + ar * 256;
+  }
+  const char* wrs = scw + (16 * g + r) * sp;
+  for (int kt = 0; kt < nk; ++kt) {
+    wait_vm<(RING - 2) * C::kPer>();
+    wait_lgkm0();
+    phase_barrier();
+    issue(kt + RING - 1);
+    if (multiplies) {
+      const int slot = (kt % RING) * C::kStage;
+      const char* base = smem + slot + (16 * g + r) * 256;
+      const v4u32 sw = *(const v4u32*)(wrs + 16 * kt);
+      v4u32 sa[MW];
+      v4i w[4], a[MW][4];
+#pragma unroll
+      for (int m = 0; m < MW; ++m) sa[m] = *(const v4u32*)(ars[m] + 16 * kt);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int c = 16 * ((4 * s + q) ^ r);
+        w[s] = *(const v4i*)(base + c);
+#pragma unroll
+        for (int m = 0; m < MW; ++m)
+          a[m][s] = FUSE ? *(const v4i*)(arc[m] + 256 * kt + 64 * s + 16 * q) : *(const v4i*)(arc[m] + slot + c);
       }
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int m = 0; m < MW; ++m)
+          acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(w[s]), fp4_operand(a[m][s]), acc[m], 4, 4, 0,
+                                                                    (int)(sw[s] >> (8 * q)), 0, (int)(sa[m][s] >> (8 * q)));
     }
   }
-  if (nfull > 0) {
-    U u[P];
-#pragma unroll
-    for (int i = 0; i < P; ++i) load(u[i], min(i, nfull - 1));
-    int k = 0;
-    for (; k + 2 * P <= nfull; k += P)
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        multiply(u[i]);
-        load(u[i], k + P + i);
-      }
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      if (k + i < nfull) multiply(u[i]);
-      if (k + P + i < nfull) load(u[i], k + P + i);
-    }
-#pragma unroll
-    for (int i = 0; i < P; ++i)
-      if (k + P + i < nfull) multiply(u[i]);
-  }
-  if (nb > 16 * nfull) multiply(last);
+  wait_vm<0>();
+  if (!multiplies) return;
   float b[4];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) b[t] = p.bias && n0 + 4 * q + t < p.N ? p.bias[n0 + 4 * q + t] : 0.0f;
+  for (int t = 0; t < 4; ++t) {
+    const int64_t n = n0 + 16 * g + 4 * q + t;
+    b[t] = p.bias && n < p.N ? p.bias[n] : 0.0f;
+  }
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    if (16 * m + r >= rows_a) continue;
+  for (int m = 0; m < MW; ++m) {
+    const int row_out = 16 * (mt + m) + r;
+    if (row_out >= rows_a) continue;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int64_t n = n0 + 4 * q + t;
-      if (n < p.N) store_out(p.out, p.out_dtype, (m0 + 16 * m + r) * p.ldo + n, p.bias ? f32_add(acc[m][t], b[t]) : acc[m][t]);
+      const int64_t n = n0 + 16 * g + 4 * q + t;
+      if (n < p.N) store_out(p.out, p.out_dtype, (m0 + row_out) * p.ldo + n, p.bias ? f32_add(acc[m][t], b[t]) : acc[m][t]);
     }
   }
 }
@@ -317,18 +397,28 @@ __global__ __launch_bounds__(64, 1) void fp4_rows_kernel(Fp4Args p) {
 // Scales [rows, nb] bytes (row stride lds) to the transposed form, 8 dwords of a row a thread.
 LSK_DEV void transpose_scales(const uint8_t* __restrict__ s, int64_t lds, int64_t rows, int nb, int64_t block,
                               uint32_t* __restrict__ t) {
-  const int nst = (nb + 3) / 4;
   const int64_t rblocks = (rows + 255) / 256;
   const int64_t c = block / rblocks, r = (block - c * rblocks) * 256 + threadIdx.x;
   if (r >= rows) return;
-  const uint8_t* p = s + r * lds;
-  for (int d = (int)c * 8; d < (int)c * 8 + 8 && d < nst; ++d) {
-    uint32_t w = 0;
-    if (4 * d + 4 <= nb) __builtin_memcpy(&w, p + 4 * d, 4);
-    else
-      for (int z = 0; 4 * d + z < nb; ++z) w |= (uint32_t)p[4 * d + z] << (8 * z);
-    t[d * rows + r] = w;
+  const uint8_t* p = s + r * lds + 32 * c;
+  uint32_t* o = t + 8 * c * rows + r;
+  const int left = nb - 32 * (int)c;
+  uint32_t w[8];
+  if (left >= 32) {
+    __builtin_memcpy(w, p, 32);
+  } else {  // a row's last blocks, zeros past them
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      w[d] = 0;
+      if (4 * d + 4 <= left) __builtin_memcpy(&w[d], p + 4 * d, 4);
+      else
+        for (int z = 0; z < 3; ++z)
+          if (4 * d + z < left) w[d] |= (uint32_t)p[4 * d + z] << (8 * z);
+    }
   }
+#pragma unroll
+  for (int d = 0; d < 8; ++d)
+    if (4 * d < left) o[d * rows] = w[d];
 }
 inline int64_t transpose_blocks(int64_t rows, int64_t K) { return ((rows + 255) / 256) * ((K / 32 + 31) / 32); }
 
@@ -366,12 +456,16 @@ __global__ __launch_bounds__(256) void fp4_prep_kernel(Fp4Prep p) {
 // A BM x BN tile: tiles walk kGroupM row tiles down a column of weight tiles inside each XCD's run
 // of them, so the row tiles that share a weight tile run together on one L2.
 template <int BM, int BN, int WM, int WN, int RING, int BKB, bool GROUPED>
-__global__ __launch_bounds__(512) void fp4_tile_kernel(Fp4Args p, const uint32_t* __restrict__ sat,
+__global__ __launch_bounds__(WM * WN * 64) void fp4_tile_kernel(Fp4Args p, const uint32_t* __restrict__ sat,
                                                        const uint32_t* __restrict__ swt, int64_t mtiles, int vec) {
   using C = Fp4Cfg<BM, BN, WM, WN, RING, BKB>;
   constexpr int kGroupM = 4;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int ntiles = (int)((p.N + BN - 1) / BN);
+  if constexpr (GROUPED) {  // (the grid holds the most tiles there can be: the ones there are go to every XCD)
+    mtiles = expert_tile_count(p.offs, p.E, (int)p.M, BM);
+    if (blockIdx.x >= mtiles * ntiles) return;
+  }
   const int L = xcd_logical_id(blockIdx.x, (int)mtiles * ntiles);
   const int first = L / (kGroupM * ntiles) * kGroupM;
   const int gsize = (int)mtiles - first < kGroupM ? (int)mtiles - first : kGroupM;
@@ -474,11 +568,18 @@ static int fp4_tile_launch(const Fp4Args& p, const uint32_t* sat, const uint32_t
                 : run(fp4_tile_kernel<BM, BN, WM, WN, RING, BKB, false>);
 }
 
-// Whether the products of M rows (R over E experts) run on the tiles, which need the operands' offsets
-// inside 31 bits.
+// Whether the products of M rows (of E experts: E > 0) run on the tiles: past 64 rows (16 an expert), and
+// where a block's scales of all of K do not fit the LDS.  (MI355X, us on the streaming blocks and on
+// the tiles: 48 rows of 4608 x 3584 11.8, 12.4; 64 of 4096 x 14336 16.6, 25.3; by expert, 16 rows each of
+// 5760 x 2880 78, 88, 32 rows 102, 93.)
+constexpr int64_t kStreamK = 32768;
 static bool fp4_takes_tiles(int64_t M, int64_t N, int64_t K, int64_t E) {
+  return K > kStreamK || (K > 0 && (E ? M > 16 * E : M > 64));
+}
+// The tiles address a tile's rows and the transposed scales with 31-bit offsets.
+static bool fp4_tiles_reach(int64_t M, int64_t N, int64_t K) {
   const int64_t nst = (K + 127) / 128;
-  return K > 0 && M > 64 * E && 4 * nst * M < 0x7fffffff && 4 * nst * N < 0x7fffffff && 256 * (K / 2) < 0x7fffffff;
+  return 4 * nst * M < 0x7fffffff && 4 * nst * N < 0x7fffffff && 256 * (K / 2) < 0x7fffffff;
 }
 
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -492,6 +593,8 @@ static int64_t fp4_prep_bytes(int64_t M, int64_t N, int64_t K, int64_t E) {
 // The tiles' products: p.a / p.sa the rows (x null), or x to be quantised into q first.
 static int fp4_tiles(Fp4Args p, const void* x, int x_dtype, int64_t ldx, uint8_t* q, char* work, hipStream_t s) {
   const int64_t nst = (p.K + 127) / 128, E = p.offs ? p.E : 1;
+  LSK_REQUIRE(fp4_tiles_reach(p.M, p.N, p.K), "mxfp4 product: M=%lld N=%lld K=%d beyond 31-bit offsets", (long long)p.M,
+              (long long)p.N, p.K);
   Fp4Prep r{};
   r.M = p.M, r.K = p.K;
   r.sat = (uint32_t*)work, r.swt = (uint32_t*)(work + up256(4 * nst * p.M));
@@ -514,29 +617,71 @@ static int fp4_tiles(Fp4Args p, const void* x, int x_dtype, int64_t ldx, uint8_t
     hipLaunchKernelGGL((fp4_prep_kernel<-1, false>), grid, blk, 0, s, r);
   const int rc = check_launch("fp4_prep_kernel");
   if (rc) return rc;
-  const int64_t per = p.M / E;  // rows an expert, on average
+  // The tile by how many there are: 256 x 256 where they fill the part; 128 x 128, then 64 x 128 where
+  // there are enough for two blocks a CU, else 64 x 64; experts of many rows 128 x 256.  (MI355X, us:
+  // 4096 rows of 28672 x 4096 328 on 256 x 256, 371 on 128 x 128; 2048 of 4096 x 14336 110, 95; 777 of 4608 x
+  // 3584 24.7 on 128 x 128, 21.2 on 64 x 128, 26.2 on 64 x 64; 200 of 3584 x 18944 49 on 64 x 128, 37 on
+  // 64 x 64; 16384 rows over 128 experts of 1536 x 2048 96 on 128 x 256, 108 on 128 x 128, 104 on 64 x 128.)
+  const int64_t per = p.M / E;
   const auto tiles = [&](int64_t bm, int64_t bn) { return ((per + bm - 1) / bm) * E * ((p.N + bn - 1) / bn); };
-  if (per > 192 && tiles(256, 256) >= 256) return fp4_tile_launch<256, 256, 2, 4, 4, 64>(p, r.sat, r.swt, s);
-  if (per > 64 && tiles(128, 128) >= 192) return fp4_tile_launch<128, 128, 4, 2, 4, 128>(p, r.sat, r.swt, s);
-  return fp4_tile_launch<64, 128, 2, 4, 5, 128>(p, r.sat, r.swt, s);
+  if (!p.offs && tiles(256, 256) >= 200) return fp4_tile_launch<256, 256, 2, 4, 4, 64>(p, r.sat, r.swt, s);
+  if (p.offs && per >= 64 && tiles(128, 256) >= 200) return fp4_tile_launch<128, 256, 2, 4, 3, 64>(p, r.sat, r.swt, s);
+  if (!p.offs && tiles(128, 128) >= 448) return fp4_tile_launch<128, 128, 2, 2, 2, 128>(p, r.sat, r.swt, s);
+  if (tiles(64, 128) >= 384) return fp4_tile_launch<64, 128, 2, 2, 2, 128>(p, r.sat, r.swt, s);
+  return fp4_tile_launch<64, 64, 2, 2, 4, 128>(p, r.sat, r.swt, s);
 }
 
-template <int MT, int P>
-static int fp4_rows_launch(const Fp4Args& p, hipStream_t s) {
+template <int NG, int MT, int RING, int DT>
+static int fp4_stream_launch(const Fp4Args& p, const void* x, int64_t ldx, hipStream_t s) {
   const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
-  const int64_t blocks = tiles * ((p.N + 15) / 16);
+  const int64_t blocks = tiles * ((p.N + 16 * NG - 1) / (16 * NG));
   LSK_REQUIRE(blocks <= 0x7fffffff, "mxfp4 product: grid too large");
-  const dim3 grid((unsigned)blocks), blk(64);
-  if (p.offs) hipLaunchKernelGGL((fp4_rows_kernel<MT, P, true>), grid, blk, 0, s, p);
-  else hipLaunchKernelGGL((fp4_rows_kernel<MT, P, false>), grid, blk, 0, s, p);
-  return check_launch("fp4_rows_kernel");
+  const int64_t lds = fp4_stream_lds<NG, MT, RING, (DT >= 0)>(p.K, (int)(p.M < 16 ? p.M : 16));
+  LSK_REQUIRE(lds <= 160 * 1024, "mxfp4 product: K=%d too long for few rows", p.K);
+  auto run = [&](auto kern) {
+    if (lds > 65536 &&
+        hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
+      return set_error("fp4_stream_kernel: cannot reserve LDS"), LSK_ERR_HIP;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), (size_t)lds, s, p, x, ldx);
+    return check_launch("fp4_stream_kernel");
+  };
+  if constexpr (DT < 0) {
+    if (p.offs) return run(fp4_stream_kernel<NG, MT, RING, DT, true>);
+  }
+  return run(fp4_stream_kernel<NG, MT, RING, DT, false>);
 }
 
-static int fp4_rows(const Fp4Args& p, hipStream_t s) {
+// The launch shape by the number of 16-row weight groups over all row tiles: one group a block while
+// there are few (deep rings: nothing else hides the latency), else blocks of four with the shortest
+// ring, several of which share a CU.  (MI355X, us for NG x RING = 1 x 4, 2 x 3, 4 x 2 at M rows of N x K:
+// 24 of 4096 x 14336 15.5, 16.3, 24.3; 48 of 4608 x 3584 12.9, 11.8, 12.3; 8 of 28672 x 4096 16.9, 17.1,
+// 14.4; by expert, 4 rows of 5760 x 2880 14.2, 9.8, 10.9; 256 rows over 32 experts of 2880 x 2880 51.3,
+// 42.0, 36.4.)
+template <int MT, int DT>
+static int fp4_stream_shape(const Fp4Args& p, const void* x, int64_t ldx, hipStream_t s) {
+  const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
+  const int64_t groups = tiles * ((p.N + 15) / 16);
+  if (groups <= 512) return fp4_stream_launch<1, MT, 4, DT>(p, x, ldx, s);
+  if (groups <= 1536) return fp4_stream_launch<2, MT, 3, DT>(p, x, ldx, s);
+  return fp4_stream_launch<4, MT, 2, DT>(p, x, ldx, s);
+}
+
+// Row tiles of 16 while that holds all rows (of an expert: twice the average, the skew of a routing).
+static int fp4_stream(const Fp4Args& p, hipStream_t s) {
   const int64_t per = p.offs ? 2 * p.M / p.E : p.M;
-  if (per <= 16) return fp4_rows_launch<1, 4>(p, s);
-  if (per <= 32) return fp4_rows_launch<2, 4>(p, s);
-  return fp4_rows_launch<4, 2>(p, s);
+  return per <= 16 ? fp4_stream_shape<1, -1>(p, nullptr, 0, s) : fp4_stream_shape<2, -1>(p, nullptr, 0, s);
+}
+
+// Whether a linear's few rows are quantised in the product's launch (one row of 4608 x 3584 13.3 -> 9.3
+// us on MI355X): whole 16-byte loads, codes and scales that fit the LDS.
+static bool fp4_fuses(const void* x, int x_dtype, int64_t ldx, int64_t M, int64_t K) {
+  return M <= 4 && K > 0 && K <= 24576 && (uintptr_t)x % 16 == 0 && (ldx * (x_dtype == LSK_F32 ? 4 : 2)) % 16 == 0;
+}
+
+static int fp4_stream_fused(const Fp4Args& p, const void* x, int x_dtype, int64_t ldx, hipStream_t s) {
+  if (x_dtype == LSK_F32) return fp4_stream_shape<1, LSK_F32>(p, x, ldx, s);
+  if (x_dtype == LSK_BF16) return fp4_stream_shape<1, LSK_BF16>(p, x, ldx, s);
+  return fp4_stream_shape<1, LSK_F16>(p, x, ldx, s);
 }
 
 static bool is_float_dtype(int d) { return d == LSK_F32 || d == LSK_BF16 || d == LSK_F16; }
@@ -563,14 +708,14 @@ extern "C" int lsk_quantize_mxfp4(const void* x, int x_dtype, int64_t M, int64_t
 static int mxfp4_check(const char* who, int64_t M, int64_t N, int64_t K, int out_dtype, int64_t ldo) {
   LSK_REQUIRE(M >= 0 && N >= 0 && K >= 0 && K % 32 == 0, "%s: bad sizes M=%lld N=%lld K=%lld (K a multiple of 32)", who,
               (long long)M, (long long)N, (long long)K);
-  LSK_REQUIRE(M <= 0x7fffffff && N <= 0x7fffffff && K <= (1 << 25), "%s: sizes beyond 31 bits (K beyond 2^25)", who);
+  LSK_REQUIRE(M <= 0x7fffffff && N <= 0x7fffffff && K < (1 << 24), "%s: sizes beyond 31 bits (K beyond 2^24)", who);
   LSK_REQUIRE(lsk::is_float_dtype(out_dtype), "%s: out_dtype must be f32, bf16 or f16", who);
   LSK_REQUIRE(ldo >= N, "%s: ldo below N", who);
   return LSK_OK;
 }
 
 extern "C" int64_t lsk_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
-  return lsk::fp4_takes_tiles(M, N, K, 1) ? lsk::fp4_prep_bytes(M, N, K, 1) : 0;
+  return lsk::fp4_takes_tiles(M, N, K, 0) ? lsk::fp4_prep_bytes(M, N, K, 1) : 0;
 }
 
 #define LSK_REQUIRE_WORK(who, need)                                                                                  \
@@ -591,14 +736,14 @@ extern "C" int lsk_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, int64_t 
   p.lda = p.ldw = K / 2, p.ldsa = p.ldsw = K / 32;
   p.M = M, p.N = N, p.K = (int)K;
   p.bias = bias, p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
-  if (lsk::fp4_takes_tiles(M, N, K, 1)) return lsk::fp4_tiles(p, nullptr, 0, 0, nullptr, (char*)workspace, (hipStream_t)stream);
-  return lsk::fp4_rows(p, (hipStream_t)stream);
+  if (lsk::fp4_takes_tiles(M, N, K, 0)) return lsk::fp4_tiles(p, nullptr, 0, 0, nullptr, (char*)workspace, (hipStream_t)stream);
+  return lsk::fp4_stream(p, (hipStream_t)stream);
 }
 
 // The quantised rows come first in the workspace, then their scales (the row kernels) or the tiles' part.
 extern "C" int64_t lsk_linear_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
   return lsk::up256(M * (K / 2)) +
-         (lsk::fp4_takes_tiles(M, N, K, 1) ? lsk::fp4_prep_bytes(M, N, K, 1) : lsk::up256(M * (K / 32)));
+         (lsk::fp4_takes_tiles(M, N, K, 0) ? lsk::fp4_prep_bytes(M, N, K, 1) : lsk::up256(M * (K / 32)));
 }
 
 extern "C" int lsk_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int64_t M, int64_t K, const uint8_t* w,
@@ -620,9 +765,10 @@ extern "C" int lsk_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int64_t
   p.lda = p.ldw = K / 2, p.ldsa = p.ldsw = K / 32;
   p.M = M, p.N = N, p.K = (int)K;
   p.bias = bias, p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
-  if (lsk::fp4_takes_tiles(M, N, K, 1)) return lsk::fp4_tiles(p, x, x_dtype, ldx, q, (char*)rest, s);
+  if (lsk::fp4_takes_tiles(M, N, K, 0)) return lsk::fp4_tiles(p, x, x_dtype, ldx, q, (char*)rest, s);
+  if (lsk::fp4_fuses(x, x_dtype, ldx, M, K)) return lsk::fp4_stream_fused(p, x, x_dtype, ldx, s);
   if (K > 0 && (rc = lsk::quantize_launch(x, x_dtype, M, K, ldx, q, rest, s))) return rc;
-  return lsk::fp4_rows(p, s);
+  return lsk::fp4_stream(p, s);
 }
 
 extern "C" int64_t lsk_grouped_gemm_mxfp4_workspace(int64_t R, int64_t E, int64_t N, int64_t K) {
@@ -640,7 +786,7 @@ extern "C" int lsk_grouped_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, 
   LSK_REQUIRE(out && offs && w_ptrs && ws_ptrs && (K == 0 || (a && a_scale)), "lsk_grouped_gemm_mxfp4: null pointer");
   LSK_REQUIRE((uintptr_t)a % 16 == 0 && ldw >= K / 2 && ldw % 16 == 0 && lds >= K / 32,
               "lsk_grouped_gemm_mxfp4: codes in rows of 16-byte multiples, strides that cover K");
-  LSK_REQUIRE(ldw <= (1 << 26) && lds <= (1 << 26), "lsk_grouped_gemm_mxfp4: row strides beyond 2^26 bytes");
+  LSK_REQUIRE(ldw < (1 << 23) && lds < (1 << 23), "lsk_grouped_gemm_mxfp4: row strides beyond 2^23 bytes");
   LSK_REQUIRE_WORK("lsk_grouped_gemm_mxfp4", lsk_grouped_gemm_mxfp4_workspace(R, E, N, K));
   lsk::Fp4Args p{};
   p.a = a, p.sa = a_scale;
@@ -649,5 +795,5 @@ extern "C" int lsk_grouped_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, 
   p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
   p.offs = offs, p.E = (int)E, p.w_ptrs = w_ptrs, p.ws_ptrs = ws_ptrs, p.b_ptrs = b_ptrs;
   if (lsk::fp4_takes_tiles(R, N, K, E)) return lsk::fp4_tiles(p, nullptr, 0, 0, nullptr, (char*)workspace, (hipStream_t)stream);
-  return lsk::fp4_rows(p, (hipStream_t)stream);
+  return lsk::fp4_stream(p, (hipStream_t)stream);
 }

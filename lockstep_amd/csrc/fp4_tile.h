@@ -1,7 +1,7 @@
-// Eight-wave ping-pong main loop of the MXFP4 products on gfx950's block-scaled matrix core.
+// Main loops of the MXFP4 products' tiles on gfx950's block-scaled matrix core.
 //
-// A block of 512 threads computes a BM x BN tile of A * W^T over all of K, as pp_tile.h does for
-// int8: two groups of four waves half a period apart, one reading its operands from LDS while the
+// A block computes a BM x BN tile of A * W^T over all of K.  With eight waves it does so as pp_tile.h
+// does for int8: two groups of four waves half a period apart, one reading its operands from LDS while the
 // other multiplies, K staged 128 (or 256) values at a time through a ring of LDS stages that direct
 // global -> LDS loads fill RING - 1 stages ahead.  A 128-value stage of a row is 64 bytes of codes and
 // one dword of four scale bytes.
@@ -30,21 +30,21 @@ LSK_DEV v8i fp4_operand(v4i x) { return v8i{x[0], x[1], x[2], x[3], 0, 0, 0, 0};
 
 template <int BM, int BN, int WM, int WN, int RING, int BKB>
 struct Fp4Cfg {
-  static_assert(WM * WN == 8, "eight waves");
-  static_assert(RING >= 3 && RING <= 5, "ring of 3..5 stages");
+  static_assert(WM * WN == 8 || WM * WN == 4, "eight waves (ping-pong) or four");
+  static_assert(RING >= (WM * WN == 8 ? 3 : 2), "ring of stages");
   static_assert(BKB == 64 || BKB == 128, "stages of 128 or 256 values");
-  static_assert(BM + BN <= 512, "one scale dword per thread and 128 values");
-  static constexpr int kThreads = 512, kBM = BM, kBN = BN, kWM = WM, kWN = WN;
+  static constexpr int kThreads = WM * WN * 64, kBM = BM, kBN = BN, kWM = WM, kWN = WN;
+  static_assert(BM + BN <= kThreads, "one scale dword per thread and 128 values");
   static constexpr int kRing = RING, kAhead = RING - 1;
   static constexpr int kChunks = BKB / 16, kSub = BKB / 64;  // 16-byte chunks and 128-value parts of a stage
   static constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 32, TN = WTN / 32;
-  static constexpr int kStageA = BM * BKB, kStageB = BN * BKB, kScale = 512 * 4 * kSub;
+  static constexpr int kStageA = BM * BKB, kStageB = BN * BKB, kScale = kThreads * 4 * kSub;
   static constexpr int kStage = kStageA + kStageB + kScale;
   static constexpr int kLA = kStageA / 16 / kThreads, kLB = kStageB / 16 / kThreads;
   static constexpr int kPer = kLA + kLB + kSub;  // loads per thread per stage
   static constexpr int kMainBytes = kRing * kStage;
   static constexpr int kLdc = WTN + 4;           // floats a row of a staged 32-row strip
-  static constexpr int kEpiBytes = 8 * 32 * kLdc * 4;
+  static constexpr int kEpiBytes = WM * WN * 32 * kLdc * 4;
   static constexpr int kSmemBytes = kMainBytes > kEpiBytes ? kMainBytes : kEpiBytes;
   static_assert(kStageA % (16 * kThreads) == 0 && kStageB % (16 * kThreads) == 0, "tile / threads");
   static_assert(WTM % 32 == 0 && WTN % 32 == 0, "wave tile must be a multiple of 32");
@@ -103,7 +103,7 @@ LSK_DEV void fp4_mainloop(typename Fp4Cfg<BM, BN, WM, WN, RING, BKB>::Acc& acc, 
 #pragma unroll
     for (int u = 0; u < C::kSub; ++u)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rs, (lds_void_t)(base + C::kStageA + C::kStageB + (u * 512 + wave * 64) * 4), 4,
+          rs, (lds_void_t)(base + C::kStageA + C::kStageB + (u * C::kThreads + wave * 64) * 4), 4,
           (!kCheck || s * C::kSub + u < nst) ? t.s : kOob, (int)((uint32_t)(s * C::kSub + u) * st), 0, 0);
   };
 
@@ -115,6 +115,51 @@ LSK_DEV void fp4_mainloop(typename Fp4Cfg<BM, BN, WM, WN, RING, BKB>::Acc& acc, 
 #pragma unroll
   for (int ks = 0; ks < 2 * C::kSub; ++ks) slot[ks] = 16 * ((2 * ks + kg) ^ sw);
 
+  if constexpr (C::kThreads == 256) {
+    // Four waves, one barrier a stage: a wave's own loads of stage kt are complete when at most the RING
+    // - 2 younger stages are outstanding, every wave's at the barrier; the slot of stage kt - 1, which
+    // no wave reads any more, takes stage kt + RING - 1.  Past the last stage the loads read zeros, so
+    // the count of outstanding loads is the same to the end.
+#pragma unroll
+    for (int s = 0; s < RING - 1; ++s) issue(s, std::true_type{});
+    for (int kt = 0; kt < nk; ++kt) {
+      wait_vm<(RING - 2) * C::kPer>();
+      phase_barrier();
+      issue(kt + RING - 1, std::true_type{});
+      const char* base = smem + (kt % RING) * C::kStage;
+#pragma unroll
+      for (int u = 0; u < C::kSub; ++u) {
+        int xa[C::TM], xb[C::TN];
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+          xa[i] = (int)(*(const uint32_t*)(base + sA + u * 4 * C::kThreads + i * 128) >> (8 * kg));
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+          xb[j] = (int)(*(const uint32_t*)(base + sB + u * 4 * C::kThreads + j * 128) >> (8 * kg));
+        v4i fa[2][C::TM], fb[2][C::TN];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int i = 0; i < C::TM; ++i) fa[h][i] = *(const v4i*)(base + offA + i * 32 * BKB + slot[2 * u + h]);
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j) fb[h][j] = *(const v4i*)(base + offB + j * 32 * BKB + slot[2 * u + h]);
+        }
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(fb[0][j]), fp4_operand(fa[0][i]),
+                                                                        acc[i][j], 4, 4, 0, xb[j], 0, xa[i]);
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(fb[1][j]), fp4_operand(fa[1][i]),
+                                                                        acc[i][j], 4, 4, 2, xb[j], 2, xa[i]);
+      }
+    }
+    wait_vm<0>();
+  } else {
   using Chk = std::true_type;
   using NoChk = std::false_type;
   using W0 = std::integral_constant<int, 0>;
@@ -127,9 +172,9 @@ LSK_DEV void fp4_mainloop(typename Fp4Cfg<BM, BN, WM, WN, RING, BKB>::Acc& acc, 
 #pragma unroll
     for (int u = 0; u < C::kSub; ++u) {
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) xa[u][i] = *(const int*)(base + sA + u * 2048 + i * 128);
+      for (int i = 0; i < C::TM; ++i) xa[u][i] = *(const int*)(base + sA + u * 4 * C::kThreads + i * 128);
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j) xb[u][j] = *(const int*)(base + sB + u * 2048 + j * 128);
+      for (int j = 0; j < C::TN; ++j) xb[u][j] = *(const int*)(base + sB + u * 4 * C::kThreads + j * 128);
     }
 #pragma unroll
     for (int ks = 0; ks < 2 * C::kSub; ++ks) {
@@ -186,6 +231,7 @@ LSK_DEV void fp4_mainloop(typename Fp4Cfg<BM, BN, WM, WN, RING, BKB>::Acc& acc, 
     for (int kt = 0; kt < nk; ++kt) step(kt, W0{}, false, NoChk{});
   }
   if (group == 0) phase_barrier();
+  }
 }
 
 }  // namespace lsk
