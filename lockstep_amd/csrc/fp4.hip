@@ -219,8 +219,8 @@ inline int64_t expert_tiles_max(int64_t R, int64_t E, int64_t bm) { return R / b
 // flight: with a few thousand weight rows there is a block of 16 of them a CU, which is why waves that
 // do not multiply load.  K is not split over waves or blocks: a row's bits would depend on the split.
 // The scale bytes of the block's rows lie together in memory and are copied into LDS whole.
-// DT >= 0: the rows of x (at most four, whole rows 16-byte aligned) are quantised by every block into
-// LDS itself, which saves a launch and the wait for it; x comes from the L2.
+// DT >= 0: the rows of x (at most four; vec: 16-byte aligned) are quantised by every block into LDS
+// itself, which saves a launch and the wait for it; x comes from the L2.
 template <int NG, int MT, bool FUSE>
 struct Fp4StreamCfg {
   static constexpr int kStageW = NG * 16 * 256, kStageA = FUSE ? 0 : MT * 16 * 256, kStage = kStageW + kStageA;
@@ -263,7 +263,8 @@ static int64_t fp4_stream_lds(int K, int rows) {
 }
 
 template <int NG, int MT, int RING, int DT, bool GROUPED>
-__global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* __restrict__ x, int64_t ldx) {
+__global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* __restrict__ x, int64_t ldx,
+                                                         int vec) {
   constexpr bool FUSE = DT >= 0;
   using C = Fp4StreamCfg<NG, MT, FUSE>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -320,7 +321,8 @@ __global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* 
     for (int m = 0; m < rows_a; ++m)
       for (int c = tid; c < K8; c += 256) {
         float v[8];
-        load8<DT, true>(x, (m0 + m) * ldx + 8 * c, v);
+        if (vec) load8<DT, true>(x, (m0 + m) * ldx + 8 * c, v);
+        else load8<DT, false>(x, (m0 + m) * ldx + 8 * c, v);
         uint32_t sc;
         *(uint32_t*)(fused + m * fp + 4 * c) = quantize8_mxfp4(v, sc);
         if ((c & 3) == 0) sca[m * sp + (c >> 2)] = (char)sc;
@@ -638,11 +640,12 @@ static int fp4_stream_launch(const Fp4Args& p, const void* x, int64_t ldx, hipSt
   LSK_REQUIRE(blocks <= 0x7fffffff, "mxfp4 product: grid too large");
   const int64_t lds = fp4_stream_lds<NG, MT, RING, (DT >= 0)>(p.K, (int)(p.M < 16 ? p.M : 16));
   LSK_REQUIRE(lds <= 160 * 1024, "mxfp4 product: K=%d too long for few rows", p.K);
+  const int vec = x && (uintptr_t)x % 16 == 0 && (ldx * (DT == LSK_F32 ? 4 : 2)) % 16 == 0;
   auto run = [&](auto kern) {
     if (lds > 65536 &&
         hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
       return set_error("fp4_stream_kernel: cannot reserve LDS"), LSK_ERR_HIP;
-    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), (size_t)lds, s, p, x, ldx);
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), (size_t)lds, s, p, x, ldx, vec);
     return check_launch("fp4_stream_kernel");
   };
   if constexpr (DT < 0) {
@@ -673,10 +676,8 @@ static int fp4_stream(const Fp4Args& p, hipStream_t s) {
 }
 
 // Whether a linear's few rows are quantised in the product's launch (one row of 4608 x 3584 13.3 -> 9.3
-// us on MI355X): whole 16-byte loads, codes and scales that fit the LDS.
-static bool fp4_fuses(const void* x, int x_dtype, int64_t ldx, int64_t M, int64_t K) {
-  return M <= 4 && K > 0 && K <= 24576 && (uintptr_t)x % 16 == 0 && (ldx * (x_dtype == LSK_F32 ? 4 : 2)) % 16 == 0;
-}
+// us on MI355X): codes and scales that fit the LDS.
+static bool fp4_fuses(int64_t M, int64_t K) { return M <= 4 && K > 0 && K <= 24576; }
 
 static int fp4_stream_fused(const Fp4Args& p, const void* x, int x_dtype, int64_t ldx, hipStream_t s) {
   if (x_dtype == LSK_F32) return fp4_stream_shape<1, LSK_F32>(p, x, ldx, s);
@@ -742,6 +743,7 @@ extern "C" int lsk_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, int64_t 
 
 // The quantised rows come first in the workspace, then their scales (the row kernels) or the tiles' part.
 extern "C" int64_t lsk_linear_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
+  if (lsk::fp4_fuses(M, K)) return 0;
   return lsk::up256(M * (K / 2)) +
          (lsk::fp4_takes_tiles(M, N, K, 0) ? lsk::fp4_prep_bytes(M, N, K, 1) : lsk::up256(M * (K / 32)));
 }
@@ -766,7 +768,7 @@ extern "C" int lsk_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int64_t
   p.M = M, p.N = N, p.K = (int)K;
   p.bias = bias, p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
   if (lsk::fp4_takes_tiles(M, N, K, 0)) return lsk::fp4_tiles(p, x, x_dtype, ldx, q, (char*)rest, s);
-  if (lsk::fp4_fuses(x, x_dtype, ldx, M, K)) return lsk::fp4_stream_fused(p, x, x_dtype, ldx, s);
+  if (lsk::fp4_fuses(M, K)) return lsk::fp4_stream_fused(p, x, x_dtype, ldx, s);
   if (K > 0 && (rc = lsk::quantize_launch(x, x_dtype, M, K, ldx, q, rest, s))) return rc;
   return lsk::fp4_stream(p, s);
 }

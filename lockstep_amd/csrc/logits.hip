@@ -134,7 +134,7 @@ __global__ __launch_bounds__(1024) void penalize_logits_kernel(PenaltyArgs p) {
       }
     }
     if (!bias && !mask) {  // nothing to do but copy
-      if (in != out) *(v4u32*)(out + (int64_t)i * SIZE) = raw;
+      if (in != out) store16_split(out + (int64_t)i * SIZE, raw);
       continue;
     }
     float l[VEC], s[VEC];

@@ -798,6 +798,7 @@ __global__ __launch_bounds__(256) void dequant_mxfp4_8_kernel(const uint32_t* __
     } else {
       store16_split((float*)out + 8 * i, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
                     __float_as_uint(v[3]));
+      __asm__ volatile("" ::: "memory");  // (keeps the two from being fused across)
       store16_split((float*)out + 8 * i + 4, __float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]),
                     __float_as_uint(v[7]));
     }

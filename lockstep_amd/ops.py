@@ -650,14 +650,16 @@ def dequant_mxfp4(packed: torch.Tensor, scale: torch.Tensor, out_dtype=torch.bfl
     K = packed.shape[-1] * 2
     if scale.shape[-1] * block != K:
         raise AssertionError((tuple(scale.shape), K))
-    p2 = packed.to(torch.uint8).reshape(-1, K // 2).contiguous()
-    s2 = scale.to(torch.uint8).reshape(-1, K // block).contiguous()
-    code = L.LSK_BF16 if out_dtype == torch.bfloat16 else L.LSK_F32
-    out = torch.empty((p2.shape[0], K), dtype=torch.bfloat16 if code == L.LSK_BF16 else torch.float32,
-                      device=packed.device)
-    L.call("lsk_dequant_mxfp4", L.ptr(p2), L.ptr(s2), p2.shape[0], K, int(block), L.ptr(out), code,
-           L.stream_of(packed))
-    out = out.reshape(*lead, K)
+    p2 = packed if packed.dtype == torch.uint8 else packed.to(torch.uint8)
+    s2 = scale if scale.dtype == torch.uint8 else scale.to(torch.uint8)
+    p2, s2 = p2.contiguous(), s2.contiguous()
+    rows = p2.numel() * 2 // K if K else 0
+    if s2.numel() * block != rows * K:
+        raise AssertionError((tuple(scale.shape), tuple(packed.shape)))
+    half = out_dtype == torch.bfloat16
+    out = torch.empty((*lead, K), dtype=torch.bfloat16 if half else torch.float32, device=packed.device)
+    L.call("lsk_dequant_mxfp4", p2.data_ptr(), s2.data_ptr(), rows, K, int(block), out.data_ptr(),
+           L.LSK_BF16 if half else L.LSK_F32, L.stream_of(packed))
     return out if out.dtype == out_dtype else out.to(out_dtype)
 
 
@@ -675,24 +677,40 @@ def pack_m2(m2: torch.Tensor):
 
 
 # ---------------------------------------------------------------- MXFP4 activations and weights
+# (written for few Python operations a call: one row of a linear is 6 us of GPU work)
+_FLOATS = {torch.float32: L.LSK_F32, torch.bfloat16: L.LSK_BF16, torch.float16: L.LSK_F16}
+
+
+def _float_rows(x: torch.Tensor, what: str):
+    """x [..., K] as (a tensor whose rows have unit stride, dtype code, rows, K, row stride)."""
+    code = _FLOATS.get(x.dtype)
+    if code is None:
+        if not x.is_floating_point():
+            raise TypeError("%s: x must be floating point, got %s" % (what, x.dtype))
+        x, code = x.to(torch.float32), L.LSK_F32
+    if x.dim() != 2:
+        if x.dim() == 0:
+            raise ValueError("%s: x must be [..., K], got a scalar" % what)
+        x = x.reshape(x.numel() // x.shape[-1], x.shape[-1]) if x.shape[-1] else x.new_empty((x.shape[:-1].numel(), 0))
+    M, K = x.shape
+    if K > 1 and x.stride(1) != 1 or M > 1 and x.stride(0) < K:
+        x = x.contiguous()
+    return x, code, M, K, x.stride(0) if M > 1 else K
+
+
 def quantize_mxfp4(x: torch.Tensor):
     """x [..., K] (f32 / bf16 / f16; other float dtypes go through f32), K % 32 == 0, to MXFP4:
     (packed E2M1 codes uint8 [..., K/2], low nibble first, E8M0 scales uint8 [..., K/32])."""
     L.require_cuda(x, what="quantize_mxfp4")
-    if x.dim() == 0 or x.shape[-1] % 32:
-        raise ValueError("quantize_mxfp4: x must be [..., K] with K a multiple of 32, got %s" % (tuple(x.shape),))
-    if not x.is_floating_point():
-        raise TypeError("quantize_mxfp4: x must be floating point, got %s" % x.dtype)
-    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        x = x.to(torch.float32)
-    lead, K = x.shape[:-1], x.shape[-1]
+    lead = x.shape[:-1]
+    x, code, M, K, ld = _float_rows(x, "quantize_mxfp4")
+    if K % 32:
+        raise ValueError("quantize_mxfp4: K=%d not a multiple of 32" % K)
     packed = torch.empty((*lead, K // 2), dtype=torch.uint8, device=x.device)
     scale = torch.empty((*lead, K // 32), dtype=torch.uint8, device=x.device)
-    if x.numel():
-        x2 = _rows(x)
-        M = x2.shape[0]
-        L.call_on(x, "lsk_quantize_mxfp4", L.ptr(x2), L.dtype_code(x2.dtype), M, K, x2.stride(0) if M > 1 else K,
-                  L.ptr(packed), L.ptr(scale), L.stream_of(x))
+    if M and K:
+        L.call_on(x, "lsk_quantize_mxfp4", x.data_ptr(), code, M, K, ld, packed.data_ptr(), scale.data_ptr(),
+                  L.stream_of(x))
     return packed, scale
 
 
@@ -701,23 +719,26 @@ def _mxfp4_codes(packed: torch.Tensor, scale: torch.Tensor, what: str):
     16-byte aligned (a copy where they are not).  Returns (packed, scale, rows, K)."""
     if packed.dtype != torch.uint8 or scale.dtype != torch.uint8:
         raise TypeError("%s: packed codes and scales must be uint8, got %s and %s" % (what, packed.dtype, scale.dtype))
-    if packed.dim() != 2 or scale.dim() != 2 or packed.shape[1] % 16 \
-            or tuple(scale.shape) != (packed.shape[0], packed.shape[1] // 16):
+    shape = packed.shape
+    if len(shape) != 2 or shape[1] % 16 or scale.shape != (shape[0], shape[1] // 16):
         raise ValueError("%s: packed [rows, K/2] and scale [rows, K/32] with K a multiple of 32 expected, got %s and %s"
-                         % (what, tuple(packed.shape), tuple(scale.shape)))
+                         % (what, tuple(shape), tuple(scale.shape)))
     if not packed.is_contiguous() or packed.data_ptr() % 16:
         packed = packed.clone(memory_format=torch.contiguous_format)
-    return packed, scale.contiguous(), packed.shape[0], packed.shape[1] * 2
+    return packed, scale.contiguous(), shape[0], shape[1] * 2
 
 
 def _mxfp4_out(what: str, out_dtype):
-    if out_dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    code = _FLOATS.get(out_dtype)
+    if code is None:
         raise TypeError("%s: out_dtype %s not supported (float32, bfloat16, float16)" % (what, out_dtype))
-    return L.dtype_code(out_dtype)
+    return code
 
 
 def _mxfp4_bias(bias, N: int, what: str):
-    if bias is not None and tuple(bias.shape) != (N,):
+    if bias is None:
+        return None
+    if bias.shape != (N,):
         raise ValueError("%s: bias must be [%d], got %s" % (what, N, tuple(bias.shape)))
     return _f32(bias)
 
@@ -738,8 +759,8 @@ def mm_mxfp4(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: t
     if M and N:
         nbytes = L.load().lsk_gemm_mxfp4_workspace(M, N, K)
         work = torch.empty((nbytes,), dtype=torch.uint8, device=a.device) if nbytes else None
-        L.call_on(a, "lsk_gemm_mxfp4", L.ptr(a), L.ptr(a_scale), M, K, L.ptr(w), L.ptr(w_scale), N, L.ptr(bias),
-                  L.ptr(out), code, N, L.ptr(work), nbytes, L.stream_of(a))
+        L.call_on(a, "lsk_gemm_mxfp4", a.data_ptr(), a_scale.data_ptr(), M, K, w.data_ptr(), w_scale.data_ptr(), N,
+                  L.ptr(bias), out.data_ptr(), code, N, L.ptr(work), nbytes, L.stream_of(a))
     return out
 
 
@@ -749,51 +770,62 @@ def linear_mxfp4(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=N
     the quantised rows, the same bits, in one call."""
     L.require_cuda(x, w, w_scale, bias, what="linear_mxfp4")
     w, w_scale, N, K = _mxfp4_codes(w, w_scale, "linear_mxfp4")
-    if x.dim() == 0 or x.shape[-1] != K:
-        raise ValueError("linear_mxfp4: x must be [..., %d], got %s" % (K, tuple(x.shape)))
-    if not x.is_floating_point():
-        raise TypeError("linear_mxfp4: x must be floating point, got %s" % x.dtype)
-    out_dtype = x.dtype if out_dtype is None else out_dtype
+    lead = x.shape[:-1]
+    out_dtype = out_dtype or x.dtype
+    x, xcode, M, Kx, ld = _float_rows(x, "linear_mxfp4")
+    if Kx != K:
+        raise ValueError("linear_mxfp4: rows of %d values for a weight of %d" % (Kx, K))
     code = _mxfp4_out("linear_mxfp4", out_dtype)
-    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        x = x.to(torch.float32)
     bias = _mxfp4_bias(bias, N, "linear_mxfp4")
-    out = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=x.device)
-    if out.numel():
-        x2 = _rows(x) if K else x.reshape(out.numel() // N, 0)
-        M = x2.shape[0]
+    out = torch.empty((*lead, N), dtype=out_dtype, device=x.device)
+    if M and N:
         nbytes = L.load().lsk_linear_mxfp4_workspace(M, N, K)
         work = torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
-        L.call_on(x, "lsk_linear_mxfp4", L.ptr(x2), L.dtype_code(x2.dtype), x2.stride(0) if M > 1 else K, M, K, L.ptr(w),
-                  L.ptr(w_scale), N, L.ptr(bias), L.ptr(out), code, N, L.ptr(work), nbytes, L.stream_of(x))
+        L.call_on(x, "lsk_linear_mxfp4", x.data_ptr(), xcode, ld, M, K, w.data_ptr(), w_scale.data_ptr(), N,
+                  L.ptr(bias), out.data_ptr(), code, N, L.ptr(work), nbytes, L.stream_of(x))
     return out
 
 
 # ---------------------------------------------------------------- logits
+_INTS = {torch.int32: 0, torch.int64: 1}
+
+
 def _history(tokens, lens, B: int, what: str):
-    """(tokens [B, L] with unit stride, lens [B] contiguous, wide flags) of one token history."""
+    """One token history as the C call takes it: (tokens, its address, row stride, columns, lengths, their
+    address, 64-bit tokens, 64-bit lengths)."""
     if tokens is None:
         if lens is not None:
             raise ValueError("penalize_logits: %s_lens without %s" % (what, what))
-        return None, None, 0, 0
-    if tokens.dim() != 2 or tokens.shape[0] != B or tokens.dtype not in (torch.int32, torch.int64):
+        return None, None, 0, 0, None, None, 0, 0
+    wide, shape = _INTS.get(tokens.dtype), tokens.shape
+    if wide is None or len(shape) != 2 or shape[0] != B:
         raise ValueError("penalize_logits: %s must be int32 or int64 [%d, L], got %s %s"
-                         % (what, B, tokens.dtype, tuple(tokens.shape)))
-    if tokens.shape[1] > 1 and tokens.stride(1) != 1:
+                         % (what, B, tokens.dtype, tuple(shape)))
+    if shape[1] > 1 and tokens.stride(1) != 1:
         tokens = tokens.contiguous()
-    if lens is not None:
-        if tuple(lens.shape) != (B,) or lens.dtype not in (torch.int32, torch.int64):
-            raise ValueError("penalize_logits: %s_lens must be int32 or int64 [%d], got %s %s"
-                             % (what, B, lens.dtype, tuple(lens.shape)))
-        lens = lens.contiguous()
-    return (tokens, lens, 1 if tokens.dtype == torch.int64 else 0,
-            1 if lens is not None and lens.dtype == torch.int64 else 0)
+    if lens is None:
+        return tokens, tokens.data_ptr(), tokens.stride(0), shape[1], None, None, wide, 0
+    lwide = _INTS.get(lens.dtype)
+    if lwide is None or lens.shape != (B,):
+        raise ValueError("penalize_logits: %s_lens must be int32 or int64 [%d], got %s %s"
+                         % (what, B, lens.dtype, tuple(lens.shape)))
+    lens = lens.contiguous()
+    return tokens, tokens.data_ptr(), tokens.stride(0), shape[1], lens, lens.data_ptr(), wide, lwide
+
+
+def _per_row(t, B: int, what: str):
+    if t is None:
+        return None
+    if t.shape != (B,) or t.dtype != torch.float32:
+        raise ValueError("penalize_logits: %s must be f32 [%d], got %s %s" % (what, B, t.dtype, tuple(t.shape)))
+    return t.contiguous()
 
 
 def penalize_logits(logits: torch.Tensor, prompt=None, prompt_lens=None, output=None, output_lens=None, repetition=None,
                     frequency=None, presence=None, bias=None, mask=None, out=None) -> torch.Tensor:
     """logits [B, V] (f32 / bf16 / f16) -> the same shape and type (into `out` when given; out=logits
-    works in place), per row b and token v, in binary32, each step one rounding:
+    works in place, any other overlap does not), per row b and token v, in binary32, each step one
+    rounding:
         l = logits + bias                                  bias f32 [V] or [B, V]
         v in the row's prompt or output:  l = l / repetition if l > 0 else l * repetition
         l = l - frequency * (times v stands in the output)
@@ -805,40 +837,41 @@ def penalize_logits(logits: torch.Tensor, prompt=None, prompt_lens=None, output=
     presence are f32 [B]; what is None is left out.  A row whose mask allows nothing is -inf throughout."""
     L.require_cuda(logits, prompt, prompt_lens, output, output_lens, repetition, frequency, presence, bias, mask, out,
                    what="penalize_logits")
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    code, shape = _FLOATS.get(logits.dtype), logits.shape
+    if code is None or len(shape) != 2:
         raise ValueError("penalize_logits: logits must be f32, bf16 or f16 [B, V], got %s %s"
-                         % (logits.dtype, tuple(logits.shape)))
-    B, V = logits.shape
-    prompt, prompt_lens, p64, pl64 = _history(prompt, prompt_lens, B, "prompt")
-    output, output_lens, o64, ol64 = _history(output, output_lens, B, "output")
-    for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
-        if t is not None and (tuple(t.shape) != (B,) or t.dtype != torch.float32):
-            raise ValueError("penalize_logits: %s must be f32 [%d], got %s %s" % (name, B, t.dtype, tuple(t.shape)))
+                         % (logits.dtype, tuple(shape)))
+    B, V = shape
+    prompt, pp, ldp, Lp, prompt_lens, plp, p64, pl64 = _history(prompt, prompt_lens, B, "prompt")
+    output, op, ldt, Lo, output_lens, olp, o64, ol64 = _history(output, output_lens, B, "output")
+    repetition = _per_row(repetition, B, "repetition")
+    frequency = _per_row(frequency, B, "frequency")
+    presence = _per_row(presence, B, "presence")
+    ldb = ldm = 0
     if bias is not None:
-        if bias.dtype != torch.float32 or tuple(bias.shape) not in ((V,), (B, V)):
+        if bias.dtype != torch.float32 or bias.shape != (V,) and bias.shape != (B, V):
             raise ValueError("penalize_logits: bias must be f32 [%d] or [%d, %d], got %s %s"
                              % (V, B, V, bias.dtype, tuple(bias.shape)))
-        bias = bias if V < 2 or bias.stride(-1) == 1 else bias.contiguous()
+        if V > 1 and bias.stride(-1) != 1:
+            bias = bias.contiguous()
+        ldb = bias.stride(0) if bias.dim() == 2 else 0
     if mask is not None:
         words = (V + 31) // 32
-        if mask.dtype != torch.int32 or tuple(mask.shape) not in ((B, words), (1, words)):
+        if mask.dtype != torch.int32 or mask.shape != (B, words) and mask.shape != (1, words):
             raise ValueError("penalize_logits: mask must be int32 [%d, %d] or [1, %d], got %s %s"
                              % (B, words, words, mask.dtype, tuple(mask.shape)))
-        mask = mask if words < 2 or mask.stride(1) == 1 else mask.contiguous()
-    if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or (V > 1 and out.stride(1) != 1)
-                            or (B > 1 and out.stride(0) < V)):
+        if words > 1 and mask.stride(1) != 1:
+            mask = mask.contiguous()
+        ldm = mask.stride(0) if mask.shape[0] > 1 else 0
+    if out is not None and (out.shape != shape or out.dtype != logits.dtype or V > 1 and out.stride(1) != 1
+                            or B > 1 and out.stride(0) < V):
         raise ValueError("penalize_logits: out must be %s [%d, %d] with rows of consecutive tokens" % (logits.dtype, B, V))
     if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
         logits = logits.contiguous()
     if out is None:
         out = torch.empty((B, V), dtype=logits.dtype, device=logits.device)
     if B and V:
-        rep, freq, pres = (None if t is None else t.contiguous() for t in (repetition, frequency, presence))
-        row = lambda t: 0 if t is None else t.stride(0)  # noqa: E731
-        cols = lambda t: 0 if t is None else t.shape[1]  # noqa: E731
-        L.call_on(logits, "lsk_penalize_logits", L.ptr(logits), L.dtype_code(logits.dtype), row(logits), B, V,
-                  L.ptr(prompt), row(prompt), cols(prompt), L.ptr(prompt_lens), L.ptr(output), row(output), cols(output),
-                  L.ptr(output_lens), p64 | o64 << 1 | pl64 << 2 | ol64 << 3, L.ptr(rep), L.ptr(freq), L.ptr(pres),
-                  L.ptr(bias), row(bias) if bias is not None and bias.dim() == 2 else 0, L.ptr(mask),
-                  row(mask) if mask is not None and mask.shape[0] > 1 else 0, L.ptr(out), row(out), L.stream_of(logits))
+        L.call_on(logits, "lsk_penalize_logits", logits.data_ptr(), code, logits.stride(0), B, V, pp, ldp, Lp, plp, op,
+                  ldt, Lo, olp, p64 | o64 << 1 | pl64 << 2 | ol64 << 3, L.ptr(repetition), L.ptr(frequency),
+                  L.ptr(presence), L.ptr(bias), ldb, L.ptr(mask), ldm, out.data_ptr(), out.stride(0), L.stream_of(logits))
     return out
