@@ -94,9 +94,17 @@ LSK_DEV void quantize_run(const void* __restrict__ x, int64_t ldx, int64_t M, in
     load8<DT, VEC>(x, row * ldx + 8 * c, v);
     uint32_t s;
     ((uint32_t*)packed)[i] = quantize8_mxfp4(v, s);
-    if ((i & 3) == 0) {
-      if constexpr (TS) store_scale_t(scale, M, row, c >> 2, K8 >> 2, s);
-      else scale[i >> 2] = (uint8_t)s;
+    if constexpr (TS) {
+      if ((K8 & 15) == 0) {  // 16 lanes hold the four bytes of a dword
+        uint32_t w = s << (2 * (c & 12));
+        w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x124, 0xf, 0xf, false);  // row_ror:4
+        w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x128, 0xf, 0xf, false);  // row_ror:8
+        if ((c & 15) == 0) ((uint32_t*)scale)[(int64_t)(c >> 4) * M + row] = w;
+      } else if ((c & 3) == 0) {
+        store_scale_t(scale, M, row, c >> 2, K8 >> 2, s);
+      }
+    } else if ((i & 3) == 0) {
+      scale[i >> 2] = (uint8_t)s;
     }
   }
 }
@@ -152,121 +160,110 @@ struct Fp4Args {
   const int64_t* b_ptrs;
 };
 
-// Row tile t of expert-sorted rows: expert e, its first row m0 and the end m1 of the expert's rows,
-// tiles of bm rows counted over the experts in order; false past the last tile.  Offsets that
-// decrease or leave [0, R] are taken as min(R, max(0, offs[0..j])), so that experts come out empty
-// or shortened and no row outside [0, R) is touched.  Every wave looks its tile up itself, 64
-// experts a step: no table to build in a launch of its own.
-LSK_DEV bool expert_tile(const int32_t* __restrict__ offs, int E, int R, int bm, int t, int& e, int& m0, int& m1) {
-  const int lane = threadIdx.x & 63;
-  int carry = min(max(offs[0], 0), R);
-  for (int e0 = 0; e0 < E; e0 += 64) {
-    int hi = min(max(offs[min(e0 + lane + 1, E)], 0), R);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(hi, d, 64);
-      if (lane >= d) hi = max(hi, o);
-    }
-    hi = max(hi, carry);
-    int lo = __shfl_up(hi, 1, 64);
-    if (lane == 0) lo = carry;
-    const int n = (hi - lo + bm - 1) / bm;
-    int sum = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(sum, d, 64);
-      if (lane >= d) sum += o;
-    }
-    const uint64_t past = __builtin_amdgcn_ballot_w64(sum > t);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      e = e0 + l;
-      m0 = __builtin_amdgcn_readlane(lo, l) + (t - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l))) * bm;
-      m1 = __builtin_amdgcn_readlane(hi, l);
-      return true;
-    }
-    t -= __builtin_amdgcn_readlane(sum, 63);
-    carry = __builtin_amdgcn_readlane(hi, 63);
-  }
-  return false;
+// Inclusive scans over the wave by DPP row shifts and broadcasts (lanes without a source keep `ident`).
+template <class Op>
+LSK_DEV int wave_scan(int v, int ident, Op op) {
+  v = op(v, __builtin_amdgcn_update_dpp(ident, v, 0x111, 0xf, 0xf, false));  // row_shr:1
+  v = op(v, __builtin_amdgcn_update_dpp(ident, v, 0x112, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(ident, v, 0x114, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(ident, v, 0x118, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(ident, v, 0x142, 0xa, 0xf, false));  // row_bcast:15
+  v = op(v, __builtin_amdgcn_update_dpp(ident, v, 0x143, 0xc, 0xf, false));  // row_bcast:31
+  return v;
 }
-// How many such tiles there are in all.
-LSK_DEV int expert_tile_count(const int32_t* __restrict__ offs, int E, int R, int bm) {
-  const int lane = threadIdx.x & 63;
-  int carry = min(max(offs[0], 0), R), total = 0;
-  for (int e0 = 0; e0 < E; e0 += 64) {
-    int hi = min(max(offs[min(e0 + lane + 1, E)], 0), R);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(hi, d, 64);
-      if (lane >= d) hi = max(hi, o);
-    }
-    hi = max(hi, carry);
-    int lo = __shfl_up(hi, 1, 64);
-    if (lane == 0) lo = carry;
-    total += wave_sum_i32((hi - lo + bm - 1) / bm);
-    carry = __builtin_amdgcn_readlane(hi, 63);
+
+// Row tiles of expert-sorted rows, bm rows each, counted over the experts in order.  Offsets that
+// decrease or leave [0, R] are taken as min(R, max(0, offs[0..j])), so that experts come out empty or
+// shortened and no row outside [0, R) is touched.  Every wave looks its tile up itself, 64 experts a
+// step: no table to build in a launch of its own.
+struct ExpertTiles {
+  const int32_t* offs;
+  int E, R, bm;
+  int carry, lo, hi, n, sum;  // of the last 64 experts looked at, one a lane; carry: the rows before them
+  LSK_DEV ExpertTiles(const int32_t* o, int e, int r, int b) : offs(o), E(e), R(r), bm(b) { restart(); }
+  LSK_DEV void restart() {
+    carry = min(max(offs[0], 0), R);
+    look(0);
   }
-  return total;
-}
+  LSK_DEV void look(int e0) {
+    const int lane = threadIdx.x & 63;
+    hi = wave_scan(min(max(offs[min(e0 + lane + 1, E)], 0), R), 0, [](int a, int b) { return max(a, b); });
+    hi = max(hi, carry);
+    lo = __shfl_up(hi, 1, 64);
+    if (lane == 0) lo = carry;
+    n = (int)((unsigned)(hi - lo + bm - 1) / (unsigned)bm);
+    sum = wave_scan(n, 0, [](int a, int b) { return a + b; });
+  }
+  LSK_DEV void next(int e0) {
+    carry = __builtin_amdgcn_readlane(hi, 63);
+    look(e0);
+  }
+  // how many tiles there are
+  LSK_DEV int count() {
+    int total = __builtin_amdgcn_readlane(sum, 63);
+    for (int e0 = 64; e0 < E; e0 += 64) {
+      next(e0);
+      total += __builtin_amdgcn_readlane(sum, 63);
+    }
+    if (E > 64) restart();
+    return total;
+  }
+  // tile t: its expert, first row and the end of the expert's rows; false past the last tile
+  LSK_DEV bool find(int t, int& e, int& m0, int& m1) {
+    for (int e0 = 0;;) {
+      const uint64_t past = __builtin_amdgcn_ballot_w64(sum > t);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        e = e0 + l;
+        m0 = __builtin_amdgcn_readlane(lo, l) +
+             (t - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l))) * bm;
+        m1 = __builtin_amdgcn_readlane(hi, l);
+        return true;
+      }
+      t -= __builtin_amdgcn_readlane(sum, 63);
+      e0 += 64;
+      if (e0 >= E) return false;
+      next(e0);
+    }
+  }
+};
 inline int64_t expert_tiles_max(int64_t R, int64_t E, int64_t bm) { return R / bm + (E < R ? E : R); }
 
 // Few rows: a block computes NG x 16 output columns of up to MT x 16 rows over all of K, streaming its
-// weight rows from HBM.  Four waves bring the codes in, 512 values (256 bytes of a row, whole lines) a
-// stage, by direct global -> LDS loads RING - 1 stages ahead; the first NG of them multiply, a group of
-// 16 weight rows each, on 16x16x128 instructions (weight rows as their rows, activation rows as their
-// columns, so a lane ends with four consecutive outputs of a row).  Bound by HBM, that is by bytes in
-// flight: with a few thousand weight rows there is a block of 16 of them a CU, which is why waves that
-// do not multiply load.  K is not split over waves or blocks: a row's bits would depend on the split.
-// The scale bytes of the block's rows lie together in memory and are copied into LDS whole.
+// weight rows from HBM.  Four waves bring the codes in, KS x 512 values (256 bytes of a row, whole lines)
+// a stage, by direct global -> LDS loads RING - 1 stages ahead; waves multiply a group of 16 weight
+// rows by a row tile each, on 16x16x128 instructions (weight rows as their rows, activation rows as
+// their columns, so a lane ends with four consecutive outputs of a row).  Bound by HBM, that is by
+// bytes in flight: with a few thousand weight rows there is a block of 16 of them a CU, which is why
+// waves that do not multiply load.  K is not split over waves or blocks: a row's bits would depend on
+// the split.  The scales of the block's rows are copied into LDS whole at the start.
 // DT >= 0: the rows of x (at most four; vec: 16-byte aligned) are quantised by every block into LDS
 // itself, which saves a launch and the wait for it; x comes from the L2.
-template <int NG, int MT, bool FUSE>
+template <int NG, int MT, int KS, bool FUSE>
 struct Fp4StreamCfg {
-  static constexpr int kStageW = NG * 16 * 256, kStageA = FUSE ? 0 : MT * 16 * 256, kStage = kStageW + kStageA;
-  static constexpr int kPer = NG + (FUSE ? 0 : MT);              // loads per thread per stage
-  static constexpr int kMW = NG * MT > 4 ? NG * MT / 4 : 1;      // row tiles of a wave
+  static constexpr int kPartW = NG * 4096, kPart = kPartW + (FUSE ? 0 : MT * 4096), kStage = KS * kPart;  // bytes
+  static constexpr int kPer = KS * (NG + (FUSE ? 0 : MT));  // loads per thread per stage
+  static constexpr int kMW = NG * MT > 4 ? NG * MT / 4 : 1;  // row tiles of a wave
   static_assert(NG * MT <= 4 || NG == 4, "a wave's row tiles share its weight rows");
 };
 
-// Bytes from one row of scales to the next in LDS: whole 16-byte pieces, an odd number of them, so that
-// 16 rows read at once lie in 16 bank groups.
-LSK_HD int scale_pitch(int nb) { return (nb + 15) / 16 * 16 | 16; }
-
-// `rows` rows of nb scale bytes (row stride ld, any alignment) into LDS at d, zeros past nb.
-LSK_DEV void copy_scales(const uint8_t* __restrict__ p, int64_t ld, int rows, int nb, char* d) {
-  const int pieces = (nb + 15) / 16, pitch = scale_pitch(nb);
-  for (int i = threadIdx.x; i < rows * pieces; i += 256) {
-    const int row = i / pieces, c = i - row * pieces;
-    const uint8_t* src = p + row * ld;
-    if (nb >= 16) {  // the last piece from the 16 bytes that end the row, shifted down
-      const int at = min(16 * c, nb - 16), sh = 8 * (16 * c - at);
-      uint64_t v[2];
-      __builtin_memcpy(v, src + at, 16);
-      if (sh >= 64) v[0] = v[1] >> (sh - 64), v[1] = 0;
-      else if (sh > 0) v[0] = v[0] >> sh | v[1] << (64 - sh), v[1] >>= sh;
-      *(ulonglong2*)(d + row * pitch + 16 * c) = make_ulonglong2(v[0], v[1]);
-      continue;
-    }
-    v4u32 v = {0, 0, 0, 0};
-    for (int z = 0; z < nb; ++z) v[z >> 2] |= (uint32_t)src[z] << (8 * (z & 3));
-    *(v4u32*)(d + row * pitch + 16 * c) = v;
-  }
-}
-
+// Bytes from one row of scales to the next in LDS: whole stages, in an odd number of 16-byte pieces (512
+// values each), so that 16 rows read at once lie in 16 bank groups.
+LSK_HD int scale_pieces(int nb, int ks) { return ((nb + 15) / 16 + ks - 1) / ks * ks; }
+LSK_HD int scale_pitch(int nb, int ks) { return scale_pieces(nb, ks) * 16 | 16; }
 // Bytes of LDS of such a block: the ring, the rows' codes (FUSE: `rows` of them) and the scales.
-LSK_HD int fused_pitch(int K) { return (K + 511) / 512 * 256 + 16; }
-template <int NG, int MT, int RING, bool FUSE>
+LSK_HD int fused_pitch(int K, int ks) { return scale_pieces(K / 32, ks) * 256 + 16; }
+template <int NG, int MT, int KS, int RING, bool FUSE>
 static int64_t fp4_stream_lds(int K, int rows) {
-  return RING * Fp4StreamCfg<NG, MT, FUSE>::kStage + (FUSE ? (int64_t)rows * fused_pitch(K) : 0) +
-         (int64_t)(NG * 16 + (FUSE ? rows : MT * 16)) * scale_pitch(K / 32);
+  return RING * Fp4StreamCfg<NG, MT, KS, FUSE>::kStage + (FUSE ? (int64_t)rows * fused_pitch(K, KS) : 0) +
+         (int64_t)(NG * 16 + (FUSE ? rows : MT * 16)) * scale_pitch(K / 32, KS);
 }
 
-template <int NG, int MT, int RING, int DT, bool GROUPED>
+template <int NG, int MT, int KS, int RING, int DT, bool GROUPED>
 __global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* __restrict__ x, int64_t ldx,
                                                          int vec) {
   constexpr bool FUSE = DT >= 0;
-  using C = Fp4StreamCfg<NG, MT, FUSE>;
+  using C = Fp4StreamCfg<NG, MT, KS, FUSE>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), r = lane & 15, q = lane >> 4;
   const int ngroups = (int)((p.N + 16 * NG - 1) / (16 * NG));
@@ -274,7 +271,7 @@ __global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* 
   int64_t m0 = (int64_t)tile * 16 * MT, m1 = p.M;
   if constexpr (GROUPED) {
     int e, first, end;
-    if (!expert_tile(p.offs, p.E, (int)p.M, 16 * MT, tile, e, first, end)) return;
+    if (!ExpertTiles(p.offs, p.E, (int)p.M, 16 * MT).find(tile, e, first, end)) return;
     m0 = first;
     m1 = end;
     p.w = (const uint8_t*)wave_uniform64(p.w_ptrs[e]);
@@ -283,42 +280,79 @@ __global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* 
   }
   const int rows_a = m1 - m0 < 16 * MT ? (int)(m1 - m0) : 16 * MT;
   const int rows_w = p.N - n0 < 16 * NG ? (int)p.N - n0 : 16 * NG;
-  const int nb = p.K / 32, Kb = p.K / 2, nk = (p.K + 511) / 512;
-  const int sp = scale_pitch(nb), fp = fused_pitch(p.K);
+  const int nb = p.K / 32, Kb = p.K / 2, pieces = scale_pieces(nb, KS), nk = pieces / KS;
+  const int sp = scale_pitch(nb, KS), fp = fused_pitch(p.K, KS);
   char* const fused = smem + RING * C::kStage;  // FUSE: the rows' codes
   char* const scw = fused + (FUSE ? rows_a * fp : 0);
   char* const sca = scw + NG * 16 * sp;
 
-  // scales first: their registers are then waited for without waiting for the stages
-  copy_scales(p.sw + n0 * p.ldsw, p.ldsw, rows_w, nb, scw);
-  if constexpr (!FUSE) copy_scales(p.sa + m0 * p.ldsa, p.ldsa, rows_a, nb, sca);
-
   const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w + (int64_t)n0 * p.ldw, (int64_t)(rows_w - 1) * p.ldw + Kb);
   const __amdgpu_buffer_rsrc_t ra = FUSE ? rw : make_rsrc(p.a + m0 * p.lda, (int64_t)(rows_a - 1) * p.lda + Kb);
-  // a thread's 16-byte slot j of a stage: row 16 j + tid / 16, chunk c of its 256 bytes in place c ^ row % 16
+  // a thread's 16-byte slot j of a part: row 16 j + tid / 16, chunk c of its 256 bytes in place c ^ row % 16
   const int row = tid >> 4, kc = 16 * ((tid & 15) ^ row);
-  auto issue = [&](int s) {
-    char* base = smem + (s % RING) * C::kStage;
-    const int k = 256 * s + kc;
+  auto issue = [&](int kt) {
+    char* base = smem + (kt % RING) * C::kStage + wave * 1024;
 #pragma unroll
-    for (int j = 0; j < NG; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_void_t)(base + j * 4096 + wave * 1024), 16,
-                                               k < Kb && 16 * j + row < rows_w ? (uint32_t)((16 * j + row) * p.ldw + k) : kOob,
-                                               0, 0, 0);
-    if constexpr (!FUSE) {
+    for (int u = 0; u < KS; ++u) {
+      const int k = 256 * (KS * kt + u);
+      const bool in = k + kc < Kb;
 #pragma unroll
-      for (int j = 0; j < MT; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            ra, (lds_void_t)(base + C::kStageW + j * 4096 + wave * 1024), 16,
-            k < Kb && 16 * j + row < rows_a ? (uint32_t)((16 * j + row) * p.lda + k) : kOob, 0, 0, 0);
+      for (int j = 0; j < NG; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_void_t)(base + u * C::kPart + j * 4096), 16, in && 16 * j + row < rows_w ? (uint32_t)((16 * j + row) * (int)p.ldw + kc) : kOob,
+                                                 k, 0, 0);
+      if constexpr (!FUSE) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void_t)(base + u * C::kPart + C::kPartW + j * 4096), 16,
+                                                   in && 16 * j + row < rows_a ? (uint32_t)((16 * j + row) * (int)p.lda + kc) : kOob,
+                                                   k, 0, 0);
+      }
     }
   };
 #pragma unroll
   for (int s = 0; s < RING - 1; ++s) issue(s);
+
+  // The scales: 16 threads a row, a 16-byte piece each, every row's first 32 pieces in flight at once and
+  // no branch around a load but uniform ones.  A row's last piece comes from the 16 bytes that end it,
+  // shifted down; zeros past it.
+  constexpr int kRows = NG + (FUSE ? 0 : MT);  // row sets of 16
+  const int c0 = tid & 15;
+  auto scale_src = [&](int j) {
+    return j < NG ? p.sw + n0 * p.ldsw + (uint32_t)(min(16 * j + row, rows_w - 1) * (int)p.ldsw)
+                  : p.sa + m0 * p.ldsa + (uint32_t)(min(16 * (j - NG) + row, rows_a - 1) * (int)p.ldsa);
+  };
+  auto store_piece = [&](int j, int c, uint64_t lo, uint64_t hi) {
+    if (c >= pieces) return;
+    const int sh = 8 * max(16 * c + 16 - nb, 0);
+    if (sh >= 128) lo = hi = 0;
+    else if (sh >= 64) lo = hi >> (sh - 64), hi = 0;
+    else if (sh > 0) lo = lo >> sh | hi << (64 - sh), hi >>= sh;
+    *(ulonglong2*)(scw + (16 * j + row) * sp + 16 * c) = make_ulonglong2(lo, hi);
+  };
+  if (nb >= 16) {
+    for (int cc = 0; cc < pieces; cc += 32) {
+      uint64_t v[2][kRows][2];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) __builtin_memcpy(v[0][j], scale_src(j) + min(16 * (cc + c0), nb - 16), 16);
+      if (cc + 16 < pieces) {
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) __builtin_memcpy(v[1][j], scale_src(j) + min(16 * (cc + 16 + c0), nb - 16), 16);
+      }
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) store_piece(j, cc + c0, v[0][j][0], v[0][j][1]);
+      if (cc + 16 < pieces) {
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) store_piece(j, cc + 16 + c0, v[1][j][0], v[1][j][1]);
+      }
+    }
+  } else {
+    for (int j = 0; j < kRows; ++j)
+      for (int c = c0; c < pieces * 16; c += 16) (scw + (16 * j + row) * sp)[c] = c < nb ? (char)scale_src(j)[c] : 0;
+  }
   if constexpr (FUSE) {
     // (codes past K stay as they were: the weights beside them are zeros; scales past K are written 0)
     const int K8 = p.K / 8;
-    for (int m = 0; m < rows_a; ++m)
+    for (int m = 0; m < rows_a; ++m) {
       for (int c = tid; c < K8; c += 256) {
         float v[8];
         if (vec) load8<DT, true>(x, (m0 + m) * ldx + 8 * c, v);
@@ -327,8 +361,8 @@ __global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* 
         *(uint32_t*)(fused + m * fp + 4 * c) = quantize8_mxfp4(v, sc);
         if ((c & 3) == 0) sca[m * sp + (c >> 2)] = (char)sc;
       }
-    for (int i = tid; i < rows_a * 16; i += 256)
-      if (nb + (i & 15) < (nb + 15) / 16 * 16) sca[(i >> 4) * sp + nb + (i & 15)] = 0;
+      if (nb + tid < 16 * pieces) sca[m * sp + nb + tid] = 0;
+    }
   }
 
   // wave w multiplies weight group w % NG with row tiles w / NG (and, NG * MT > 4, the next ones)
@@ -343,36 +377,74 @@ __global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* 
     // (rows past the end: whatever lies there, their results are not stored)
     const int ar = FUSE ? min(r, rows_a - 1) : 16 * (mt + m) + r;
     ars[m] = sca + ar * sp;
-    arc[m] = FUSE ? fused + ar * fp : smem + C::kStageW + ar * 256;
+    arc[m] = FUSE ? fused + ar * fp : smem + C::kPartW + ar * 256;
   }
   const char* wrs = scw + (16 * g + r) * sp;
-  for (int kt = 0; kt < nk; ++kt) {
-    wait_vm<(RING - 2) * C::kPer>();
-    wait_lgkm0();
-    phase_barrier();
-    issue(kt + RING - 1);
-    if (multiplies) {
-      const int slot = (kt % RING) * C::kStage;
-      const char* base = smem + slot + (16 * g + r) * 256;
-      const v4u32 sw = *(const v4u32*)(wrs + 16 * kt);
-      v4u32 sa[MW];
-      v4i w[4], a[MW][4];
+  // a stage's fragments are read a stage ahead where the ring is deep enough (fp4_tile.h)
+  struct Frag {
+    v4u32 sw[KS], sa[KS][MW];
+    v4i w[KS][4], a[KS][MW][4];
+  };
+  auto read = [&](int kt, Frag& f) {
 #pragma unroll
-      for (int m = 0; m < MW; ++m) sa[m] = *(const v4u32*)(ars[m] + 16 * kt);
+    for (int u = 0; u < KS; ++u) {
+      const int slot = (kt % RING) * C::kStage + u * C::kPart, part = KS * kt + u;
+      const char* base = smem + slot + (16 * g + r) * 256;
+      f.sw[u] = *(const v4u32*)(wrs + 16 * part);
+#pragma unroll
+      for (int m = 0; m < MW; ++m) f.sa[u][m] = *(const v4u32*)(ars[m] + 16 * part);
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         const int c = 16 * ((4 * s + q) ^ r);
-        w[s] = *(const v4i*)(base + c);
+        f.w[u][s] = *(const v4i*)(base + c);
 #pragma unroll
         for (int m = 0; m < MW; ++m)
-          a[m][s] = FUSE ? *(const v4i*)(arc[m] + 256 * kt + 64 * s + 16 * q) : *(const v4i*)(arc[m] + slot + c);
+          f.a[u][m][s] = FUSE ? *(const v4i*)(arc[m] + 256 * part + 64 * s + 16 * q) : *(const v4i*)(arc[m] + slot + c);
       }
+    }
+  };
+  auto multiply = [&](const Frag& f) {
+#pragma unroll
+    for (int u = 0; u < KS; ++u)
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int m = 0; m < MW; ++m)
-          acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(w[s]), fp4_operand(a[m][s]), acc[m], 4, 4, 0,
-                                                                    (int)(sw[s] >> (8 * q)), 0, (int)(sa[m][s] >> (8 * q)));
+          acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(f.w[u][s]), fp4_operand(f.a[u][m][s]), acc[m],
+                                                                    4, 4, 0, (int)(f.sw[u][s] >> (8 * q)), 0,
+                                                                    (int)(f.sa[u][m][s] >> (8 * q)));
+  };
+  Frag f[2];
+  if constexpr (RING >= 4) {
+    wait_vm<(RING - 2) * C::kPer>();
+    wait_lgkm0();
+    phase_barrier();
+    if (multiplies) read(0, f[0]);
+    auto step = [&](int kt, Frag& now, Frag& next) {
+      wait_vm<(RING - 3) * C::kPer>();
+      phase_barrier();
+      issue(kt + RING - 1);
+      if (multiplies) {
+        if (kt + 1 < nk) read(kt + 1, next);
+        multiply(now);
+      }
+    };
+    int kt = 0;
+    for (; kt + 2 <= nk; kt += 2) {
+      step(kt, f[0], f[1]);
+      step(kt + 1, f[1], f[0]);
+    }
+    if (kt < nk) step(kt, f[0], f[1]);
+  } else {
+    for (int kt = 0; kt < nk; ++kt) {
+      wait_vm<(RING - 2) * C::kPer>();
+      wait_lgkm0();
+      phase_barrier();
+      issue(kt + RING - 1);
+      if (multiplies) {
+        read(kt, f[0]);
+        multiply(f[0]);
+      }
     }
   }
   wait_vm<0>();
@@ -455,6 +527,24 @@ __global__ __launch_bounds__(256) void fp4_prep_kernel(Fp4Prep p) {
                    p.swt + e * p.N * ((p.K + 127) / 128));
 }
 
+// Four outputs to consecutive places (8-byte, for binary32 16-byte aligned), rounded to the type; a NaN
+// to bf16 becomes 0x7FC0, off the common path (v0 + v1 + v2 + v3 is a NaN where one of them is).
+LSK_DEV void store_quad(char* o, int dtype, v4f v) {
+  if (dtype == LSK_F32) {
+    store16_split(o, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  } else if (dtype == LSK_BF16) {
+    const float s = (v[0] + v[1]) + (v[2] + v[3]);
+    uint2 u = make_uint2(pack_bf16x2_nonan(v[0], v[1]), pack_bf16x2_nonan(v[2], v[3]));
+    if (__builtin_amdgcn_ballot_w64(s != s)) u = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    *(uint2*)o = u;
+  } else {
+    uint2 u;
+    u.x = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[0]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[1]) << 16);
+    u.y = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[3]) << 16);
+    *(uint2*)o = u;
+  }
+}
+
 // A BM x BN tile: tiles walk kGroupM row tiles down a column of weight tiles inside each XCD's run
 // of them, so the row tiles that share a weight tile run together on one L2.
 template <int BM, int BN, int WM, int WN, int RING, int BKB, bool GROUPED>
@@ -464,24 +554,30 @@ __global__ __launch_bounds__(WM * WN * 64) void fp4_tile_kernel(Fp4Args p, const
   constexpr int kGroupM = 4;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int ntiles = (int)((p.N + BN - 1) / BN);
-  if constexpr (GROUPED) {  // (the grid holds the most tiles there can be: the ones there are go to every XCD)
-    mtiles = expert_tile_count(p.offs, p.E, (int)p.M, BM);
-    if (blockIdx.x >= mtiles * ntiles) return;
-  }
-  const int L = xcd_logical_id(blockIdx.x, (int)mtiles * ntiles);
-  const int first = L / (kGroupM * ntiles) * kGroupM;
-  const int gsize = (int)mtiles - first < kGroupM ? (int)mtiles - first : kGroupM;
-  const int in = L - first * ntiles;
-  const int n0 = in / gsize * BN;
-  int m0 = (first + in % gsize) * BM, m1 = (int)p.M;
+  // logical tile L: row tile mt, first weight row n0
+  int mt, n0;
+  auto place = [&](int L) {
+    const int first = L / (kGroupM * ntiles) * kGroupM;
+    const int gsize = (int)mtiles - first < kGroupM ? (int)mtiles - first : kGroupM;
+    const int in = L - first * ntiles;
+    mt = first + in % gsize;
+    n0 = in / gsize * BN;
+  };
   const int nst = (p.K + 127) / 128;
-  if constexpr (GROUPED) {
-    int e, f, l;
-    if (!expert_tile(p.offs, p.E, (int)p.M, BM, first + in % gsize, e, f, l)) return;
-    m0 = f, m1 = l;
+  int m0, m1;
+  if constexpr (GROUPED) {  // (the grid holds the most tiles there can be: the ones there are go to every XCD)
+    ExpertTiles tiles(p.offs, p.E, (int)p.M, BM);
+    mtiles = tiles.count();
+    if (blockIdx.x >= mtiles * ntiles) return;
+    place(xcd_logical_id(blockIdx.x, (int)mtiles * ntiles));
+    int e;
+    if (!tiles.find(mt, e, m0, m1)) return;
     p.w = (const uint8_t*)wave_uniform64(p.w_ptrs[e]);
     p.bias = p.b_ptrs ? (const float*)wave_uniform64(p.b_ptrs[e]) : nullptr;
     swt += (int64_t)e * nst * p.N;
+  } else {
+    place(xcd_logical_id(blockIdx.x, (int)mtiles * ntiles));
+    m0 = mt * BM, m1 = (int)p.M;
   }
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int rows_a = m1 - m0 < BM ? m1 - m0 : BM, rows_w = (int)p.N - n0 < BN ? (int)p.N - n0 : BN;
@@ -522,12 +618,16 @@ __global__ __launch_bounds__(WM * WN * 64) void fp4_tile_kernel(Fp4Args p, const
   const int wm = wave / C::kWN, wn = wave % C::kWN;
   float* strip = (float*)(smem + wave * 32 * C::kLdc * 4);
   constexpr int kLanes = C::WTN / 4, kRows = 64 / kLanes;  // lanes a row, rows an instruction
-  const int col = wn * C::WTN + lane % kLanes * 4;
+  const int col = wn * C::WTN + lane % kLanes * 4, size = p.out_dtype == LSK_F32 ? 4 : 2;
   float b[4] = {0, 0, 0, 0};
   if (p.bias)
 #pragma unroll
     for (int z = 0; z < 4; ++z)
       if (col + z < rows_w) b[z] = p.bias[n0 + col + z];
+  int row = wm * C::WTM + lane / kLanes;
+  const int64_t step = (int64_t)kRows * p.ldo * size;
+  char* o = (char*)p.out + ((int64_t)(m0 + row) * p.ldo + n0 + col) * size;
+  const bool whole = vec && col + 4 <= rows_w;
 #pragma unroll
   for (int i = 0; i < C::TM; ++i) {
 #pragma unroll
@@ -538,17 +638,17 @@ __global__ __launch_bounds__(WM * WN * 64) void fp4_tile_kernel(Fp4Args p, const
             v4f{acc[i][j][4 * h], acc[i][j][4 * h + 1], acc[i][j][4 * h + 2], acc[i][j][4 * h + 3]};
     // (a wave's own LDS operations run in order)
 #pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += kRows) {
-      const int r = r0 + lane / kLanes, row = wm * C::WTM + i * 32 + r;
-      v4f v = *(const v4f*)(strip + r * C::kLdc + lane % kLanes * 4);
+    for (int r0 = 0; r0 < 32; r0 += kRows, row += kRows, o += step) {
+      v4f v = *(const v4f*)(strip + (r0 + lane / kLanes) * C::kLdc + lane % kLanes * 4);
       if (row >= rows_a || col >= rows_w) continue;
-      float y[4];
+      if (p.bias)
 #pragma unroll
-      for (int z = 0; z < 4; ++z) y[z] = p.bias ? f32_add(v[z], b[z]) : v[z];
-      const int64_t o = (int64_t)(m0 + row) * p.ldo + n0 + col;
-      if (vec && col + 4 <= rows_w) store4_out(p.out, LSK_EPI_V21, p.out_dtype, o, y, zero4());
-      else
-        for (int z = 0; z < 4 && col + z < rows_w; ++z) store_out(p.out, p.out_dtype, o + z, y[z]);
+        for (int z = 0; z < 4; ++z) v[z] = f32_add(v[z], b[z]);
+      if (whole) {
+        store_quad(o, p.out_dtype, v);
+      } else {
+        for (int z = 0; z < 4 && col + z < rows_w; ++z) store_out(o, p.out_dtype, z, v[z]);
+      }
     }
   }
 }
@@ -633,12 +733,12 @@ static int fp4_tiles(Fp4Args p, const void* x, int x_dtype, int64_t ldx, uint8_t
   return fp4_tile_launch<64, 64, 2, 2, 4, 128>(p, r.sat, r.swt, s);
 }
 
-template <int NG, int MT, int RING, int DT>
+template <int NG, int MT, int KS, int RING, int DT>
 static int fp4_stream_launch(const Fp4Args& p, const void* x, int64_t ldx, hipStream_t s) {
   const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
   const int64_t blocks = tiles * ((p.N + 16 * NG - 1) / (16 * NG));
   LSK_REQUIRE(blocks <= 0x7fffffff, "mxfp4 product: grid too large");
-  const int64_t lds = fp4_stream_lds<NG, MT, RING, (DT >= 0)>(p.K, (int)(p.M < 16 ? p.M : 16));
+  const int64_t lds = fp4_stream_lds<NG, MT, KS, RING, (DT >= 0)>(p.K, (int)(p.M < 16 ? p.M : 16));
   LSK_REQUIRE(lds <= 160 * 1024, "mxfp4 product: K=%d too long for few rows", p.K);
   const int vec = x && (uintptr_t)x % 16 == 0 && (ldx * (DT == LSK_F32 ? 4 : 2)) % 16 == 0;
   auto run = [&](auto kern) {
@@ -649,24 +749,24 @@ static int fp4_stream_launch(const Fp4Args& p, const void* x, int64_t ldx, hipSt
     return check_launch("fp4_stream_kernel");
   };
   if constexpr (DT < 0) {
-    if (p.offs) return run(fp4_stream_kernel<NG, MT, RING, DT, true>);
+    if (p.offs) return run(fp4_stream_kernel<NG, MT, KS, RING, DT, true>);
   }
-  return run(fp4_stream_kernel<NG, MT, RING, DT, false>);
+  return run(fp4_stream_kernel<NG, MT, KS, RING, DT, false>);
 }
 
 // The launch shape by the number of 16-row weight groups over all row tiles: one group a block while
-// there are few (deep rings: nothing else hides the latency), else blocks of four with the shortest
-// ring, several of which share a CU.  (MI355X, us for NG x RING = 1 x 4, 2 x 3, 4 x 2 at M rows of N x K:
-// 24 of 4096 x 14336 15.5, 16.3, 24.3; 48 of 4608 x 3584 12.9, 11.8, 12.3; 8 of 28672 x 4096 16.9, 17.1,
-// 14.4; by expert, 4 rows of 5760 x 2880 14.2, 9.8, 10.9; 256 rows over 32 experts of 2880 x 2880 51.3,
-// 42.0, 36.4.)
+// there are few (long stages, a deep ring: nothing else hides the latency), else blocks of two, then of
+// four with the shortest ring, several of which share a CU.  (MI355X, kernel us for NG x KS x RING = 1 x 2
+// x 4, 2 x 1 x 3: 24 rows of 4096 x 14336 11.0, 12.4; 16 of 4096 x 7168 7.3, 8.1.  Calls, us, for 1 x 1 x 4, 2 x 1 x
+// 3, 4 x 1 x 2: 48 rows of 4608 x 3584 11.9, 10.2, 10.5; 8 of 28672 x 4096 16.8, 16.9, 14.0; by expert, 4 rows
+// of 5760 x 2880 13.9, 10.0, 10.4; 256 rows over 32 experts of 2880 x 2880 50, 41, 36.)
 template <int MT, int DT>
 static int fp4_stream_shape(const Fp4Args& p, const void* x, int64_t ldx, hipStream_t s) {
   const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
   const int64_t groups = tiles * ((p.N + 15) / 16);
-  if (groups <= 512) return fp4_stream_launch<1, MT, 4, DT>(p, x, ldx, s);
-  if (groups <= 1536) return fp4_stream_launch<2, MT, 3, DT>(p, x, ldx, s);
-  return fp4_stream_launch<4, MT, 2, DT>(p, x, ldx, s);
+  if (groups <= 512) return fp4_stream_launch<1, MT, 2, 4, DT>(p, x, ldx, s);
+  if (groups <= 1536) return fp4_stream_launch<2, MT, 1, 3, DT>(p, x, ldx, s);
+  return fp4_stream_launch<4, MT, 1, 2, DT>(p, x, ldx, s);
 }
 
 // Row tiles of 16 while that holds all rows (of an expert: twice the average, the skew of a routing).

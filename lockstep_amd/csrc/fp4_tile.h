@@ -116,47 +116,87 @@ LSK_DEV void fp4_mainloop(typename Fp4Cfg<BM, BN, WM, WN, RING, BKB>::Acc& acc, 
   for (int ks = 0; ks < 2 * C::kSub; ++ks) slot[ks] = 16 * ((2 * ks + kg) ^ sw);
 
   if constexpr (C::kThreads == 256) {
-    // Four waves, one barrier a stage: a wave's own loads of stage kt are complete when at most the RING
-    // - 2 younger stages are outstanding, every wave's at the barrier; the slot of stage kt - 1, which
-    // no wave reads any more, takes stage kt + RING - 1.  Past the last stage the loads read zeros, so
-    // the count of outstanding loads is the same to the end.
-#pragma unroll
-    for (int s = 0; s < RING - 1; ++s) issue(s, std::true_type{});
-    for (int kt = 0; kt < nk; ++kt) {
-      wait_vm<(RING - 2) * C::kPer>();
-      phase_barrier();
-      issue(kt + RING - 1, std::true_type{});
+    // Four waves, one barrier a stage.  RING > 2: a stage's fragments are read into registers a stage ahead,
+    // so that the LDS works under the matrix core's chain (200 rows of 3584 x 18944 on 64 x 64 tiles 28.4 ->
+    // 24.2 us on MI355X).  A wave's own loads of stage kt + 1 are complete when at most the RING - 3 younger
+    // stages are outstanding, every wave's at the barrier; the slot of stage kt - 1, whose fragments every
+    // wave has multiplied, takes stage kt + RING - 1.  RING 2 reads a stage when it multiplies it, and loads
+    // the next one meanwhile: with two or three blocks a CU the other blocks fill the gaps (777 rows of 4608
+    // x 3584 on 64 x 128 tiles 16.6 us, 18.4 with the longer ring).  Past the last stage the loads read
+    // zeros, so the count of outstanding loads is the same to the end.
+    struct Frag {
+      v4i a[2 * C::kSub][C::TM], b[2 * C::kSub][C::TN];
+      int xa[C::kSub][C::TM], xb[C::kSub][C::TN];
+    };
+    auto read = [&](int kt, Frag& f) {
       const char* base = smem + (kt % RING) * C::kStage;
 #pragma unroll
       for (int u = 0; u < C::kSub; ++u) {
-        int xa[C::TM], xb[C::TN];
 #pragma unroll
-        for (int i = 0; i < C::TM; ++i)
-          xa[i] = (int)(*(const uint32_t*)(base + sA + u * 4 * C::kThreads + i * 128) >> (8 * kg));
+        for (int i = 0; i < C::TM; ++i) f.xa[u][i] = *(const int*)(base + sA + u * 4 * C::kThreads + i * 128);
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j)
-          xb[j] = (int)(*(const uint32_t*)(base + sB + u * 4 * C::kThreads + j * 128) >> (8 * kg));
-        v4i fa[2][C::TM], fb[2][C::TN];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int i = 0; i < C::TM; ++i) fa[h][i] = *(const v4i*)(base + offA + i * 32 * BKB + slot[2 * u + h]);
-#pragma unroll
-          for (int j = 0; j < C::TN; ++j) fb[h][j] = *(const v4i*)(base + offB + j * 32 * BKB + slot[2 * u + h]);
-        }
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-          for (int j = 0; j < C::TN; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(fb[0][j]), fp4_operand(fa[0][i]),
-                                                                        acc[i][j], 4, 4, 0, xb[j], 0, xa[i]);
-#pragma unroll
-        for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-          for (int j = 0; j < C::TN; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(fb[1][j]), fp4_operand(fa[1][i]),
-                                                                        acc[i][j], 4, 4, 2, xb[j], 2, xa[i]);
+        for (int j = 0; j < C::TN; ++j) f.xb[u][j] = *(const int*)(base + sB + u * 4 * C::kThreads + j * 128);
       }
+#pragma unroll
+      for (int h = 0; h < 2 * C::kSub; ++h) {
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) f.a[h][i] = *(const v4i*)(base + offA + i * 32 * BKB + slot[h]);
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) f.b[h][j] = *(const v4i*)(base + offB + j * 32 * BKB + slot[h]);
+      }
+    };
+    auto multiply = [&](Frag& f) {
+#pragma unroll
+      for (int u = 0; u < C::kSub; ++u) {
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i) f.xa[u][i] = (int)((uint32_t)f.xa[u][i] >> (8 * kg));
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) f.xb[u][j] = (int)((uint32_t)f.xb[u][j] >> (8 * kg));
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(f.b[2 * u][j]), fp4_operand(f.a[2 * u][i]),
+                                                                        acc[i][j], 4, 4, 0, f.xb[u][j], 0, f.xa[u][i]);
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+          for (int j = 0; j < C::TN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(f.b[2 * u + 1][j]),
+                                                                        fp4_operand(f.a[2 * u + 1][i]), acc[i][j], 4, 4, 2,
+                                                                        f.xb[u][j], 2, f.xa[u][i]);
+      }
+    };
+    if constexpr (RING == 2) {
+      Frag f;
+      issue(0, std::true_type{});
+      for (int kt = 0; kt < nk; ++kt) {
+        wait_vm<0>();
+        phase_barrier();
+        issue(kt + 1, std::true_type{});
+        read(kt, f);
+        multiply(f);
+      }
+    } else {
+    Frag f[2];
+#pragma unroll
+    for (int s = 0; s < RING - 1; ++s) issue(s, std::true_type{});
+    wait_vm<(RING - 2) * C::kPer>();
+    phase_barrier();
+    read(0, f[0]);
+    auto step = [&](int kt, Frag& now, Frag& next) {
+      wait_vm<(RING - 3) * C::kPer>();
+      phase_barrier();
+      issue(kt + RING - 1, std::true_type{});
+      read(kt + 1, next);
+      multiply(now);
+    };
+    int kt = 0;
+    for (; kt + 2 <= nk; kt += 2) {
+      step(kt, f[0], f[1]);
+      step(kt + 1, f[1], f[0]);
+    }
+    if (kt < nk) step(kt, f[0], f[1]);
     }
     wait_vm<0>();
   } else {

@@ -4,14 +4,12 @@
 // prompt or output:
 //   l = fl32(l + bias[v]);  seen: l = l > 0 ? fl32(l / r) : fl32(l * r);
 //   l = fl32(l - fl32(f * n));  n > 0: l = fl32(l - p);  mask bit 0: l = -inf;  out = round(l)
-// A block owns a run of one row's tokens.  It counts the row's history into a table of that run in LDS
-// (the output count, and the top bit for the prompt; integer atomics, so the order of tokens changes
-// nothing), streams the run once with bias and mask, leaving the counted tokens as they came, and then
-// walks the history again: the first thread to take a token's count out of the table computes that
-// token from its logit and stores it.  So the penalties cost their few tokens, not every token, and
-// the stream is a copy at the rate of HBM.  Every block of a row reads the whole history, which stays
-// in the L2: runs are as long as the LDS of two blocks a CU allows, and shorter where there are too
-// few rows to fill the part with them.
+// A block owns a run of one row's tokens.  It requests its first logits, counts the row's history into
+// a table of that run in LDS meanwhile (the output count, and the top bit for the prompt; integer
+// atomics, so the order of tokens changes nothing), and then streams the run: a vector of tokens none
+// of which stands in the history, without bias and mask, is a copy.  Bound by HBM.  Every block of a
+// row reads the whole history, which stays in the L2: runs are as long as the LDS of two blocks a CU
+// allows, and shorter where there are too few rows to fill the part with them.
 #include <hip/hip_runtime.h>
 
 #include "lsk_common.h"
@@ -51,7 +49,6 @@ struct CountTable {
   LSK_DEV void mark_prompt(int i) { atomicOr(&w[word(i)], kPrompt << shift(i)); }
   LSK_DEV void count(int i) { atomicAdd(&w[word(i)], 1u << shift(i)); }
   LSK_DEV uint32_t at(int i) const { return (w[word(i)] >> shift(i)) & kAll; }
-  LSK_DEV uint32_t take(int i) { return (atomicAnd(&w[word(i)], ~(kAll << shift(i))) >> shift(i)) & kAll; }
 };
 
 // f(local token) for each token of a row's history that lies in the block's run [v0, v0 + n).
@@ -68,7 +65,7 @@ LSK_DEV void each_token(const void* tok, int wide, int64_t ld, int64_t L, const 
 }
 
 template <int DT, int BITS>
-__global__ __launch_bounds__(1024) void penalize_logits_kernel(PenaltyArgs p) {
+__global__ __launch_bounds__(1024, 8) void penalize_logits_kernel(PenaltyArgs p) {
   extern __shared__ __attribute__((aligned(16))) uint32_t smem[];
   constexpr int VEC = DT == LSK_F32 ? 4 : 8, SIZE = DT == LSK_F32 ? 4 : 2;
   const int tid = threadIdx.x, nt = blockDim.x, chunks = (int)((p.V + p.chunk - 1) / p.chunk);
@@ -86,71 +83,87 @@ __global__ __launch_bounds__(1024) void penalize_logits_kernel(PenaltyArgs p) {
   head = head < n ? head : n;
   const int pad = (VEC - head % VEC) % VEC;
   CountTable<BITS> table{smem};
-  auto prompt = [&](auto f) { each_token(p.prompt, p.p64, p.ldp, p.Lp, p.prompt_lens, p.pl64, b, v0, n, f); };
-  auto output = [&](auto f) { each_token(p.output, p.o64, p.ldo_tok, p.Lo, p.output_lens, p.ol64, b, v0, n, f); };
+
+  // a thread's first vectors, on their way while the history is counted
+  constexpr int kAhead = 5;
+  const int nvec = (n - head) / VEC;
+  v4u32 ahead[kAhead];
+#pragma unroll
+  for (int z = 0; z < kAhead; ++z)
+    if (tid + z * nt < nvec) ahead[z] = *(const v4u32*)(in + (int64_t)(head + (tid + z * nt) * VEC) * SIZE);
+
   if (counted) {
     const int words = ((n + pad) * BITS + 31) / 32;
     for (int i = tid; i < (words + 3) / 4; i += nt) ((uint4*)smem)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    prompt([&](int t) { table.mark_prompt(t + pad); });
-    output([&](int t) { table.count(t + pad); });
+    each_token(p.prompt, p.p64, p.ldp, p.Lp, p.prompt_lens, p.pl64, b, v0, n, [&](int t) { table.mark_prompt(t + pad); });
+    each_token(p.output, p.o64, p.ldo_tok, p.Lo, p.output_lens, p.ol64, b, v0, n, [&](int t) { table.count(t + pad); });
     __syncthreads();
   }
-
-  auto allowed = [&](int i) {
-    const int64_t v = v0 + i;
-    return !mask || ((mask[v >> 5] >> (v & 31)) & 1u);
+  const float rep = p.rep ? p.rep[b] : 1.0f, freq = p.freq ? p.freq[b] : 0.0f, pres = p.pres ? p.pres[b] : 0.0f;
+  // the penalties of a token with count word c != 0
+  auto penalized = [&](float l, uint32_t c) {
+    if (p.rep) l = l > 0.0f ? f32_div(l, rep) : f32_mul(l, rep);
+    const uint32_t k = c & (CountTable<BITS>::kPrompt - 1);
+    if (k) {
+      if (p.freq) l = l - f32_mul(freq, (float)k);
+      if (p.pres) l = l - pres;
+    }
+    return l;
   };
   auto one = [&](int i) {
     float l = load_as_f32(in, DT, i);
-    if (counted && table.at(i + pad)) {
-      if (in != out) store_out(out, DT, i, l);
-      return;
-    }
     if (bias) l = f32_add(l, bias[i]);
-    store_out(out, DT, i, allowed(i) ? l : -__builtin_inff());
+    const uint32_t c = counted ? table.at(i + pad) : 0;
+    if (c) l = penalized(l, c);
+    const int64_t v = v0 + i;
+    if (mask && !((mask[v >> 5] >> (v & 31)) & 1u)) l = -__builtin_inff();
+    store_out(out, DT, i, l);
   };
   for (int i = tid; i < head; i += nt) one(i);
-  const int nvec = (n - head) / VEC;
-  for (int g = tid; g < nvec; g += nt) {
+
+  auto vector = [&](int g, v4u32 raw) {
     const int i = head + g * VEC;
-    const v4u32 raw = *(const v4u32*)(in + (int64_t)i * SIZE);
-    uint32_t live = 0;  // a bit per counted token
+    uint32_t cw[VEC * BITS / 32] = {};
+    bool any = false;
     if (counted) {
       const uint4* c = (const uint4*)((const char*)smem + (int64_t)(i + pad) * (BITS / 8));
 #pragma unroll
       for (int q = 0; q < VEC * BITS / 128; ++q) {
         const uint4 u = c[q];
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          if constexpr (BITS == 32) {
-            live |= (w[z] ? 1u : 0u) << (4 * q + z);
-          } else {
-            live |= ((w[z] & 0xffffu) ? 1u : 0u) << (8 * q + 2 * z);
-            live |= ((w[z] >> 16) ? 1u : 0u) << (8 * q + 2 * z + 1);
-          }
-        }
+        cw[4 * q] = u.x, cw[4 * q + 1] = u.y, cw[4 * q + 2] = u.z, cw[4 * q + 3] = u.w;
+        any = any || (u.x | u.y | u.z | u.w);
+      }
+      if constexpr (VEC * BITS < 128) {
+        const uint2 u = *(const uint2*)c;
+        cw[0] = u.x, cw[1] = u.y;
+        any = u.x | u.y;
       }
     }
-    if (!bias && !mask) {  // nothing to do but copy
+    if (!any && !bias && !mask) {
       if (in != out) store16_split(out + (int64_t)i * SIZE, raw);
-      continue;
+      return;
     }
-    float l[VEC], s[VEC];
+    float l[VEC];
     const uint32_t rw[4] = {raw[0], raw[1], raw[2], raw[3]};
 #pragma unroll
     for (int z = 0; z < VEC; ++z) {
       if constexpr (DT == LSK_F32) l[z] = __uint_as_float(rw[z]);
       else if constexpr (DT == LSK_BF16) l[z] = bf16_to_f32((uint16_t)(rw[z / 2] >> (z % 2 * 16)));
       else l[z] = (float)__builtin_bit_cast(_Float16, (uint16_t)(rw[z / 2] >> (z % 2 * 16)));
-      s[z] = l[z];
     }
     if (bias) {
       float bv[VEC];
       __builtin_memcpy(bv, bias + i, VEC * 4);
 #pragma unroll
-      for (int z = 0; z < VEC; ++z) s[z] = f32_add(s[z], bv[z]);
+      for (int z = 0; z < VEC; ++z) l[z] = f32_add(l[z], bv[z]);
+    }
+    if (any) {
+#pragma unroll
+      for (int z = 0; z < VEC; ++z) {
+        const uint32_t c = BITS == 32 ? cw[z] : (cw[z * BITS / 32] >> (z * BITS % 32)) & 0xffffu;
+        if (c) l[z] = penalized(l[z], c);
+      }
     }
     if (mask) {
       const int64_t v = v0 + i;
@@ -158,46 +171,28 @@ __global__ __launch_bounds__(1024) void penalize_logits_kernel(PenaltyArgs p) {
       const uint32_t m = (uint32_t)(((hi << 32) | lo) >> (v & 31));  // (VEC bits at most: inside 64)
 #pragma unroll
       for (int z = 0; z < VEC; ++z)
-        if (!((m >> z) & 1u)) s[z] = -__builtin_inff();
+        if (!((m >> z) & 1u)) l[z] = -__builtin_inff();
     }
     uint32_t o[4];
-#pragma unroll
-    for (int z = 0; z < VEC; ++z)
-      if ((live >> z) & 1u) s[z] = l[z];
     if constexpr (DT == LSK_F32) {
 #pragma unroll
-      for (int z = 0; z < 4; ++z) o[z] = __float_as_uint(s[z]);
+      for (int z = 0; z < 4; ++z) o[z] = __float_as_uint(l[z]);
     } else if constexpr (DT == LSK_BF16) {
 #pragma unroll
-      for (int z = 0; z < 4; ++z) o[z] = pack_bf16x2(s[2 * z], s[2 * z + 1]);
+      for (int z = 0; z < 4; ++z) o[z] = pack_bf16x2(l[2 * z], l[2 * z + 1]);
     } else {
 #pragma unroll
       for (int z = 0; z < 4; ++z)
-        o[z] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)s[2 * z]) |
-               ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)s[2 * z + 1]) << 16);
+        o[z] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)l[2 * z]) |
+               ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)l[2 * z + 1]) << 16);
     }
     store16_split(out + (int64_t)i * SIZE, o[0], o[1], o[2], o[3]);
-  }
-  for (int i = head + nvec * VEC + tid; i < n; i += nt) one(i);
-  if (!counted) return;
-
-  __syncthreads();
-  const float rep = p.rep ? p.rep[b] : 1.0f, freq = p.freq ? p.freq[b] : 0.0f, pres = p.pres ? p.pres[b] : 0.0f;
-  auto penalize = [&](int i) {
-    const uint32_t c = table.take(i + pad);
-    if (!c) return;  // another thread has it
-    float l = load_as_f32(in, DT, i);
-    if (bias) l = f32_add(l, bias[i]);
-    if (p.rep) l = l > 0.0f ? f32_div(l, rep) : f32_mul(l, rep);
-    const uint32_t k = c & (CountTable<BITS>::kPrompt - 1);
-    if (k) {
-      if (p.freq) l = l - f32_mul(freq, (float)k);
-      if (p.pres) l = l - pres;
-    }
-    store_out(out, DT, i, allowed(i) ? l : -__builtin_inff());
   };
-  prompt(penalize);
-  output(penalize);
+#pragma unroll
+  for (int z = 0; z < kAhead; ++z)
+    if (tid + z * nt < nvec) vector(tid + z * nt, ahead[z]);
+  for (int g = tid + kAhead * nt; g < nvec; g += nt) vector(g, *(const v4u32*)(in + (int64_t)(head + g * VEC) * SIZE));
+  for (int i = head + nvec * VEC + tid; i < n; i += nt) one(i);
 }
 
 }  // namespace lsk
