@@ -95,17 +95,35 @@ LSK_DEV void quantize_run(const void* __restrict__ x, int64_t ldx, int64_t M, in
     uint32_t s;
     ((uint32_t*)packed)[i] = quantize8_mxfp4(v, s);
     if constexpr (TS) {
-      if ((K8 & 15) == 0) {  // 16 lanes hold the four bytes of a dword
-        uint32_t w = s << (2 * (c & 12));
-        w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x124, 0xf, 0xf, false);  // row_ror:4
-        w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x128, 0xf, 0xf, false);  // row_ror:8
-        if ((c & 15) == 0) ((uint32_t*)scale)[(int64_t)(c >> 4) * M + row] = w;
-      } else if ((c & 3) == 0) {
-        store_scale_t(scale, M, row, c >> 2, K8 >> 2, s);
-      }
+      if ((c & 3) == 0) store_scale_t(scale, M, row, c >> 2, K8 >> 2, s);
     } else if ((i & 3) == 0) {
       scale[i >> 2] = (uint8_t)s;
     }
+  }
+}
+
+// The same with transposed scales for K % 128 == 0: 16 rows by 512 values a block, 16 lanes a row, so that
+// a block stores 16 rows' dwords of a stage side by side (scattered over blocks, a line of 32 rows was
+// written in pieces from several XCDs).
+template <int DT, bool VEC>
+LSK_DEV void quantize_rows16(const void* __restrict__ x, int64_t ldx, int64_t M, int K, int64_t block,
+                             uint8_t* __restrict__ packed, uint32_t* __restrict__ sat) {
+  const int chunks = (K + 511) / 512, tid = threadIdx.x;
+  const int64_t rb = block / chunks, row = rb * 16 + (tid >> 4);
+  const int k0 = (int)(block - rb * chunks) * 512 + 8 * (tid & 15);
+  float v[4][8];
+#pragma unroll
+  for (int z = 0; z < 4; ++z)
+    if (row < M && k0 + 128 * z < K) load8<DT, VEC>(x, row * ldx + k0 + 128 * z, v[z]);
+#pragma unroll
+  for (int z = 0; z < 4; ++z) {
+    if (row >= M || k0 + 128 * z >= K) continue;  // (16 lanes alike)
+    uint32_t s;
+    *(uint32_t*)(packed + (row * K + k0 + 128 * z) / 2) = quantize8_mxfp4(v[z], s);
+    uint32_t w = s << (2 * (tid & 12));  // the four bytes of a dword, from 16 lanes
+    w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x124, 0xf, 0xf, false);  // row_ror:4
+    w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x128, 0xf, 0xf, false);  // row_ror:8
+    if ((tid & 15) == 0) sat[(int64_t)((k0 >> 7) + z) * M + row] = w;
   }
 }
 
@@ -468,33 +486,41 @@ __global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* 
 }
 
 // ---------------------------------------------------------------- tiles
-// Scales [rows, nb] bytes (row stride lds) to the transposed form, 8 dwords of a row a thread.
+// Scales [rows, nb] bytes (row stride lds) to the transposed form: 64 rows by 128 bytes a block, read in
+// whole lines (eight lanes a row), turned in LDS, stored 64 rows' dwords side by side.
+constexpr int kTurnPitch = 33;  // dwords
 LSK_DEV void transpose_scales(const uint8_t* __restrict__ s, int64_t lds, int64_t rows, int nb, int64_t block,
-                              uint32_t* __restrict__ t) {
-  const int64_t rblocks = (rows + 255) / 256;
-  const int64_t c = block / rblocks, r = (block - c * rblocks) * 256 + threadIdx.x;
-  if (r >= rows) return;
-  const uint8_t* p = s + r * lds + 32 * c;
-  uint32_t* o = t + 8 * c * rows + r;
-  const int left = nb - 32 * (int)c;
-  uint32_t w[8];
-  if (left >= 32) {
-    __builtin_memcpy(w, p, 32);
-  } else {  // a row's last blocks, zeros past them
+                              uint32_t* __restrict__ t, uint32_t* turn) {
+  const int64_t rblocks = (rows + 63) / 64, c = block / rblocks, r0 = (block - c * rblocks) * 64;
+  const int nst = (nb + 3) / 4, tid = threadIdx.x, at = (int)(128 * c) + 16 * (tid & 7);
 #pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      w[d] = 0;
-      if (4 * d + 4 <= left) __builtin_memcpy(&w[d], p + 4 * d, 4);
-      else
-        for (int z = 0; z < 3; ++z)
-          if (4 * d + z < left) w[d] |= (uint32_t)p[4 * d + z] << (8 * z);
+  for (int half = 0; half < 2; ++half) {
+    const int row = 32 * half + (tid >> 3);
+    const uint8_t* p = s + (r0 + row < rows ? r0 + row : rows - 1) * lds;
+    uint64_t v[2] = {0, 0};
+    if (at < nb) {
+      if (nb >= 16) {  // the last piece from the 16 bytes that end the row, shifted down
+        const int sh = 8 * max(at + 16 - nb, 0);
+        __builtin_memcpy(v, p + min(at, nb - 16), 16);
+        if (sh >= 64) v[0] = v[1] >> (sh - 64), v[1] = 0;
+        else if (sh > 0) v[0] = v[0] >> sh | v[1] << (64 - sh), v[1] >>= sh;
+      } else {
+        for (int z = 0; z < nb; ++z) (z < 8 ? v[0] : v[1]) |= (uint64_t)p[z] << (8 * (z & 7));
+      }
     }
+    uint32_t* d = turn + row * kTurnPitch + 4 * (tid & 7);
+    d[0] = (uint32_t)v[0], d[1] = (uint32_t)(v[0] >> 32), d[2] = (uint32_t)v[1], d[3] = (uint32_t)(v[1] >> 32);
   }
+  __syncthreads();
+  const int row = tid & 63;
+  if (r0 + row >= rows) return;
 #pragma unroll
-  for (int d = 0; d < 8; ++d)
-    if (4 * d < left) o[d * rows] = w[d];
+  for (int z = 0; z < 8; ++z) {
+    const int d = 4 * z + (tid >> 6);
+    if (32 * (int)c + d < nst) t[(32 * c + d) * rows + r0 + row] = turn[row * kTurnPitch + d];
+  }
 }
-inline int64_t transpose_blocks(int64_t rows, int64_t K) { return ((rows + 255) / 256) * ((K / 32 + 31) / 32); }
+inline int64_t transpose_blocks(int64_t rows, int64_t K) { return ((rows + 63) / 64) * ((K / 32 + 127) / 128); }
 
 // What the tiles need beside the codes, in one launch: the rows quantised with transposed scales (DT an
 // input type) or their scales transposed (DT < 0), and the weights' scales transposed, every expert's
@@ -515,16 +541,18 @@ struct Fp4Prep {
 };
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void fp4_prep_kernel(Fp4Prep p) {
+  __shared__ uint32_t turn[64 * kTurnPitch];
   if (blockIdx.x < p.ablocks) {
     if constexpr (DT >= 0)
-      quantize_run<DT, VEC, true>(p.x, p.ldx, p.M, p.total, p.K / 8, blockIdx.x, (int)p.ablocks, p.q, (uint8_t*)p.sat);
+      if (p.K % 128 == 0) quantize_rows16<DT, VEC>(p.x, p.ldx, p.M, p.K, blockIdx.x, p.q, p.sat);
+      else quantize_run<DT, VEC, true>(p.x, p.ldx, p.M, p.total, p.K / 8, blockIdx.x, (int)p.ablocks, p.q, (uint8_t*)p.sat);
     else
-      transpose_scales(p.sa, p.ldsa, p.M, p.K / 32, blockIdx.x, p.sat);
+      transpose_scales(p.sa, p.ldsa, p.M, p.K / 32, blockIdx.x, p.sat, turn);
     return;
   }
   const int64_t b = blockIdx.x - p.ablocks, e = b / p.wblocks;
   transpose_scales(p.ws_ptrs ? (const uint8_t*)p.ws_ptrs[e] : p.sw, p.ldsw, p.N, p.K / 32, b - e * p.wblocks,
-                   p.swt + e * p.N * ((p.K + 127) / 128));
+                   p.swt + e * p.N * ((p.K + 127) / 128), turn);
 }
 
 // Four outputs to consecutive places (8-byte, for binary32 16-byte aligned), rounded to the type; a NaN
@@ -705,6 +733,7 @@ static int fp4_tiles(Fp4Args p, const void* x, int x_dtype, int64_t ldx, uint8_t
   if (x) {
     r.x = x, r.ldx = ldx, r.total = p.M * (p.K / 8), r.q = q;
     r.ablocks = (r.total + 255) / 256 < 65536 ? (r.total + 255) / 256 : 65536;
+    if (p.K % 128 == 0) r.ablocks = (p.M + 15) / 16 * ((p.K + 511) / 512);
     p.a = q;
   } else {
     r.sa = p.sa, r.ldsa = p.ldsa, r.ablocks = transpose_blocks(p.M, p.K);
