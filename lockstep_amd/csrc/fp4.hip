@@ -557,19 +557,24 @@ __global__ __launch_bounds__(256) void fp4_prep_kernel(Fp4Prep p) {
 
 // Four outputs to consecutive places (8-byte, for binary32 16-byte aligned), rounded to the type; a NaN
 // to bf16 becomes 0x7FC0, off the common path (v0 + v1 + v2 + v3 is a NaN where one of them is).
+// Non-temporal: an output stays in no L2 past its launch, and within it leaves the L2 to the operands
+// (4096 rows of 28672 x 4096 321 -> 293 us on MI355X, 777 of 4608 x 3584 21.9 -> 20.6).
 LSK_DEV void store_quad(char* o, int dtype, v4f v) {
+  auto put = [&](char* at, uint32_t lo, uint32_t hi) {
+    __builtin_nontemporal_store((uint64_t)hi << 32 | lo, (uint64_t*)at);
+  };
   if (dtype == LSK_F32) {
-    store16_split(o, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    put(o, __float_as_uint(v[0]), __float_as_uint(v[1]));
+    __asm__ volatile("" ::: "memory");  // (no 16-byte stores: store16_split)
+    put(o + 8, __float_as_uint(v[2]), __float_as_uint(v[3]));
   } else if (dtype == LSK_BF16) {
     const float s = (v[0] + v[1]) + (v[2] + v[3]);
-    uint2 u = make_uint2(pack_bf16x2_nonan(v[0], v[1]), pack_bf16x2_nonan(v[2], v[3]));
-    if (__builtin_amdgcn_ballot_w64(s != s)) u = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-    *(uint2*)o = u;
+    uint32_t lo = pack_bf16x2_nonan(v[0], v[1]), hi = pack_bf16x2_nonan(v[2], v[3]);
+    if (__builtin_amdgcn_ballot_w64(s != s)) lo = pack_bf16x2(v[0], v[1]), hi = pack_bf16x2(v[2], v[3]);
+    put(o, lo, hi);
   } else {
-    uint2 u;
-    u.x = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[0]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[1]) << 16);
-    u.y = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[3]) << 16);
-    *(uint2*)o = u;
+    put(o, (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[0]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[1]) << 16),
+        (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[3]) << 16));
   }
 }
 

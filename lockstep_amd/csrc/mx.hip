@@ -776,31 +776,36 @@ __global__ __launch_bounds__(256) void dequant_mxfp4_kernel(const uint8_t* __res
   }
 }
 
-// The same values for K and block multiples of 8: eight a thread, one 4-byte load and whole 16-byte
-// stores side by side (28672 x 4096 to bf16 on MI355X: 205 us a byte a thread).  A code's value comes
-// exactly from the conversion instruction under a unit scale; the product with the block's power of
-// two is the same binary32 multiply.
+// The same values for K and block multiples of 4: four a thread and step, so that a wave's stores are whole
+// lines side by side, and those past the caches (28672 x 4096 to bf16 on MI355X: 205 us a byte a thread).
+// A code's value comes exactly from the conversion instruction under a unit scale; the product with the
+// block's power of two is the same binary32 multiply.
 template <int ODT>
-__global__ __launch_bounds__(256) void dequant_mxfp4_8_kernel(const uint32_t* __restrict__ packed,
+__global__ __launch_bounds__(256) void dequant_mxfp4_4_kernel(const uint16_t* __restrict__ packed,
                                                               const uint8_t* __restrict__ scale, int64_t total,
-                                                              int block8, void* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const uint32_t u = packed[i];
-    const int e = (int)scale[i / block8] - 127;
-    const float sc = e > 127 ? __builtin_inff() : pow2f(e);
-    const v2f_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 1);
-    const v2f_t c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, 3);
-    const float v[8] = {f32_mul(a[0], sc), f32_mul(a[1], sc), f32_mul(b[0], sc), f32_mul(b[1], sc),
-                        f32_mul(c[0], sc), f32_mul(c[1], sc), f32_mul(d[0], sc), f32_mul(d[1], sc)};
+                                                              int block4, void* __restrict__ out) {
+  constexpr int kStep = 4;
+  const int64_t i0 = (int64_t)blockIdx.x * (256 * kStep) + threadIdx.x;
+  uint32_t u[kStep];
+  int e[kStep];
+#pragma unroll
+  for (int z = 0; z < kStep; ++z) {
+    const int64_t i = min(i0 + 256 * z, total - 1);
+    u[z] = packed[i];
+    e[z] = (int)scale[(total >> 31) == 0 ? (int64_t)((uint32_t)i / (uint32_t)block4) : i / block4] - 127;
+  }
+#pragma unroll
+  for (int z = 0; z < kStep; ++z) {
+    if (i0 + 256 * z >= total) return;
+    const float sc = e[z] > 127 ? __builtin_inff() : pow2f(e[z]);
+    const v2f_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u[z], 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u[z], 1.0f, 1);
+    const float v[4] = {f32_mul(a[0], sc), f32_mul(a[1], sc), f32_mul(b[0], sc), f32_mul(b[1], sc)};
     if constexpr (ODT == LSK_BF16) {
-      store16_split((uint16_t*)out + 8 * i, pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                    pack_bf16x2(v[6], v[7]));
+      __builtin_nontemporal_store((uint64_t)pack_bf16x2(v[2], v[3]) << 32 | pack_bf16x2(v[0], v[1]),
+                                  (uint64_t*)out + i0 + 256 * z);
     } else {
-      store16_split((float*)out + 8 * i, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+      store16_split((float*)out + 4 * (i0 + 256 * z), __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
                     __float_as_uint(v[3]));
-      __asm__ volatile("" ::: "memory");  // (keeps the two from being fused across)
-      store16_split((float*)out + 8 * i + 4, __float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]),
-                    __float_as_uint(v[7]));
     }
   }
 }
@@ -1704,16 +1709,16 @@ extern "C" int lsk_dequant_mxfp4(const uint8_t* packed, const uint8_t* scale, in
   LSK_REQUIRE(out_dtype == LSK_BF16 || out_dtype == LSK_F32, "lsk_dequant_mxfp4: out_dtype must be bf16 or f32");
   if (rows == 0 || K == 0) return LSK_OK;
   LSK_REQUIRE(packed && scale && out, "lsk_dequant_mxfp4: null pointer");
-  if (K % 8 == 0 && block % 8 == 0 && (uintptr_t)packed % 4 == 0 && (uintptr_t)out % 8 == 0) {
-    const int64_t total = rows * K / 8;
-    const dim3 grid(grid_for(total)), blk(256);
+  const int64_t total = rows * (K / 4), blocks = (total + 1023) / 1024;
+  if (K % 4 == 0 && block % 4 == 0 && (uintptr_t)packed % 2 == 0 && (uintptr_t)out % 8 == 0 && blocks <= 0x7fffffff) {
+    const dim3 grid((unsigned)blocks), blk(256);
     if (out_dtype == LSK_BF16)
-      hipLaunchKernelGGL(dequant_mxfp4_8_kernel<LSK_BF16>, grid, blk, 0, (hipStream_t)stream, (const uint32_t*)packed,
-                         scale, total, block / 8, out);
+      hipLaunchKernelGGL(dequant_mxfp4_4_kernel<LSK_BF16>, grid, blk, 0, (hipStream_t)stream, (const uint16_t*)packed,
+                         scale, total, block / 4, out);
     else
-      hipLaunchKernelGGL(dequant_mxfp4_8_kernel<LSK_F32>, grid, blk, 0, (hipStream_t)stream, (const uint32_t*)packed,
-                         scale, total, block / 8, out);
-    return lsk::check_launch("dequant_mxfp4_8_kernel");
+      hipLaunchKernelGGL(dequant_mxfp4_4_kernel<LSK_F32>, grid, blk, 0, (hipStream_t)stream, (const uint16_t*)packed,
+                         scale, total, block / 4, out);
+    return lsk::check_launch("dequant_mxfp4_4_kernel");
   }
   hipLaunchKernelGGL(dequant_mxfp4_kernel, dim3(grid_for(rows * K / 2)), dim3(256), 0, (hipStream_t)stream, packed, scale,
                      rows, K, block, out, out_dtype);
