@@ -316,7 +316,8 @@ __global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* 
       const bool in = k + kc < Kb;
 #pragma unroll
       for (int j = 0; j < NG; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_void_t)(base + u * C::kPart + j * 4096), 16, in && 16 * j + row < rows_w ? (uint32_t)((16 * j + row) * (int)p.ldw + kc) : kOob,
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_void_t)(base + u * C::kPart + j * 4096), 16,
+                                                 in && 16 * j + row < rows_w ? (uint32_t)((16 * j + row) * (int)p.ldw + kc) : kOob,
                                                  k, 0, 0);
       if constexpr (!FUSE) {
 #pragma unroll
@@ -439,6 +440,7 @@ __global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* 
     phase_barrier();
     if (multiplies) read(0, f[0]);
     auto step = [&](int kt, Frag& now, Frag& next) {
+      compiler_fence();  // (the reads of the stage before stay on their side of the barrier)
       wait_vm<(RING - 3) * C::kPer>();
       phase_barrier();
       issue(kt + RING - 1);

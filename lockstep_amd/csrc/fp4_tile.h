@@ -178,99 +178,100 @@ LSK_DEV void fp4_mainloop(typename Fp4Cfg<BM, BN, WM, WN, RING, BKB>::Acc& acc, 
         multiply(f);
       }
     } else {
-    Frag f[2];
+      Frag f[2];
 #pragma unroll
-    for (int s = 0; s < RING - 1; ++s) issue(s, std::true_type{});
-    wait_vm<(RING - 2) * C::kPer>();
-    phase_barrier();
-    read(0, f[0]);
-    auto step = [&](int kt, Frag& now, Frag& next) {
-      wait_vm<(RING - 3) * C::kPer>();
+      for (int s = 0; s < RING - 1; ++s) issue(s, std::true_type{});
+      wait_vm<(RING - 2) * C::kPer>();
       phase_barrier();
-      issue(kt + RING - 1, std::true_type{});
-      read(kt + 1, next);
-      multiply(now);
-    };
-    int kt = 0;
-    for (; kt + 2 <= nk; kt += 2) {
-      step(kt, f[0], f[1]);
-      step(kt + 1, f[1], f[0]);
-    }
-    if (kt < nk) step(kt, f[0], f[1]);
+      read(0, f[0]);
+      auto step = [&](int kt, Frag& now, Frag& next) {
+        compiler_fence();  // (the reads of the stage before stay on their side of the barrier)
+        wait_vm<(RING - 3) * C::kPer>();
+        phase_barrier();
+        issue(kt + RING - 1, std::true_type{});
+        read(kt + 1, next);
+        multiply(now);
+      };
+      int kt = 0;
+      for (; kt + 2 <= nk; kt += 2) {
+        step(kt, f[0], f[1]);
+        step(kt + 1, f[1], f[0]);
+      }
+      if (kt < nk) step(kt, f[0], f[1]);
     }
     wait_vm<0>();
   } else {
-  using Chk = std::true_type;
-  using NoChk = std::false_type;
-  using W0 = std::integral_constant<int, 0>;
-  auto step = [&](int kt, auto wait_n, bool do_issue, auto check) {
-    constexpr int kWait = decltype(wait_n)::value;
-    if (do_issue) issue(kt + C::kAhead, check);
-    const char* base = smem + (kt % C::kRing) * C::kStage;
-    v4i fa[2 * C::kSub][C::TM], fb[2 * C::kSub][C::TN];
-    int xa[C::kSub][C::TM], xb[C::kSub][C::TN];
+    using Chk = std::true_type;
+    using NoChk = std::false_type;
+    using W0 = std::integral_constant<int, 0>;
+    auto step = [&](int kt, auto wait_n, bool do_issue, auto check) {
+      constexpr int kWait = decltype(wait_n)::value;
+      if (do_issue) issue(kt + C::kAhead, check);
+      const char* base = smem + (kt % C::kRing) * C::kStage;
+      v4i fa[2 * C::kSub][C::TM], fb[2 * C::kSub][C::TN];
+      int xa[C::kSub][C::TM], xb[C::kSub][C::TN];
 #pragma unroll
-    for (int u = 0; u < C::kSub; ++u) {
+      for (int u = 0; u < C::kSub; ++u) {
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) xa[u][i] = *(const int*)(base + sA + u * 4 * C::kThreads + i * 128);
+        for (int i = 0; i < C::TM; ++i) xa[u][i] = *(const int*)(base + sA + u * 4 * C::kThreads + i * 128);
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j) xb[u][j] = *(const int*)(base + sB + u * 4 * C::kThreads + j * 128);
-    }
+        for (int j = 0; j < C::TN; ++j) xb[u][j] = *(const int*)(base + sB + u * 4 * C::kThreads + j * 128);
+      }
 #pragma unroll
-    for (int ks = 0; ks < 2 * C::kSub; ++ks) {
+      for (int ks = 0; ks < 2 * C::kSub; ++ks) {
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) fa[ks][i] = *(const v4i*)(base + offA + i * 32 * BKB + slot[ks]);
+        for (int i = 0; i < C::TM; ++i) fa[ks][i] = *(const v4i*)(base + offA + i * 32 * BKB + slot[ks]);
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j) fb[ks][j] = *(const v4i*)(base + offB + j * 32 * BKB + slot[ks]);
-    }
-    wait_vm<kWait>();
-    wait_lgkm0();
+        for (int j = 0; j < C::TN; ++j) fb[ks][j] = *(const v4i*)(base + offB + j * 32 * BKB + slot[ks]);
+      }
+      wait_vm<kWait>();
+      wait_lgkm0();
 #pragma unroll
-    for (int u = 0; u < C::kSub; ++u) {
+      for (int u = 0; u < C::kSub; ++u) {
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) xa[u][i] = (int)((uint32_t)xa[u][i] >> (8 * kg));
+        for (int i = 0; i < C::TM; ++i) xa[u][i] = (int)((uint32_t)xa[u][i] >> (8 * kg));
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j) xb[u][j] = (int)((uint32_t)xb[u][j] >> (8 * kg));
-    }
-    phase_barrier();
+        for (int j = 0; j < C::TN; ++j) xb[u][j] = (int)((uint32_t)xb[u][j] >> (8 * kg));
+      }
+      phase_barrier();
 #pragma unroll
-    for (int u = 0; u < C::kSub; ++u) {
+      for (int u = 0; u < C::kSub; ++u) {
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i)
+        for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(fb[2 * u][j]), fp4_operand(fa[2 * u][i]),
-                                                                      acc[i][j], 4, 4, 0, xb[u][j], 0, xa[u][i]);
+          for (int j = 0; j < C::TN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(fb[2 * u][j]), fp4_operand(fa[2 * u][i]),
+                                                                        acc[i][j], 4, 4, 0, xb[u][j], 0, xa[u][i]);
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i)
+        for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-        for (int j = 0; j < C::TN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-              fp4_operand(fb[2 * u + 1][j]), fp4_operand(fa[2 * u + 1][i]), acc[i][j], 4, 4, 2, xb[u][j], 2, xa[u][i]);
-    }
-    phase_barrier();
-  };
+          for (int j = 0; j < C::TN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                fp4_operand(fb[2 * u + 1][j]), fp4_operand(fa[2 * u + 1][i]), acc[i][j], 4, 4, 2, xb[u][j], 2, xa[u][i]);
+      }
+      phase_barrier();
+    };
 
 #pragma unroll
-  for (int s = 0; s < C::kAhead; ++s)
-    if (s < nk) issue(s, Chk{});
-  wait_vm<0>();
-  phase_barrier();
-  if (group == 1) phase_barrier();
-  if (nk >= C::kAhead) {
-    using WSteady = std::integral_constant<int, (C::kAhead - 1) * C::kPer>;
-    const int nfull = Kb / BKB;
-    int kt = 0;
-    for (; kt + C::kAhead < nfull; ++kt) step(kt, WSteady{}, true, NoChk{});
-    for (; kt + C::kAhead < nk; ++kt) step(kt, WSteady{}, true, Chk{});
-    step(kt, std::integral_constant<int, (C::kAhead - 2) * C::kPer>{}, false, NoChk{});
-    step(kt + 1, std::integral_constant<int, (C::kAhead >= 3 ? C::kAhead - 3 : 0) * C::kPer>{}, false, NoChk{});
-    if (C::kAhead >= 3) step(kt + 2, std::integral_constant<int, (C::kAhead >= 4 ? C::kAhead - 4 : 0) * C::kPer>{}, false, NoChk{});
-    if (C::kAhead >= 4) step(kt + 3, W0{}, false, NoChk{});
-  } else {
-    for (int kt = 0; kt < nk; ++kt) step(kt, W0{}, false, NoChk{});
-  }
-  if (group == 0) phase_barrier();
+    for (int s = 0; s < C::kAhead; ++s)
+      if (s < nk) issue(s, Chk{});
+    wait_vm<0>();
+    phase_barrier();
+    if (group == 1) phase_barrier();
+    if (nk >= C::kAhead) {
+      using WSteady = std::integral_constant<int, (C::kAhead - 1) * C::kPer>;
+      const int nfull = Kb / BKB;
+      int kt = 0;
+      for (; kt + C::kAhead < nfull; ++kt) step(kt, WSteady{}, true, NoChk{});
+      for (; kt + C::kAhead < nk; ++kt) step(kt, WSteady{}, true, Chk{});
+      step(kt, std::integral_constant<int, (C::kAhead - 2) * C::kPer>{}, false, NoChk{});
+      step(kt + 1, std::integral_constant<int, (C::kAhead >= 3 ? C::kAhead - 3 : 0) * C::kPer>{}, false, NoChk{});
+      if (C::kAhead >= 3) step(kt + 2, std::integral_constant<int, (C::kAhead >= 4 ? C::kAhead - 4 : 0) * C::kPer>{}, false, NoChk{});
+      if (C::kAhead >= 4) step(kt + 3, W0{}, false, NoChk{});
+    } else {
+      for (int kt = 0; kt < nk; ++kt) step(kt, W0{}, false, NoChk{});
+    }
+    if (group == 0) phase_barrier();
   }
 }
 

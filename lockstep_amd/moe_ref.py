@@ -498,6 +498,12 @@ class ExpertTablesMX:
         self.b13 = table(b13) if any(b13) else None
         self.b2 = table(b2) if any(b2) else None
         self._keep = keep
+        # what grouped_linear_mxfp4 reads beyond the fused layer's needs: every expert in the first one's
+        # shape, and codes 16-byte aligned
+        H, I = self.H, self.I
+        shapes = ((2 * I, H // 2), (H, I // 2), (2 * I, H // 32), (H, I // 32), (2 * I,), (H,))
+        self.grouped_mxfp4 = all(t is None or t.shape == s for ts in zip(*[iter(keep)] * 6) for t, s in zip(ts, shapes)) \
+            and H % 32 == 0 and I % 32 == 0 and all(p % 16 == 0 for p in p13 + p2)
         self._derived = _derived(pairs)
         # the codes' skinny-layout copies (lsk_mx_skinny_pack), which the skinny grouped MX GEMM
         # reads a kilobyte per wave load: made by make_skinny() on the first call that reads them,
@@ -614,6 +620,8 @@ def grouped_linear_mxfp4(tables, which: str, a, a_scale, offs, out_dtype=BF):
     if which not in ("w13", "w2"):
         raise ValueError("%s: which must be 'w13' or 'w2'" % what)
     L.require_cuda(a, a_scale, offs, tables.w13, what=what)
+    if not tables.grouped_mxfp4:
+        raise ValueError("%s: experts of one shape, H and I multiples of 32, with 16-byte aligned codes expected" % what)
     if offs.dtype != torch.int32 or offs.dim() != 1 or offs.numel() != tables.E + 1:
         raise ValueError("%s: offs must be int32 [E + 1] = [%d]" % (what, tables.E + 1))
     N, K = (2 * tables.I, tables.H) if which == "w13" else (tables.H, tables.I)

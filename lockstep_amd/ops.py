@@ -658,8 +658,8 @@ def dequant_mxfp4(packed: torch.Tensor, scale: torch.Tensor, out_dtype=torch.bfl
         raise AssertionError((tuple(scale.shape), tuple(packed.shape)))
     half = out_dtype == torch.bfloat16
     out = torch.empty((*lead, K), dtype=torch.bfloat16 if half else torch.float32, device=packed.device)
-    L.call("lsk_dequant_mxfp4", p2.data_ptr(), s2.data_ptr(), rows, K, int(block), out.data_ptr(),
-           L.LSK_BF16 if half else L.LSK_F32, L.stream_of(packed))
+    L.call_on(packed, "lsk_dequant_mxfp4", p2.data_ptr(), s2.data_ptr(), rows, K, int(block), out.data_ptr(),
+              L.LSK_BF16 if half else L.LSK_F32, L.stream_of(packed))
     return out if out.dtype == out_dtype else out.to(out_dtype)
 
 

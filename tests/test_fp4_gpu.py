@@ -141,6 +141,41 @@ def test_product_exact(M, N, K):
         assert np.array_equal(bits(_mm(ca, sa, cw, sw, bias, dt)), bits(want.to(dt))), dt
 
 
+@pytest.mark.parametrize("M,N,K", [(3, 8213, 96), (7, 25003, 64), (40, 4200, 160), (33, 13001, 96), (64, 6500, 1088),
+                                   (700, 4500, 96), (2050, 3500, 160), (3700, 3400, 288), (3600, 3600, 64)])
+def test_product_exact_over_many_columns(M, N, K):
+    """The same where there are enough blocks for the larger ones: of 32 and 64 columns for few rows, and
+    tiles of 64 x 128, 128 x 128 and 256 x 256."""
+    say("product many columns", M, N, K)
+    g = np.random.default_rng(M + N + K)
+    ca, sa = _operand(g, M, K, 1)
+    cw, sw = _operand(g, N, K, 1)
+    y, _ = U.product(ca, sa, cw, sw)
+    assert np.array_equal(_mm(ca, sa, cw, sw).double().cpu().numpy(), y)
+    bias = g.standard_normal(N).astype(np.float32)
+    want = torch.from_numpy(y.astype(np.float32) + bias)
+    assert np.array_equal(bits(_mm(ca, sa, cw, sw, bias, torch.bfloat16)), bits(want.to(torch.bfloat16)))
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 50, 24576), (4, 50, 24608), (2, 40, 32768), (20, 70, 32768), (3, 40, 32800),
+                                   (33, 100, 65600), (70, 30, 24608)])
+def test_long_rows(M, N, K):
+    """Around the lengths of K where few rows stop being quantised in the product's launch, and where they
+    go to the tiles."""
+    from lockstep_amd import moe_mxfp4 as X
+    say("long rows", M, N, K)
+    g = np.random.default_rng(M + N + K)
+    x = torch.from_numpy(g.standard_normal((M, K)).astype(np.float32)).to(torch.bfloat16)
+    cw, sw = _operand(g, N, K, 4)
+    ca, sa = U.quantize(x.double().numpy())
+    y, mag = U.product(ca, sa, cw, sw)
+    w, ws = to_dev(U.pack(cw)), to_dev(sw)
+    got = X.linear_mxfp4(x.to(dev()), w, ws, out_dtype=torch.float32)
+    assert (np.abs(got.double().cpu().numpy() - y) <= U.bound(y, mag, K, 2.0 ** -24)).all()
+    assert np.array_equal(bits(got), bits(_mm(ca, sa, cw, sw)))
+    assert np.array_equal(bits(got[:1]), bits(X.linear_mxfp4(x[:1].to(dev()), w, ws, out_dtype=torch.float32)))
+
+
 @pytest.mark.parametrize("M,N,K,out", [(1, 200, 3584, torch.bfloat16), (24, 129, 14336, torch.float32),
                                        (7, 64, 18944, torch.float16), (150, 300, 2880, torch.float32),
                                        (300, 513, 2048, torch.bfloat16), (64, 2000, 1056, torch.float32)])
@@ -165,6 +200,18 @@ def test_product_rows_do_not_depend_on_the_batch():
         full = bits(_mm(ca, sa, cw, sw))
         for lo, hi in ((0, 1), (3, 5), (7, 16), (100, 117), (30, 63), (5, 100), (590, 600), (10, 140), (0, 260), (99, 599)):
             assert np.array_equal(bits(_mm(ca[lo:hi], sa[lo:hi], cw, sw)), full[lo:hi]), (N, K, lo, hi)
+
+
+def test_product_rows_do_not_depend_on_a_large_batch():
+    """The same up to 256 x 256 tiles, and over every number of columns a block takes."""
+    g = np.random.default_rng(13)
+    M, N, K = 3600, 3600, 544
+    ca, sa = _operand(g, M, K, 6)
+    cw, sw = _operand(g, N, K, 6)
+    full = bits(_mm(ca, sa, cw, sw))
+    for lo, hi in ((0, 1), (17, 19), (300, 340), (3500, 3600), (1000, 1700), (900, 3000)):
+        assert np.array_equal(bits(_mm(ca[lo:hi], sa[lo:hi], cw, sw)), full[lo:hi]), (lo, hi)
+        assert np.array_equal(bits(_mm(ca[lo:hi], sa[lo:hi], cw[77:190], sw[77:190])), full[lo:hi, 77:190]), (lo, hi)
 
 
 def test_product_special_scales():
@@ -216,7 +263,7 @@ def test_product_empty_and_layouts():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("M,N,K", [(1, 100, 3584), (2, 130, 96), (4, 64, 2880), (9, 77, 448), (40, 300, 1024),
+@pytest.mark.parametrize("M,N,K", [(1, 100, 3584), (2, 130, 96), (4, 64, 2880), (3, 9001, 160), (1, 25001, 64), (9, 77, 448), (40, 300, 1024),
                                    (130, 260, 288), (300, 300, 512)])
 def test_linear_is_the_product_of_the_quantised_rows(M, N, K, dtype):
     from lockstep_amd import moe_mxfp4 as X
@@ -269,7 +316,9 @@ def _check_grouped(tables, host, which, R, offs, g, dt):
 @pytest.mark.parametrize("R,E,H,I,bias,dt", [(1, 3, 64, 32, True, torch.bfloat16), (4, 32, 160, 96, True, torch.bfloat16),
                                              (50, 6, 288, 64, False, torch.float32), (256, 32, 96, 160, True, torch.bfloat16),
                                              (700, 5, 128, 256, False, torch.float16), (1500, 70, 64, 96, True, torch.bfloat16),
-                                             (900, 2, 320, 544, True, torch.float32)])
+                                             (900, 2, 320, 544, True, torch.float32), (4000, 20, 96, 640, True, torch.bfloat16),
+                                             (800, 40, 96, 640, False, torch.bfloat16), (400, 130, 64, 1024, True, torch.float32),
+                                             (9000, 130, 32, 256, True, torch.float16)])
 def test_grouped(R, E, H, I, bias, dt):
     say("grouped", R, E, H, I, bias, dt)
     g = np.random.default_rng(R + E)
@@ -287,6 +336,31 @@ def test_grouped_bad_offsets():
     tables, host = _experts(g, 6, 96, 64, False)
     for offs in ([0, 100, 80, 300, 700, 650, 900], [-5, -2, 10, 10, 9, 400, 499], [500] * 7, [0] * 7, [7, 7, 8, 500, 500, 501, 2]):
         _check_grouped(tables, host, "w13", 500, offs, g, torch.float32)
+
+
+def test_grouped_some_biases_and_refused_experts():
+    from lockstep_amd import moe_ref as MR
+    g = np.random.default_rng(25)
+    ex, host = [], []
+    for e in range(3):
+        c13, s13 = _operand(g, 64, 96, 1)
+        c2, s2 = _operand(g, 96, 32, 1)
+        b = g.standard_normal(64).astype(np.float32) if e == 1 else None
+        host.append({"w13": (c13, s13, b)})
+        ex.append(((to_dev(U.pack(c13)), to_dev(s13)), (to_dev(U.pack(c2)), to_dev(s2)), None if b is None else to_dev(b), None))
+    tables = MR.ExpertTablesMX(ex, packed=True)
+    for R, offs in ((30, [0, 4, 20, 30]), (100, [0, 1, 60, 100])):
+        _check_grouped(tables, host, "w13", R, offs, g, torch.float32)
+    a, s, o = to_dev(np.zeros((2, 48), np.uint8)), to_dev(np.zeros((2, 3), np.uint8)), torch.zeros(4, dtype=torch.int32, device=dev())
+    moved = torch.zeros((64 * 48 + 1,), dtype=torch.uint8, device=dev())[1:].view(64, 48)
+    other = (to_dev(np.zeros((32, 48), np.uint8)), to_dev(np.zeros((32, 3), np.uint8)))
+    for bad in ((moved, ex[2][0][1]), other):
+        with pytest.raises(ValueError):
+            MR.grouped_linear_mxfp4(MR.ExpertTablesMX(ex[:2] + [(bad,) + ex[2][1:]], packed=True), "w13", a, s, o)
+    for args in ((tables, "w3", a, s, o), (tables, "w13", a, s, o[:3]), (tables, "w13", a, s, o.long()),
+                 (tables, "w2", a, s, o), (tables, "w13", a, s[:, :2], o)):
+        with pytest.raises(ValueError):
+            MR.grouped_linear_mxfp4(*args)
 
 
 def test_grouped_leaves_other_rows_alone():

@@ -58,6 +58,22 @@ def test_each_part_may_be_left_out(left):
     _check(l, {k: v for k, v in c.items() if k in left and k.replace("_lens", "") in left})   # (lengths need tokens)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_histories(dtype):
+    """Counts of 2^15 and more, and one token over the whole of a long output."""
+    g = np.random.default_rng(11)
+    for Lo in (32767, 32768, 70000):
+        l, c = _case(g, 2, 40003, 3, Lo, dtype)
+        c["output"][0] = 40002
+        c["output_lens"][0], c["prompt"][0], c["prompt_lens"][0] = Lo, 40002, 1
+        _check(l, c)
+
+
+def test_many_rows():
+    l, c = _case(np.random.default_rng(12), 1500, 2100, 5, 9, torch.bfloat16)
+    _check(l, c)
+
+
 def test_special_values():
     """Infinite and NaN logits, also in masked and penalised places, and a row whose mask allows nothing."""
     g = np.random.default_rng(8)
