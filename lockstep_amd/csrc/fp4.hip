@@ -255,7 +255,7 @@ inline int64_t expert_tiles_max(int64_t R, int64_t E, int64_t bm) { return R / b
 // bytes in flight: with a few thousand weight rows there is a block of 16 of them a CU, which is why
 // waves that do not multiply load.  K is not split over waves or blocks: a row's bits would depend on
 // the split.  The scales of the block's rows are copied into LDS whole at the start.
-// DT >= 0: the rows of x (at most four; vec: 16-byte aligned) are quantised by every block into LDS
+// DT >= 0: the rows of x (at most 16; vec: 16-byte aligned) are quantised by every block into LDS
 // itself, which saves a launch and the wait for it; x comes from the L2.
 template <int NG, int MT, int KS, bool FUSE>
 struct Fp4StreamCfg {
@@ -370,17 +370,42 @@ __global__ __launch_bounds__(256) void fp4_stream_kernel(Fp4Args p, const void* 
   }
   if constexpr (FUSE) {
     // (codes past K stay as they were: the weights beside them are zeros; scales past K are written 0)
-    const int K8 = p.K / 8;
-    for (int m = 0; m < rows_a; ++m) {
+    const int K8 = p.K / 8, all = rows_a * K8;
+    auto load = [&](int m, int c, float (&v)[8]) {
+      if (vec) load8<DT, true>(x, (m0 + m) * ldx + 8 * c, v);
+      else load8<DT, false>(x, (m0 + m) * ldx + 8 * c, v);
+    };
+    auto put = [&](int m, int c, const float (&v)[8]) {
+      uint32_t sc;
+      *(uint32_t*)(fused + m * fp + 4 * c) = quantize8_mxfp4(v, sc);
+      if ((c & 3) == 0) sca[m * sp + (c >> 2)] = (char)sc;
+    };
+    if (rows_a == 1) {
       for (int c = tid; c < K8; c += 256) {
         float v[8];
-        if (vec) load8<DT, true>(x, (m0 + m) * ldx + 8 * c, v);
-        else load8<DT, false>(x, (m0 + m) * ldx + 8 * c, v);
-        uint32_t sc;
-        *(uint32_t*)(fused + m * fp + 4 * c) = quantize8_mxfp4(v, sc);
-        if ((c & 3) == 0) sca[m * sp + (c >> 2)] = (char)sc;
+        load(0, c, v);
+        put(0, c, v);
       }
-      if (nb + tid < 16 * pieces) sca[m * sp + nb + tid] = 0;
+    } else {  // the rows end to end, kBatch loads of a thread in flight
+      constexpr int kBatch = 4;
+      for (int i0 = tid; i0 < all; i0 += 256 * kBatch) {
+        float v[kBatch][8];
+        int m[kBatch];
+#pragma unroll
+        for (int z = 0; z < kBatch; ++z) {
+          const int i = i0 + 256 * z;
+          m[z] = (int)((uint32_t)i / (uint32_t)K8);
+          if (i < all) load(m[z], i - m[z] * K8, v[z]);
+        }
+#pragma unroll
+        for (int z = 0; z < kBatch; ++z)
+          if (i0 + 256 * z < all) put(m[z], i0 + 256 * z - m[z] * K8, v[z]);  // (a quad of lanes alike)
+      }
+    }
+    const int past = 16 * pieces - nb;
+    for (int i = tid; i < rows_a * past; i += 256) {
+      const int m = (int)((uint32_t)i / (uint32_t)past);
+      sca[m * sp + nb + i - m * past] = 0;
     }
   }
 
@@ -811,9 +836,14 @@ static int fp4_stream(const Fp4Args& p, hipStream_t s) {
   return per <= 16 ? fp4_stream_shape<1, -1>(p, nullptr, 0, s) : fp4_stream_shape<2, -1>(p, nullptr, 0, s);
 }
 
-// Whether a linear's few rows are quantised in the product's launch (one row of 4608 x 3584 13.3 -> 9.3
-// us on MI355X): codes and scales that fit the LDS.
-static bool fp4_fuses(int64_t M, int64_t K) { return M <= 4 && K > 0 && K <= 24576; }
+// Whether a linear's few rows are quantised in the product's launch: one row whose codes fit the LDS beside
+// the ring, or up to 16 of few values together, since every block quantises them all.  (MI355X, GPU us in one
+// launch and in two, N = 4608: one row of 4096 5.2, 7.0, of 18944 11.7, 11.7 (N = 1024); 4 of 1024 4.6, 6.2,
+// of 4096 7.9, 7.1, of 8192 13.6, 9.0; 16 of 512 5.7, 6.4, of 1024 7.0, 6.3.  A launch less is 3 us of a
+// caller's time besides.)
+static bool fp4_fuses(int64_t M, int64_t K) {
+  return K > 0 && (M == 1 ? K <= 24576 : M <= 16 && M * K <= 16384);
+}
 
 static int fp4_stream_fused(const Fp4Args& p, const void* x, int x_dtype, int64_t ldx, hipStream_t s) {
   if (x_dtype == LSK_F32) return fp4_stream_shape<1, LSK_F32>(p, x, ldx, s);

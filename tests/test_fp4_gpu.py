@@ -263,7 +263,8 @@ def test_product_empty_and_layouts():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("M,N,K", [(1, 100, 3584), (2, 130, 96), (4, 64, 2880), (3, 9001, 160), (1, 25001, 64), (9, 77, 448), (40, 300, 1024),
+@pytest.mark.parametrize("M,N,K", [(1, 100, 3584), (2, 130, 96), (4, 64, 2880), (3, 9001, 160), (1, 25001, 64), (16, 333, 1024), (15, 90, 32),
+                                   (13, 20000, 96), (16, 9000, 160), (17, 100, 96), (9, 77, 448), (40, 300, 1024),
                                    (130, 260, 288), (300, 300, 512)])
 def test_linear_is_the_product_of_the_quantised_rows(M, N, K, dtype):
     from lockstep_amd import moe_mxfp4 as X

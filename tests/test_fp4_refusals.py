@@ -41,10 +41,10 @@ def test_product_refusals():
     _refused(gemm(M=1 << 32), b"31 bits")
     assert gemm(M=0, a=None, w=None, out=None) == 0
     assert gemm(N=0, ldo=0, a=None, w=None, out=None) == 0
-    need = lib.lsk_linear_mxfp4_workspace(5, 8, 64)
+    need = lib.lsk_linear_mxfp4_workspace(17, 8, 64)
     assert need > 0
-    _refused(lib.lsk_linear_mxfp4(P, L.LSK_F32, 64, 5, 64, P, P, 8, None, P, L.LSK_F32, 8, P, need - 1, None), b"workspace")
-    _refused(lib.lsk_linear_mxfp4(P, L.LSK_F32, 64, 5, 64, P, P, 8, None, P, L.LSK_F32, 8, P + 16, need, None), b"workspace")
+    _refused(lib.lsk_linear_mxfp4(P, L.LSK_F32, 64, 17, 64, P, P, 8, None, P, L.LSK_F32, 8, P, need - 1, None), b"workspace")
+    _refused(lib.lsk_linear_mxfp4(P, L.LSK_F32, 64, 17, 64, P, P, 8, None, P, L.LSK_F32, 8, P + 16, need, None), b"workspace")
     _refused(lib.lsk_linear_mxfp4(P, L.LSK_I32, 64, 5, 64, P, P, 8, None, P, L.LSK_F32, 8, P, need, None), b"x_dtype")
 
 
