@@ -752,6 +752,39 @@ static int64_t fp4_prep_bytes(int64_t M, int64_t N, int64_t K, int64_t E) {
   return up256(4 * nst * M) + up256(4 * nst * N * E);
 }
 
+// About how long a product takes on tiles of one size, in us: the CU with the most blocks, ceil(tiles / 256)
+// of them, works through them `blocks` at a time, a round of o blocks at once in round[o] + k[o] * K / 1000
+// (round[0]: the launches); every million outputs costs `out` and `area` * K / 1000, and every 10^9 weights
+// of experts (E > 0, whose last rows take half a tile each) `weights`.  Fitted to 368 products on MI355X (65
+// to 4096 rows, 512 to 28672 columns, K = 96 to 14336; 100 to 16384 rows over 4 to 128 experts).  The tile it
+// picks is 0.4 % slower than the best of the five on average and 17 % at most; thresholds on the number of
+// tiles were 5 % and 44 % (4096 rows of 4608 x 512 on 1.1 rounds of 256 x 256).
+struct Fp4TileCost {
+  int bm, bn, blocks;
+  double out, area, weights, round[4], k[4];
+};
+constexpr Fp4TileCost kFp4Tiles[5] = {
+    {256, 256, 1, 0.053, 0.16, 0, {4.9, 9.9}, {0, 4.9}},
+    {128, 256, 2, 0.11, 0.15, 21, {6.5, 4.5, 4.8}, {0, 4.1, 7.0}},
+    {128, 128, 2, 0.12, 0.15, 27, {6.5, 3.7, 4.2}, {0, 2.9, 3.4}},
+    {64, 128, 3, 0.13, 0.15, 50, {7.3, 0.88, 1.6, 2.4}, {0, 2.4, 2.6, 3.4}},
+    {64, 64, 2, 0.71, 0.11, 50, {6.6, 0.56, 0.99}, {0, 1.3, 1.7}},
+};
+static double fp4_tile_us(const Fp4TileCost& t, int64_t M, int64_t N, int64_t K, int64_t E) {
+  const int64_t down = E ? (M / t.bm + E / 2 > E ? M / t.bm + E / 2 : E) : (M + t.bm - 1) / t.bm;
+  const int64_t tiles = down * ((N + t.bn - 1) / t.bn), most = (tiles + 255) / 256;
+  const double kk = K * 1e-3, outs = tiles * 1e-6 * t.bm * t.bn;
+  const int o = t.blocks, rest = (int)(most % o);
+  return t.round[0] + outs * (t.out + t.area * kk) + E * N * kk * 1e-6 * t.weights +
+         (double)(most / o) * (t.round[o] + t.k[o] * kk) + (rest ? t.round[rest] + t.k[rest] * kk : 0);
+}
+static int fp4_cheapest_tile(int64_t M, int64_t N, int64_t K, int64_t E) {
+  int best = 0;
+  for (int c = 1; c < 5; ++c)
+    if (fp4_tile_us(kFp4Tiles[c], M, N, K, E) < fp4_tile_us(kFp4Tiles[best], M, N, K, E)) best = c;
+  return best;
+}
+
 // The tiles' products: p.a / p.sa the rows (x null), or x to be quantised into q first.
 static int fp4_tiles(Fp4Args p, const void* x, int x_dtype, int64_t ldx, uint8_t* q, char* work, hipStream_t s) {
   const int64_t nst = (p.K + 127) / 128, E = p.offs ? p.E : 1;
@@ -780,18 +813,13 @@ static int fp4_tiles(Fp4Args p, const void* x, int x_dtype, int64_t ldx, uint8_t
     hipLaunchKernelGGL((fp4_prep_kernel<-1, false>), grid, blk, 0, s, r);
   const int rc = check_launch("fp4_prep_kernel");
   if (rc) return rc;
-  // The tile by how many there are: 256 x 256 where they fill the part; 128 x 128, then 64 x 128 where
-  // there are enough for two blocks a CU, else 64 x 64; experts of many rows 128 x 256.  (MI355X, us:
-  // 4096 rows of 28672 x 4096 328 on 256 x 256, 371 on 128 x 128; 2048 of 4096 x 14336 110, 95; 777 of 4608 x
-  // 3584 24.7 on 128 x 128, 21.2 on 64 x 128, 26.2 on 64 x 64; 200 of 3584 x 18944 49 on 64 x 128, 37 on
-  // 64 x 64; 16384 rows over 128 experts of 1536 x 2048 96 on 128 x 256, 108 on 128 x 128, 104 on 64 x 128.)
-  const int64_t per = p.M / E;
-  const auto tiles = [&](int64_t bm, int64_t bn) { return ((per + bm - 1) / bm) * E * ((p.N + bn - 1) / bn); };
-  if (!p.offs && tiles(256, 256) >= 200) return fp4_tile_launch<256, 256, 2, 4, 4, 64>(p, r.sat, r.swt, s);
-  if (p.offs && per >= 64 && tiles(128, 256) >= 200) return fp4_tile_launch<128, 256, 2, 4, 3, 64>(p, r.sat, r.swt, s);
-  if (!p.offs && tiles(128, 128) >= 448) return fp4_tile_launch<128, 128, 2, 2, 2, 128>(p, r.sat, r.swt, s);
-  if (tiles(64, 128) >= 384) return fp4_tile_launch<64, 128, 2, 2, 2, 128>(p, r.sat, r.swt, s);
-  return fp4_tile_launch<64, 64, 2, 2, 4, 128>(p, r.sat, r.swt, s);
+  switch (fp4_cheapest_tile(p.M, p.N, p.K, p.offs ? E : 0)) {  // (all give the same bits)
+    case 0: return fp4_tile_launch<256, 256, 2, 4, 4, 64>(p, r.sat, r.swt, s);
+    case 1: return fp4_tile_launch<128, 256, 2, 4, 3, 64>(p, r.sat, r.swt, s);
+    case 2: return fp4_tile_launch<128, 128, 2, 2, 2, 128>(p, r.sat, r.swt, s);
+    case 3: return fp4_tile_launch<64, 128, 2, 2, 2, 128>(p, r.sat, r.swt, s);
+    default: return fp4_tile_launch<64, 64, 2, 2, 4, 128>(p, r.sat, r.swt, s);
+  }
 }
 
 template <int NG, int MT, int KS, int RING, int DT>
