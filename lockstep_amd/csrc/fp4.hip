@@ -730,13 +730,18 @@ static int fp4_tile_launch(const Fp4Args& p, const uint32_t* sat, const uint32_t
                 : run(fp4_tile_kernel<BM, BN, WM, WN, RING, BKB, false>);
 }
 
-// Whether the products of M rows (of E experts: E > 0) run on the tiles: past 64 rows (16 an expert), and
-// where a block's scales of all of K do not fit the LDS.  (MI355X, us on the streaming blocks and on
-// the tiles: 48 rows of 4608 x 3584 11.8, 12.4; 64 of 4096 x 14336 16.6, 25.3; by expert, 16 rows each of
-// 5760 x 2880 78, 88, 32 rows 102, 93.)
+// Whether the products of M rows (of E experts: E > 0) run on the tiles: where the streaming blocks would be
+// many, by groups of 16 columns of 32 rows, since each streams its weight rows again for its 32; and where a
+// block's scales of all of K do not fit the LDS.  (MI355X, GPU us of a linear on streaming blocks and on
+// tiles, groups: 64 rows of 8192 x 2048 8.9, 9.6 at 1024; 64 of 12000 x 2048 11.1, 10.2, 256 of 3584 x 14336 43,
+// 25 at 1500 - 1800; 128 of 3584 x 14336 19, 24 at 896; 24 of 28672 x 2048 11.0, 12.2 at 1792, 17 of 37888 x 2048
+// 17.6, 15.2 at 2368.  By expert: 192 rows over 4 of 4096 x 1024 7.7, 10.0 at 2560; 128 over 4 of 5760 x 2880 20,
+// 16 at 2880; 16 rows each over 32 of 5760 x 2880 69, 70, 24 each 80, 72.)
 constexpr int64_t kStreamK = 32768;
 static bool fp4_takes_tiles(int64_t M, int64_t N, int64_t K, int64_t E) {
-  return K > kStreamK || (K > 0 && (E ? M > 16 * E : M > 64));
+  if (K == 0 || K > kStreamK) return K > 0;
+  const int64_t groups = (E ? expert_tiles_max(M, E, 32) : (M + 31) / 32) * ((N + 15) / 16);
+  return E ? M > 16 * E && groups > 2560 : M > 16 && groups > (M <= 32 ? 2048 : 1024);
 }
 // The tiles address a tile's rows and the transposed scales with 31-bit offsets.
 static bool fp4_tiles_reach(int64_t M, int64_t N, int64_t K) {
@@ -845,16 +850,17 @@ static int fp4_stream_launch(const Fp4Args& p, const void* x, int64_t ldx, hipSt
 
 // The launch shape by the number of 16-row weight groups over all row tiles: one group a block while
 // there are few (long stages, a deep ring: nothing else hides the latency), else blocks of two, then of
-// four with the shortest ring, several of which share a CU.  (MI355X, kernel us for NG x KS x RING = 1 x 2
-// x 4, 2 x 1 x 3: 24 rows of 4096 x 14336 11.0, 12.4; 16 of 4096 x 7168 7.3, 8.1.  Calls, us, for 1 x 1 x 4, 2 x 1 x
-// 3, 4 x 1 x 2: 48 rows of 4608 x 3584 11.9, 10.2, 10.5; 8 of 28672 x 4096 16.8, 16.9, 14.0; by expert, 4 rows
-// of 5760 x 2880 13.9, 10.0, 10.4; 256 rows over 32 experts of 2880 x 2880 50, 41, 36.)
+// four with the shortest ring, several of which share a CU; sooner with two row tiles, whose blocks of one
+// group do not share a CU.  (MI355X, kernel us for NG x KS x RING = 1 x 2 x 4, 2 x 1 x 3: 24 rows of 4096 x 14336
+// 11.0, 12.4; 16 of 4096 x 7168 7.3, 8.1; calls 64 of 3584 x 2048 11.4, 8.3.  Calls for 1 x 1 x 4, 2 x 1 x 3, 4 x
+// 1 x 2: 8 of 28672 x 4096 16.8, 16.9, 14.0; by expert, 4 rows of 5760 x 2880 13.9, 10.0, 10.4; 256 rows over 32
+// experts of 2880 x 2880 50, 41, 36; 64 over 2 of 5760 x 2880 -, 12.6, 10.1.)
 template <int MT, int DT>
 static int fp4_stream_shape(const Fp4Args& p, const void* x, int64_t ldx, hipStream_t s) {
   const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
   const int64_t groups = tiles * ((p.N + 15) / 16);
-  if (groups <= 512) return fp4_stream_launch<1, MT, 2, 4, DT>(p, x, ldx, s);
-  if (groups <= 1536) return fp4_stream_launch<2, MT, 1, 3, DT>(p, x, ldx, s);
+  if (groups <= (MT == 1 ? 512 : 256)) return fp4_stream_launch<1, MT, 2, 4, DT>(p, x, ldx, s);
+  if (groups <= (MT == 1 ? 1536 : 1024)) return fp4_stream_launch<2, MT, 1, 3, DT>(p, x, ldx, s);
   return fp4_stream_launch<4, MT, 1, 2, DT>(p, x, ldx, s);
 }
 

@@ -121,7 +121,8 @@ def _mm(ca, sa, cw, sw, bias=None, out_dtype=torch.float32):
 
 SIZES = [(1, 1, 32), (1, 17, 64), (2, 48, 96), (5, 33, 128), (16, 16, 160), (17, 100, 224), (31, 64, 512), (33, 257, 288),
          (64, 130, 1024), (65, 129, 352), (100, 300, 640), (129, 255, 256), (200, 520, 480), (257, 260, 544),
-         (300, 1030, 128), (513, 512, 96)]
+         (300, 1030, 128), (513, 512, 96), (600, 900, 32), (65, 5500, 64), (1100, 480, 96), (129, 3301, 160), (600, 901, 224),
+         (600, 900, 288), (257, 1830, 352), (600, 907, 480), (1030, 515, 544), (2000, 280, 1056)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
@@ -218,9 +219,8 @@ def test_product_rows_do_not_depend_on_a_large_batch():
 def test_product_special_scales():
     """255 is a NaN for its row or column alone, also under zero codes; the largest scales overflow to
     infinity, the smallest reach zero or a subnormal; no neighbour changes."""
-    for M, K in ((5, 96), (40, 288), (200, 160)):
+    for M, K, N in ((5, 96, 70), (40, 288, 70), (200, 160, 70), (600, 160, 900), (3600, 96, 3600)):
         g = np.random.default_rng(M)
-        N = 70
         ca, sa = _operand(g, M, K, 1)
         cw, sw = _operand(g, N, K, 1)
         sa[2, 1], sw[33, 0] = 255, 255
@@ -266,7 +266,7 @@ def test_product_empty_and_layouts():
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("M,N,K", [(1, 100, 3584), (2, 130, 96), (4, 64, 2880), (3, 9001, 160), (1, 25001, 64), (16, 333, 1024), (15, 90, 32),
                                    (13, 20000, 96), (16, 9000, 160), (17, 100, 96), (9, 77, 448), (40, 300, 1024),
-                                   (130, 260, 288), (300, 300, 512)])
+                                   (130, 260, 288), (300, 300, 512), (600, 900, 288), (601, 900, 512), (65, 5500, 96)])
 def test_linear_is_the_product_of_the_quantised_rows(M, N, K, dtype):
     from lockstep_amd import moe_mxfp4 as X
     say("linear", M, N, K, dtype)
@@ -335,9 +335,10 @@ def test_grouped(R, E, H, I, bias, dt):
         _check_grouped(tables, host, which, R, offs, g, dt)
 
 
-def test_grouped_bad_offsets():
+@pytest.mark.parametrize("I", [64, 992])
+def test_grouped_bad_offsets(I):
     g = np.random.default_rng(21)
-    tables, host = _experts(g, 6, 96, 64, False)
+    tables, host = _experts(g, 6, 96, I, False)
     for offs in ([0, 100, 80, 300, 700, 650, 900], [-5, -2, 10, 10, 9, 400, 499], [500] * 7, [0] * 7, [7, 7, 8, 500, 500, 501, 2]):
         _check_grouped(tables, host, "w13", 500, offs, g, torch.float32)
 
@@ -367,29 +368,32 @@ def test_grouped_some_biases_and_refused_experts():
             MR.grouped_linear_mxfp4(*args)
 
 
-def test_grouped_leaves_other_rows_alone():
+@pytest.mark.parametrize("I", [64, 1024])
+def test_grouped_leaves_other_rows_alone(I):
     """Rows of no expert keep what the buffer held."""
     from lockstep_amd import _lib as L
     g = np.random.default_rng(22)
-    tables, host = _experts(g, 3, 64, 64, False)
+    tables, host = _experts(g, 3, 64, I, False)
+    N = 2 * I
     for R, offs in ((40, [3, 10, 10, 30]), (600, [5, 200, 300, 580])):
         ca, sa = _operand(g, R, 64, 1)
         a, s, o = to_dev(U.pack(ca)), to_dev(sa), to_dev(np.asarray(offs, np.int32))
-        out = torch.full((R, 128), 7.0, device=dev())
-        need = L.load().lsk_grouped_gemm_mxfp4_workspace(R, 3, 128, 64)
+        out = torch.full((R, N), 7.0, device=dev())
+        need = L.load().lsk_grouped_gemm_mxfp4_workspace(R, 3, N, 64)
         work = torch.empty((max(need, 1),), dtype=torch.uint8, device=dev())
         L.call("lsk_grouped_gemm_mxfp4", L.ptr(a), L.ptr(s), L.ptr(o), 3, R, L.ptr(tables.w13), tables.ldw13,
-               L.ptr(tables.ws13), tables.lds13, None, 128, 64, L.ptr(out), L.LSK_F32, 128, L.ptr(work), need,
+               L.ptr(tables.ws13), tables.lds13, None, N, 64, L.ptr(out), L.LSK_F32, N, L.ptr(work), need,
                L.stream_of(a))
         assert (out[:offs[0]] == 7).all() and (out[offs[3]:] == 7).all()
         y, _ = U.product(ca[offs[0]:offs[1]], sa[offs[0]:offs[1]], *host[0]["w13"][:2])
         assert np.array_equal(out[offs[0]:offs[1]].double().cpu().numpy(), y)
 
 
-def test_grouped_rows_are_the_dense_products():
+@pytest.mark.parametrize("I", [96, 736])
+def test_grouped_rows_are_the_dense_products(I):
     from lockstep_amd import moe_mxfp4 as X, moe_ref as MR
     g = np.random.default_rng(23)
-    E, H, I, R = 4, 2880, 96, 777
+    E, H, R = 4, 2880, 777
     tables, host = _experts(g, E, H, I, True)
     ca, sa = _operand(g, R, H, 7)
     offs = [0, 1, 40, 41, 777]
@@ -467,7 +471,7 @@ def test_other_streams():
     from lockstep_amd import moe_mxfp4 as X
     g = torch.Generator().manual_seed(1)
     w, ws = X.quantize_mxfp4(torch.randn((520, 1024), generator=g).to(dev()))
-    xs = [torch.randn((m, 1024), generator=g).to(dev()) for m in (1, 20, 300)]
+    xs = [torch.randn((m, 1024), generator=g).to(dev()) for m in (1, 20, 300, 1100)]
     want = [X.linear_mxfp4(x, w, ws) for x in xs]
     streams = [torch.cuda.Stream() for _ in xs]
     torch.cuda.synchronize()
@@ -480,11 +484,11 @@ def test_other_streams():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
-@pytest.mark.parametrize("M", [1, 12, 40, 300])
+@pytest.mark.parametrize("M", [1, 12, 40, 300, 1700])
 def test_captured_and_replayed(M):
     from lockstep_amd import moe_mxfp4 as X, moe_ref as MR, t16h_lmvariants as TH
     g = np.random.default_rng(41)
-    E, H, I = 5, 288, 64
+    E, H, I = 5, 288, 704
     tables, _ = _experts(g, E, H, I, True)
     w, ws = X.quantize_mxfp4(torch.from_numpy(g.standard_normal((330, H)).astype(np.float32)).to(dev()))
     x = torch.zeros((M, H), device=dev(), dtype=torch.bfloat16)
