@@ -173,10 +173,13 @@ def call(name: str, *args):
 def call_on(t: torch.Tensor, name: str, *args):
     """call() with t's device current: a launch goes to the current device, whose streams t's are not
     when t lives on another."""
-    if t.get_device() == torch._C._cuda_getDevice():
-        return call(name, *args)
-    with torch.cuda.device(t.device):
-        return call(name, *args)
+    if t.get_device() != torch._C._cuda_getDevice():
+        with torch.cuda.device(t.device):
+            return call(name, *args)
+    rc = getattr(_lib or load(), name)(*args)
+    if rc != 0:
+        raise LockstepError("%s failed (code %d): %s" % (name, rc, last_error()))
+    return rc
 
 
 def dtype_code(dt: torch.dtype) -> int:

@@ -632,10 +632,10 @@ def grouped_linear_mxfp4(tables, which: str, a, a_scale, offs, out_dtype=BF):
     w, ws, b = (tables.w13, tables.ws13, tables.b13) if which == "w13" else (tables.w2, tables.ws2, tables.b2)
     ldw, lds = (tables.ldw13, tables.lds13) if which == "w13" else (tables.ldw2, tables.lds2)
     offs = offs.contiguous()
-    out = torch.empty((R, N), dtype=out_dtype, device=a.device)
+    out = a.new_empty((R, N), dtype=out_dtype)
     if R:
         nbytes = L.load().lsk_grouped_gemm_mxfp4_workspace(R, tables.E, N, K)
-        work = torch.empty((nbytes,), dtype=torch.uint8, device=a.device) if nbytes else None
+        work = a.new_empty((nbytes,)) if nbytes else None
         L.call_on(a, "lsk_grouped_gemm_mxfp4", L.ptr(a), L.ptr(a_scale), L.ptr(offs), tables.E, R,
                   L.ptr(w), ldw, L.ptr(ws), lds, L.ptr(b), N, K, L.ptr(out), code, N, L.ptr(work), nbytes,
                   L.stream_of(a))

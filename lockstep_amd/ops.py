@@ -657,7 +657,7 @@ def dequant_mxfp4(packed: torch.Tensor, scale: torch.Tensor, out_dtype=torch.bfl
     if s2.numel() * block != rows * K:
         raise AssertionError((tuple(scale.shape), tuple(packed.shape)))
     half = out_dtype == torch.bfloat16
-    out = torch.empty((*lead, K), dtype=torch.bfloat16 if half else torch.float32, device=packed.device)
+    out = packed.new_empty((*lead, K), dtype=torch.bfloat16 if half else torch.float32)
     L.call_on(packed, "lsk_dequant_mxfp4", p2.data_ptr(), s2.data_ptr(), rows, K, int(block), out.data_ptr(),
               L.LSK_BF16 if half else L.LSK_F32, L.stream_of(packed))
     return out if out.dtype == out_dtype else out.to(out_dtype)
@@ -693,6 +693,8 @@ def _float_rows(x: torch.Tensor, what: str):
             raise ValueError("%s: x must be [..., K], got a scalar" % what)
         x = x.reshape(x.numel() // x.shape[-1], x.shape[-1]) if x.shape[-1] else x.new_empty((x.shape[:-1].numel(), 0))
     M, K = x.shape
+    if x.is_contiguous():
+        return x, code, M, K, K
     if K > 1 and x.stride(1) != 1 or M > 1 and x.stride(0) < K:
         x = x.contiguous()
     return x, code, M, K, x.stride(0) if M > 1 else K
@@ -706,8 +708,8 @@ def quantize_mxfp4(x: torch.Tensor):
     x, code, M, K, ld = _float_rows(x, "quantize_mxfp4")
     if K % 32:
         raise ValueError("quantize_mxfp4: K=%d not a multiple of 32" % K)
-    packed = torch.empty((*lead, K // 2), dtype=torch.uint8, device=x.device)
-    scale = torch.empty((*lead, K // 32), dtype=torch.uint8, device=x.device)
+    packed = x.new_empty((*lead, K // 2), dtype=torch.uint8)
+    scale = packed.new_empty((*lead, K // 32))
     if M and K:
         L.call_on(x, "lsk_quantize_mxfp4", x.data_ptr(), code, M, K, ld, packed.data_ptr(), scale.data_ptr(),
                   L.stream_of(x))
@@ -725,7 +727,7 @@ def _mxfp4_codes(packed: torch.Tensor, scale: torch.Tensor, what: str):
                          % (what, tuple(shape), tuple(scale.shape)))
     if not packed.is_contiguous() or packed.data_ptr() % 16:
         packed = packed.clone(memory_format=torch.contiguous_format)
-    return packed, scale.contiguous(), shape[0], shape[1] * 2
+    return packed, scale if scale.is_contiguous() else scale.contiguous(), shape[0], shape[1] * 2
 
 
 def _mxfp4_out(what: str, out_dtype):
@@ -755,10 +757,10 @@ def mm_mxfp4(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: t
         raise ValueError("mm_mxfp4: K mismatch %d vs %d" % (K, K2))
     code = _mxfp4_out("mm_mxfp4", out_dtype)
     bias = _mxfp4_bias(bias, N, "mm_mxfp4")
-    out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    out = a.new_empty((M, N), dtype=out_dtype)
     if M and N:
         nbytes = L.load().lsk_gemm_mxfp4_workspace(M, N, K)
-        work = torch.empty((nbytes,), dtype=torch.uint8, device=a.device) if nbytes else None
+        work = a.new_empty((nbytes,)) if nbytes else None
         L.call_on(a, "lsk_gemm_mxfp4", a.data_ptr(), a_scale.data_ptr(), M, K, w.data_ptr(), w_scale.data_ptr(), N,
                   L.ptr(bias), out.data_ptr(), code, N, L.ptr(work), nbytes, L.stream_of(a))
     return out
@@ -777,10 +779,10 @@ def linear_mxfp4(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=N
         raise ValueError("linear_mxfp4: rows of %d values for a weight of %d" % (Kx, K))
     code = _mxfp4_out("linear_mxfp4", out_dtype)
     bias = _mxfp4_bias(bias, N, "linear_mxfp4")
-    out = torch.empty((*lead, N), dtype=out_dtype, device=x.device)
+    out = x.new_empty((*lead, N), dtype=out_dtype)
     if M and N:
         nbytes = L.load().lsk_linear_mxfp4_workspace(M, N, K)
-        work = torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
+        work = w.new_empty((nbytes,)) if nbytes else None
         L.call_on(x, "lsk_linear_mxfp4", x.data_ptr(), xcode, ld, M, K, w.data_ptr(), w_scale.data_ptr(), N,
                   L.ptr(bias), out.data_ptr(), code, N, L.ptr(work), nbytes, L.stream_of(x))
     return out
@@ -869,7 +871,7 @@ def penalize_logits(logits: torch.Tensor, prompt=None, prompt_lens=None, output=
     if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
         logits = logits.contiguous()
     if out is None:
-        out = torch.empty((B, V), dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty((B, V))
     if B and V:
         L.call_on(logits, "lsk_penalize_logits", logits.data_ptr(), code, logits.stride(0), B, V, pp, ldp, Lp, plp, op,
                   ldt, Lo, olp, p64 | o64 << 1 | pl64 << 2 | ol64 << 3, L.ptr(repetition), L.ptr(frequency),

@@ -144,7 +144,7 @@ def test_product_exact(M, N, K):
 
 @pytest.mark.parametrize("M,N,K", [(3, 8213, 96), (7, 25003, 64), (40, 4200, 160), (33, 13001, 96), (64, 6500, 1088),
                                    (700, 4500, 96), (2050, 3500, 160), (3700, 3400, 288), (3600, 3600, 64),
-                                   (720, 8250, 96), (1760, 5800, 1472)])
+                                   (720, 8250, 96), (1760, 5800, 1472), (24, 20000, 96), (3000, 40, 1056), (9000, 16, 96)])
 def test_product_exact_over_many_columns(M, N, K):
     """The same where there are enough blocks for the larger ones: of 32 and 64 columns for few rows, and
     tiles of every size."""
@@ -321,7 +321,7 @@ def _check_grouped(tables, host, which, R, offs, g, dt):
                                              (900, 2, 320, 544, True, torch.float32), (4000, 20, 96, 640, True, torch.bfloat16),
                                              (800, 40, 96, 640, False, torch.bfloat16), (400, 130, 64, 1024, True, torch.float32),
                                              (9000, 130, 32, 256, True, torch.float16), (96, 4, 96, 2272, True, torch.bfloat16),
-                                             (512, 6, 96, 4448, False, torch.float32), (720, 8, 96, 4384, True, torch.bfloat16),
+                                             (512, 6, 96, 4448, False, torch.float32), (64, 32, 64, 1024, True, torch.bfloat16), (720, 8, 96, 4384, True, torch.bfloat16),
                                              (720, 8, 1696, 3680, True, torch.bfloat16)])
 def test_grouped(R, E, H, I, bias, dt):
     say("grouped", R, E, H, I, bias, dt)
