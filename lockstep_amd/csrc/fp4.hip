@@ -736,12 +736,20 @@ static int fp4_tile_launch(const Fp4Args& p, const uint32_t* sat, const uint32_t
 // tiles, groups: 64 rows of 8192 x 2048 8.9, 9.6 at 1024; 64 of 12000 x 2048 11.1, 10.2, 256 of 3584 x 14336 43,
 // 25 at 1500 - 1800; 128 of 3584 x 14336 19, 24 at 896; 24 of 28672 x 2048 11.0, 12.2 at 1792, 17 of 37888 x 2048
 // 17.6, 15.2 at 2368.  By expert: 192 rows over 4 of 4096 x 1024 7.7, 10.0 at 2560; 128 over 4 of 5760 x 2880 20,
-// 16 at 2880; 16 rows each over 32 of 5760 x 2880 69, 70, 24 each 80, 72.)
+// 16 at 2880; 16 rows each over 32 of 5760 x 2880 69, 70, 24 each 80, 72.)  The counts are what one round of
+// blocks takes with two of them a CU; a long K, whose scales leave the LDS room for one, halves them (64 rows
+// of 7000 x 18944 31.6 on streaming blocks, 28.7 on tiles).
 constexpr int64_t kStreamK = 32768;
+template <int NG, int MT, int KS, int RING, int DT>
+static int fp4_stream_per_cu(int64_t K, int rows) {  // blocks that a CU's LDS holds, counted to two
+  return 2 * fp4_stream_lds<NG, MT, KS, RING, (DT >= 0)>((int)K, rows) <= 160 * 1024 ? 2 : 1;
+}
 static bool fp4_takes_tiles(int64_t M, int64_t N, int64_t K, int64_t E) {
   if (K == 0 || K > kStreamK) return K > 0;
   const int64_t groups = (E ? expert_tiles_max(M, E, 32) : (M + 31) / 32) * ((N + 15) / 16);
-  return E ? M > 16 * E && groups > 2560 : M > 16 && groups > (M <= 32 ? 2048 : 1024);
+  const int64_t of4 = fp4_stream_per_cu<4, 2, 1, 2, -1>(K, 16), of2 = fp4_stream_per_cu<2, 2, 1, 3, -1>(K, 16);
+  if (E) return M > 16 * E && groups > 1280 * of4;
+  return M > 16 && groups > (M <= 32 ? 1024 * of4 : 512 * of2);
 }
 // The tiles address a tile's rows and the transposed scales with 31-bit offsets.
 static bool fp4_tiles_reach(int64_t M, int64_t N, int64_t K) {
@@ -850,8 +858,8 @@ static int fp4_stream_launch(const Fp4Args& p, const void* x, int64_t ldx, hipSt
 
 // The launch shape by the number of 16-row weight groups over all row tiles: one group a block while
 // there are few (long stages, a deep ring: nothing else hides the latency), else blocks of two, then of
-// four with the shortest ring, several of which share a CU; sooner with two row tiles, whose blocks of one
-// group do not share a CU.  (MI355X, kernel us for NG x KS x RING = 1 x 2 x 4, 2 x 1 x 3: 24 rows of 4096 x 14336
+// four with the shortest ring, several of which share a CU: each for one round of blocks, as many a CU as its
+// LDS holds.  (MI355X, kernel us for NG x KS x RING = 1 x 2 x 4, 2 x 1 x 3: 24 rows of 4096 x 14336
 // 11.0, 12.4; 16 of 4096 x 7168 7.3, 8.1; calls 64 of 3584 x 2048 11.4, 8.3.  Calls for 1 x 1 x 4, 2 x 1 x 3, 4 x
 // 1 x 2: 8 of 28672 x 4096 16.8, 16.9, 14.0; by expert, 4 rows of 5760 x 2880 13.9, 10.0, 10.4; 256 rows over 32
 // experts of 2880 x 2880 50, 41, 36; 64 over 2 of 5760 x 2880 -, 12.6, 10.1.)
@@ -859,8 +867,10 @@ template <int MT, int DT>
 static int fp4_stream_shape(const Fp4Args& p, const void* x, int64_t ldx, hipStream_t s) {
   const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
   const int64_t groups = tiles * ((p.N + 15) / 16);
-  if (groups <= (MT == 1 ? 512 : 256)) return fp4_stream_launch<1, MT, 2, 4, DT>(p, x, ldx, s);
-  if (groups <= (MT == 1 ? 1536 : 1024)) return fp4_stream_launch<2, MT, 1, 3, DT>(p, x, ldx, s);
+  const int rows = (int)(p.M < 16 ? p.M : 16);
+  if (groups <= 256 * fp4_stream_per_cu<1, MT, 2, 4, DT>(p.K, rows)) return fp4_stream_launch<1, MT, 2, 4, DT>(p, x, ldx, s);
+  if (groups <= (MT == 1 ? 1536 : 512 * fp4_stream_per_cu<2, 2, 1, 3, -1>(p.K, 16)))
+    return fp4_stream_launch<2, MT, 1, 3, DT>(p, x, ldx, s);
   return fp4_stream_launch<4, MT, 1, 2, DT>(p, x, ldx, s);
 }
 

@@ -193,6 +193,25 @@ def test_product_wide_scales(M, N, K, out):
     assert (np.abs(got - y) <= U.bound(y, mag, K, HALF[out])).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(24, 8400, 15200), (40, 4400, 15200), (16, 6000, 18944), (3, 9000, 5440)])
+def test_long_rows_over_many_columns(M, N, K):
+    """Long K over blocks of every number of columns: a column's bits are those of a product of its own."""
+    g = np.random.default_rng(M + N + K)
+    ca, sa = _operand(g, M, K, 5)
+    w = torch.from_numpy(g.integers(0, 256, (N, K // 2), dtype=np.uint8)).to(dev())
+    ws = torch.from_numpy(g.integers(120, 130, (N, K // 32), dtype=np.uint8)).to(dev())
+    from lockstep_amd import moe_mxfp4 as X
+    a, s = to_dev(U.pack(ca)), to_dev(sa)
+    full = bits(X.mm_mxfp4(a, s, w, ws))
+    for lo in (0, 1000, N - 33):
+        cols = slice(lo, lo + 33)
+        p = bits(w[cols])
+        y, mag = U.product(ca, sa, np.stack((p & 15, p >> 4), -1).reshape(33, K), bits(ws[cols]))
+        one = X.mm_mxfp4(a, s, w[cols], ws[cols])
+        assert np.array_equal(bits(one), full[:, cols])
+        assert (np.abs(one.double().cpu().numpy() - y) <= U.bound(y, mag, K, 2.0 ** -24)).all()
+
+
 def test_product_rows_do_not_depend_on_the_batch():
     """The bits of a row are the same alone, in every batch and at every place in it."""
     g = np.random.default_rng(11)
