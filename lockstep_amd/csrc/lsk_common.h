@@ -598,6 +598,9 @@ inline bool out_vec_ok(const void* out, int out_dtype, int64_t ldo) {
   return ((uintptr_t)out % (4 * esz) == 0) && ((ldo * esz) % (4 * esz) == 0);
 }
 
+// Whether HIP can launch that many blocks: fewer than 2^32 threads along a grid's dimension.
+inline bool grid_ok(int64_t blocks, int threads) { return blocks <= 0xffffffffLL / threads; }
+
 // Thread-local last-error string shared by every entry point.
 namespace lsk {
 void set_error(const char* fmt, ...);

@@ -776,10 +776,11 @@ __global__ __launch_bounds__(256) void dequant_mxfp4_kernel(const uint8_t* __res
   }
 }
 
-// The same values for K and block multiples of 4: four a thread and step, so that a wave's stores are whole
-// lines side by side, and those past the caches (28672 x 4096 to bf16 on MI355X: 205 us a byte a thread).
-// A code's value comes exactly from the conversion instruction under a unit scale; the product with the
-// block's power of two is the same binary32 multiply.
+// The same values for K and block multiples of 4, while one launch holds a thread for every 16 of them (2^36
+// values): four a thread and step, so that a wave's stores are whole lines side by side, and those past the
+// caches (28672 x 4096 to bf16 on MI355X: 205 us a byte a thread).  A code's value comes exactly from the
+// conversion instruction under a unit scale; the product with the block's power of two is the same binary32
+// multiply.
 template <int ODT>
 __global__ __launch_bounds__(256) void dequant_mxfp4_4_kernel(const uint16_t* __restrict__ packed,
                                                               const uint8_t* __restrict__ scale, int64_t total,
@@ -1710,7 +1711,7 @@ extern "C" int lsk_dequant_mxfp4(const uint8_t* packed, const uint8_t* scale, in
   if (rows == 0 || K == 0) return LSK_OK;
   LSK_REQUIRE(packed && scale && out, "lsk_dequant_mxfp4: null pointer");
   const int64_t total = rows * (K / 4), blocks = (total + 1023) / 1024;
-  if (K % 4 == 0 && block % 4 == 0 && (uintptr_t)packed % 2 == 0 && (uintptr_t)out % 8 == 0 && blocks <= 0x7fffffff) {
+  if (K % 4 == 0 && block % 4 == 0 && (uintptr_t)packed % 2 == 0 && (uintptr_t)out % 8 == 0 && grid_ok(blocks, 256)) {
     const dim3 grid((unsigned)blocks), blk(256);
     if (out_dtype == LSK_BF16)
       hipLaunchKernelGGL(dequant_mxfp4_4_kernel<LSK_BF16>, grid, blk, 0, (hipStream_t)stream, (const uint16_t*)packed,

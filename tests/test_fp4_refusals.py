@@ -97,3 +97,15 @@ def test_head_variant_names():
     assert t16h_lmvariants.build("mxfp4").gemms() == 0 and t16h_lmvariants.build("mxfp4").nbytes() == 0
     with pytest.raises(ValueError):
         t16h_lmvariants.build("mxfp6")
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: only where no launch can start")
+def test_dequant_beyond_one_grid():
+    """The quad kernel takes a launch of fewer than 2^32 threads (2^36 values); a larger tensor goes to the
+    kernel that strides over its grid.  Without a GPU each says which one it tried to launch."""
+    lib = L.load()
+    for rows, kernel in ((1, b"dequant_mxfp4_4_kernel:"), ((1 << 30) - 64, b"dequant_mxfp4_4_kernel:"),
+                         ((1 << 30), b"dequant_mxfp4_kernel:"), ((1 << 34), b"dequant_mxfp4_kernel:")):
+        for odt in (L.LSK_BF16, L.LSK_F32):
+            assert lib.lsk_dequant_mxfp4(P, P, rows, 64, 32, P, odt, None) == 2
+            assert kernel in lib.lsk_last_error(), (rows, lib.lsk_last_error())
