@@ -704,7 +704,8 @@ int lsk_quantize_mxfp4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t
  * E8M0 bytes, all contiguous, the codes 16-byte aligned; K % 32 == 0 (K = 0: the bias alone); bias [N] or
  * NULL; out [M, N] (row stride ldo).  A row's results are the same bits whatever the other rows are and
  * however many, and on every launch.  workspace: lsk_gemm_mxfp4_workspace(M, N, K) bytes, 256-byte
- * aligned (none needed when that is 0). */
+ * aligned (none needed when that is 0).  Products whose blocks one launch does not hold (2^32 threads)
+ * are refused. */
 int64_t lsk_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K);
 int lsk_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, int64_t M, int64_t K, const uint8_t* w,
                    const uint8_t* w_scale, int64_t N, const float* bias, void* out, int out_dtype, int64_t ldo,
@@ -745,7 +746,8 @@ int lsk_grouped_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, const int32
  * hold int64 (int32 where the bit is 0).  repetition, frequency, presence: f32 [B] or NULL (left out).
  * bias: f32, row b at bias + b * ldb (ldb 0: one row for all), or NULL.  mask: row b at mask + b * ldm
  * (words; ldm 0: one for all), bit v % 32 of word v / 32 allows v, ceil(V / 32) words, or NULL.  out
- * [B, V] (row stride ldo) may be logits itself. */
+ * [B, V] (row stride ldo) may be logits itself.  At most 2^24 - 1 rows, fewer of more than 8160 tokens (one
+ * launch holds 2^32 threads). */
 int lsk_penalize_logits(const void* logits, int dtype, int64_t ldl, int64_t B, int64_t V, const void* prompt, int64_t ldp,
                         int64_t Lp, const void* prompt_lens, const void* output, int64_t ldo_tok, int64_t Lo,
                         const void* output_lens, int wide, const float* repetition, const float* frequency,

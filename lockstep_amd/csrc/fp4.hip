@@ -713,12 +713,15 @@ __global__ __launch_bounds__(WM * WN * 64) void fp4_tile_kernel(Fp4Args p, const
   }
 }
 
+static int64_t fp4_row_tiles(const Fp4Args& p, int bm) {
+  return p.offs ? expert_tiles_max(p.M, p.E, bm) : (p.M + bm - 1) / bm;
+}
+
+// (fp4_tiles has checked the grid)
 template <int BM, int BN, int WM, int WN, int RING, int BKB>
 static int fp4_tile_launch(const Fp4Args& p, const uint32_t* sat, const uint32_t* swt, hipStream_t s) {
   using C = Fp4Cfg<BM, BN, WM, WN, RING, BKB>;
-  const int64_t mtiles = p.offs ? expert_tiles_max(p.M, p.E, BM) : (p.M + BM - 1) / BM;
-  const int64_t blocks = mtiles * ((p.N + BN - 1) / BN);
-  LSK_REQUIRE(blocks <= 0x7fffffff, "mxfp4 product: grid too large");
+  const int64_t mtiles = fp4_row_tiles(p, BM), blocks = mtiles * ((p.N + BN - 1) / BN);
   const int vec = out_vec_ok(p.out, p.out_dtype, p.ldo);
   auto run = [&](auto kern) {
     if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes) != hipSuccess)
@@ -816,7 +819,11 @@ static int fp4_tiles(Fp4Args p, const void* x, int x_dtype, int64_t ldx, uint8_t
   } else {
     r.sa = p.sa, r.ldsa = p.ldsa, r.ablocks = transpose_blocks(p.M, p.K);
   }
-  LSK_REQUIRE(r.ablocks + r.wblocks * E <= 0x7fffffff, "mxfp4 product: grid too large");
+  const int tile = fp4_cheapest_tile(p.M, p.N, p.K, p.offs ? E : 0);
+  const Fp4TileCost& size = kFp4Tiles[tile];
+  const int64_t blocks = fp4_row_tiles(p, size.bm) * ((p.N + size.bn - 1) / size.bn);
+  LSK_REQUIRE(grid_ok(r.ablocks + r.wblocks * E, 256) && grid_ok(blocks, tile < 2 ? 512 : 256),
+              "mxfp4 product: grid too large");
   const dim3 grid((unsigned)(r.ablocks + r.wblocks * E)), blk(256);
   if (x)
     by_input(x, x_dtype, ldx, [&](auto dt, auto vec) {
@@ -826,7 +833,7 @@ static int fp4_tiles(Fp4Args p, const void* x, int x_dtype, int64_t ldx, uint8_t
     hipLaunchKernelGGL((fp4_prep_kernel<-1, false>), grid, blk, 0, s, r);
   const int rc = check_launch("fp4_prep_kernel");
   if (rc) return rc;
-  switch (fp4_cheapest_tile(p.M, p.N, p.K, p.offs ? E : 0)) {  // (all give the same bits)
+  switch (tile) {  // (all give the same bits)
     case 0: return fp4_tile_launch<256, 256, 2, 4, 4, 64>(p, r.sat, r.swt, s);
     case 1: return fp4_tile_launch<128, 256, 2, 4, 3, 64>(p, r.sat, r.swt, s);
     case 2: return fp4_tile_launch<128, 128, 2, 2, 2, 128>(p, r.sat, r.swt, s);
@@ -839,7 +846,7 @@ template <int NG, int MT, int KS, int RING, int DT>
 static int fp4_stream_launch(const Fp4Args& p, const void* x, int64_t ldx, hipStream_t s) {
   const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
   const int64_t blocks = tiles * ((p.N + 16 * NG - 1) / (16 * NG));
-  LSK_REQUIRE(blocks <= 0x7fffffff, "mxfp4 product: grid too large");
+  LSK_REQUIRE(grid_ok(blocks, 256), "mxfp4 product: grid too large");
   const int64_t lds = fp4_stream_lds<NG, MT, KS, RING, (DT >= 0)>(p.K, (int)(p.M < 16 ? p.M : 16));
   LSK_REQUIRE(lds <= 160 * 1024, "mxfp4 product: K=%d too long for few rows", p.K);
   const int vec = x && (uintptr_t)x % 16 == 0 && (ldx * (DT == LSK_F32 ? 4 : 2)) % 16 == 0;

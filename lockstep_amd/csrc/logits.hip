@@ -229,9 +229,10 @@ extern "C" int lsk_penalize_logits(const void* logits, int dtype, int64_t ldl, i
   if (chunks < (V + most - 1) / most) chunks = (V + most - 1) / most;
   p.chunk = (int)(((V + chunks - 1) / chunks + 31) / 32 * 32);
   const int64_t blocks = B * ((V + p.chunk - 1) / p.chunk);
-  LSK_REQUIRE(blocks <= 0x7fffffff, "lsk_penalize_logits: grid too large");
+  const int threads = p.chunk >= 8192 ? 1024 : 256;
+  LSK_REQUIRE(grid_ok(blocks, threads), "lsk_penalize_logits: grid too large");
   const size_t smem = counted ? ((size_t)p.chunk + 8) * (narrow ? 2 : 4) + 16 : 0;
-  const dim3 grid((unsigned)blocks), blk(p.chunk >= 8192 ? 1024 : 256);
+  const dim3 grid((unsigned)blocks), blk(threads);
   hipStream_t s = (hipStream_t)stream;
   auto run = [&](auto kern) {
     if (smem > 65536 &&

@@ -109,3 +109,26 @@ def test_dequant_beyond_one_grid():
         for odt in (L.LSK_BF16, L.LSK_F32):
             assert lib.lsk_dequant_mxfp4(P, P, rows, 64, 32, P, odt, None) == 2
             assert kernel in lib.lsk_last_error(), (rows, lib.lsk_last_error())
+
+
+def test_grids_beyond_hip_are_refused():
+    """HIP launches fewer than 2^32 threads along a grid: what would take more is refused before anything is
+    launched."""
+    lib = L.load()
+
+    def pen(B, V):
+        return lib.lsk_penalize_logits(P, L.LSK_F32, V, B, V, None, 0, 0, None, None, 0, 0, None, 0, None, None, None,
+                                       None, 0, None, 0, P, V, None)
+    _refused(pen(1 << 24, 1), b"grid too large")             # a block of 256 threads a row
+    _refused(pen(1 << 22, 8192), b"grid too large")          # of 1024
+    _refused(pen((1 << 31) - 1, 33), b"grid too large")
+    for M, N in ((1, (1 << 31) - 1), (1 << 21, 1 << 21), ((1 << 29) - 1, 2000)):
+        need = lib.lsk_gemm_mxfp4_workspace(M, N, 32)
+        _refused(lib.lsk_gemm_mxfp4(P, P, M, 32, P, P, N, None, P, L.LSK_BF16, N, P, need, None), b"grid too large")
+    need = lib.lsk_linear_mxfp4_workspace(1 << 28, 64, 128)  # 16 rows a block of the quantiser
+    _refused(lib.lsk_linear_mxfp4(P, L.LSK_BF16, 128, 1 << 28, 128, P, P, 64, None, P, L.LSK_BF16, 64, P, need, None),
+             b"grid too large")
+    E = 1 << 20
+    need = lib.lsk_grouped_gemm_mxfp4_workspace(E, E, 8192, 32)
+    _refused(lib.lsk_grouped_gemm_mxfp4(P, P, P, E, E, P, 16, P, 1, None, 8192, 32, P, L.LSK_BF16, 8192, P, need, None),
+             b"grid too large")
