@@ -12,6 +12,8 @@
 // allows, and shorter where there are too few rows to fill the part with them.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "lsk_common.h"
 
 namespace lsk {
@@ -64,7 +66,8 @@ LSK_DEV void each_token(const void* tok, int wide, int64_t ld, int64_t L, const 
   }
 }
 
-template <int DT, int BITS>
+// PLAIN: without bias and mask, where a token outside the history keeps its bits, a NaN's payload too.
+template <int DT, int BITS, bool PLAIN>
 __global__ __launch_bounds__(1024, 8) void penalize_logits_kernel(PenaltyArgs p) {
   extern __shared__ __attribute__((aligned(16))) uint32_t smem[];
   constexpr int VEC = DT == LSK_F32 ? 4 : 8, SIZE = DT == LSK_F32 ? 4 : 2;
@@ -74,8 +77,8 @@ __global__ __launch_bounds__(1024, 8) void penalize_logits_kernel(PenaltyArgs p)
   const bool counted = p.prompt || p.output;
   const char* in = (const char*)p.logits + (b * p.ldl + v0) * SIZE;
   char* out = (char*)p.out + (b * p.ldo + v0) * SIZE;
-  const float* bias = p.bias ? p.bias + b * p.ldb + v0 : nullptr;
-  const uint32_t* mask = p.mask ? p.mask + b * p.ldm : nullptr;
+  const float* bias = !PLAIN && p.bias ? p.bias + b * p.ldb + v0 : nullptr;
+  const uint32_t* mask = !PLAIN && p.mask ? p.mask + b * p.ldm : nullptr;
   // the run's first 16-byte boundary, where the vectors start (rows of in and out that differ modulo
   // 16 bytes go token by token); the table starts `pad` entries in, so that vectors of it are whole too
   const bool vec = ((uintptr_t)in & 15) == ((uintptr_t)out & 15) && (uintptr_t)in % SIZE == 0;
@@ -112,9 +115,14 @@ __global__ __launch_bounds__(1024, 8) void penalize_logits_kernel(PenaltyArgs p)
     return l;
   };
   auto one = [&](int i) {
+    const uint32_t c = counted ? table.at(i + pad) : 0;
+    if (PLAIN && !c) {
+      if constexpr (DT == LSK_F32) ((uint32_t*)out)[i] = ((const uint32_t*)in)[i];
+      else ((uint16_t*)out)[i] = ((const uint16_t*)in)[i];
+      return;
+    }
     float l = load_as_f32(in, DT, i);
     if (bias) l = f32_add(l, bias[i]);
-    const uint32_t c = counted ? table.at(i + pad) : 0;
     if (c) l = penalized(l, c);
     const int64_t v = v0 + i;
     if (mask && !((mask[v >> 5] >> (v & 31)) & 1u)) l = -__builtin_inff();
@@ -140,51 +148,72 @@ __global__ __launch_bounds__(1024, 8) void penalize_logits_kernel(PenaltyArgs p)
         any = u.x | u.y;
       }
     }
-    if (!any && !bias && !mask) {
+    if (PLAIN && !any) {
       if (in != out) store16_split(out + (int64_t)i * SIZE, raw);
       return;
     }
-    float l[VEC];
     const uint32_t rw[4] = {raw[0], raw[1], raw[2], raw[3]};
+    uint32_t o[4];
+    auto value = [&](int z) {
+      if constexpr (DT == LSK_F32) return __uint_as_float(rw[z]);
+      else if constexpr (DT == LSK_BF16) return bf16_to_f32((uint16_t)(rw[z / 2] >> (z % 2 * 16)));
+      else return (float)__builtin_bit_cast(_Float16, (uint16_t)(rw[z / 2] >> (z % 2 * 16)));
+    };
+    auto counted_at = [&](int z) -> uint32_t {
+      return BITS == 32 ? cw[z] : (cw[z * BITS / 32] >> (z * BITS % 32)) & 0xffffu;
+    };
+    if constexpr (PLAIN) {  // the counted tokens alone, in their places among the others' bits
 #pragma unroll
-    for (int z = 0; z < VEC; ++z) {
-      if constexpr (DT == LSK_F32) l[z] = __uint_as_float(rw[z]);
-      else if constexpr (DT == LSK_BF16) l[z] = bf16_to_f32((uint16_t)(rw[z / 2] >> (z % 2 * 16)));
-      else l[z] = (float)__builtin_bit_cast(_Float16, (uint16_t)(rw[z / 2] >> (z % 2 * 16)));
-    }
-    if (bias) {
-      float bv[VEC];
-      __builtin_memcpy(bv, bias + i, VEC * 4);
-#pragma unroll
-      for (int z = 0; z < VEC; ++z) l[z] = f32_add(l[z], bv[z]);
-    }
-    if (any) {
+      for (int z = 0; z < 4; ++z) o[z] = rw[z];
 #pragma unroll
       for (int z = 0; z < VEC; ++z) {
-        const uint32_t c = BITS == 32 ? cw[z] : (cw[z * BITS / 32] >> (z * BITS % 32)) & 0xffffu;
-        if (c) l[z] = penalized(l[z], c);
+        const uint32_t c = counted_at(z);
+        if (!c) continue;
+        const float l = penalized(value(z), c);
+        if constexpr (DT == LSK_F32) {
+          o[z] = __float_as_uint(l);
+        } else {
+          const uint32_t h = DT == LSK_BF16 ? f32_to_bf16(l) : __builtin_bit_cast(uint16_t, (_Float16)l);
+          o[z / 2] = z % 2 ? (o[z / 2] & 0xffffu) | h << 16 : (o[z / 2] & 0xffff0000u) | h;
+        }
       }
-    }
-    if (mask) {
-      const int64_t v = v0 + i;
-      const uint64_t lo = mask[v >> 5], hi = mask[(v + VEC - 1) >> 5];
-      const uint32_t m = (uint32_t)(((hi << 32) | lo) >> (v & 31));  // (VEC bits at most: inside 64)
-#pragma unroll
-      for (int z = 0; z < VEC; ++z)
-        if (!((m >> z) & 1u)) l[z] = -__builtin_inff();
-    }
-    uint32_t o[4];
-    if constexpr (DT == LSK_F32) {
-#pragma unroll
-      for (int z = 0; z < 4; ++z) o[z] = __float_as_uint(l[z]);
-    } else if constexpr (DT == LSK_BF16) {
-#pragma unroll
-      for (int z = 0; z < 4; ++z) o[z] = pack_bf16x2(l[2 * z], l[2 * z + 1]);
     } else {
+      float l[VEC];
 #pragma unroll
-      for (int z = 0; z < 4; ++z)
-        o[z] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)l[2 * z]) |
-               ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)l[2 * z + 1]) << 16);
+      for (int z = 0; z < VEC; ++z) l[z] = value(z);
+      if (bias) {
+        float bv[VEC];
+        __builtin_memcpy(bv, bias + i, VEC * 4);
+#pragma unroll
+        for (int z = 0; z < VEC; ++z) l[z] = f32_add(l[z], bv[z]);
+      }
+      if (any) {
+#pragma unroll
+        for (int z = 0; z < VEC; ++z) {
+          const uint32_t c = counted_at(z);
+          if (c) l[z] = penalized(l[z], c);
+        }
+      }
+      if (mask) {
+        const int64_t v = v0 + i;
+        const uint64_t lo = mask[v >> 5], hi = mask[(v + VEC - 1) >> 5];
+        const uint32_t m = (uint32_t)(((hi << 32) | lo) >> (v & 31));  // (VEC bits at most: inside 64)
+#pragma unroll
+        for (int z = 0; z < VEC; ++z)
+          if (!((m >> z) & 1u)) l[z] = -__builtin_inff();
+      }
+      if constexpr (DT == LSK_F32) {
+#pragma unroll
+        for (int z = 0; z < 4; ++z) o[z] = __float_as_uint(l[z]);
+      } else if constexpr (DT == LSK_BF16) {
+#pragma unroll
+        for (int z = 0; z < 4; ++z) o[z] = pack_bf16x2(l[2 * z], l[2 * z + 1]);
+      } else {
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          o[z] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)l[2 * z]) |
+                 ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)l[2 * z + 1]) << 16);
+      }
     }
     store16_split(out + (int64_t)i * SIZE, o[0], o[1], o[2], o[3]);
   };
@@ -241,9 +270,13 @@ extern "C" int lsk_penalize_logits(const void* logits, int dtype, int64_t ldl, i
     hipLaunchKernelGGL(kern, grid, blk, smem, s, p);
     return lsk::check_launch("penalize_logits_kernel");
   };
-  if (dtype == LSK_F32)
-    return narrow ? run(lsk::penalize_logits_kernel<LSK_F32, 16>) : run(lsk::penalize_logits_kernel<LSK_F32, 32>);
-  if (dtype == LSK_BF16)
-    return narrow ? run(lsk::penalize_logits_kernel<LSK_BF16, 16>) : run(lsk::penalize_logits_kernel<LSK_BF16, 32>);
-  return narrow ? run(lsk::penalize_logits_kernel<LSK_F16, 16>) : run(lsk::penalize_logits_kernel<LSK_F16, 32>);
+  auto with = [&](auto dt) {
+    constexpr int kDt = decltype(dt)::value;
+    if (!p.bias && !p.mask)
+      return narrow ? run(lsk::penalize_logits_kernel<kDt, 16, true>) : run(lsk::penalize_logits_kernel<kDt, 32, true>);
+    return narrow ? run(lsk::penalize_logits_kernel<kDt, 16, false>) : run(lsk::penalize_logits_kernel<kDt, 32, false>);
+  };
+  if (dtype == LSK_F32) return with(std::integral_constant<int, LSK_F32>{});
+  if (dtype == LSK_BF16) return with(std::integral_constant<int, LSK_BF16>{});
+  return with(std::integral_constant<int, LSK_F16>{});
 }

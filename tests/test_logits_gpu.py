@@ -139,3 +139,38 @@ def test_bad_arguments():
         TH.penalize_logits(l[0])
     with pytest.raises(ValueError):
         TH.penalize_logits(l.to(torch.int32))
+
+
+@pytest.mark.parametrize("Lo", [6, 32768])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_untouched_tokens_keep_their_bits(dtype, Lo):
+    """Without bias and mask a token outside the history keeps its bits, a NaN's payload too, whatever the
+    row's alignment and its neighbours (every 16-bit pattern; binary32 ones of every exponent)."""
+    from lockstep_amd import t16h_lmvariants as TH
+    g = np.random.default_rng(21)
+    B, V = 3, 65536 + 11
+    raw = np.arange(B * V, dtype=np.uint32)
+    if dtype == torch.float32:
+        raw = ((raw << 16) ^ g.integers(0, 1 << 16, raw.size, dtype=np.uint32)).view(np.int32)
+    else:
+        raw = raw.astype(np.uint16).view(np.int16)
+    l = torch.from_numpy(raw).view(dtype).view(B, V)
+    out_tok = g.integers(0, V, (B, Lo))
+    out_tok[:, :6] = np.array([0x7f81, 0x7fff, 0xffc1, 0x7c01, 0xfe00, V - 1]) + np.arange(B)[:, None]   # (some past V)
+    kw = dict(output=out_tok, output_lens=np.full(B, 6), repetition=np.full(B, 1.25, np.float32),
+              presence=np.full(B, 0.5, np.float32))
+    seen = U.counts(out_tok, kw["output_lens"], V) > 0
+    with np.errstate(invalid="ignore"):
+        want = torch.from_numpy(U.penalize(l.float().numpy(), **kw)).to(dtype)
+    d = {k: to_dev(v) for k, v in kw.items()}
+    for off, to in ((0, 0), (1, 1), (5, 5), (0, 1), (3, 0)):
+        wide, out = (torch.zeros((B, V + 8), dtype=dtype, device=dev()) for _ in range(2))
+        wide[:, off:off + V].copy_(l)
+        assert np.array_equal(bits(wide[:, off:off + V]), bits(l))      # (the copy there kept them)
+        got = TH.penalize_logits(wide[:, off:off + V], **d, out=out[:, to:to + V])
+        assert np.array_equal(bits(got)[~seen], bits(l)[~seen]), (off, to)
+        nan = want.isnan().numpy()
+        assert np.array_equal(got.isnan().cpu().numpy(), nan) and np.array_equal(bits(got)[~nan], bits(want)[~nan])
+        if off == to:
+            TH.penalize_logits(wide[:, off:off + V], **d, out=wide[:, off:off + V])
+            assert np.array_equal(bits(wide[:, off:off + V]), bits(got)), off
