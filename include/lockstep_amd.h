@@ -738,7 +738,7 @@ int lsk_grouped_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, const int32
  * stands in the row's output and seen = v stands in its prompt or output, each step one binary32
  * operation:
  *   l = logits + bias;  seen: l = l > 0 ? l / repetition : l * repetition;
- *   l = l - frequency * n (the product rounded first);  n > 0: l = l - presence;
+ *   n > 0: l = l - frequency * n (the product rounded first), then l = l - presence;
  *   mask bit 0: l = -inf;  out = l rounded to dtype.
  * prompt [B, Lp] (row stride ldp) and output [B, Lo] (row stride ldo_tok): tokens, NULL for none; the
  * first prompt_lens[b] / output_lens[b] of a row count (NULL: all; lengths are taken inside [0, L]), and

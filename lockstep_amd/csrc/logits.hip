@@ -3,7 +3,7 @@
 // Per row and token v, with n = how often v stands in the row's output and `seen` = v stands in its
 // prompt or output:
 //   l = fl32(l + bias[v]);  seen: l = l > 0 ? fl32(l / r) : fl32(l * r);
-//   l = fl32(l - fl32(f * n));  n > 0: l = fl32(l - p);  mask bit 0: l = -inf;  out = round(l)
+//   n > 0: l = fl32(fl32(l - fl32(f * n)) - p);  mask bit 0: l = -inf;  out = round(l)
 // A block owns a run of one row's tokens.  It requests its first logits, counts the row's history into
 // a table of that run in LDS meanwhile (the output count, and the top bit for the prompt; integer
 // atomics, so the order of tokens changes nothing), and then streams the run: a vector of tokens none

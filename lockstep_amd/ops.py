@@ -830,8 +830,7 @@ def penalize_logits(logits: torch.Tensor, prompt=None, prompt_lens=None, output=
     rounding:
         l = logits + bias                                  bias f32 [V] or [B, V]
         v in the row's prompt or output:  l = l / repetition if l > 0 else l * repetition
-        l = l - frequency * (times v stands in the output)
-        v in the output:  l = l - presence
+        v in the output:  l = l - frequency * (times it stands there), then l = l - presence
         v not allowed by mask:  l = -inf                   mask int32 [B, ceil(V / 32)] (or [1, ...] for
                                                            all rows): bit v % 32 of word v // 32 allows v
     prompt [B, Lp] and output [B, Lo] are int32 or int64 tokens of which prompt_lens / output_lens [B]

@@ -174,3 +174,19 @@ def test_untouched_tokens_keep_their_bits(dtype, Lo):
         if off == to:
             TH.penalize_logits(wide[:, off:off + V], **d, out=wide[:, off:off + V])
             assert np.array_equal(bits(wide[:, off:off + V]), bits(got)), off
+
+
+def test_a_frequency_of_infinity_or_nan_reaches_counted_tokens_only():
+    """The frequency step, as the presence step, is for tokens that stand in the output: the others keep
+    their logits (and a zero its sign) under any frequency."""
+    g = np.random.default_rng(22)
+    l, c = _case(g, 4, 3000, 50, 40, torch.float32)
+    c["frequency"] = np.array([np.inf, -np.inf, np.nan, -0.5], np.float32)
+    l[:, ::5] = -0.0
+    for left in ((), ("bias", "mask")):
+        kw = {k: v for k, v in c.items() if k not in left}
+        got, want = _run(l, kw).cpu().numpy(), U.penalize(l.numpy(), **kw)
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        assert np.array_equal(got[~np.isnan(got)].view(np.uint32), want[~np.isnan(want)].view(np.uint32))
+        no = U.counts(kw["output"], kw["output_lens"], 3000) == 0
+        assert not np.isnan(got[no]).any()
