@@ -7,9 +7,9 @@
 // memory: a lane holds the 16 code bytes of one block of one row and that block's scale byte.
 //
 // Every output is one chain of such instructions over ascending K from +0.  Chained 32x32x64 and
-// 16x16x128 give the same bits (measured on MI355X: 245,760 sums of 128 to 1024 products, exponents
-// spread over up to 40 octaves, zero and nonzero accumulators), so a row's result depends neither on
-// the tile that computes it nor on the other rows of the call.
+// 16x16x128 give the same bits (MI355X: tested with scale bytes from one octave to all that a byte holds,
+// through subnormal sums and overflows), so a row's result depends neither on the tile that computes it nor
+// on the other rows of the call.
 #include <hip/hip_runtime.h>
 
 #include "lsk_common.h"

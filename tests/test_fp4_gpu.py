@@ -235,6 +235,22 @@ def test_product_rows_do_not_depend_on_a_large_batch():
         assert np.array_equal(bits(_mm(ca[lo:hi], sa[lo:hi], cw[77:190], sw[77:190])), full[lo:hi, 77:190]), (lo, hi)
 
 
+@pytest.mark.parametrize("M,N,K", [(3700, 3400, 224), (2050, 515, 128), (700, 4500, 1088), (300, 1030, 2880), (129, 255, 64)])
+def test_product_rows_do_not_depend_on_the_batch_at_any_scale(M, N, K):
+    """The same with scale bytes spread over up to 121 octaves in either operand, over all that a byte holds,
+    and where products turn subnormal or overflow: few rows on one shape of the matrix instruction and many
+    on the other sum alike."""
+    g = np.random.default_rng(M + N + K)
+    ca, cw = g.integers(0, 16, (M, K), dtype=np.uint8), g.integers(0, 16, (N, K), dtype=np.uint8)
+    for lo, hi in ((107, 147), (67, 187), (40, 70), (180, 195), (0, 254)):
+        say("scales", lo, hi)
+        sa = g.integers(lo, hi + 1, (M, K // 32), dtype=np.uint8)
+        sw = g.integers(lo, hi + 1, (N, K // 32), dtype=np.uint8)
+        full = bits(_mm(ca, sa, cw, sw))
+        for r0, r1 in ((0, 1), (5, 14), (60, 90), (0, min(M, 257)), (100, M)):
+            assert np.array_equal(bits(_mm(ca[r0:r1], sa[r0:r1], cw, sw)), full[r0:r1]), (lo, hi, r0, r1)
+
+
 def test_product_special_scales():
     """255 is a NaN for its row or column alone, also under zero codes; the largest scales overflow to
     infinity, the smallest reach zero or a subnormal; no neighbour changes."""
