@@ -746,8 +746,8 @@ int lsk_grouped_gemm_mxfp4(const uint8_t* a, const uint8_t* a_scale, const int32
  * hold int64 (int32 where the bit is 0).  repetition, frequency, presence: f32 [B] or NULL (left out).
  * bias: f32, row b at bias + b * ldb (ldb 0: one row for all), or NULL.  mask: row b at mask + b * ldm
  * (words; ldm 0: one for all), bit v % 32 of word v / 32 allows v, ceil(V / 32) words, or NULL.  out
- * [B, V] (row stride ldo) may be logits itself.  At most 2^24 - 1 rows, fewer of more than 8160 tokens (one
- * launch holds 2^32 threads). */
+ * [B, V] (row stride ldo) may be logits itself (ldo = ldl then); any other overlap gives wrong rows.  At
+ * most 2^24 - 1 rows, fewer of more than 8160 tokens (one launch holds 2^32 threads). */
 int lsk_penalize_logits(const void* logits, int dtype, int64_t ldl, int64_t B, int64_t V, const void* prompt, int64_t ldp,
                         int64_t Lp, const void* prompt_lens, const void* output, int64_t ldo_tok, int64_t Lo,
                         const void* output_lens, int wide, const float* repetition, const float* frequency,

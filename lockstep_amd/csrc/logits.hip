@@ -240,6 +240,7 @@ extern "C" int lsk_penalize_logits(const void* logits, int dtype, int64_t ldl, i
   if (B == 0 || V == 0) return LSK_OK;
   LSK_REQUIRE(logits && out, "lsk_penalize_logits: null pointer");
   LSK_REQUIRE(B == 1 || (ldl >= V && ldo >= V), "lsk_penalize_logits: row strides below V");
+  LSK_REQUIRE(B == 1 || out != logits || ldo == ldl, "lsk_penalize_logits: in place with two row strides");
   LSK_REQUIRE(!mask || B == 1 || ldm >= 0, "lsk_penalize_logits: negative mask stride");
   lsk::PenaltyArgs p{};
   p.logits = logits, p.ldl = ldl, p.B = B, p.V = V;

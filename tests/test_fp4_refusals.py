@@ -132,3 +132,14 @@ def test_grids_beyond_hip_are_refused():
     need = lib.lsk_grouped_gemm_mxfp4_workspace(E, E, 8192, 32)
     _refused(lib.lsk_grouped_gemm_mxfp4(P, P, P, E, E, P, 16, P, 1, None, 8192, 32, P, L.LSK_BF16, 8192, P, need, None),
              b"grid too large")
+
+
+def test_logits_in_place_needs_one_stride():
+    """In place with two row strides, a row's output lies in another row's input."""
+    lib = L.load()
+
+    def pen(B, ldl, ldo):
+        return lib.lsk_penalize_logits(P, L.LSK_F32, ldl, B, 100, None, 0, 0, None, None, 0, 0, None, 0, None, None, None,
+                                       None, 0, None, 0, P, ldo, None)
+    _refused(pen(2, 128, 100), b"in place")
+    _refused(pen(2, 100, 128), b"in place")
