@@ -253,8 +253,10 @@ inline int64_t expert_tiles_max(int64_t R, int64_t E, int64_t bm) { return R / b
 // rows by a row tile each, on 16x16x128 instructions (weight rows as their rows, activation rows as
 // their columns, so a lane ends with four consecutive outputs of a row).  Bound by HBM, that is by
 // bytes in flight: with a few thousand weight rows there is a block of 16 of them a CU, which is why
-// waves that do not multiply load.  K is not split over waves or blocks: a row's bits would depend on
-// the split.  The scales of the block's rows are copied into LDS whole at the start.
+// waves that do not multiply load.  K is not split over waves or blocks: every kernel here sums an output in
+// one chain, and a split by the number of rows would make a row's bits depend on its batch.  (One at places
+// that depend on K alone, in every kernel, would not; it needs a second set of accumulators, for which the
+// 256 x 256 tiles, at 204 of 256 registers, have no room.)  The scales of the block's rows are copied into LDS whole at the start.
 // DT >= 0: the rows of x (at most 16; vec: 16-byte aligned) are quantised by every block into LDS
 // itself, which saves a launch and the wait for it; x comes from the L2.
 template <int NG, int MT, int KS, bool FUSE>
@@ -740,8 +742,9 @@ static int fp4_tile_launch(const Fp4Args& p, const uint32_t* sat, const uint32_t
 // 25 at 1500 - 1800; 128 of 3584 x 14336 19, 24 at 896; 24 of 28672 x 2048 11.0, 12.2 at 1792, 17 of 37888 x 2048
 // 17.6, 15.2 at 2368.  By expert: 192 rows over 4 of 4096 x 1024 7.7, 10.0 at 2560; 128 over 4 of 5760 x 2880 20,
 // 16 at 2880; 16 rows each over 32 of 5760 x 2880 69, 70, 24 each 80, 72.)  The counts are what one round of
-// blocks takes with two of them a CU; a long K, whose scales leave the LDS room for one, halves them (64 rows
-// of 7000 x 18944 31.6 on streaming blocks, 28.7 on tiles).
+// blocks takes with two of them a CU; by expert, where the count is the most tiles there can be and part of
+// them stay empty, a fitted two and a half.  A long K, whose scales leave the LDS room for one, halves them (64
+// rows of 7000 x 18944 31.6 on streaming blocks, 28.7 on tiles).
 constexpr int64_t kStreamK = 32768;
 template <int NG, int MT, int KS, int RING, int DT>
 static int fp4_stream_per_cu(int64_t K, int rows) {  // blocks that a CU's LDS holds, counted to two
@@ -774,7 +777,9 @@ static int64_t fp4_prep_bytes(int64_t M, int64_t N, int64_t K, int64_t E) {
 // of experts (E > 0, whose last rows take half a tile each) `weights`.  Fitted to 368 products on MI355X (65
 // to 4096 rows, 512 to 28672 columns, K = 96 to 14336; 100 to 16384 rows over 4 to 128 experts).  The tile it
 // picks is 0.4 % slower than the best of the five on average and 17 % at most; thresholds on the number of
-// tiles were 5 % and 44 % (4096 rows of 4608 x 512 on 1.1 rounds of 256 x 256).
+// tiles were 5 % and 44 % (4096 rows of 4608 x 512 on 1.1 rounds of 256 x 256).  Dense weight bytes are no term
+// of it, so it says less than they take where they bound the product (64 rows of 152064 x 3584: 39 us by the
+// fit, 78 measured); its choice past 28672 columns is an extrapolation.
 struct Fp4TileCost {
   int bm, bn, blocks;
   double out, area, weights, round[4], k[4];
@@ -866,7 +871,10 @@ static int fp4_stream_launch(const Fp4Args& p, const void* x, int64_t ldx, hipSt
 // The launch shape by the number of 16-row weight groups over all row tiles: one group a block while
 // there are few (long stages, a deep ring: nothing else hides the latency), else blocks of two, then of
 // four with the shortest ring, several of which share a CU: each for one round of blocks, as many a CU as its
-// LDS holds.  (MI355X, kernel us for NG x KS x RING = 1 x 2 x 4, 2 x 1 x 3: 24 rows of 4096 x 14336
+// LDS holds, counted to two.  For row tiles of 16 the second bound is fixed: three blocks of two groups a CU, which
+// fit up to K = 7168 or so; at 14336 two do and at 32768 one, so just below the bound such products take up to
+// three rounds (16 rows of 20000 x 14336 32.8 us where the weights' bytes take 25, of 24000 x 32768 110 and 69; not
+// measured against blocks of four there).  (MI355X, kernel us for NG x KS x RING = 1 x 2 x 4, 2 x 1 x 3: 24 rows of 4096 x 14336
 // 11.0, 12.4; 16 of 4096 x 7168 7.3, 8.1; calls 64 of 3584 x 2048 11.4, 8.3.  Calls for 1 x 1 x 4, 2 x 1 x 3, 4 x
 // 1 x 2: 8 of 28672 x 4096 16.8, 16.9, 14.0; by expert, 4 rows of 5760 x 2880 13.9, 10.0, 10.4; 256 rows over 32
 // experts of 2880 x 2880 50, 41, 36; 64 over 2 of 5760 x 2880 -, 12.6, 10.1.)
@@ -891,7 +899,9 @@ static int fp4_stream(const Fp4Args& p, hipStream_t s) {
 // the ring, or up to 16 of few values together, since every block quantises them all.  (MI355X, GPU us in one
 // launch and in two, N = 4608: one row of 4096 5.2, 7.0, of 18944 11.7, 11.7 (N = 1024); 4 of 1024 4.6, 6.2,
 // of 4096 7.9, 7.1, of 8192 13.6, 9.0; 16 of 512 5.7, 6.4, of 1024 7.0, 6.3.  A launch less is 3 us of a
-// caller's time besides.)
+// caller's time besides, but nothing in a replayed graph.  The rule does not look at N, and the border was set at
+// 4608: in a graph, 16 rows of 1024 take 10.1, 8.5 at N = 28672 and 32.8, 24.6 at 152064, 4 of 4096 15.6, 14.0
+// and 78, 68, 8 of 1024 8.0, 8.3 and 22.2, 23.8, 16 of 512 6.2, 6.7 and 20.1, 19.9.)
 static bool fp4_fuses(int64_t M, int64_t K) {
   return K > 0 && (M == 1 ? K <= 24576 : M <= 16 && M * K <= 16384);
 }

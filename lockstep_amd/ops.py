@@ -836,7 +836,9 @@ def penalize_logits(logits: torch.Tensor, prompt=None, prompt_lens=None, output=
     prompt [B, Lp] and output [B, Lo] are int32 or int64 tokens of which prompt_lens / output_lens [B]
     (all when None) count; tokens outside [0, V) (padding) count for nothing.  repetition, frequency and
     presence are f32 [B]; what is None is left out.  A row whose mask allows nothing is -inf throughout.
-    Without bias and mask a token outside the history keeps its bits, a NaN's payload among them."""
+    Without bias and mask a token outside the history keeps its bits, a NaN's payload among them.
+    Rows that lie at different places modulo 16 bytes in logits and out go token by token: for the first V
+    columns of a padded head, out=logits or an out of the same row stride keeps the vectors."""
     L.require_cuda(logits, prompt, prompt_lens, output, output_lens, repetition, frequency, presence, bias, mask, out,
                    what="penalize_logits")
     code, shape = _FLOATS.get(logits.dtype), logits.shape
