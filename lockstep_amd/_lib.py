@@ -117,6 +117,17 @@ SIGNATURES = {
                                     _P]),
     "lsk_penalize_logits": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _P, _P, _P, _P,
                                  _I64, _P, _I64, _P, _I64, _P]),
+    "lsk_quantize_rows_fp8": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _I64, _P]),
+    "lsk_quantize_weight_fp8": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P]),
+    "lsk_dequant_fp8": (_I, [_P, _P, _I64, _I64, _I, _I64, _I64, _P, _I, _P]),
+    "lsk_gemm_fp8": (_I, [_P, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I, _I64, _P]),
+    "lsk_linear_fp8_workspace": (_I64, [_I64, _I64, _I64]),
+    "lsk_linear_fp8": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I, _I64, _P, _I64, _P]),
+    "lsk_grouped_gemm_fp8": (_I, [_P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I, _I64,
+                                  _P]),
+    "lsk_add_rmsnorm_fp8": (_I, [_P, _I, _I64, _P, _I64, _I64, _I64, _P, _I, ctypes.c_float, ctypes.c_double, _P, _I64, _P,
+                                 _P, _I64, _I64, _P, _P]),
+    "lsk_route_experts": (_I, [_P, _I, _I64, _I64, _I64, _I, _I, _P, _I, _I, _I, _I, ctypes.c_double, _P, _P, _I, _P]),
 }
 
 

@@ -35,11 +35,12 @@ FLAGS = [
 ]
 
 
-# Per-file code generation options.  mx.hip: the MX block update consumes every MFMA result
+# Per-file code generation options.  mx.hip, fp8.hip: the block update consumes every MFMA result
 # with VALU FMAs, so MFMA results go straight to VGPRs (no accumulation-register copies between
 # an MFMA and its FMAs).
 FILE_FLAGS = {
     "mx.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "fp8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -1,0 +1,178 @@
+// Main loop of the fp8 products' tiles on gfx950's matrix core.
+//
+// A block computes a BM x BN tile of A * W^T over all of K, a stage of 128 values (one block of the scales)
+// at a time through a ring of LDS stages that direct global -> LDS loads fill.  A stage's products are one
+// v_mfma_f32_16x16x128_f8f6f4 per 16 x 16 outputs from +0, added to the running sum times the two scales
+// with one FMA an output (fp8.hip): four VALU cycles of every eight of the matrix core, in its shadow.
+//
+// Lane l of that instruction supplies 32 bytes of row l % 16 of either operand: bytes 16 q .. + 15 and
+// 64 + 16 q .. + 15 of the 128, q = l / 16 (any division of the 128 that both operands share gives the
+// product; this one makes each half one 16-byte LDS read without bank conflicts).  Weight rows go in as
+// the instruction's rows and activation rows as its columns, so register r of lane l holds output row
+// l % 16 and column 4 (l / 16) + r: four consecutive outputs of one row, and one activation scale a lane.
+#pragma once
+#include <type_traits>
+
+#include "mfma_tile.h"
+#include "pp_tile.h"
+
+namespace lsk {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+
+LSK_DEV v8i fp8_operand(v4i lo, v4i hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// The sums of products of one block of 128 values, from +0.  EXACT: the values widened to bf16 (which holds
+// e4m3) and multiplied there, products kept whole and summed in binary32.  The fp8 instruction sums eight
+// products at a time on the scale of the largest, keeping 13 bits below it (MI355X: 2^16 + 2^3 is kept, 2^2
+// dropped): 1.4e-5 of the result on normal data, nothing next to a bf16's or f16's 2^-9 or 2^-12, but not what a
+// binary32 output is for.
+template <bool EXACT>
+LSK_DEV v4f fp8_block(v8i w, v8i a) {
+  const v4f zero = {0, 0, 0, 0};
+  if constexpr (!EXACT) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, zero, 0, 0, 0, 0, 0, 0);
+  } else {
+    typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+    v4f p = zero;
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      v8b x, y;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const v2b x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)w[k + h], 1.0f, false);
+        const v2b x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)w[k + h], 1.0f, true);
+        const v2b y0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)a[k + h], 1.0f, false);
+        const v2b y1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)a[k + h], 1.0f, true);
+        x[4 * h] = x0[0], x[4 * h + 1] = x0[1], x[4 * h + 2] = x1[0], x[4 * h + 3] = x1[1];
+        y[4 * h] = y0[0], y[4 * h + 1] = y0[1], y[4 * h + 2] = y1[0], y[4 * h + 3] = y1[1];
+      }
+      p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, p, 0, 0, 0);
+    }
+    return p;
+  }
+}
+
+// acc + p * s, one rounding an output.
+LSK_DEV v4f fp8_scaled(v4f p, float s, v4f acc) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) acc[t] = __builtin_fmaf(p[t], s, acc[t]);
+  return acc;
+}
+
+template <int BM, int BN, int WM, int WN, int RING>
+struct Fp8Cfg {
+  static_assert(WM * WN == 4, "four waves");
+  static_assert(RING >= 2, "ring of stages");
+  static constexpr int kThreads = WM * WN * 64, kBM = BM, kBN = BN, kWM = WM, kWN = WN, kRing = RING;
+  static constexpr int kNB = BN > 128 ? BN / 128 : 1;  // weight scales of a stage
+  static_assert(BM % 64 == 0 && BM + kNB <= kThreads, "one scale a thread");
+  static constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
+  static_assert(WTM % 16 == 0 && WTN % 16 == 0 && 128 % WTN == 0, "a wave's columns share a weight scale");
+  static constexpr int kStageA = BM * 128, kStageB = BN * 128, kStage = kStageA + kStageB + kThreads * 4;  // bytes
+  static constexpr int kLA = kStageA / 16 / kThreads, kLB = kStageB / 16 / kThreads;
+  static constexpr int kPer = kLA + kLB + 1;  // loads per thread per stage
+  static_assert(kStageA % (16 * kThreads) == 0 && kStageB % (16 * kThreads) == 0, "tile / threads");
+  static constexpr int kMainBytes = kRing * kStage;
+  static constexpr int kLdc = WTN + 4;  // floats a row of a staged 16-row strip
+  static constexpr int kEpiBytes = WM * WN * 16 * kLdc * 4;
+  static constexpr int kSmemBytes = kMainBytes > kEpiBytes ? kMainBytes : kEpiBytes;
+  static_assert(kSmemBytes <= 160 * 1024, "LDS");
+  typedef v4f Acc[TM][TN];
+};
+
+// This thread's part of a tile's loads: its rows' offsets in the resources over the tile's codes, its
+// scale's in the one over the tile's scales (kOob: no row), and the bytes between the scales of two stages.
+template <class C>
+struct Fp8Rows {
+  uint32_t a[C::kLA], b[C::kLB], s;
+  uint32_t sta;
+};
+
+template <int BM, int BN, int WM, int WN, int RING, bool EXACT>
+LSK_DEV void fp8_mainloop(typename Fp8Cfg<BM, BN, WM, WN, RING>::Acc& acc, __amdgpu_buffer_rsrc_t ra,
+                          __amdgpu_buffer_rsrc_t rb, __amdgpu_buffer_rsrc_t rsa, __amdgpu_buffer_rsrc_t rsb,
+                          const Fp8Rows<Fp8Cfg<BM, BN, WM, WN, RING>>& t, int K, char* smem) {
+  using C = Fp8Cfg<BM, BN, WM, WN, RING>;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+  const int wm = wave / C::kWN, wn = wave % C::kWN;
+  const int nk = (K + 127) / 128;
+  const bool sc_a = wave * 64 < C::kBM;  // (a wave's scales are all the rows' or all the weights')
+  const __amdgpu_buffer_rsrc_t rs = sc_a ? rsa : rsb;
+  const uint32_t st = sc_a ? t.sta : 4;
+
+  int ka[C::kLA], kb[C::kLB];
+#pragma unroll
+  for (int j = 0; j < C::kLA; ++j) {
+    int r;
+    pp_slot<C::kThreads, 8>(tid, j, r, ka[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < C::kLB; ++j) {
+    int r;
+    pp_slot<C::kThreads, 8>(tid, j, r, kb[j]);
+  }
+  // (chunks past K, and past the last stage, read zeros)
+  auto issue = [&](int s) {
+    char* base = smem + (s % C::kRing) * C::kStage;
+    const int k0 = s * 128;
+#pragma unroll
+    for (int j = 0; j < C::kLA; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void_t)(base + (j * C::kThreads + wave * 64) * 16), 16,
+                                               k0 + ka[j] < K ? t.a[j] + (uint32_t)(k0 + ka[j]) : kOob, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < C::kLB; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void_t)(base + C::kStageA + (j * C::kThreads + wave * 64) * 16), 16,
+                                               k0 + kb[j] < K ? t.b[j] + (uint32_t)(k0 + kb[j]) : kOob, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t)(base + C::kStageA + C::kStageB + wave * 256), 4,
+                                             s < nk ? t.s + (uint32_t)s * st : kOob, 0, 0, 0);
+  };
+
+  const int lr = lane & 15, q = lane >> 4, sw = pp_swz<8>(lr);
+  const int offA = (wm * C::WTM + lr) * 128, offB = C::kStageA + (wn * C::WTN + lr) * 128;
+  const int offS = C::kStageA + C::kStageB, sA = offS + 4 * (wm * C::WTM + lr), sB = offS + 4 * (C::kBM + wn * C::WTN / 128);
+  const int lo = 16 * (q ^ sw), hi = 16 * ((q + 4) ^ sw);
+
+  struct Frag {
+    v8i a[C::TM], b[C::TN];
+    float sa[C::TM], sb;
+  };
+  auto read = [&](int kt, Frag& f) {
+    const char* base = smem + (kt % C::kRing) * C::kStage;
+    f.sb = *(const float*)(base + sB);
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) f.sa[i] = *(const float*)(base + sA + i * 64);
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+      f.b[j] = fp8_operand(*(const v4i*)(base + offB + j * 2048 + lo), *(const v4i*)(base + offB + j * 2048 + hi));
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+      f.a[i] = fp8_operand(*(const v4i*)(base + offA + i * 2048 + lo), *(const v4i*)(base + offA + i * 2048 + hi));
+  };
+  auto multiply = [&](const Frag& f) {
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+      const float s = f32_mul(f.sa[i], f.sb);
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) acc[i][j] = fp8_scaled(fp8_block<EXACT>(f.b[j], f.a[i]), s, acc[i][j]);
+    }
+  };
+
+  // One barrier a stage: a wave's own loads of stage kt are complete when at most the RING - 2 younger
+  // stages are outstanding, every wave's at the barrier; the slot of stage kt - 1, which every wave has read
+  // by then, takes stage kt + RING - 1.
+  Frag f;
+#pragma unroll
+  for (int s = 0; s < RING - 1; ++s) issue(s);
+  for (int kt = 0; kt < nk; ++kt) {
+    wait_vm<(RING - 2) * C::kPer>();
+    phase_barrier();
+    issue(kt + RING - 1);
+    read(kt, f);
+    multiply(f);
+  }
+  wait_vm<0>();
+}
+
+}  // namespace lsk

@@ -10,6 +10,12 @@ arithmetic runs in the HIP kernels of liblockstep_amd.so (GPU tensors only).
     silu_contract(x), fwht_blocks(x2, blk, scale), pow2_f32(e)   :590-604, :533-546, :280-284
     outlier_side(ho, wo)                        lockstep_fullstack.py:549-557
     w8a8_outlier_linear(x, oidx, wo, W8, ws, bias, out_dtype, rot)   lockstep_fullstack.py:560-578
+
+and, beside the int8 linear, 8-bit floating point (e4m3) with a binary32 scale for each block of 128 values
+(no counterpart in the reference):
+
+    quantize_rows_fp8(x), quantize_weight_fp8(W), dequant_fp8(q, scale, out_dtype)
+    mm_fp8(a, a_scale, w, w_scale, bias, out_dtype), linear_fp8(x, w, w_scale, bias, out_dtype)
 """
 from __future__ import annotations
 
@@ -99,6 +105,14 @@ def quantize_weight_int8(W):
     """Per-out-channel int8 weight (the row quant applied to W [N, K]) -> (W8, ws)."""
     W8, ws = ops.rowquant(W.detach())
     return W8.contiguous(), ws.contiguous()
+
+
+# 8-bit floating point with a scale for each block of 128 values (rows) or 128 x 128 (weights)
+quantize_rows_fp8 = ops.quantize_rows_fp8
+quantize_weight_fp8 = ops.quantize_weight_fp8
+dequant_fp8 = ops.dequant_fp8
+mm_fp8 = ops.mm_fp8
+linear_fp8 = ops.linear_fp8
 
 
 def silu_contract(x):

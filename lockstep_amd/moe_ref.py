@@ -13,6 +13,8 @@ Same names and signatures; GPU tensors only; results bit-identical to the refere
     moe_forward, moe_forward_b                             moe_ref.py:117-140, 213-230
     int_mm_mx, lin_epilogue_mx, expert_block_mx, moe_forward_mx   moe_ref.py:243-290
     blockquant, int_mm_mx2, expert_block_mx2, moe_forward_mx2     moe_ref.py:299-352
+
+and, with no counterpart in the reference: grouped_linear_mxfp4, grouped_linear_fp8 (ExpertTablesFP8), route_experts.
 """
 from __future__ import annotations
 
@@ -102,6 +104,11 @@ def router_b(x, gate_w8, gate_ws, k, renormalize, tab, win, gate_bias=None):
     q, asc = rowquant(x)
     g = linear(q, asc, gate_w8, gate_ws, gate_bias).to(BF)
     return router_from_logits(g, k, renormalize, tab, win)
+
+
+# by softmax or sigmoid scores, with a balancing bias, groups and renormalised weights (no counterpart in the
+# reference, whose scores are the table's); its (idx, w) go into the layers as routing=(idx, w)
+route_experts = ops.route_experts
 
 
 # ============================================================================ activations (moe_ref.py:150-186)
@@ -628,7 +635,7 @@ def grouped_linear_mxfp4(tables, which: str, a, a_scale, offs, out_dtype=BF):
     a, a_scale, R, Ka = ops._mxfp4_codes(a, a_scale, what)
     if Ka != K:
         raise ValueError("%s: rows of %d values for experts of %d" % (what, Ka, K))
-    code = ops._mxfp4_out(what, out_dtype)
+    code = ops._out_code(what, out_dtype)
     w, ws, b = (tables.w13, tables.ws13, tables.b13) if which == "w13" else (tables.w2, tables.ws2, tables.b2)
     ldw, lds = (tables.ldw13, tables.lds13) if which == "w13" else (tables.ldw2, tables.lds2)
     offs = offs.contiguous()
@@ -639,6 +646,77 @@ def grouped_linear_mxfp4(tables, which: str, a, a_scale, offs, out_dtype=BF):
         L.call_on(a, "lsk_grouped_gemm_mxfp4", L.ptr(a), L.ptr(a_scale), L.ptr(offs), tables.E, R,
                   L.ptr(w), ldw, L.ptr(ws), lds, L.ptr(b), N, K, L.ptr(out), code, N, L.ptr(work), nbytes,
                   L.stream_of(a))
+    return out
+
+
+class ExpertTablesFP8:
+    """Device address tables of fp8 experts for grouped_linear_fp8: experts[e] = ((w13 [2I, H], scale_13), (w2 [H, I],
+    scale_2), b13 | None, b2 | None), weights and scales as lockstep_fullstack.quantize_weight_fp8 gives them, every
+    expert in the first one's shape.  What is not contiguous (codes: 16-byte aligned) is copied, once; the rest is
+    read where it lies, so in-place updates are seen."""
+
+    def __init__(self, experts):
+        if not experts:
+            raise ValueError("no experts")
+        L.require_cuda(*(t for ex in experts for pair in ex[:2] for t in pair), *(b for ex in experts for b in ex[2:4]),
+                       what="experts")
+        self.device = experts[0][0][0].device
+        self.E = len(experts)
+        self._keep = []
+        cols = [[] for _ in range(6)]
+        shape = None
+        for ex in experts:
+            (w13, s13, N13, H), (w2, s2, N2, I) = (ops._fp8_weight(*pair, "ExpertTablesFP8") for pair in ex[:2])
+            b13, b2 = (ex[j] if len(ex) > j else None for j in (2, 3))
+            shape = shape or (I, H)
+            if (I, H) != shape or N13 != 2 * I or N2 != H:
+                raise ValueError("ExpertTablesFP8: w13 %s and w2 %s, experts of [%d, %d] and [%d, %d] expected"
+                                 % (tuple(w13.shape), tuple(w2.shape), 2 * shape[0], shape[1], shape[1], shape[0]))
+            b13, b2 = ops._bias_of(b13, N13, "ExpertTablesFP8"), ops._bias_of(b2, N2, "ExpertTablesFP8")
+            for col, t in zip(cols, (w13, s13, w2, s2, b13, b2)):
+                col.append(t)
+        self.I, self.H = shape
+        self._keep = cols
+
+        def table(ts, what=None):
+            some = [t is not None for t in ts]
+            if not any(some):
+                return None
+            if not all(some):
+                raise ValueError("ExpertTablesFP8: %s of every expert or of none" % what)
+            return torch.tensor([t.data_ptr() for t in ts], dtype=torch.int64).to(self.device)
+        self.w13, self.ws13, self.w2, self.ws2, self.b13, self.b2 = (
+            table(c, n) for c, n in zip(cols, ("w13", "scale_13", "w2", "scale_2", "b13", "b2")))
+
+
+def grouped_linear_fp8(tables, which: str, a, a_scale, offs, out_dtype=BF):
+    """The form with fp8 rows and weights (no counterpart in the reference): per expert
+    lockstep_fullstack.mm_fp8(a[rows], a_scale[rows], w_e, scale_e[, b_e]) over expert-sorted rows, the same bits.
+    tables: ExpertTablesFP8; a float8_e4m3fn [R, K], a_scale f32 [R, ceil(K / 128)] (any strides) as
+    lockstep_fullstack.quantize_rows_fp8 gives them; offs int32 [E + 1] on the device; out [R, N] of out_dtype.  Rows past
+    offs[E] belong to no expert and are not written."""
+    what = "grouped_linear_fp8"
+    if which not in ("w13", "w2"):
+        raise ValueError("%s: which must be 'w13' or 'w2'" % what)
+    if not isinstance(tables, ExpertTablesFP8):
+        raise TypeError("%s: ExpertTablesFP8 expected, got %s" % (what, type(tables).__name__))
+    L.require_cuda(a, a_scale, offs, tables.w13, what=what)
+    if offs.dtype != torch.int32 or offs.dim() != 1 or offs.numel() != tables.E + 1:
+        raise ValueError("%s: offs must be int32 [E + 1] = [%d]" % (what, tables.E + 1))
+    N, K = (2 * tables.I, tables.H) if which == "w13" else (tables.H, tables.I)
+    a = ops._fp8_codes(a, what)
+    R = a.shape[0]
+    if a.shape[1] != K:
+        raise ValueError("%s: rows of %d values for experts of %d" % (what, a.shape[1], K))
+    ops._fp8_row_scales(a_scale, R, K, what)
+    code = ops._out_code(what, out_dtype)
+    w, ws, b = (tables.w13, tables.ws13, tables.b13) if which == "w13" else (tables.w2, tables.ws2, tables.b2)
+    offs = offs.contiguous()
+    out = a.new_empty((R, N), dtype=out_dtype)
+    if R:
+        L.call_on(a, "lsk_grouped_gemm_fp8", a.data_ptr(), a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1),
+                  offs.data_ptr(), tables.E, R, w.data_ptr(), K, ws.data_ptr(), (K + 127) // 128, L.ptr(b), N, K,
+                  out.data_ptr(), code, N, L.stream_of(a))
     return out
 
 

@@ -730,14 +730,14 @@ def _mxfp4_codes(packed: torch.Tensor, scale: torch.Tensor, what: str):
     return packed, scale if scale.is_contiguous() else scale.contiguous(), shape[0], shape[1] * 2
 
 
-def _mxfp4_out(what: str, out_dtype):
+def _out_code(what: str, out_dtype):
     code = _FLOATS.get(out_dtype)
     if code is None:
         raise TypeError("%s: out_dtype %s not supported (float32, bfloat16, float16)" % (what, out_dtype))
     return code
 
 
-def _mxfp4_bias(bias, N: int, what: str):
+def _bias_of(bias, N: int, what: str):
     if bias is None:
         return None
     if bias.shape != (N,):
@@ -755,8 +755,8 @@ def mm_mxfp4(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: t
     w, w_scale, N, K2 = _mxfp4_codes(w, w_scale, "mm_mxfp4")
     if K != K2:
         raise ValueError("mm_mxfp4: K mismatch %d vs %d" % (K, K2))
-    code = _mxfp4_out("mm_mxfp4", out_dtype)
-    bias = _mxfp4_bias(bias, N, "mm_mxfp4")
+    code = _out_code("mm_mxfp4", out_dtype)
+    bias = _bias_of(bias, N, "mm_mxfp4")
     out = a.new_empty((M, N), dtype=out_dtype)
     if M and N:
         nbytes = L.load().lsk_gemm_mxfp4_workspace(M, N, K)
@@ -777,8 +777,8 @@ def linear_mxfp4(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=N
     x, xcode, M, Kx, ld = _float_rows(x, "linear_mxfp4")
     if Kx != K:
         raise ValueError("linear_mxfp4: rows of %d values for a weight of %d" % (Kx, K))
-    code = _mxfp4_out("linear_mxfp4", out_dtype)
-    bias = _mxfp4_bias(bias, N, "linear_mxfp4")
+    code = _out_code("linear_mxfp4", out_dtype)
+    bias = _bias_of(bias, N, "linear_mxfp4")
     out = x.new_empty((*lead, N), dtype=out_dtype)
     if M and N:
         nbytes = L.load().lsk_linear_mxfp4_workspace(M, N, K)
@@ -786,6 +786,177 @@ def linear_mxfp4(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=N
         L.call_on(x, "lsk_linear_mxfp4", x.data_ptr(), xcode, ld, M, K, w.data_ptr(), w_scale.data_ptr(), N,
                   L.ptr(bias), out.data_ptr(), code, N, L.ptr(work), nbytes, L.stream_of(x))
     return out
+
+
+# ---------------------------------------------------------------- fp8 rows and weights, a scale for each block of 128
+FP8 = torch.float8_e4m3fn
+FP8_BLOCK = 128
+
+
+def quantize_rows_fp8(x: torch.Tensor):
+    """x [..., K] (f32 / bf16 / f16; other float dtypes go through f32), K % 16 == 0, to (q float8_e4m3fn [..., K],
+    scale f32 [..., ceil(K / 128)]).  The scales of one block lie side by side in memory (stride 1 along the rows),
+    as the products read them fastest."""
+    L.require_cuda(x, what="quantize_rows_fp8")
+    lead = x.shape[:-1]
+    x, code, M, K, ld = _float_rows(x, "quantize_rows_fp8")
+    if K % 16:
+        raise ValueError("quantize_rows_fp8: K=%d not a multiple of 16" % K)
+    nb = (K + 127) // 128
+    q = x.new_empty((M, K), dtype=FP8)
+    scale = x.new_empty((nb, M), dtype=torch.float32)
+    if M and K:
+        L.call_on(x, "lsk_quantize_rows_fp8", x.data_ptr(), code, M, K, ld, q.data_ptr(), scale.data_ptr(), 1, M,
+                  L.stream_of(x))
+    if len(lead) == 1:
+        return q, scale.t()
+    return q.view(*lead, K), scale.t().view(*lead, nb)
+
+
+def quantize_weight_fp8(w: torch.Tensor):
+    """w [N, K] (f32 / bf16 / f16), K % 16 == 0, to (w8 float8_e4m3fn [N, K], scale f32 [ceil(N / 128), ceil(K / 128)])."""
+    L.require_cuda(w, what="quantize_weight_fp8")
+    if w.dim() != 2:
+        raise ValueError("quantize_weight_fp8: a weight [N, K] expected, got %s" % (tuple(w.shape),))
+    w, code, N, K, ld = _float_rows(w, "quantize_weight_fp8")
+    if K % 16:
+        raise ValueError("quantize_weight_fp8: K=%d not a multiple of 16" % K)
+    q = w.new_empty((N, K), dtype=FP8)
+    scale = w.new_empty(((N + 127) // 128, (K + 127) // 128), dtype=torch.float32)
+    if N and K:
+        L.call_on(w, "lsk_quantize_weight_fp8", w.data_ptr(), code, N, K, ld, q.data_ptr(), scale.data_ptr(),
+                  L.stream_of(w))
+    return q, scale
+
+
+def _fp8_codes(q: torch.Tensor, what: str):
+    """Codes [rows, K] as the kernels read them: contiguous, 16-byte aligned (a copy where they are not)."""
+    if q.dtype != FP8 or q.dim() != 2 or q.shape[1] % 16:
+        raise ValueError("%s: float8_e4m3fn [rows, K] with K a multiple of 16 expected, got %s %s"
+                         % (what, q.dtype, tuple(q.shape)))
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.view(torch.uint8).clone(memory_format=torch.contiguous_format).view(FP8)
+    return q
+
+
+def _fp8_row_scales(scale: torch.Tensor, M: int, K: int, what: str):
+    if scale.dtype != torch.float32 or scale.shape != (M, (K + 127) // 128):
+        raise ValueError("%s: scales f32 [%d, %d] expected for rows [%d, %d], got %s %s"
+                         % (what, M, (K + 127) // 128, M, K, scale.dtype, tuple(scale.shape)))
+    return scale
+
+
+def _fp8_weight(w: torch.Tensor, scale: torch.Tensor, what: str):
+    w = _fp8_codes(w, what)
+    N, K = w.shape
+    if scale.dtype != torch.float32 or scale.shape != ((N + 127) // 128, (K + 127) // 128):
+        raise ValueError("%s: scales f32 [%d, %d] expected for a weight [%d, %d], got %s %s"
+                         % (what, (N + 127) // 128, (K + 127) // 128, N, K, scale.dtype, tuple(scale.shape)))
+    return w, scale if scale.is_contiguous() else scale.contiguous(), N, K
+
+
+def dequant_fp8(q: torch.Tensor, scale: torch.Tensor, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """What codes stand for: q [..., K] with the scales of rows ([..., ceil(K / 128)]) or q [N, K] with those of a
+    weight ([ceil(N / 128), ceil(K / 128)]), as the two quantisers give them -> [..., K] of out_dtype."""
+    L.require_cuda(q, scale, what="dequant_fp8")
+    code = _out_code("dequant_fp8", out_dtype)
+    shape = q.shape
+    if not shape:
+        raise ValueError("dequant_fp8: q must be [..., K], got a scalar")
+    K, nb = shape[-1], (shape[-1] + 127) // 128
+    if scale.dtype != torch.float32 or not (scale.shape == (*shape[:-1], nb) or len(shape) == 2
+                                            and scale.shape == ((shape[0] + 127) // 128, nb)):
+        raise ValueError("dequant_fp8: q %s with f32 scales of rows or of 128 x 128 blocks expected, got %s %s"
+                         % (tuple(shape), scale.dtype, tuple(scale.shape)))
+    rows = 1 if scale.shape[:-1] == shape[:-1] else 128
+    if len(shape) != 2:
+        M = shape[:-1].numel()
+        q, scale = q.reshape(M, K), scale.reshape(M, nb)
+    q = _fp8_codes(q, "dequant_fp8")
+    out = q.new_empty(shape, dtype=out_dtype)
+    if out.numel():
+        L.call_on(q, "lsk_dequant_fp8", q.data_ptr(), scale.data_ptr(), scale.stride(0), scale.stride(1), rows, q.shape[0],
+                  K, out.data_ptr(), code, L.stream_of(q))
+    return out
+
+
+def mm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=None,
+           out_dtype=torch.float32) -> torch.Tensor:
+    """fp8 rows a [M, K], a_scale [M, ceil(K / 128)] (any strides) times fp8 weight rows w [N, K], w_scale
+    [ceil(N / 128), ceil(K / 128)] (+ bias [N]) -> [M, N] of out_dtype.  The blocks' sums are added in binary32 over
+    ascending K, one rounding at the end.  A row's result is the same bits whatever the other rows are and
+    however many.  Products are whole for float32; for 16-bit outputs the matrix core's fp8 instruction drops what lies
+    below 2^-13 of the largest of eight (1.4e-5 of the result on normal data)."""
+    L.require_cuda(a, a_scale, w, w_scale, bias, what="mm_fp8")
+    a = _fp8_codes(a, "mm_fp8")
+    w, w_scale, N, K = _fp8_weight(w, w_scale, "mm_fp8")
+    M = a.shape[0]
+    if a.shape[1] != K:
+        raise ValueError("mm_fp8: rows of %d values for a weight of %d" % (a.shape[1], K))
+    _fp8_row_scales(a_scale, M, K, "mm_fp8")
+    code = _out_code("mm_fp8", out_dtype)
+    bias = _bias_of(bias, N, "mm_fp8")
+    out = a.new_empty((M, N), dtype=out_dtype)
+    if M and N:
+        L.call_on(a, "lsk_gemm_fp8", a.data_ptr(), a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1), M, K,
+                  w.data_ptr(), w_scale.data_ptr(), N, L.ptr(bias), out.data_ptr(), code, N, L.stream_of(a))
+    return out
+
+
+def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=None, out_dtype=None) -> torch.Tensor:
+    """x [..., K] (f32 / bf16 / f16) quantised to fp8 (quantize_rows_fp8) and multiplied with fp8 weight rows w [N, K],
+    w_scale [ceil(N / 128), ceil(K / 128)] (+ bias [N]) -> [..., N] of out_dtype (x's by default): mm_fp8 of the
+    quantised rows, the same bits, in one call."""
+    L.require_cuda(x, w, w_scale, bias, what="linear_fp8")
+    w, w_scale, N, K = _fp8_weight(w, w_scale, "linear_fp8")
+    lead = x.shape[:-1]
+    out_dtype = out_dtype or x.dtype
+    x, xcode, M, Kx, ld = _float_rows(x, "linear_fp8")
+    if Kx != K:
+        raise ValueError("linear_fp8: rows of %d values for a weight of %d" % (Kx, K))
+    code = _out_code("linear_fp8", out_dtype)
+    bias = _bias_of(bias, N, "linear_fp8")
+    out = x.new_empty((*lead, N), dtype=out_dtype)
+    if M and N:
+        nbytes = L.load().lsk_linear_fp8_workspace(M, N, K)
+        work = x.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+        L.call_on(x, "lsk_linear_fp8", x.data_ptr(), xcode, ld, M, K, w.data_ptr(), w_scale.data_ptr(), N, L.ptr(bias),
+                  out.data_ptr(), code, N, L.ptr(work), nbytes, L.stream_of(x))
+    return out
+
+
+# ---------------------------------------------------------------- the choice of experts
+_SCORING = {"softmax": 0, "sigmoid": 1}
+
+
+def route_experts(g: torch.Tensor, k: int, scoring: str = "softmax", bias=None, groups: int = 1, keep_groups=None,
+                  group_top: int = 2, renormalize: bool = True, scale: float = 1.0, out_dtype=torch.float32):
+    """k experts a token by the scores of its logits g [T, E] (f32 / bf16 / f16; E <= 1024): (idx int64 [T, k],
+    w [T, k] of out_dtype).  p = softmax over the experts or the logits' sigmoids; c = p + bias (f32 [E]) decides.
+    groups > 1: the experts form so many runs of one size, a group counts the sum of its group_top (1 or 2)
+    largest c, and the keep_groups (all by default) that count most stay.  Of their experts the k of largest c are
+    chosen, larger first, of equals the lower index; a NaN ranks below every number.  w = p of the chosen, over
+    their sum when renormalize (0 where that is 0), times scale.  Everything is computed in binary64."""
+    L.require_cuda(g, bias, what="route_experts")
+    code = _FLOATS.get(g.dtype)
+    if code is None or g.dim() != 2:
+        raise ValueError("route_experts: logits must be f32, bf16 or f16 [T, E], got %s %s" % (g.dtype, tuple(g.shape)))
+    if scoring not in _SCORING:
+        raise ValueError("route_experts: scoring must be 'softmax' or 'sigmoid', got %r" % (scoring,))
+    T, E = g.shape
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.shape != (E,):
+            raise ValueError("route_experts: bias must be f32 [%d], got %s %s" % (E, bias.dtype, tuple(bias.shape)))
+        bias = bias.contiguous()
+    wcode = _out_code("route_experts", out_dtype)
+    if g.stride(1) != 1 and E > 1 or T > 1 and g.stride(0) < E:
+        g = g.contiguous()
+    idx = g.new_empty((T, k), dtype=torch.int64)
+    w = g.new_empty((T, k), dtype=out_dtype)
+    L.call_on(g, "lsk_route_experts", g.data_ptr(), code, g.stride(0), T, E, k, _SCORING[scoring], L.ptr(bias), groups,
+              groups if keep_groups is None else keep_groups, group_top if groups > 1 else 1, renormalize, scale,
+              idx.data_ptr(), w.data_ptr(), wcode, L.stream_of(g))
+    return idx, w
 
 
 # ---------------------------------------------------------------- logits

@@ -14,6 +14,10 @@ reference; it is rmsnorm_float followed by lockstep_fullstack.quantize_rows_int8
 in one kernel):
 
     rmsnorm_float_rowquant(x, weight, sN, eps, want_out)  -> (q int8, asc f32, out bf16 or None)
+
+and of the fp8 linears (with the residual's addition; no counterpart in the reference either):
+
+    add_rmsnorm_fp8(x, residual, weight, sN, eps, want_out)  -> (q e4m3, scale f32, h, out bf16 or None)
 """
 from __future__ import annotations
 
@@ -23,6 +27,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
+from . import ops
 
 FLT_MIN = 2.0 ** -126
 
@@ -123,3 +128,45 @@ def rmsnorm_float_rowquant(x, weight, sN=None, eps=0.0, want_out=False):
            L.ptr(g), L.dtype_code(g.dtype), float(sqrt_n(N) if sN is None else sN), float(eps or 0.0), L.ptr(out),
            L.LSK_BF16, N, L.ptr(q), N, L.ptr(asc), None, L.stream_of(x))
     return q.reshape(shp), asc.reshape(shp[:-1]), (None if out is None else out.reshape(shp))
+
+
+def add_rmsnorm_fp8(x, residual, weight, sN=None, eps=0.0, want_out=False):
+    """h = x + residual, rounded once to x's type (h = x when residual is None); the norm of h in binary32;
+    its fp8 rows (lockstep_fullstack.quantize_rows_fp8 of that, without a rounding between), in one pass.
+    x and residual [..., N] of one type (f32 / bf16 / f16), N % 16 == 0, N <= 65536; weight [N] gain.
+    Returns (q float8_e4m3fn [..., N], scale f32 [..., ceil(N / 128)], h [..., N], out bf16 [..., N] =
+    rmsnorm_float(h, weight) when want_out else None)."""
+    L.require_cuda(x, residual, what="add_rmsnorm_fp8")
+    shp = x.shape
+    if x.dtype not in _ODT or x.dim() == 0:
+        raise TypeError("add_rmsnorm_fp8: x must be f32, bf16 or f16 [..., N], got %s %s" % (x.dtype, tuple(shp)))
+    if residual is not None and (residual.shape != shp or residual.dtype != x.dtype):
+        raise ValueError("add_rmsnorm_fp8: residual %s %s for x %s %s"
+                         % (residual.dtype, tuple(residual.shape), x.dtype, tuple(shp)))
+    N = shp[-1]
+    if N % 16 or N > 65536:
+        raise ValueError("add_rmsnorm_fp8: N=%d is not a multiple of 16 up to 65536" % N)
+    R, nb = shp[:-1].numel(), (N + 127) // 128
+    x2, ldx = _rows_of(x, R, N)
+    r2, ldr = (None, 0) if residual is None else _rows_of(residual, R, N)
+    g = _gain(weight, N, x.device)
+    q = x.new_empty((R, N), dtype=ops.FP8)
+    scale = x.new_empty((nb, R), dtype=torch.float32)
+    h = x if residual is None else x.new_empty(shp)
+    out = x.new_empty(shp, dtype=torch.bfloat16) if want_out else None
+    if R and N:
+        L.call_on(x, "lsk_add_rmsnorm_fp8", x2.data_ptr(), _ODT[x.dtype], ldx, L.ptr(r2), ldr, R, N, g.data_ptr(),
+                  _ODT[g.dtype], float(sqrt_n(N) if sN is None else sN), float(eps or 0.0),
+                  None if residual is None else h.data_ptr(), N, q.data_ptr(), scale.data_ptr(), 1, R, L.ptr(out),
+                  L.stream_of(x))
+    return q.view(shp), scale.t().view(*shp[:-1], nb), h, out
+
+
+def _rows_of(x, R, N):
+    """x [..., N] as R rows of unit stride: (tensor, row stride)."""
+    if x.is_contiguous():
+        return x, N
+    x = x.reshape(R, N)
+    if N > 1 and x.stride(1) != 1 or R > 1 and x.stride(0) < N:
+        x = x.contiguous()
+    return x, x.stride(0)
