@@ -128,9 +128,7 @@ __global__ __launch_bounds__(256) void dequant_fp8_kernel(const uint8_t* __restr
 #pragma unroll
       for (int t = 0; t < 8; ++t) __asm__("" : "+v"(v[t]));
     }
-    char* o = (char*)out + i * (ODT == LSK_F32 ? 32 : 16);
-    store_quad(o, ODT, v4f{v[0], v[1], v[2], v[3]});
-    store_quad(o + (ODT == LSK_F32 ? 16 : 8), ODT, v4f{v[4], v[5], v[6], v[7]});
+    store_eight((char*)out + i * (ODT == LSK_F32 ? 32 : 16), ODT, v);
   }
 }
 

@@ -47,12 +47,13 @@ LSK_DEV float wave_tree(float v) {
 template <int DT, bool VEC>
 LSK_DEV void store8(void* o, int64_t i, const float (&v)[8]) {
   if constexpr (VEC) {
-    char* at = (char*)o + i * (DT == LSK_F32 ? 4 : 2);
-    store_quad(at, DT, v4f{v[0], v[1], v[2], v[3]});
-    store_quad(at + (DT == LSK_F32 ? 16 : 8), DT, v4f{v[4], v[5], v[6], v[7]});
+    store_eight((char*)o + i * (DT == LSK_F32 ? 4 : 2), DT, v);
   } else {
 #pragma unroll
-    for (int t = 0; t < 8; ++t) store_out(o, DT, i + t, v[t]);
+    for (int t = 0; t < 8; ++t) {
+      store_out(o, DT, i + t, v[t]);
+      __asm__ volatile("" ::: "memory");  // (no 16-byte stores: store16_split)
+    }
   }
 }
 

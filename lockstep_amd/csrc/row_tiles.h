@@ -121,6 +121,14 @@ LSK_DEV void store_quad(char* o, int dtype, v4f v) {
   }
 }
 
+// Eight of them, in 8-byte stores too.
+LSK_DEV void store_eight(char* o, int dtype, const float (&v)[8]) {
+  store_quad(o, dtype, v4f{v[0], v[1], v[2], v[3]});
+  __asm__ volatile("" ::: "memory");
+  store_quad(o + (dtype == LSK_F32 ? 16 : 8), dtype, v4f{v[4], v[5], v[6], v[7]});
+  __asm__ volatile("" ::: "memory");
+}
+
 inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 inline bool is_float_dtype(int d) { return d == LSK_F32 || d == LSK_BF16 || d == LSK_F16; }
