@@ -15,6 +15,8 @@
 #include "mfma_tile.h"
 #include "row_tiles.h"
 
+#define LSK_HD __host__ __device__ inline
+
 namespace lsk {
 
 // ---------------------------------------------------------------- the quantisers
@@ -154,6 +156,253 @@ struct Fp8Args {
   const int64_t* b_ptrs;
 };
 
+// Few rows: a block computes NG x 16 output columns of up to MT x 16 rows over all of K, streaming its
+// weight rows from HBM.  Four waves bring the codes in, KS x 256 values (256 bytes of a row, whole lines)
+// a stage, by direct global -> LDS loads RING - 1 stages ahead; waves multiply a group of 16 weight
+// rows by a row tile each.  Bound by HBM, that is by bytes in flight: with a few thousand weight rows there is
+// a block of 16 of them a CU, which is why waves that do not multiply load.  K is not split over waves or
+// blocks: every kernel here sums an output in one chain, and a split by the number of rows would make a
+// row's bits depend on its batch.  The products of the rows' scales with the weight's (a block's columns share
+// one weight scale) are put into LDS whole at the start; their loads go out before the ring's, which they would
+// wait for otherwise.
+// DT >= 0: the rows of x (at most 16; vec: 16-byte aligned) are quantised by every block into LDS
+// itself, which saves a launch and the wait for it; x comes from the L2.
+template <int NG, int MT, int KS, bool FUSE>
+struct Fp8StreamCfg {
+  static constexpr int kPartW = NG * 4096, kPart = kPartW + (FUSE ? 0 : MT * 4096), kStage = KS * kPart;  // bytes
+  static constexpr int kPer = KS * (NG + (FUSE ? 0 : MT));  // loads per thread per stage
+  static constexpr int kMW = NG * MT > 4 ? NG * MT / 4 : 1;  // row tiles of a wave
+  static constexpr int kPre = 16;                            // scales of a thread loaded ahead of the ring
+  static_assert(NG * MT <= 4 || NG == 4, "a wave's row tiles share its weight rows");
+  static_assert(NG <= 8 && 128 % (16 * NG) == 0, "a block's columns share a weight scale");
+};
+
+// Parts of 256 values, whole stages of them; floats from one row of scales to the next (two of four banks
+// further each row: 16 rows' pairs read at once lie in 32 banks), bytes from one row of codes to the next.
+LSK_HD int fp8_parts(int K, int ks) { return ((K + 255) / 256 + ks - 1) / ks * ks; }
+LSK_HD int fp8_scale_pitch(int K, int ks) { return 2 * fp8_parts(K, ks) | 2; }
+LSK_HD int fp8_fused_pitch(int K, int ks) { return fp8_parts(K, ks) * 256 + 16; }
+template <int NG, int MT, int KS, int RING, bool FUSE>
+static int64_t fp8_stream_lds(int K, int rows) {
+  return RING * Fp8StreamCfg<NG, MT, KS, FUSE>::kStage + (FUSE ? (int64_t)rows * fp8_fused_pitch(K, KS) : 0) +
+         (int64_t)(FUSE ? rows : MT * 16) * fp8_scale_pitch(K, KS) * 4;
+}
+
+template <int NG, int MT, int KS, int RING, int DT, bool EXACT, bool GROUPED>
+__global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args p, const void* __restrict__ x, int64_t ldx, int vec) {
+  constexpr bool FUSE = DT >= 0;
+  using C = Fp8StreamCfg<NG, MT, KS, FUSE>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), r = lane & 15, q = lane >> 4;
+  const int ngroups = (int)((p.N + 16 * NG - 1) / (16 * NG));
+  const int tile = blockIdx.x / ngroups, n0 = (blockIdx.x - tile * ngroups) * 16 * NG;
+  int64_t m0 = (int64_t)tile * 16 * MT, m1 = p.M;
+  if constexpr (GROUPED) {
+    int e, first, end;
+    if (!ExpertTiles(p.offs, p.E, (int)p.M, 16 * MT).find(tile, e, first, end)) return;
+    m0 = first;
+    m1 = end;
+    p.w = (const uint8_t*)wave_uniform64(p.w_ptrs[e]);
+    p.sw = (const float*)wave_uniform64(p.ws_ptrs[e]);
+    p.bias = p.b_ptrs ? (const float*)wave_uniform64(p.b_ptrs[e]) : nullptr;
+  }
+  const int rows_a = m1 - m0 < 16 * MT ? (int)(m1 - m0) : 16 * MT;
+  const int rows_w = p.N - n0 < 16 * NG ? (int)p.N - n0 : 16 * NG;
+  const int nb = (p.K + 127) / 128, parts = fp8_parts(p.K, KS), nk = parts / KS;
+  const int sp = fp8_scale_pitch(p.K, KS), fp = fp8_fused_pitch(p.K, KS);
+  char* const fused = smem + RING * C::kStage;  // FUSE: the rows' codes
+  float* const scales = (float*)(fused + (FUSE ? rows_a * fp : 0));
+  const float* const sw = p.sw + (int64_t)(n0 >> 7) * p.ldsw;
+
+  // the scales' table: row m of it, block b; 0 past the rows and past K
+  constexpr int kRows = 16 * MT;
+  const int total = FUSE ? 0 : kRows * 2 * parts;
+  const float* const sa = p.sa + m0 * p.sm;
+  float pa[C::kPre], pw[C::kPre];
+  if constexpr (!FUSE) {
+#pragma unroll
+    for (int z = 0; z < C::kPre; ++z) {
+      const int i = tid + 256 * z, m = i % kRows, b = i / kRows;
+      pa[z] = pw[z] = 0.0f;
+      if (256 * z < total && m < rows_a && b < nb) pa[z] = sa[m * p.sm + b * p.sb], pw[z] = sw[b];
+    }
+  }
+
+  const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w + (int64_t)n0 * p.ldw, (int64_t)(rows_w - 1) * p.ldw + p.K);
+  const __amdgpu_buffer_rsrc_t ra = FUSE ? rw : make_rsrc(p.a + m0 * p.lda, (int64_t)(rows_a - 1) * p.lda + p.K);
+  // a thread's 16-byte slot j of a part: row 16 j + tid / 16, chunk c of its 256 bytes in place c ^ row % 16
+  const int row = tid >> 4, kc = 16 * ((tid & 15) ^ row);
+  auto issue = [&](int kt) {
+    char* base = smem + (kt % RING) * C::kStage + wave * 1024;
+#pragma unroll
+    for (int u = 0; u < KS; ++u) {
+      const int k = 256 * (KS * kt + u);
+      const bool in = k + kc < p.K;
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_void_t)(base + u * C::kPart + j * 4096), 16,
+                                                 in && 16 * j + row < rows_w ? (uint32_t)((16 * j + row) * (int)p.ldw + kc) : kOob,
+                                                 k, 0, 0);
+      if constexpr (!FUSE) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void_t)(base + u * C::kPart + C::kPartW + j * 4096), 16,
+                                                   in && 16 * j + row < rows_a ? (uint32_t)((16 * j + row) * (int)p.lda + kc) : kOob,
+                                                   k, 0, 0);
+      }
+    }
+  };
+  compiler_fence();
+#pragma unroll
+  for (int s = 0; s < RING - 1; ++s) issue(s);
+
+  if constexpr (!FUSE) {
+#pragma unroll
+    for (int z = 0; z < C::kPre; ++z) {
+      const int i = tid + 256 * z;
+      if (i < total) scales[i % kRows * sp + i / kRows] = f32_mul(pa[z], pw[z]);
+    }
+    for (int i = tid + 256 * C::kPre; i < total; i += 256) {
+      const int m = i % kRows, b = i / kRows;
+      scales[m * sp + b] = m < rows_a && b < nb ? f32_mul(sa[m * p.sm + b * p.sb], sw[b]) : 0.0f;
+    }
+  } else {
+    // 16 lanes a block of 128 values, the rows end to end (zeros past K), kBatch loads of a thread in flight
+    const int slots = 32 * parts, all = rows_a * slots;  // pieces of eight values
+    constexpr int kBatch = 4;
+    for (int i0 = tid; i0 < all; i0 += 256 * kBatch) {
+      float v[kBatch][8];
+      int m[kBatch];
+#pragma unroll
+      for (int z = 0; z < kBatch; ++z) {
+        const int i = i0 + 256 * z;
+        m[z] = (int)((uint32_t)i / (uint32_t)slots);
+        const int k = 8 * (i - m[z] * slots);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) v[z][t] = 0.0f;
+        if (i < all && k < p.K) {
+          if (vec) load8<DT, true>(x, (m0 + m[z]) * ldx + k, v[z]);
+          else load8<DT, false>(x, (m0 + m[z]) * ldx + k, v[z]);
+        }
+      }
+#pragma unroll
+      for (int z = 0; z < kBatch; ++z) {
+        const int i = i0 + 256 * z, c = i - m[z] * slots;
+        if (i >= all) continue;  // (16 lanes alike: `slots` is a multiple of 32)
+        float s;
+        *(uint2*)(fused + m[z] * fp + 8 * c) = quantize_row_fp8(v[z], s);
+        if ((c & 15) == 0) scales[m[z] * sp + (c >> 4)] = (c >> 4) < nb ? f32_mul(s, sw[c >> 4]) : 0.0f;
+      }
+    }
+  }
+
+  // wave w multiplies weight group w % NG with row tiles w / NG (and, NG * MT > 4, the next ones)
+  constexpr int MW = C::kMW;
+  const int g = wave % NG, mt = wave / NG * MW;
+  const bool multiplies = NG * MT >= 4 || wave < NG * MT;
+  v4f acc[MW];
+  const float* ars[MW];
+  const char* arc[MW];
+#pragma unroll
+  for (int m = 0; m < MW; ++m) {
+    acc[m] = v4f{0, 0, 0, 0};
+    // (rows past the end: whatever lies there, their results are not stored)
+    const int ar = FUSE ? min(r, rows_a - 1) : 16 * (mt + m) + r;
+    ars[m] = scales + ar * sp;
+    arc[m] = FUSE ? fused + ar * fp : smem + C::kPartW + ar * 256;
+  }
+  // a stage's fragments are read a stage ahead where the ring is deep enough, so that the LDS works under the
+  // matrix core's and the FMAs' chain
+  struct Frag {
+    v2f_t s[KS][MW];
+    v8i w[KS][2], a[KS][MW][2];
+  };
+  auto read = [&](int kt, Frag& f) {
+#pragma unroll
+    for (int u = 0; u < KS; ++u) {
+      const int slot = (kt % RING) * C::kStage + u * C::kPart, part = KS * kt + u;
+      const char* base = smem + slot + (16 * g + r) * 256;
+#pragma unroll
+      for (int m = 0; m < MW; ++m) f.s[u][m] = *(const v2f_t*)(ars[m] + 2 * part);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c0 = 16 * ((8 * h + q) ^ r), c1 = 16 * ((8 * h + 4 + q) ^ r);
+        f.w[u][h] = fp8_operand(*(const v4i*)(base + c0), *(const v4i*)(base + c1));
+#pragma unroll
+        for (int m = 0; m < MW; ++m) {
+          const char* a = FUSE ? arc[m] + 256 * part + 128 * h + 16 * q : arc[m] + slot;
+          f.a[u][m][h] = FUSE ? fp8_operand(*(const v4i*)a, *(const v4i*)(a + 64))
+                              : fp8_operand(*(const v4i*)(a + c0), *(const v4i*)(a + c1));
+        }
+      }
+    }
+  };
+  auto multiply = [&](const Frag& f) {
+#pragma unroll
+    for (int u = 0; u < KS; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < MW; ++m)
+          acc[m] = fp8_scaled(fp8_block<EXACT>(f.w[u][h], f.a[u][m][h]), f.s[u][m][h], acc[m]);
+  };
+  Frag f[2];
+  if constexpr (RING >= 4) {
+    wait_vm<(RING - 2) * C::kPer>();
+    wait_lgkm0();
+    phase_barrier();
+    if (multiplies) read(0, f[0]);
+    auto step = [&](int kt, Frag& now, Frag& next) {
+      compiler_fence();  // (the reads of the stage before stay on their side of the barrier)
+      wait_vm<(RING - 3) * C::kPer>();
+      phase_barrier();
+      issue(kt + RING - 1);
+      if (multiplies) {
+        if (kt + 1 < nk) read(kt + 1, next);
+        multiply(now);
+      }
+    };
+    int kt = 0;
+    for (; kt + 2 <= nk; kt += 2) {
+      step(kt, f[0], f[1]);
+      step(kt + 1, f[1], f[0]);
+    }
+    if (kt < nk) step(kt, f[0], f[1]);
+  } else {
+    for (int kt = 0; kt < nk; ++kt) {
+      wait_vm<(RING - 2) * C::kPer>();
+      wait_lgkm0();
+      phase_barrier();
+      issue(kt + RING - 1);
+      if (multiplies) {
+        read(kt, f[0]);
+        multiply(f[0]);
+      }
+    }
+  }
+  wait_vm<0>();
+  if (!multiplies) return;
+  float b[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int64_t n = n0 + 16 * g + 4 * q + t;
+    b[t] = p.bias && n < p.N ? p.bias[n] : 0.0f;
+  }
+#pragma unroll
+  for (int m = 0; m < MW; ++m) {
+    const int row_out = 16 * (mt + m) + r;
+    if (row_out >= rows_a) continue;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int64_t n = n0 + 16 * g + 4 * q + t;
+      float y = acc[m][t];
+      __asm__("" : "+v"(y));  // (a binary32 sum first, as the tiles have it: not one FMA that rounds to f16)
+      if (n < p.N) store_out(p.out, p.out_dtype, (m0 + row_out) * p.ldo + n, p.bias ? f32_add(y, b[t]) : y);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- tiles
 // A BM x BN tile: tiles walk kGroupM row tiles down a column of weight tiles inside each XCD's run
 // of them, so the row tiles that share a weight tile run together on one L2.
 template <int BM, int BN, int WM, int WN, int RING, bool EXACT, bool GROUPED>
@@ -190,25 +439,13 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8Args p, int64
   const int rows_a = m1 - m0 < BM ? m1 - m0 : BM, rows_w = (int)p.N - n0 < BN ? (int)p.N - n0 : BN;
   const int nb = (p.K + 127) / 128, blocks_w = (rows_w + 127) / 128;
 
-  Fp8Rows<C> t;
-  const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.a + (int64_t)m0 * p.lda, (int64_t)(rows_a - 1) * p.lda + p.K);
-  const __amdgpu_buffer_rsrc_t rb = make_rsrc(p.w + (int64_t)n0 * p.ldw, (int64_t)(rows_w - 1) * p.ldw + p.K);
-  const __amdgpu_buffer_rsrc_t rsa =
-      make_rsrc(p.sa + m0 * p.sm, nb ? 4 * ((rows_a - 1) * p.sm + (nb - 1) * p.sb + 1) : 0);
-  const __amdgpu_buffer_rsrc_t rsb = make_rsrc(p.sw + (n0 >> 7) * p.ldsw, nb ? 4 * ((blocks_w - 1) * p.ldsw + nb) : 0);
+  Fp8Tile t;
+  t.ra = make_rsrc(p.a + (int64_t)m0 * p.lda, (int64_t)(rows_a - 1) * p.lda + p.K);
+  t.rb = make_rsrc(p.w + (int64_t)n0 * p.ldw, (int64_t)(rows_w - 1) * p.ldw + p.K);
+  t.rsa = make_rsrc(p.sa + m0 * p.sm, nb ? 4 * ((rows_a - 1) * p.sm + (nb - 1) * p.sb + 1) : 0);
+  t.rsb = make_rsrc(p.sw + (n0 >> 7) * p.ldsw, nb ? 4 * ((blocks_w - 1) * p.ldsw + nb) : 0);
+  t.lda = (int)p.lda, t.ldb = (int)p.ldw, t.rows_a = rows_a, t.rows_b = rows_w;
   t.sta = (uint32_t)(4 * p.sb);
-#pragma unroll
-  for (int j = 0; j < C::kLA; ++j) {
-    int row, kb;
-    pp_slot<C::kThreads, 8>(tid, j, row, kb);
-    t.a[j] = row < rows_a ? (uint32_t)(row * p.lda) : kOob;
-  }
-#pragma unroll
-  for (int j = 0; j < C::kLB; ++j) {
-    int row, kb;
-    pp_slot<C::kThreads, 8>(tid, j, row, kb);
-    t.b[j] = row < rows_w ? (uint32_t)(row * p.ldw) : kOob;
-  }
   t.s = tid < BM ? (tid < rows_a ? (uint32_t)(4 * tid * p.sm) : kOob)
                  : (tid - BM < blocks_w ? (uint32_t)(4 * (tid - BM) * p.ldsw) : kOob);
 
@@ -218,7 +455,7 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8Args p, int64
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass does not instantiate the main loop twice)
-  fp8_mainloop<BM, BN, WM, WN, RING, EXACT>(acc, ra, rb, rsa, rsb, t, p.K, smem);
+  fp8_mainloop<BM, BN, WM, WN, RING, EXACT>(acc, t, p.K, smem);
 #endif
   __syncthreads();
 
@@ -273,9 +510,11 @@ static int fp8_tile_launch(const Fp8Args& p, hipStream_t s) {
     hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(C::kThreads), C::kSmemBytes, s, p, mtiles, vec);
     return check_launch("fp8_tile_kernel");
   };
-  if (p.out_dtype == LSK_F32)  // binary32 outputs from products kept whole (fp8_block)
-    return p.offs ? run(fp8_tile_kernel<BM, BN, WM, WN, RING, true, true>)
-                  : run(fp8_tile_kernel<BM, BN, WM, WN, RING, true, false>);
+  if constexpr (C::kThreads == 256) {
+    if (p.out_dtype == LSK_F32)  // from products kept whole (fp8_block)
+      return p.offs ? run(fp8_tile_kernel<BM, BN, WM, WN, RING, true, true>)
+                    : run(fp8_tile_kernel<BM, BN, WM, WN, RING, true, false>);
+  }
   return p.offs ? run(fp8_tile_kernel<BM, BN, WM, WN, RING, false, true>)
                 : run(fp8_tile_kernel<BM, BN, WM, WN, RING, false, false>);
 }
@@ -287,9 +526,71 @@ static bool fp8_reach(const Fp8Args& p) {
          4 * (4 * p.ldsw + nb) < 0x7fffffff;
 }
 
+template <int NG, int MT, int KS, int RING, int DT>
+static int fp8_stream_launch(const Fp8Args& p, const void* x, int64_t ldx, hipStream_t s) {
+  const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
+  const int64_t blocks = tiles * ((p.N + 16 * NG - 1) / (16 * NG));
+  LSK_REQUIRE(grid_ok(blocks, 256) && blocks <= 0x7fffffff, "fp8 product: grid too large");
+  const int64_t lds = fp8_stream_lds<NG, MT, KS, RING, (DT >= 0)>(p.K, (int)(p.M < 16 ? p.M : 16));
+  LSK_REQUIRE(lds <= 160 * 1024, "fp8 product: K=%d too long for few rows", p.K);
+  const int vec = x && (uintptr_t)x % 16 == 0 && (ldx * (DT == LSK_F32 ? 4 : 2)) % 16 == 0;
+  auto run = [&](auto kern) {
+    if (lds > 65536 &&
+        hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
+      return set_error("fp8_stream_kernel: cannot reserve LDS"), LSK_ERR_HIP;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), (size_t)lds, s, p, x, ldx, vec);
+    return check_launch("fp8_stream_kernel");
+  };
+  const bool exact = p.out_dtype == LSK_F32;  // (fp8_block)
+  if constexpr (DT < 0) {
+    if (p.offs)
+      return exact ? run(fp8_stream_kernel<NG, MT, KS, RING, DT, true, true>)
+                   : run(fp8_stream_kernel<NG, MT, KS, RING, DT, false, true>);
+  }
+  return exact ? run(fp8_stream_kernel<NG, MT, KS, RING, DT, true, false>)
+               : run(fp8_stream_kernel<NG, MT, KS, RING, DT, false, false>);
+}
+
+// The launch shape by the number of 16-row weight groups over all row tiles: one group a block while
+// there are few (long stages, a deep ring: nothing else hides the latency), else blocks of two, then of
+// four with the shortest ring, several of which share a CU.
+template <int MT, int DT>
+static int fp8_stream_shape(const Fp8Args& p, const void* x, int64_t ldx, hipStream_t s) {
+  const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
+  const int64_t groups = tiles * ((p.N + 15) / 16);
+  if (groups <= 256) return fp8_stream_launch<1, MT, 2, 4, DT>(p, x, ldx, s);
+  if (groups <= 1024) return fp8_stream_launch<2, MT, 1, 3, DT>(p, x, ldx, s);
+  return fp8_stream_launch<4, MT, 1, 2, DT>(p, x, ldx, s);
+}
+
+// Whether the products of M rows (of E experts: E > 0) run on the tiles: each streaming block brings its weight rows
+// in again for its 32 rows, and a block's scales of all of K have to fit the LDS.
+constexpr int64_t kStreamK = 16384;
+static bool fp8_takes_tiles(int64_t M, int64_t N, int64_t K, int64_t E) {
+  if (K == 0 || K > kStreamK) return true;
+  const int64_t groups = (E ? expert_tiles_max(M, E, 32) : (M + 31) / 32) * ((N + 15) / 16);
+  return E ? M > 16 * E : M > 16 && groups > 1024;
+}
+
 static int fp8_product(const Fp8Args& p, hipStream_t s) {
   LSK_REQUIRE(fp8_reach(p), "fp8 product: M=%lld N=%lld K=%d beyond 31-bit offsets", (long long)p.M, (long long)p.N, p.K);
-  return fp8_tile_launch<64, 64, 2, 2, 2>(p, s);
+  const int64_t E = p.offs ? p.E : 0, per = E ? 2 * p.M / E : p.M;
+  if (!fp8_takes_tiles(p.M, p.N, p.K, E))
+    return per <= 16 ? fp8_stream_shape<1, -1>(p, nullptr, 0, s) : fp8_stream_shape<2, -1>(p, nullptr, 0, s);
+  auto tiles = [&](int64_t bm, int64_t bn) { return fp8_row_tiles(p, (int)bm) * ((p.N + bn - 1) / bn); };
+  if (p.out_dtype != LSK_F32 && tiles(256, 256) >= 200) return fp8_tile_launch<256, 256, 2, 4, 2>(p, s);
+  if (tiles(128, 128) >= 400) return fp8_tile_launch<128, 128, 2, 2, 2>(p, s);
+  if (tiles(64, 128) >= 400) return fp8_tile_launch<64, 128, 2, 2, 2>(p, s);
+  return fp8_tile_launch<64, 64, 2, 2, 4>(p, s);
+}
+
+// Whether a linear's few rows are quantised in the product's launch: every block quantises them all.
+static bool fp8_fuses(int64_t M, int64_t K) { return K > 0 && (M == 1 ? K <= kStreamK : M <= 16 && M * K <= 8192); }
+
+static int fp8_stream_fused(const Fp8Args& p, const void* x, int x_dtype, int64_t ldx, hipStream_t s) {
+  if (x_dtype == LSK_F32) return fp8_stream_shape<1, LSK_F32>(p, x, ldx, s);
+  if (x_dtype == LSK_BF16) return fp8_stream_shape<1, LSK_BF16>(p, x, ldx, s);
+  return fp8_stream_shape<1, LSK_F16>(p, x, ldx, s);
 }
 
 }  // namespace lsk
@@ -383,6 +684,7 @@ extern "C" int lsk_gemm_fp8(const uint8_t* a, const float* a_scale, int64_t scal
 
 // The quantised rows come first in the workspace, then their scales, block by block.
 extern "C" int64_t lsk_linear_fp8_workspace(int64_t M, int64_t N, int64_t K) {
+  if (lsk::fp8_fuses(M, K)) return 0;
   return lsk::up256(M * K) + lsk::up256(4 * M * ((K + 127) / 128));
 }
 
@@ -407,6 +709,10 @@ extern "C" int lsk_linear_fp8(const void* x, int x_dtype, int64_t ldx, int64_t M
   p.lda = p.ldw = K, p.sm = 1, p.sb = M, p.ldsw = (K + 127) / 128;
   p.M = M, p.N = N, p.K = (int)K;
   p.bias = bias, p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
+  if (lsk::fp8_fuses(M, K)) {
+    LSK_REQUIRE(lsk::fp8_reach(p), "lsk_linear_fp8: N=%lld K=%lld beyond 31-bit offsets", (long long)N, (long long)K);
+    return lsk::fp8_stream_fused(p, x, x_dtype, ldx, s);
+  }
   int rows;
   LSK_REQUIRE(K == 0 || grid_ok(lsk::quantize_rows_blocks(M, K, rows), 256), "lsk_linear_fp8: grid too large");
   if (K > 0 && (rc = lsk::quantize_rows_launch(x, x_dtype, M, K, ldx, q, qs, 1, M, s))) return rc;

@@ -63,8 +63,8 @@ LSK_DEV v4f fp8_scaled(v4f p, float s, v4f acc) {
 
 template <int BM, int BN, int WM, int WN, int RING>
 struct Fp8Cfg {
-  static_assert(WM * WN == 4, "four waves");
-  static_assert(RING >= 2, "ring of stages");
+  static_assert(WM * WN == 8 || WM * WN == 4, "eight waves (ping-pong) or four");
+  static_assert(RING >= 2 && (WM * WN == 4 || RING == 2), "ring of stages");
   static constexpr int kThreads = WM * WN * 64, kBM = BM, kBN = BN, kWM = WM, kWN = WN, kRing = RING;
   static constexpr int kNB = BN > 128 ? BN / 128 : 1;  // weight scales of a stage
   static_assert(BM % 64 == 0 && BM + kNB <= kThreads, "one scale a thread");
@@ -82,51 +82,51 @@ struct Fp8Cfg {
   typedef v4f Acc[TM][TN];
 };
 
-// This thread's part of a tile's loads: its rows' offsets in the resources over the tile's codes, its
-// scale's in the one over the tile's scales (kOob: no row), and the bytes between the scales of two stages.
-template <class C>
-struct Fp8Rows {
-  uint32_t a[C::kLA], b[C::kLB], s;
-  uint32_t sta;
+// Where a tile's operands lie: resources over its rows from its first one on, the bytes from a row to the next, how
+// many rows there are, and this thread's scale in the resource over the tile's scales (kOob: none) with the bytes
+// between the scales of two stages.
+struct Fp8Tile {
+  __amdgpu_buffer_rsrc_t ra, rb, rsa, rsb;
+  int lda, ldb, rows_a, rows_b;
+  uint32_t s, sta;
 };
 
 template <int BM, int BN, int WM, int WN, int RING, bool EXACT>
-LSK_DEV void fp8_mainloop(typename Fp8Cfg<BM, BN, WM, WN, RING>::Acc& acc, __amdgpu_buffer_rsrc_t ra,
-                          __amdgpu_buffer_rsrc_t rb, __amdgpu_buffer_rsrc_t rsa, __amdgpu_buffer_rsrc_t rsb,
-                          const Fp8Rows<Fp8Cfg<BM, BN, WM, WN, RING>>& t, int K, char* smem) {
+LSK_DEV void fp8_mainloop(typename Fp8Cfg<BM, BN, WM, WN, RING>::Acc& acc, const Fp8Tile& t, int K, char* smem) {
   using C = Fp8Cfg<BM, BN, WM, WN, RING>;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int wm = wave / C::kWN, wn = wave % C::kWN;
   const int nk = (K + 127) / 128;
   const bool sc_a = wave * 64 < C::kBM;  // (a wave's scales are all the rows' or all the weights')
-  const __amdgpu_buffer_rsrc_t rs = sc_a ? rsa : rsb;
+  const __amdgpu_buffer_rsrc_t rs = sc_a ? t.rsa : t.rsb;
   const uint32_t st = sc_a ? t.sta : 4;
 
-  int ka[C::kLA], kb[C::kLB];
-#pragma unroll
-  for (int j = 0; j < C::kLA; ++j) {
-    int r;
-    pp_slot<C::kThreads, 8>(tid, j, r, ka[j]);
-  }
-#pragma unroll
-  for (int j = 0; j < C::kLB; ++j) {
-    int r;
-    pp_slot<C::kThreads, 8>(tid, j, r, kb[j]);
-  }
-  // (chunks past K, and past the last stage, read zeros)
-  auto issue = [&](int s) {
-    char* base = smem + (s % C::kRing) * C::kStage;
+  // A thread loads one chunk of every kThreads / 8-th row, the same chunk of each: its first row's offset is a
+  // lane's, the rest is added by a scalar, which the range check leaves out.
+  constexpr int kStep = C::kThreads / 8;
+  static_assert(kStep % 16 == 0, "rows a step apart share their swizzle");
+  int r0, kc;
+  pp_slot<C::kThreads, 8>(tid, 0, r0, kc);
+  const uint32_t offa = (uint32_t)(r0 * t.lda + kc), offb = (uint32_t)(r0 * t.ldb + kc);
+  // Load l of stage s (chunks past K, and past the last stage, read zeros, and so do rows past the last).
+  auto load = [&](int s, int l) {
+    char* base = smem + (s % C::kRing) * C::kStage + wave * 1024;
     const int k0 = s * 128;
+    const bool in = k0 + kc < K;
+    if (l < C::kLA)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(t.ra, (lds_void_t)(base + l * C::kThreads * 16), 16,
+                                               in && r0 + l * kStep < t.rows_a ? offa : kOob, k0 + l * kStep * t.lda, 0, 0);
+    else if (l < C::kLA + C::kLB)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(t.rb, (lds_void_t)(base + l * C::kThreads * 16), 16,
+                                               in && r0 + (l - C::kLA) * kStep < t.rows_b ? offb : kOob,
+                                               k0 + (l - C::kLA) * kStep * t.ldb, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t)(base + C::kStageA + C::kStageB - wave * 768), 4,
+                                               s < nk ? t.s : kOob, (int)((uint32_t)s * st), 0, 0);
+  };
+  auto issue = [&](int s) {
 #pragma unroll
-    for (int j = 0; j < C::kLA; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void_t)(base + (j * C::kThreads + wave * 64) * 16), 16,
-                                               k0 + ka[j] < K ? t.a[j] + (uint32_t)(k0 + ka[j]) : kOob, 0, 0, 0);
-#pragma unroll
-    for (int j = 0; j < C::kLB; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void_t)(base + C::kStageA + (j * C::kThreads + wave * 64) * 16), 16,
-                                               k0 + kb[j] < K ? t.b[j] + (uint32_t)(k0 + kb[j]) : kOob, 0, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t)(base + C::kStageA + C::kStageB + wave * 256), 4,
-                                             s < nk ? t.s + (uint32_t)s * st : kOob, 0, 0, 0);
+    for (int l = 0; l < C::kPer; ++l) load(s, l);
   };
 
   const int lr = lane & 15, q = lane >> 4, sw = pp_swz<8>(lr);
@@ -136,13 +136,13 @@ LSK_DEV void fp8_mainloop(typename Fp8Cfg<BM, BN, WM, WN, RING>::Acc& acc, __amd
 
   struct Frag {
     v8i a[C::TM], b[C::TN];
-    float sa[C::TM], sb;
+    float s[C::TM];
   };
   auto read = [&](int kt, Frag& f) {
     const char* base = smem + (kt % C::kRing) * C::kStage;
-    f.sb = *(const float*)(base + sB);
+    const float sb = *(const float*)(base + sB);
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i) f.sa[i] = *(const float*)(base + sA + i * 64);
+    for (int i = 0; i < C::TM; ++i) f.s[i] = f32_mul(*(const float*)(base + sA + i * 64), sb);
 #pragma unroll
     for (int j = 0; j < C::TN; ++j)
       f.b[j] = fp8_operand(*(const v4i*)(base + offB + j * 2048 + lo), *(const v4i*)(base + offB + j * 2048 + hi));
@@ -150,29 +150,114 @@ LSK_DEV void fp8_mainloop(typename Fp8Cfg<BM, BN, WM, WN, RING>::Acc& acc, __amd
     for (int i = 0; i < C::TM; ++i)
       f.a[i] = fp8_operand(*(const v4i*)(base + offA + i * 2048 + lo), *(const v4i*)(base + offA + i * 2048 + hi));
   };
-  auto multiply = [&](const Frag& f) {
+  // Three products ahead of the FMAs that use them: a result takes the matrix core's eight passes and three more to
+  // come back, and a wave that waited for each would leave the core idle as long (256 x 256 tiles, 4096 rows of 28672
+  // x 4096: 577 us as the compiler ordered it, 452 two ahead, 439 three).
+  constexpr int kTiles = C::TM * C::TN, kDepth = kTiles < 3 ? kTiles : 3;
+  constexpr int kEvery = kTiles / C::kPer > 0 ? kTiles / C::kPer : 1;  // products to a load
+  static_assert(C::kThreads == 256 || kTiles >= C::kPer, "a stage's loads fit among its products");
+  // with: the loads of stage s among the products.
+  auto multiply = [&](const Frag& f, auto with, int s) {
+    constexpr bool kWith = decltype(with)::value;
+    if constexpr (EXACT) {
+      if (kWith) issue(s);
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i) {
-      const float s = f32_mul(f.sa[i], f.sb);
+      for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-      for (int j = 0; j < C::TN; ++j) acc[i][j] = fp8_scaled(fp8_block<EXACT>(f.b[j], f.a[i]), s, acc[i][j]);
+        for (int j = 0; j < C::TN; ++j) acc[i][j] = fp8_scaled(fp8_block<true>(f.b[j], f.a[i]), f.s[i], acc[i][j]);
+    } else {
+      v4f p[kDepth + 1];
+#pragma unroll
+      for (int n = 0; n < kDepth; ++n) p[n] = fp8_block<false>(f.b[n % C::TN], f.a[n / C::TN]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        const int z = n + kDepth;
+        if (z < kTiles) p[z % (kDepth + 1)] = fp8_block<false>(f.b[z % C::TN], f.a[z / C::TN]);
+        if constexpr (kWith)
+          if (n % kEvery == 0 && n / kEvery < C::kPer) load(s, n / kEvery);
+        acc[n / C::TN][n % C::TN] = fp8_scaled(p[n % (kDepth + 1)], f.s[n / C::TN], acc[n / C::TN][n % C::TN]);
+        __builtin_amdgcn_sched_barrier(0);  // (in this order)
+      }
     }
   };
 
-  // One barrier a stage: a wave's own loads of stage kt are complete when at most the RING - 2 younger
-  // stages are outstanding, every wave's at the barrier; the slot of stage kt - 1, which every wave has read
-  // by then, takes stage kt + RING - 1.
   Frag f;
+  if constexpr (C::kThreads == 256) {
+    if constexpr (RING < 4) {
+      // One barrier a stage: a wave's own loads of stage kt are complete when at most the RING - 2 younger
+      // stages are outstanding, every wave's at the barrier; the slot of stage kt - 1, which every wave has read
+      // by then, takes stage kt + RING - 1.
 #pragma unroll
-  for (int s = 0; s < RING - 1; ++s) issue(s);
-  for (int kt = 0; kt < nk; ++kt) {
-    wait_vm<(RING - 2) * C::kPer>();
+      for (int s = 0; s < RING - 1; ++s) issue(s);
+      for (int kt = 0; kt < nk; ++kt) {
+        wait_vm<(RING - 2) * C::kPer>();
+        phase_barrier();
+        issue(kt + RING - 1);
+        read(kt, f);
+        multiply(f, std::false_type{}, 0);
+      }
+    } else {
+      // The same with a stage's fragments read a stage ahead of its products.
+      Frag g;
+#pragma unroll
+      for (int s = 0; s < RING - 1; ++s) issue(s);
+      wait_vm<(RING - 2) * C::kPer>();
+      phase_barrier();
+      read(0, f);
+      auto step = [&](int kt, Frag& now, Frag& next) {
+        compiler_fence();  // (the reads of the stage before stay on their side of the barrier)
+        wait_vm<(RING - 3) * C::kPer>();
+        phase_barrier();
+        issue(kt + RING - 1);
+        read(kt + 1, next);
+        multiply(now, std::false_type{}, 0);
+      };
+      int kt = 0;
+      for (; kt + 2 <= nk; kt += 2) {
+        step(kt, f, g);
+        step(kt + 1, g, f);
+      }
+      if (kt < nk) step(kt, f, g);
+    }
+    wait_vm<0>();
+  } else {
+    // Two groups of four waves, half a period apart: while one multiplies stage kt the other reads its fragments
+    // (group 0 reads in period 2 kt and multiplies in 2 kt + 1, group 1 a period later).  Both request stage kt + 1 in
+    // period 2 kt, into the slot of stage kt - 1, which group 1 has read by the end of 2 kt - 1, and wait for it at the
+    // end of 2 kt + 1.  A CU has about 32 KB of requests on their way, half a stage, and a wave that issues more
+    // waits: so group 0 issues behind its reads and group 1 one request to every three products (all of them ahead of
+    // the products 495 us for the case above, so 452).
+    issue(0);
+    wait_vm<0>();
     phase_barrier();
-    issue(kt + RING - 1);
-    read(kt, f);
-    multiply(f);
+    if (wave < 4) {
+      for (int kt = 0; kt < nk; ++kt) {
+        read(kt, f);
+        __builtin_amdgcn_sched_barrier(0);
+        issue(kt + 1);
+        wait_lgkm0();
+        phase_barrier();
+        multiply(f, std::false_type{}, 0);
+        __builtin_amdgcn_sched_barrier(0);  // (the wait stays behind the products)
+        wait_vm<0>();
+        phase_barrier();
+      }
+      phase_barrier();
+    } else {
+      issue(1);
+      phase_barrier();
+      for (int kt = 0; kt < nk; ++kt) {
+        read(kt, f);
+        wait_lgkm0();
+        wait_vm<0>();
+        phase_barrier();
+        multiply(f, std::true_type{}, kt + 2);
+        phase_barrier();
+      }
+      wait_vm<0>();
+    }
   }
-  wait_vm<0>();
 }
 
 }  // namespace lsk
