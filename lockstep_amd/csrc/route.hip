@@ -11,6 +11,8 @@
 // gfx950 computes 64-bit FMAs at the rate of 32-bit ones.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "lsk_common.h"
 
 namespace lsk {
@@ -47,47 +49,122 @@ LSK_DEV double wave_sum(double v) {
   return v;
 }
 
-// A wave a token; lane l holds experts l, l + 64, ...
+LSK_DEV double lane_value(double v, int l) {  // l the same in every lane
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, l);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), l);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+// The value of the lane that a DPP control names; without one (or in a row that the mask leaves out), `old`.
+template <int CTRL, int ROWS = 0xf>
+LSK_DEV double dpp_value(double old, double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v), o = (uint64_t)__double_as_longlong(old);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)o, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)(o >> 32), (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+  return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+// The larger one; a NaN is passed over.
+LSK_DEV double larger(double a, double b) { return __builtin_fmax(a, b); }
+constexpr double kOut = __builtin_nan("");  // not to be chosen, where no score is a NaN
+
+// larger() over the wave, in every lane.
+LSK_DEV double wave_larger(double v) {
+  v = larger(v, dpp_value<0xb1>(v, v));        // quad [1,0,3,2]
+  v = larger(v, dpp_value<0x4e>(v, v));        // quad [2,3,0,1]
+  v = larger(v, dpp_value<0x141>(v, v));       // half-row mirror
+  v = larger(v, dpp_value<0x140>(v, v));       // row mirror
+  v = larger(v, dpp_value<0x142, 0xa>(v, v));  // row bcast 15
+  v = larger(v, dpp_value<0x143, 0xc>(v, v));  // row bcast 31
+  return lane_value(v, 63);
+}
+
+// The choice among c (no NaNs but kOut), a round for each of the k: the largest upper word of rank_of over the wave, of
+// those that hold it the largest lower word where there are several (scores within 2^-20 of each other), and of those the
+// lowest expert.  Lane z gets the z-th expert and its score.  (A maximum of whole numbers over the wave is one instruction
+// a step, of 64-bit numbers three: 8192 tokens, 256 experts, 8 of them: 13.6 us with those.)
 template <int EPL>
-__global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
-  __shared__ double score[4][64];
-  const int lane = threadIdx.x & 63, wave = wave_id();
-  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
-  if (t >= p.T) return;
-  double s[EPL], c[EPL];
+LSK_DEV void choose(const RouteArgs& p, const double (&s)[EPL], const double (&c)[EPL], double& chosen, int& expert, double& sum) {
+  const int lane = threadIdx.x & 63;
+  uint32_t hi[EPL], lo[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    const uint64_t r = c[j] != c[j] ? 0 : rank_of(c[j]);
+    hi[j] = (uint32_t)(r >> 32), lo[j] = (uint32_t)r;
+  }
+  for (int z = 0; z < p.k; ++z) {
+    uint32_t top = hi[0];
+#pragma unroll
+    for (int j = 1; j < EPL; ++j) top = top > hi[j] ? top : hi[j];
+    top = wave_max_u32(top);
+    uint64_t at[EPL];
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) at[j] = __builtin_amdgcn_ballot_w64(hi[j] == top), n += __builtin_popcountll(at[j]);
+    if (n > 1) {
+      uint32_t low = 0;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) low = hi[j] == top && lo[j] > low ? lo[j] : low;
+      low = wave_max_u32(low);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) at[j] &= __builtin_amdgcn_ballot_w64(lo[j] == low);
+    }
+    double v = 0;
+    int e = 0;
+#pragma unroll
+    for (int j = EPL - 1; j >= 0; --j) {  // (the lowest j last)
+      if (!at[j]) continue;
+      const int l = __builtin_ctzll(at[j]);
+      v = lane_value(s[j], l);
+      e = l + 64 * j;
+    }
+    sum = z ? sum + v : v;
+    if (lane == z) chosen = v, expert = e;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j)
+      if (e == lane + 64 * j) hi[j] = lo[j] = 0;
+  }
+}
+
+// The groups that stay (no NaNs in c; a sum may be one, of both infinities): 64 / groups lanes, rounded down to a power of two, look a group over from LDS for
+// its two largest; then lane g compares group g with every other.
+LSK_DEV uint64_t kept_groups(const RouteArgs& p, const double* c) {
+  const int lane = threadIdx.x & 63, size = p.E / p.groups;
+  int per = 1;
+  while (2 * per * p.groups <= 64) per *= 2;
+  const int g = lane / per;
+  double a = kOut, b = kOut;  // the two largest
+  auto put = [&](double x, double y) {  // two more, x the larger
+    const double lo = __builtin_fmin(a, x);  // (of a and nothing: a, which then is x: nothing)
+    const bool none = a != a || x != x;
+    a = larger(a, x);
+    b = larger(larger(b, y), none ? kOut : lo);
+  };
+  if (g < p.groups)
+    for (int i = lane % per; i < size; i += per) put(c[g * size + i], kOut);
+  if (per > 1) put(dpp_value<0xb1>(kOut, a), dpp_value<0xb1>(kOut, b));
+  if (per > 2) put(dpp_value<0x4e>(kOut, a), dpp_value<0x4e>(kOut, b));
+  if (per > 4) put(dpp_value<0x141>(kOut, a), dpp_value<0x141>(kOut, b));  // (a quad's lanes hold the same by now)
+  if (per > 8) put(dpp_value<0x140>(kOut, a), dpp_value<0x140>(kOut, b));
+  if (per > 16) put(__shfl_xor(a, 16, 64), __shfl_xor(b, 16, 64));
+  const double sum = p.group_top == 2 ? a + b : a;
+  // (bring group g's to lane g)
+  const double mine = __shfl(sum, lane * per & 63, 64);
+  int ahead = 0;
+  for (int h = 0; h < p.groups; ++h) {
+    const double o = lane_value(sum, h * per);
+    ahead += (o == o && mine != mine) || o > mine || ((o == mine || (o != o && mine != mine)) && h < lane);
+  }
+  return __builtin_amdgcn_ballot_w64(lane < p.groups && ahead < p.keep);
+}
+
+// The same two where scores are NaNs: by rank_of, the slow way.
+template <int EPL>
+LSK_DEV void choose_ranked(const RouteArgs& p, const double (&s)[EPL], const double (&c)[EPL], double& chosen, int& expert,
+                           double& total) {
+  const int lane = threadIdx.x & 63;
   uint64_t r[EPL];
-  double top = -__builtin_inf();
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int e = lane + 64 * j;
-    s[j] = e < p.E ? (double)load_as_f32(p.g, p.g_dtype, t * p.ldg + e) : -__builtin_inf();
-    top = s[j] > top ? s[j] : top;
-  }
-  if (p.sigmoid) {
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) s[j] = 1.0 / (1.0 + exp(-s[j]));
-  } else {
-    for (int o = 32; o > 0; o >>= 1) {
-      const double q = __shfl_xor(top, o, 64);
-      top = q > top ? q : top;
-    }
-    double sum = 0;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      // (nothing above -infinity: every score is 0; a NaN makes the sum one)
-      s[j] = s[j] == -__builtin_inf() ? 0.0 : exp(s[j] - top);
-      sum += s[j];
-    }
-    sum = wave_sum(sum);
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) s[j] = sum == 0.0 ? 0.0 : s[j] / sum;
-  }
-#pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int e = lane + 64 * j;
-    c[j] = e < p.E && p.bias ? s[j] + (double)p.bias[e] : s[j];
-    r[j] = e < p.E ? rank_of(c[j]) : 0;
-  }
+  for (int j = 0; j < EPL; ++j) r[j] = lane + 64 * j < p.E ? rank_of(c[j]) : 0;
   if (p.keep < p.groups) {
     const int size = p.E / p.groups;
     double mine = 0;
@@ -103,13 +180,11 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
           const int e = lane + 64 * j;
           if (e / size == g && e != skip && r[j] > best) best = r[j], at = e;
         }
-        const int own = at;
         wave_best(best, at);
 #pragma unroll
         for (int j = 0; j < EPL; ++j)
           if (lane + 64 * j == at) v = c[j];
         v = __shfl(v, at & 63, 64);
-        (void)own;
         sum = z ? sum + v : v;
         skip = at;
       }
@@ -129,8 +204,6 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
       if (e < p.E && !(kept >> (e / size) & 1)) r[j] = 0;
     }
   }
-  double chosen = 0;  // lane z: the z-th chosen expert's score
-  int expert = 0;
   for (int z = 0; z < p.k; ++z) {
     uint64_t best = 0;
     int at = 1 << 30;
@@ -143,11 +216,78 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
     for (int j = 0; j < EPL; ++j)
       if (lane + 64 * j == at) v = s[j], r[j] = 0;
     v = __shfl(v, at & 63, 64);
+    total = z ? total + v : v;
     if (lane == z) chosen = v, expert = at;
   }
-  double sum = 0;
-  score[wave][lane] = chosen;
-  for (int z = 0; z < p.k; ++z) sum += score[wave][z];  // (a wave's own LDS operations run in order)
+}
+
+// A wave a token; lane l holds experts l, l + 64, ...
+template <int EPL, bool GROUPS>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
+  __shared__ double values[GROUPS ? 4 : 1][GROUPS ? 64 * EPL : 1];
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+  if (t >= p.T) return;
+  double s[EPL], c[EPL];
+  double top = -__builtin_inf();
+  // (one switch for all of a lane's loads: they go out together)
+  auto load = [&](auto dt) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      const int e = lane + 64 * j;
+      s[j] = e < p.E ? (double)load_as_f32(p.g, decltype(dt)::value, t * p.ldg + e) : -__builtin_inf();
+    }
+  };
+  float bias[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) bias[j] = p.bias && lane + 64 * j < p.E ? p.bias[lane + 64 * j] : 0.0f;
+  if (p.g_dtype == LSK_F32) load(std::integral_constant<int, LSK_F32>{});
+  else if (p.g_dtype == LSK_BF16) load(std::integral_constant<int, LSK_BF16>{});
+  else load(std::integral_constant<int, LSK_F16>{});
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) top = larger(top, s[j]);
+  if (p.sigmoid) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) s[j] = 1.0 / (1.0 + exp(-s[j]));
+  } else {
+    top = wave_larger(top);
+    double sum = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      // (nothing above -infinity: every score is 0; a NaN makes the sum one)
+      s[j] = s[j] == -__builtin_inf() ? 0.0 : exp(s[j] - top);
+      sum += s[j];
+    }
+    sum = wave_sum(sum);
+    const double scale = 1.0 / sum;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) s[j] = sum == 0.0 ? 0.0 : s[j] * scale;
+  }
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    const int e = lane + 64 * j;
+    c[j] = s[j] + (double)bias[j];
+    nan |= e < p.E && c[j] != c[j];
+    if (e >= p.E) c[j] = kOut;
+  }
+  double chosen = 0, sum = 0;
+  int expert = 0;
+  if (__builtin_amdgcn_ballot_w64(nan)) {
+    choose_ranked<EPL>(p, s, c, chosen, expert, sum);
+  } else {
+    if constexpr (GROUPS) {
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) values[wave][lane + 64 * j] = c[j];
+      // (a wave's own LDS operations run in order)
+      const uint64_t kept = kept_groups(p, values[wave]);
+      const uint32_t recip = (1u << 20) / (uint32_t)(p.E / p.groups) + 1;  // e / size for e < 1024, size < 1024
+#pragma unroll
+      for (int j = 0; j < EPL; ++j)
+        if (!(kept >> ((lane + 64 * j) * recip >> 20 & 63) & 1)) c[j] = kOut;
+    }
+    choose<EPL>(p, s, c, chosen, expert, sum);
+  }
   if (lane < p.k) {
     double w = p.renorm ? (sum == 0.0 ? 0.0 : chosen / sum) : chosen;
     w *= p.factor;
@@ -180,7 +320,10 @@ extern "C" int lsk_route_experts(const void* g, int g_dtype, int64_t ldg, int64_
                    idx, w, w_dtype};
   const dim3 grid((unsigned)((T + 3) / 4)), blk(256);
   hipStream_t s = (hipStream_t)stream;
-  auto run = [&](auto epl) { hipLaunchKernelGGL((lsk::route_kernel<decltype(epl)::value>), grid, blk, 0, s, p); };
+  auto run = [&](auto epl) {
+    if (keep_groups < groups) hipLaunchKernelGGL((lsk::route_kernel<decltype(epl)::value, true>), grid, blk, 0, s, p);
+    else hipLaunchKernelGGL((lsk::route_kernel<decltype(epl)::value, false>), grid, blk, 0, s, p);
+  };
   if (E <= 64) run(std::integral_constant<int, 1>{});
   else if (E <= 128) run(std::integral_constant<int, 2>{});
   else if (E <= 256) run(std::integral_constant<int, 4>{});

@@ -109,7 +109,9 @@ def test_infinities_nans_and_rows_without_an_expert(scoring):
     bias = (0.1 * g.standard_normal(E)).astype(np.float32)
     banned = bias.copy()
     banned[10:] = -np.inf
-    for b in (None, bias, banned):
+    both = bias.copy()
+    both[[0, 9, 17]], both[[1, 2, 16, 18]] = np.inf, -np.inf
+    for b in (None, bias, banned, both):
         for renorm in (True, False):
             _compare(torch.from_numpy(l), 8, scoring, b, renormalize=renorm)
         _compare(torch.from_numpy(l), 8, scoring, b, 6, 2, 2)
