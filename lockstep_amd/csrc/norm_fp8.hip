@@ -22,7 +22,7 @@ struct NormFp8Args {
   const void* r;  // or null
   int64_t ldx, ldr, R;
   int N;
-  const void* g;  // [N] or null
+  const void* g;  // [N]
   int g_dtype;
   float sN, ne;
   void* h;  // [R, N] or null, row stride ldh
@@ -63,26 +63,45 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_fp8_kernel(NormFp8Args p) {
   const int lane = threadIdx.x & 63, wave = wave_id(), W = blockDim.x >> 6;
   const int64_t m = blockIdx.x;
   const int G = p.N / 8, g0 = wave * C * 64 + lane;
-  float v[C][8];
+  // (one switch on the gain's type for all of a lane's loads)
+  auto gain = [&](auto& g, int first) {
+    auto load = [&](auto gdt) {
+#pragma unroll
+      for (int c = 0; c < (int)(sizeof(g) / sizeof(g[0])); ++c)
+        if (g0 + 64 * (first + c) < G) load8<decltype(gdt)::value, VEC>(p.g, 8 * (g0 + 64 * (first + c)), g[c]);
+    };
+    if (p.g_dtype == LSK_F32) load(std::integral_constant<int, LSK_F32>{});
+    else if (p.g_dtype == LSK_BF16) load(std::integral_constant<int, LSK_BF16>{});
+    else load(std::integral_constant<int, LSK_F16>{});
+  };
+  constexpr bool kEarly = C <= 4;  // (eight groups' residuals and gains beside the values would not fit the registers)
+  constexpr int kE = kEarly ? C : 1;
+  float v[C][8], r[kE][8], g[kE][8];
+  auto residual = [&](int c, float (&w)[8]) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) w[t] = 0.0f;
+    if (p.r && g0 + 64 * c < G) load8<DT, VEC>(p.r, m * p.ldr + 8 * (g0 + 64 * c), w);
+  };
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) v[c][t] = 0.0f;
+    if (g0 + 64 * c < G) load8<DT, VEC>(p.x, m * p.ldx + 8 * (g0 + 64 * c), v[c]);
+    if constexpr (kEarly) residual(c, r[c]);
+  }
+  if constexpr (kEarly) gain(g, 0);
   float S[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int grp = g0 + 64 * c;
+    if constexpr (!kEarly) residual(c, r[0]);
+    if (p.r)
 #pragma unroll
-    for (int t = 0; t < 8; ++t) v[c][t] = 0.0f;
-    if (grp < G) {
-      load8<DT, VEC>(p.x, m * p.ldx + 8 * grp, v[c]);
-      if (p.r) {
-        float r[8];
-        load8<DT, VEC>(p.r, m * p.ldr + 8 * grp, r);
-#pragma unroll
-        for (int t = 0; t < 8; ++t) v[c][t] = round_out(DT, f32_add(v[c][t], r[t]));
-      }
-    }
+      for (int t = 0; t < 8; ++t) v[c][t] = round_out(DT, f32_add(v[c][t], r[kEarly ? c : 0][t]));
     float s = f32_mul(v[c][0], v[c][0]);
 #pragma unroll
     for (int t = 1; t < 8; ++t) s = f32_add(s, f32_mul(v[c][t], v[c][t]));
-    S[c] = grp < G ? s : -0.0f;
+    S[c] = g0 + 64 * c < G ? s : -0.0f;
+    if (p.h && g0 + 64 * c < G) store8<DT, VEC>(p.h, m * p.ldh + 8 * (g0 + 64 * c), v[c]);
   }
 #pragma unroll
   for (int c = 0; c < C; ++c) S[c] = wave_tree(S[c]);
@@ -109,17 +128,12 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_fp8_kernel(NormFp8Args p) {
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int grp = g0 + 64 * c;
-    if (p.h && grp < G) store8<DT, VEC>(p.h, m * p.ldh + 8 * grp, v[c]);
+    if constexpr (!kEarly) gain(g, c);
     float y[8];
 #pragma unroll
-    for (int t = 0; t < 8; ++t) y[t] = f32_mul(v[c][t], rs);
-    if (p.g && grp < G) {
-#pragma unroll
-      for (int t = 0; t < 8; ++t) y[t] = f32_mul(y[t], load_as_f32(p.g, p.g_dtype, 8 * grp + t));
-    }
-    if (grp >= G) {  // (beside a row's end: not to weigh in the block's maximum, a NaN sum's NaNs among them)
-#pragma unroll
-      for (int t = 0; t < 8; ++t) y[t] = 0.0f;
+    for (int t = 0; t < 8; ++t) {
+      y[t] = f32_mul(f32_mul(v[c][t], rs), g[kEarly ? c : 0][t]);
+      if (grp >= G) y[t] = 0.0f;  // (beside a row's end: not to weigh in the block's maximum, a NaN sum's NaNs among them)
     }
     float s;
     const uint2 code = quantize_row_fp8(y, s);
@@ -137,23 +151,28 @@ extern "C" int lsk_add_rmsnorm_fp8(const void* x, int x_dtype, int64_t ldx, cons
                                    int64_t N, const void* g, int g_dtype, float sN, double eps, void* h, int64_t ldh,
                                    uint8_t* q, float* scale, int64_t scale_m, int64_t scale_b, void* out, void* stream) {
   LSK_REQUIRE(lsk::is_float_dtype(x_dtype), "lsk_add_rmsnorm_fp8: x_dtype must be f32, bf16 or f16");
-  LSK_REQUIRE(!g || lsk::is_float_dtype(g_dtype), "lsk_add_rmsnorm_fp8: the gain must be f32, bf16 or f16");
+  LSK_REQUIRE(lsk::is_float_dtype(g_dtype), "lsk_add_rmsnorm_fp8: the gain must be f32, bf16 or f16");
   LSK_REQUIRE(R >= 0 && N >= 0 && N % 16 == 0 && N <= 65536, "lsk_add_rmsnorm_fp8: R=%lld, N=%lld (N a multiple of 16 up to 65536)",
               (long long)R, (long long)N);
   if (R == 0 || N == 0) return LSK_OK;
-  LSK_REQUIRE(x && q && scale, "lsk_add_rmsnorm_fp8: null pointer");
+  LSK_REQUIRE(x && g && q && scale, "lsk_add_rmsnorm_fp8: null pointer");
   LSK_REQUIRE(R == 1 || (ldx >= N && (!residual || ldr >= N) && (!h || ldh >= N)), "lsk_add_rmsnorm_fp8: leading dimension below N");
   LSK_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0, "lsk_add_rmsnorm_fp8: codes and out must be 16-byte aligned");
+  // One group a lane while 16 waves hold the row (MI355X, 1, 2, 4 and 8 groups a lane: 8192 rows of 4096 53.6, 58.5, 63.5,
+  // 64.3 us, 512 of them 6.6, 7.3, 10.4, 15.3, 16384 of 1024 27.3, 28.3, 28.2, 28.4; 235 MB in 53.6 us are 4.4 TB/s, a
+  // large copy reaches 5.0).
   int64_t P = 64;
   while (P < N / 8) P *= 2;
-  const int W = (int)(P / 64 < 16 ? P / 64 : 16), C = (int)(P / 64 / W);
+  int C = 1;
+  while (P / 64 > 16 * C) C *= 2;
+  const int W = (int)(P / 64 / C);
   LSK_REQUIRE(R <= 0x7fffffff && grid_ok(R, 64 * W), "lsk_add_rmsnorm_fp8: grid too large");
   lsk::NormFp8Args p{x, residual, ldx, ldr, R, (int)N, g, g_dtype, sN, 0.0f, h, ldh, q, scale, scale_m, scale_b, out};
   if (!(sN > 0.0f)) p.sN = (float)__builtin_sqrt((double)N);  // the width constant fl32(sqrt(N))
   p.ne = (float)((double)N * eps);  // one binary64 product, one rounding
   const int size = x_dtype == LSK_F32 ? 4 : 2;
   auto even = [&](const void* a, int64_t ld) { return !a || ((uintptr_t)a % 16 == 0 && (R == 1 || ld * size % 16 == 0)); };
-  const bool vec = even(x, ldx) && even(residual, ldr) && even(h, ldh);
+  const bool vec = even(x, ldx) && even(residual, ldr) && even(h, ldh) && (uintptr_t)g % 16 == 0;
   auto run = [&](auto dt, auto v, auto c) {
     hipLaunchKernelGGL((lsk::add_rmsnorm_fp8_kernel<decltype(dt)::value, decltype(v)::value, decltype(c)::value>),
                        dim3((unsigned)R), dim3(64 * W), 0, (hipStream_t)stream, p);

@@ -137,29 +137,33 @@ def add_rmsnorm_fp8(x, residual, weight, sN=None, eps=0.0, want_out=False):
     Returns (q float8_e4m3fn [..., N], scale f32 [..., ceil(N / 128)], h [..., N], out bf16 [..., N] =
     rmsnorm_float(h, weight) when want_out else None)."""
     L.require_cuda(x, residual, what="add_rmsnorm_fp8")
-    shp = x.shape
-    if x.dtype not in _ODT or x.dim() == 0:
+    shp, code = x.shape, _ODT.get(x.dtype)
+    if code is None or not shp:
         raise TypeError("add_rmsnorm_fp8: x must be f32, bf16 or f16 [..., N], got %s %s" % (x.dtype, tuple(shp)))
-    if residual is not None and (residual.shape != shp or residual.dtype != x.dtype):
-        raise ValueError("add_rmsnorm_fp8: residual %s %s for x %s %s"
-                         % (residual.dtype, tuple(residual.shape), x.dtype, tuple(shp)))
     N = shp[-1]
     if N % 16 or N > 65536:
         raise ValueError("add_rmsnorm_fp8: N=%d is not a multiple of 16 up to 65536" % N)
-    R, nb = shp[:-1].numel(), (N + 127) // 128
+    R, nb = x.numel() // N if N else shp[:-1].numel(), (N + 127) // 128
     x2, ldx = _rows_of(x, R, N)
-    r2, ldr = (None, 0) if residual is None else _rows_of(residual, R, N)
-    g = _gain(weight, N, x.device)
-    q = x.new_empty((R, N), dtype=ops.FP8)
+    if residual is None:
+        r2, ldr, h = None, 0, x
+    else:
+        if residual.shape != shp or residual.dtype != x.dtype:
+            raise ValueError("add_rmsnorm_fp8: residual %s %s for x %s %s"
+                             % (residual.dtype, tuple(residual.shape), x.dtype, tuple(shp)))
+        r2, ldr = _rows_of(residual, R, N)
+        h = x.new_empty(shp)
+    g = weight if weight.shape == (N,) and weight.dtype in _ODT and weight.device == x.device and weight.is_contiguous() \
+        else _gain(weight, N, x.device)
+    q = x.new_empty(shp, dtype=ops.FP8)
     scale = x.new_empty((nb, R), dtype=torch.float32)
-    h = x if residual is None else x.new_empty(shp)
     out = x.new_empty(shp, dtype=torch.bfloat16) if want_out else None
     if R and N:
-        L.call_on(x, "lsk_add_rmsnorm_fp8", x2.data_ptr(), _ODT[x.dtype], ldx, L.ptr(r2), ldr, R, N, g.data_ptr(),
-                  _ODT[g.dtype], float(sqrt_n(N) if sN is None else sN), float(eps or 0.0),
-                  None if residual is None else h.data_ptr(), N, q.data_ptr(), scale.data_ptr(), 1, R, L.ptr(out),
-                  L.stream_of(x))
-    return q.view(shp), scale.t().view(*shp[:-1], nb), h, out
+        # (sN 0: the C call computes fl32(sqrt(N)) itself)
+        L.call_on(x, "lsk_add_rmsnorm_fp8", x2.data_ptr(), code, ldx, L.ptr(r2), ldr, R, N, g.data_ptr(), _ODT[g.dtype],
+                  sN or 0.0, eps or 0.0, None if residual is None else h.data_ptr(), N, q.data_ptr(), scale.data_ptr(), 1, R,
+                  L.ptr(out), L.stream_of(x))
+    return q, scale.t() if len(shp) == 2 else scale.t().view(*shp[:-1], nb), h, out
 
 
 def _rows_of(x, R, N):
