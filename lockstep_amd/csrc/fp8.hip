@@ -403,6 +403,45 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args p, const void* 
 }
 
 // ---------------------------------------------------------------- tiles
+// The tile's outputs: a 16-row strip at a time through the wave's part of LDS, out of it four consecutive columns a lane.
+template <class C, int ODT>
+LSK_DEV void fp8_tile_out(const Fp8Args& p, const typename C::Acc& acc, char* smem, int m0, int n0, int rows_a, int rows_w,
+                          int vec) {
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int wm = wave / C::kWN, wn = wave % C::kWN;
+  float* strip = (float*)(smem + wave * 16 * C::kLdc * 4);
+  constexpr int kLanes = C::WTN / 4, kRows = 64 / kLanes;  // lanes a row, rows an instruction
+  const int col = wn * C::WTN + lane % kLanes * 4, size = ODT == LSK_F32 ? 4 : 2;
+  float b[4] = {0, 0, 0, 0};
+  if (p.bias)
+#pragma unroll
+    for (int z = 0; z < 4; ++z)
+      if (col + z < rows_w) b[z] = p.bias[n0 + col + z];
+  int row = wm * C::WTM + lane / kLanes;
+  const int64_t step = (int64_t)kRows * p.ldo * size;
+  char* o = (char*)p.out + ((int64_t)(m0 + row) * p.ldo + n0 + col) * size;
+  const bool whole = vec && col + 4 <= rows_w;
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) *(v4f*)(strip + (lane & 15) * C::kLdc + j * 16 + 4 * (lane >> 4)) = acc[i][j];
+    // (a wave's own LDS operations run in order)
+#pragma unroll
+    for (int r0 = 0; r0 < 16; r0 += kRows, row += kRows, o += step) {
+      v4f v = *(const v4f*)(strip + (r0 + lane / kLanes) * C::kLdc + lane % kLanes * 4);
+      if (row >= rows_a || col >= rows_w) continue;
+      if (p.bias)
+#pragma unroll
+        for (int z = 0; z < 4; ++z) v[z] = f32_add(v[z], b[z]);
+      if (whole) {
+        store_quad(o, ODT, v);
+      } else {
+        for (int z = 0; z < 4 && col + z < rows_w; ++z) store_out(o, ODT, z, v[z]);
+      }
+    }
+  }
+}
+
 // A BM x BN tile: tiles walk kGroupM row tiles down a column of weight tiles inside each XCD's run
 // of them, so the row tiles that share a weight tile run together on one L2.
 template <int BM, int BN, int WM, int WN, int RING, bool EXACT, bool GROUPED>
@@ -459,39 +498,9 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8Args p, int64
 #endif
   __syncthreads();
 
-  // a 16-row strip at a time through the wave's part of LDS, out of it four consecutive columns a lane
-  const int wm = wave / C::kWN, wn = wave % C::kWN;
-  float* strip = (float*)(smem + wave * 16 * C::kLdc * 4);
-  constexpr int kLanes = C::WTN / 4, kRows = 64 / kLanes;  // lanes a row, rows an instruction
-  const int col = wn * C::WTN + lane % kLanes * 4, size = p.out_dtype == LSK_F32 ? 4 : 2;
-  float b[4] = {0, 0, 0, 0};
-  if (p.bias)
-#pragma unroll
-    for (int z = 0; z < 4; ++z)
-      if (col + z < rows_w) b[z] = p.bias[n0 + col + z];
-  int row = wm * C::WTM + lane / kLanes;
-  const int64_t step = (int64_t)kRows * p.ldo * size;
-  char* o = (char*)p.out + ((int64_t)(m0 + row) * p.ldo + n0 + col) * size;
-  const bool whole = vec && col + 4 <= rows_w;
-#pragma unroll
-  for (int i = 0; i < C::TM; ++i) {
-#pragma unroll
-    for (int j = 0; j < C::TN; ++j) *(v4f*)(strip + (lane & 15) * C::kLdc + j * 16 + 4 * (lane >> 4)) = acc[i][j];
-    // (a wave's own LDS operations run in order)
-#pragma unroll
-    for (int r0 = 0; r0 < 16; r0 += kRows, row += kRows, o += step) {
-      v4f v = *(const v4f*)(strip + (r0 + lane / kLanes) * C::kLdc + lane % kLanes * 4);
-      if (row >= rows_a || col >= rows_w) continue;
-      if (p.bias)
-#pragma unroll
-        for (int z = 0; z < 4; ++z) v[z] = f32_add(v[z], b[z]);
-      if (whole) {
-        store_quad(o, p.out_dtype, v);
-      } else {
-        for (int z = 0; z < 4 && col + z < rows_w; ++z) store_out(o, p.out_dtype, z, v[z]);
-      }
-    }
-  }
+  if constexpr (EXACT) fp8_tile_out<C, LSK_F32>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
+  else if (p.out_dtype == LSK_BF16) fp8_tile_out<C, LSK_BF16>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
+  else fp8_tile_out<C, LSK_F16>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
 }
 
 static int64_t fp8_row_tiles(const Fp8Args& p, int bm) {
