@@ -404,7 +404,10 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args p, const void* 
 
 // ---------------------------------------------------------------- tiles
 // The tile's outputs: a 16-row strip at a time through the wave's part of LDS, out of it four consecutive columns a lane.
-template <class C, int ODT>
+// LINES: rows begin on lines of 128 bytes, and whole lines go past the caches (store_quad; MI355X, past them and not:
+// 4096 rows of 28672 x 4096 426 us, 456; 4096 of 4096 x 2048 39.4, 41.5); lines that two rows share are put together in
+// the L2 (3102 rows of 13016 x 128 47.9, 41.7).
+template <class C, int ODT, bool LINES>
 LSK_DEV void fp8_tile_out(const Fp8Args& p, const typename C::Acc& acc, char* smem, int m0, int n0, int rows_a, int rows_w,
                           int vec) {
   const int lane = threadIdx.x & 63, wave = wave_id();
@@ -434,7 +437,8 @@ LSK_DEV void fp8_tile_out(const Fp8Args& p, const typename C::Acc& acc, char* sm
 #pragma unroll
         for (int z = 0; z < 4; ++z) v[z] = f32_add(v[z], b[z]);
       if (whole) {
-        store_quad(o, ODT, v);
+        store_quad<LINES>(o, ODT, v);
+        __asm__ volatile("" ::: "memory");  // (no 16-byte stores: store16_split)
       } else {
         for (int z = 0; z < 4 && col + z < rows_w; ++z) store_out(o, ODT, z, v[z]);
       }
@@ -498,9 +502,13 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8Args p, int64
 #endif
   __syncthreads();
 
-  if constexpr (EXACT) fp8_tile_out<C, LSK_F32>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
-  else if (p.out_dtype == LSK_BF16) fp8_tile_out<C, LSK_BF16>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
-  else fp8_tile_out<C, LSK_F16>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
+  auto out = [&](auto odt) {
+    if (vec == 2) fp8_tile_out<C, decltype(odt)::value, true>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
+    else fp8_tile_out<C, decltype(odt)::value, false>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
+  };
+  if constexpr (EXACT) out(std::integral_constant<int, LSK_F32>{});
+  else if (p.out_dtype == LSK_BF16) out(std::integral_constant<int, LSK_BF16>{});
+  else out(std::integral_constant<int, LSK_F16>{});
 }
 
 static int64_t fp8_row_tiles(const Fp8Args& p, int bm) {
@@ -512,7 +520,8 @@ static int fp8_tile_launch(const Fp8Args& p, hipStream_t s) {
   using C = Fp8Cfg<BM, BN, WM, WN, RING>;
   const int64_t mtiles = fp8_row_tiles(p, BM), blocks = mtiles * ((p.N + BN - 1) / BN);
   LSK_REQUIRE(grid_ok(blocks, C::kThreads) && blocks <= 0x7fffffff, "fp8 product: grid too large");
-  const int vec = out_vec_ok(p.out, p.out_dtype, p.ldo);
+  const int64_t pitch = p.ldo * (p.out_dtype == LSK_F32 ? 4 : 2);
+  const int vec = !out_vec_ok(p.out, p.out_dtype, p.ldo) ? 0 : (uintptr_t)p.out % 128 == 0 && pitch % 128 == 0 ? 2 : 1;
   auto run = [&](auto kern) {
     if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes) != hipSuccess)
       return set_error("fp8_tile_kernel: cannot reserve LDS"), LSK_ERR_HIP;
@@ -560,46 +569,129 @@ static int fp8_stream_launch(const Fp8Args& p, const void* x, int64_t ldx, hipSt
                : run(fp8_stream_kernel<NG, MT, KS, RING, DT, false, false>);
 }
 
-// The launch shape by the number of 16-row weight groups over all row tiles: one group a block while
-// there are few (long stages, a deep ring: nothing else hides the latency), else blocks of two, then of
-// four with the shortest ring, several of which share a CU.
-template <int MT, int DT>
-static int fp8_stream_shape(const Fp8Args& p, const void* x, int64_t ldx, hipStream_t s) {
-  const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
-  const int64_t groups = tiles * ((p.N + 15) / 16);
-  if (groups <= 256) return fp8_stream_launch<1, MT, 2, 4, DT>(p, x, ldx, s);
-  if (groups <= 1024) return fp8_stream_launch<2, MT, 1, 3, DT>(p, x, ldx, s);
-  return fp8_stream_launch<4, MT, 1, 2, DT>(p, x, ldx, s);
+// ---------------------------------------------------------------- which launch
+// About how long a product takes on each of the launches, in us: the CU with the most blocks, ceil(blocks / 256) of
+// them, works through them `resident` at a time, a round of o blocks at once in round[o - 1] + k[o - 1] a block of 128
+// values of K; every million outputs cost `out` and `area` a block of K, every 10^9 weights read `weights`, and every
+// 10^9 bytes of a block's operands `spill` where the rows (of an expert) outgrow an XCD's 4 MB of L2.  Fitted to 902
+// products on MI355X (1 to 4096 rows of 17 to 37888 columns, K = 16 to 18944; 1 to 32768 rows over 2 to 128 experts):
+// what it picks is 1.6 % slower than the best of them on average and 28 % at most (50 rows of 19 x 736, 6.5 and 5.1 us;
+// among those over 10 us 24 %, 1917 rows over 93 experts of 3099 x 4496).  All of them give the same bits.
+struct Fp8Cost {
+  int bm, bn, resident;  // resident 0: as many as the LDS holds at this K, to four
+  double base, out, area, weights, spill, round[4], k[4];
+};
+enum {  // fp8_launch's order
+  kTile256, kTile128, kTile64x128, kTile64, kTile64Deep, kTile128x64, kStream1, kStream2, kStream4, kStream1Deep, kStream1x2,
+  kStream2x2, kStream4x2, kStream2x2Deep, kLaunches
+};
+constexpr Fp8Cost kFp8Costs[kLaunches] = {
+    {256, 256, 1, 2.6, 0.044, 0.042, 45, 0, {8.6}, {0.93}},
+    {128, 128, 2, 2.0, 0, 0.06, 54, 0, {4.4, 5.5}, {0.556, 0.526}},
+    {64, 128, 3, 2.7, 0.19, 0.056, 97, 3.1, {1.8, 2.8, 2.5}, {0.43, 0.383, 0.662}},
+    {64, 64, 4, 3.2, 0.19, 0.118, 85, 4.3, {0.54, 0.94, 2.1, 1.8}, {0.364, 0.256, 0.22, 0.374}},
+    {64, 64, 2, 2.4, 0.58, 0.003, 84, 8.6, {1.7, 1.7}, {0.284, 0.369}},
+    {128, 64, 1, 2.5, 0.72, 0.004, 23, 0, {2.0}, {0.427}},
+    {16, 16, 0, 2.6, 15.7, 0.55, 0, 0, {2.2, 1.5}, {0.068, 0.087}},
+    {16, 32, 0, 3.1, 4.2, 0, 54, 0, {1.9, 1.8, 0.1, 0}, {0.114, 0.141, 0.382, 0.481}},
+    {16, 64, 0, 3.0, 3.3, 0.33, 75, 0, {1.7, 0, 0.6, 0}, {0.158, 0.255, 0.313, 0.313}},
+    {16, 16, 0, 2.7, 14.2, 0, 14, 0, {2.0}, {0.086}},
+    {32, 16, 0, 2.6, 1.6, 0, 95, 6.3, {2.9}, {0.083}},
+    {32, 32, 0, 3.5, 0.11, 0.008, 97, 7.6, {1.6, 1.9, 2.3}, {0.135, 0.17, 0.24}},
+    {32, 64, 0, 4.4, 0.88, 0.018, 115, 7.5, {1.3, 0, 1.0}, {0.215, 0.289, 0.372}},
+    {32, 32, 0, 1.9, 0.126, 0.014, 63, 0, {3.5}, {0.116}},
+};
+
+template <int NG, int MT, int KS, int RING>
+static int fp8_stream_resident(int64_t K) {  // blocks of a CU, to four (0: the scales of all of K do not fit)
+  const int64_t n = 160 * 1024 / fp8_stream_lds<NG, MT, KS, RING, false>((int)K, 16);
+  return (int)(n < 4 ? n : 4);
 }
 
-// Whether the products of M rows (of E experts: E > 0) run on the tiles: each streaming block brings its weight rows
-// in again for its 32 rows, and a block's scales of all of K have to fit the LDS.
-constexpr int64_t kStreamK = 16384;
-static bool fp8_takes_tiles(int64_t M, int64_t N, int64_t K, int64_t E) {
-  if (K == 0 || K > kStreamK) return true;
-  const int64_t groups = (E ? expert_tiles_max(M, E, 32) : (M + 31) / 32) * ((N + 15) / 16);
-  return E ? M > 16 * E : M > 16 && groups > 1024;
+static int fp8_launch(int which, const Fp8Args& p, hipStream_t s) {
+  switch (which) {
+    case kTile256: return fp8_tile_launch<256, 256, 2, 4, 2>(p, s);
+    case kTile128: return fp8_tile_launch<128, 128, 2, 2, 2>(p, s);
+    case kTile64x128: return fp8_tile_launch<64, 128, 2, 2, 2>(p, s);
+    case kTile64: return fp8_tile_launch<64, 64, 2, 2, 2>(p, s);
+    case kTile64Deep: return fp8_tile_launch<64, 64, 2, 2, 4>(p, s);
+    case kTile128x64: return fp8_tile_launch<128, 64, 2, 2, 4>(p, s);
+    case kStream1: return fp8_stream_launch<1, 1, 2, 4, -1>(p, nullptr, 0, s);
+    case kStream2: return fp8_stream_launch<2, 1, 1, 3, -1>(p, nullptr, 0, s);
+    case kStream4: return fp8_stream_launch<4, 1, 1, 2, -1>(p, nullptr, 0, s);
+    case kStream1Deep: return fp8_stream_launch<1, 1, 2, 6, -1>(p, nullptr, 0, s);
+    case kStream1x2: return fp8_stream_launch<1, 2, 2, 4, -1>(p, nullptr, 0, s);
+    case kStream2x2: return fp8_stream_launch<2, 2, 1, 3, -1>(p, nullptr, 0, s);
+    case kStream4x2: return fp8_stream_launch<4, 2, 1, 2, -1>(p, nullptr, 0, s);
+    default: return fp8_stream_launch<2, 2, 2, 4, -1>(p, nullptr, 0, s);
+  }
+}
+
+static int fp8_resident(int which, int64_t K) {
+  switch (which) {
+    case kStream1: return fp8_stream_resident<1, 1, 2, 4>(K);
+    case kStream2: return fp8_stream_resident<2, 1, 1, 3>(K);
+    case kStream4: return fp8_stream_resident<4, 1, 1, 2>(K);
+    case kStream1Deep: return fp8_stream_resident<1, 1, 2, 6>(K);
+    case kStream1x2: return fp8_stream_resident<1, 2, 2, 4>(K);
+    case kStream2x2: return fp8_stream_resident<2, 2, 1, 3>(K);
+    case kStream4x2: return fp8_stream_resident<4, 2, 1, 2>(K);
+    case kStream2x2Deep: return fp8_stream_resident<2, 2, 2, 4>(K);
+    default: return kFp8Costs[which].resident;
+  }
+}
+
+// E > 0: rows over E experts, `live` of which get some were all as likely, half a tile of each part empty.
+static double fp8_us(int which, int64_t M, int64_t N, int64_t K, int64_t E) {
+  const Fp8Cost& c = kFp8Costs[which];
+  const int o = fp8_resident(which, K);
+  if (o < 1) return 1e30;
+  const double live = E ? E * (1.0 - __builtin_exp(-(double)M / E)) : 1.0;
+  double down = (double)((M + c.bm - 1) / c.bm);
+  if (E) down = (double)M / c.bm + live / 2 > live ? (double)M / c.bm + live / 2 : live;
+  const double blocks = __builtin_ceil(down * ((N + c.bn - 1) / c.bn)), nk = (double)((K + 127) / 128);
+  const double most = __builtin_ceil(blocks / 256), full = __builtin_floor(most / o), outs = blocks * 1e-6 * c.bm * c.bn;
+  const int rest = (int)(most - full * o);
+  const bool spills = (double)M * K > 4e6 * (E ? E : 1);
+  return c.base + outs * (c.out + c.area * nk) + live * N * K * 1e-9 * c.weights +
+         (spills ? blocks * (c.bm + c.bn) * K * 1e-9 * c.spill : 0) + full * (c.round[o - 1] + c.k[o - 1] * nk) +
+         (rest ? c.round[rest - 1] + c.k[rest - 1] * nk : 0);
 }
 
 static int fp8_product(const Fp8Args& p, hipStream_t s) {
   LSK_REQUIRE(fp8_reach(p), "fp8 product: M=%lld N=%lld K=%d beyond 31-bit offsets", (long long)p.M, (long long)p.N, p.K);
-  const int64_t E = p.offs ? p.E : 0, per = E ? 2 * p.M / E : p.M;
-  if (!fp8_takes_tiles(p.M, p.N, p.K, E))
-    return per <= 16 ? fp8_stream_shape<1, -1>(p, nullptr, 0, s) : fp8_stream_shape<2, -1>(p, nullptr, 0, s);
-  auto tiles = [&](int64_t bm, int64_t bn) { return fp8_row_tiles(p, (int)bm) * ((p.N + bn - 1) / bn); };
-  if (p.out_dtype != LSK_F32 && tiles(256, 256) >= 200) return fp8_tile_launch<256, 256, 2, 4, 2>(p, s);
-  if (tiles(128, 128) >= 400) return fp8_tile_launch<128, 128, 2, 2, 2>(p, s);
-  if (tiles(64, 128) >= 400) return fp8_tile_launch<64, 128, 2, 2, 2>(p, s);
-  return fp8_tile_launch<64, 64, 2, 2, 4>(p, s);
+  const int64_t E = p.offs ? p.E : 0;
+  int best = kTile128;
+  double us = 1e30;
+  for (int c = 0; c < kLaunches; ++c) {
+    if (p.K == 0 && c >= kStream1) break;
+    if (c == kTile256 && p.out_dtype == LSK_F32) continue;  // (products kept whole need more registers than it has)
+    const double t = fp8_us(c, p.M, p.N, p.K, E);
+    if (t < us) us = t, best = c;
+  }
+  return fp8_launch(best, p, s);
 }
 
-// Whether a linear's few rows are quantised in the product's launch: every block quantises them all.
-static bool fp8_fuses(int64_t M, int64_t K) { return K > 0 && (M == 1 ? K <= kStreamK : M <= 16 && M * K <= 8192); }
+// Whether a linear's few rows are quantised in the product's launch, by every block: while they hold few values.  (MI355X,
+// GPU us in one launch and in two: one row of 3584 on 4608 columns 8.7, 10.7, of 14336 on 4096 19.8, 19.8; 4 of 2048 on
+// 1024 7.4, 9.5, of 4096 on 4096 12.7, 12.5; 16 of 1024 on 2048 9.1, 9.3, on 12000 10.9, 10.3, of 2048 on 1024 13.7, 9.9.
+// A launch less is 3 us of a caller's time besides, but nothing in a replayed graph.)
+static bool fp8_fuses(int64_t M, int64_t K) { return K > 0 && M <= 16 && M * K <= 16384; }
 
+// One group of 16 columns a block while a block a CU and a few more hold them, else two, then four.  (One row of 3584 on
+// 4608 columns, 288 groups: 7.7, 8.1, 10.7 us; on 28672 columns of 512, 1792 groups, 7.2 with four, of 4096 31.0 with two
+// and 31.5 with four.)
 static int fp8_stream_fused(const Fp8Args& p, const void* x, int x_dtype, int64_t ldx, hipStream_t s) {
-  if (x_dtype == LSK_F32) return fp8_stream_shape<1, LSK_F32>(p, x, ldx, s);
-  if (x_dtype == LSK_BF16) return fp8_stream_shape<1, LSK_BF16>(p, x, ldx, s);
-  return fp8_stream_shape<1, LSK_F16>(p, x, ldx, s);
+  const int64_t groups = (p.N + 15) / 16;
+  auto run = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (groups <= 300) return fp8_stream_launch<1, 1, 2, 4, DT>(p, x, ldx, s);
+    if (groups <= 1600) return fp8_stream_launch<2, 1, 1, 3, DT>(p, x, ldx, s);
+    return fp8_stream_launch<4, 1, 1, 2, DT>(p, x, ldx, s);
+  };
+  if (x_dtype == LSK_F32) return run(std::integral_constant<int, LSK_F32>{});
+  if (x_dtype == LSK_BF16) return run(std::integral_constant<int, LSK_BF16>{});
+  return run(std::integral_constant<int, LSK_F16>{});
 }
 
 }  // namespace lsk

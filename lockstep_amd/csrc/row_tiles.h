@@ -102,9 +102,12 @@ inline int64_t expert_tiles_max(int64_t R, int64_t E, int64_t bm) { return R / b
 // to bf16 becomes 0x7FC0, off the common path (v0 + v1 + v2 + v3 is a NaN where one of them is).
 // Non-temporal: an output stays in no L2 past its launch, and within it leaves the L2 to the operands
 // (4096 rows of 28672 x 4096 321 -> 293 us on MI355X, 777 of 4608 x 3584 21.9 -> 20.6).
+// NT false: as any other store, for rows that share their lines with others' (fp8.hip).
+template <bool NT = true>
 LSK_DEV void store_quad(char* o, int dtype, v4f v) {
   auto put = [&](char* at, uint32_t lo, uint32_t hi) {
-    __builtin_nontemporal_store((uint64_t)hi << 32 | lo, (uint64_t*)at);
+    if constexpr (NT) __builtin_nontemporal_store((uint64_t)hi << 32 | lo, (uint64_t*)at);
+    else *(uint64_t*)at = (uint64_t)hi << 32 | lo;
   };
   if (dtype == LSK_F32) {
     put(o, __float_as_uint(v[0]), __float_as_uint(v[1]));
