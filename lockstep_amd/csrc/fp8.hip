@@ -171,9 +171,8 @@ template <int NG, int MT, int KS, bool FUSE>
 struct Fp8StreamCfg {
   static constexpr int kPartW = NG * 4096, kPart = kPartW + (FUSE ? 0 : MT * 4096), kStage = KS * kPart;  // bytes
   static constexpr int kPer = KS * (NG + (FUSE ? 0 : MT));  // loads per thread per stage
-  static constexpr int kMW = NG * MT > 4 ? NG * MT / 4 : 1;  // row tiles of a wave
   static constexpr int kPre = 16;                            // scales of a thread loaded ahead of the ring
-  static_assert(NG * MT <= 4 || NG == 4, "a wave's row tiles share its weight rows");
+  static_assert(NG * MT <= 4, "a wave multiplies at most one weight group with one row tile");
   static_assert(NG <= 8 && 128 % (16 * NG) == 0, "a block's columns share a weight scale");
 };
 
@@ -296,44 +295,33 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args p, const void* 
     }
   }
 
-  // wave w multiplies weight group w % NG with row tiles w / NG (and, NG * MT > 4, the next ones)
-  constexpr int MW = C::kMW;
-  const int g = wave % NG, mt = wave / NG * MW;
-  const bool multiplies = NG * MT >= 4 || wave < NG * MT;
-  v4f acc[MW];
-  const float* ars[MW];
-  const char* arc[MW];
-#pragma unroll
-  for (int m = 0; m < MW; ++m) {
-    acc[m] = v4f{0, 0, 0, 0};
-    // (rows past the end: whatever lies there, their results are not stored)
-    const int ar = FUSE ? min(r, rows_a - 1) : 16 * (mt + m) + r;
-    ars[m] = scales + ar * sp;
-    arc[m] = FUSE ? fused + ar * fp : smem + C::kPartW + ar * 256;
-  }
+  // wave w multiplies weight group w % NG with row tile w / NG
+  const int g = wave % NG, mt = wave / NG;
+  const bool multiplies = wave < NG * MT;
+  v4f acc = v4f{0, 0, 0, 0};
+  // (rows past the end: whatever lies there, their results are not stored)
+  const int ar = FUSE ? min(r, rows_a - 1) : 16 * mt + r;
+  const float* const ars = scales + ar * sp;
+  const char* const arc = FUSE ? fused + ar * fp : smem + C::kPartW + ar * 256;
   // a stage's fragments are read a stage ahead where the ring is deep enough, so that the LDS works under the
   // matrix core's and the FMAs' chain
   struct Frag {
-    v2f_t s[KS][MW];
-    v8i w[KS][2], a[KS][MW][2];
+    v2f_t s[KS];
+    v8i w[KS][2], a[KS][2];
   };
   auto read = [&](int kt, Frag& f) {
 #pragma unroll
     for (int u = 0; u < KS; ++u) {
       const int slot = (kt % RING) * C::kStage + u * C::kPart, part = KS * kt + u;
       const char* base = smem + slot + (16 * g + r) * 256;
-#pragma unroll
-      for (int m = 0; m < MW; ++m) f.s[u][m] = *(const v2f_t*)(ars[m] + 2 * part);
+      f.s[u] = *(const v2f_t*)(ars + 2 * part);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int c0 = 16 * ((8 * h + q) ^ r), c1 = 16 * ((8 * h + 4 + q) ^ r);
         f.w[u][h] = fp8_operand(*(const v4i*)(base + c0), *(const v4i*)(base + c1));
-#pragma unroll
-        for (int m = 0; m < MW; ++m) {
-          const char* a = FUSE ? arc[m] + 256 * part + 128 * h + 16 * q : arc[m] + slot;
-          f.a[u][m][h] = FUSE ? fp8_operand(*(const v4i*)a, *(const v4i*)(a + 64))
-                              : fp8_operand(*(const v4i*)(a + c0), *(const v4i*)(a + c1));
-        }
+        const char* a = FUSE ? arc + 256 * part + 128 * h + 16 * q : arc + slot;
+        f.a[u][h] = FUSE ? fp8_operand(*(const v4i*)a, *(const v4i*)(a + 64))
+                         : fp8_operand(*(const v4i*)(a + c0), *(const v4i*)(a + c1));
       }
     }
   };
@@ -341,10 +329,7 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args p, const void* 
 #pragma unroll
     for (int u = 0; u < KS; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int m = 0; m < MW; ++m)
-          acc[m] = fp8_scaled(fp8_block<EXACT>(f.w[u][h], f.a[u][m][h]), f.s[u][m][h], acc[m]);
+      for (int h = 0; h < 2; ++h) acc = fp8_scaled(fp8_block<EXACT>(f.w[u][h], f.a[u][h]), f.s[u][h], acc);
   };
   Frag f[2];
   if constexpr (RING >= 4) {
@@ -388,17 +373,14 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args p, const void* 
     const int64_t n = n0 + 16 * g + 4 * q + t;
     b[t] = p.bias && n < p.N ? p.bias[n] : 0.0f;
   }
+  const int row_out = 16 * mt + r;
+  if (row_out >= rows_a) return;
 #pragma unroll
-  for (int m = 0; m < MW; ++m) {
-    const int row_out = 16 * (mt + m) + r;
-    if (row_out >= rows_a) continue;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int64_t n = n0 + 16 * g + 4 * q + t;
-      float y = acc[m][t];
-      __asm__("" : "+v"(y));  // (a binary32 sum first, as the tiles have it: not one FMA that rounds to f16)
-      if (n < p.N) store_out(p.out, p.out_dtype, (m0 + row_out) * p.ldo + n, p.bias ? f32_add(y, b[t]) : y);
-    }
+  for (int t = 0; t < 4; ++t) {
+    const int64_t n = n0 + 16 * g + 4 * q + t;
+    float y = acc[t];
+    __asm__("" : "+v"(y));  // (a binary32 sum first, as the tiles have it: not one FMA that rounds to f16)
+    if (n < p.N) store_out(p.out, p.out_dtype, (m0 + row_out) * p.ldo + n, p.bias ? f32_add(y, b[t]) : y);
   }
 }
 
@@ -575,15 +557,15 @@ static int fp8_stream_launch(const Fp8Args& p, const void* x, int64_t ldx, hipSt
 // values of K; every million outputs cost `out` and `area` a block of K, every 10^9 weights read `weights`, and every
 // 10^9 bytes of a block's operands `spill` where the rows (of an expert) outgrow an XCD's 4 MB of L2.  Fitted to 902
 // products on MI355X (1 to 4096 rows of 17 to 37888 columns, K = 16 to 18944; 1 to 32768 rows over 2 to 128 experts):
-// what it picks is 1.6 % slower than the best of them on average and 28 % at most (50 rows of 19 x 736, 6.5 and 5.1 us;
-// among those over 10 us 24 %, 1917 rows over 93 experts of 3099 x 4496).  All of them give the same bits.
+// what it picks is 1.3 % slower than the best of these on average and 27 % at most (50 rows of 19 x 736, 6.5 and 5.1 us;
+// among those over 10 us 18 %, 256 rows over 8 experts of 4096 x 4096).  All of them give the same bits.
 struct Fp8Cost {
   int bm, bn, resident;  // resident 0: as many as the LDS holds at this K, to four
   double base, out, area, weights, spill, round[4], k[4];
 };
 enum {  // fp8_launch's order
   kTile256, kTile128, kTile64x128, kTile64, kTile64Deep, kTile128x64, kStream1, kStream2, kStream4, kStream1Deep, kStream1x2,
-  kStream2x2, kStream4x2, kStream2x2Deep, kLaunches
+  kStream2x2, kStream2x2Deep, kLaunches
 };
 constexpr Fp8Cost kFp8Costs[kLaunches] = {
     {256, 256, 1, 2.6, 0.044, 0.042, 45, 0, {8.6}, {0.93}},
@@ -598,7 +580,6 @@ constexpr Fp8Cost kFp8Costs[kLaunches] = {
     {16, 16, 0, 2.7, 14.2, 0, 14, 0, {2.0}, {0.086}},
     {32, 16, 0, 2.6, 1.6, 0, 95, 6.3, {2.9}, {0.083}},
     {32, 32, 0, 3.5, 0.11, 0.008, 97, 7.6, {1.6, 1.9, 2.3}, {0.135, 0.17, 0.24}},
-    {32, 64, 0, 4.4, 0.88, 0.018, 115, 7.5, {1.3, 0, 1.0}, {0.215, 0.289, 0.372}},
     {32, 32, 0, 1.9, 0.126, 0.014, 63, 0, {3.5}, {0.116}},
 };
 
@@ -622,7 +603,6 @@ static int fp8_launch(int which, const Fp8Args& p, hipStream_t s) {
     case kStream1Deep: return fp8_stream_launch<1, 1, 2, 6, -1>(p, nullptr, 0, s);
     case kStream1x2: return fp8_stream_launch<1, 2, 2, 4, -1>(p, nullptr, 0, s);
     case kStream2x2: return fp8_stream_launch<2, 2, 1, 3, -1>(p, nullptr, 0, s);
-    case kStream4x2: return fp8_stream_launch<4, 2, 1, 2, -1>(p, nullptr, 0, s);
     default: return fp8_stream_launch<2, 2, 2, 4, -1>(p, nullptr, 0, s);
   }
 }
@@ -635,7 +615,6 @@ static int fp8_resident(int which, int64_t K) {
     case kStream1Deep: return fp8_stream_resident<1, 1, 2, 6>(K);
     case kStream1x2: return fp8_stream_resident<1, 2, 2, 4>(K);
     case kStream2x2: return fp8_stream_resident<2, 2, 1, 3>(K);
-    case kStream4x2: return fp8_stream_resident<4, 2, 1, 2>(K);
     case kStream2x2Deep: return fp8_stream_resident<2, 2, 2, 4>(K);
     default: return kFp8Costs[which].resident;
   }

@@ -171,6 +171,27 @@ def test_product_exact(M, N, K):
         assert got.dtype == odt and torch.equal(got.cpu(), want.to(odt))
 
 
+# sizes that between them reach every launch a product may take, one expert's and (below) several experts'
+LAUNCHES = [(6278, 1934, 16), (2100, 3900, 400), (579, 10033, 16), (1500, 2050, 656), (278, 13067, 16), (500, 2050, 272),
+            (1, 16, 16), (700, 2050, 144), (1419, 20, 560), (78, 13670, 2656), (1, 17, 1056), (15, 4078, 688), (4175, 17, 480),
+            (17, 8206, 16), (224, 18, 432), (2118, 21, 1792), (2433, 18, 848), (6689, 17, 1632)]
+
+
+@pytest.mark.parametrize("M,N,K", LAUNCHES)
+def test_product_exact_on_every_launch(M, N, K):
+    """As above; the largest sizes' rows in 64 bits are the same few, so that the oracle's product stays small."""
+    say("product exact", M, N, K)
+    g = np.random.default_rng(M + N * K)
+    R, octaves = min(M, 300), 1 if K < 1820 else 0
+    qa, sa = _exact_operand(g, R, K, octaves, False)
+    qw, sw = _exact_operand(g, N, K, octaves, True)
+    pick = g.integers(0, R, M)
+    y = U.product(qa, sa, qw, sw)[0][pick]
+    for odt in HALF:
+        got = _mm(qa[pick], sa[pick], qw, sw, None, odt)
+        assert torch.equal(got.cpu(), torch.from_numpy(y.astype(np.float32)).to(odt))
+
+
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("M,N,K", [(1, 300, 4096), (7, 513, 2880), (32, 256, 14336), (50, 1000, 400), (150, 700, 3584),
                                    (333, 300, 1040), (700, 1100, 912)])
@@ -326,6 +347,37 @@ def test_grouped_is_mm_of_each_expert(counts, H, I, bias, out_dtype):
                 rows = slice(offs[e], offs[e + 1])
                 want = FS.mm_fp8(a[rows], s[rows], *ex[e][j], ex[e][2 + j], out_dtype)
                 assert np.array_equal(bits(got[rows]), bits(want)), (which, e)
+
+
+@pytest.mark.parametrize("R,N,K,E", [(1880, 6048, 272, 6), (443, 9920, 16, 6), (10, 13504, 16, 6), (1, 16, 16, 6), (1185, 32, 528, 6),
+                                     (362, 2560, 2896, 6), (1, 16, 1040, 6), (3, 13856, 32, 6), (9, 3648, 16, 6), (357, 16, 416, 6),
+                                     (4593, 16, 1360, 6), (3682, 16, 784, 6), (70, 1104, 1024, 6), (3235, 1408, 16, 40),
+                                     (56, 2144, 16, 40), (50, 544, 16, 40), (541, 144, 1088, 40)])
+def test_grouped_exact_on_every_launch(R, N, K, E):
+    """Random counts, some experts empty, rows behind the last expert: those stay what they were."""
+    from lockstep_amd import _lib as L
+    say("grouped exact", R, N, K, E)
+    g = np.random.default_rng(R * E + N)
+    octaves = 1 if K < 1820 else 0
+    qa, sa = _exact_operand(g, min(R, 300), K, octaves, False)
+    pick = g.integers(0, len(qa), R)
+    qa, sa = qa[pick], sa[pick]
+    weights = [_exact_operand(g, N, K, octaves, True) for _ in range(min(E, 7))]
+    held = [(to_dev(q), to_dev(s)) for q, s in weights]
+    part = g.random(E) * (g.random(E) < 0.8) + 1e-9
+    offs = np.concatenate([[0], np.cumsum(part) / part.sum() * R * (0.9 if R > 20 else 1)]).astype(np.int32)
+    y = np.full((R, N), 7.0)
+    for e in range(E):
+        rows = slice(offs[e], offs[e + 1])
+        y[rows] = U.product(qa[rows], sa[rows], *weights[e % len(weights)])[0]
+    a, s, o = to_dev(qa), to_dev(sa), to_dev(offs)
+    wp, sp = (to_dev(np.array([held[e % len(held)][j].data_ptr() for e in range(E)], np.int64)) for j in (0, 1))
+    for odt in (torch.float32, torch.bfloat16):
+        out = torch.full((R, N), 7.0, dtype=odt, device=dev())
+        L.call("lsk_grouped_gemm_fp8", a.data_ptr(), s.data_ptr(), s.stride(0), s.stride(1), o.data_ptr(), E, R, wp.data_ptr(), K,
+               sp.data_ptr(), (K + 127) // 128, None, N, K, out.data_ptr(), L.LSK_F32 if odt == torch.float32 else L.LSK_BF16, N,
+               L.stream_of(a))
+        assert torch.equal(out.cpu(), torch.from_numpy(y.astype(np.float32)).to(odt))
 
 
 def test_grouped_offsets_out_of_order_and_rows_of_no_expert():
