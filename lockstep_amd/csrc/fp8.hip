@@ -741,8 +741,12 @@ static int fp8_check(const char* who, int64_t M, int64_t N, int64_t K, int out_d
   return LSK_OK;
 }
 
-static int fp8_scales_check(const char* who, int64_t sm, int64_t sb) {
-  LSK_REQUIRE(sm >= 0 && sb >= 0 && sm < (1LL << 31) && sb < (1LL << 31), "%s: bad scale strides", who);
+// (a stride that nothing steps by may be any size)
+static int fp8_scales_check(const char* who, int64_t M, int64_t K, int64_t& sm, int64_t& sb) {
+  LSK_REQUIRE(sm >= 0 && sb >= 0, "%s: bad scale strides", who);
+  if (M <= 1) sm = 0;
+  if (K <= 128) sb = 0;
+  LSK_REQUIRE(sm < (1LL << 31) && sb < (1LL << 31), "%s: bad scale strides", who);
   return LSK_OK;
 }
 
@@ -750,7 +754,7 @@ extern "C" int lsk_gemm_fp8(const uint8_t* a, const float* a_scale, int64_t scal
                             const uint8_t* w, const float* w_scale, int64_t N, const float* bias, void* out, int out_dtype,
                             int64_t ldo, void* stream) {
   int rc = fp8_check("lsk_gemm_fp8", M, N, K, out_dtype, ldo);
-  if (rc || (rc = fp8_scales_check("lsk_gemm_fp8", scale_m, scale_b))) return rc;
+  if (rc || (rc = fp8_scales_check("lsk_gemm_fp8", M, K, scale_m, scale_b))) return rc;
   if (M == 0 || N == 0) return LSK_OK;
   LSK_REQUIRE(out && (K == 0 || (a && a_scale && w && w_scale)), "lsk_gemm_fp8: null pointer");
   LSK_REQUIRE((uintptr_t)a % 16 == 0 && (uintptr_t)w % 16 == 0, "lsk_gemm_fp8: codes must be 16-byte aligned");
@@ -804,7 +808,7 @@ extern "C" int lsk_grouped_gemm_fp8(const uint8_t* a, const float* a_scale, int6
                                     const int64_t* ws_ptrs, int64_t ldsw, const int64_t* b_ptrs, int64_t N, int64_t K,
                                     void* out, int out_dtype, int64_t ldo, void* stream) {
   int rc = fp8_check("lsk_grouped_gemm_fp8", R, N, K, out_dtype, ldo);
-  if (rc || (rc = fp8_scales_check("lsk_grouped_gemm_fp8", scale_m, scale_b))) return rc;
+  if (rc || (rc = fp8_scales_check("lsk_grouped_gemm_fp8", R, K, scale_m, scale_b))) return rc;
   LSK_REQUIRE(E >= 1 && E <= (1 << 20), "lsk_grouped_gemm_fp8: E=%lld not in [1, 2^20]", (long long)E);
   if (R == 0 || N == 0) return LSK_OK;
   LSK_REQUIRE(out && offs && w_ptrs && ws_ptrs && (K == 0 || (a && a_scale)), "lsk_grouped_gemm_fp8: null pointer");

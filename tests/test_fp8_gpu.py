@@ -228,6 +228,12 @@ def test_product_scales_of_any_stride():
             assert not other.is_contiguous() and torch.equal(FS.mm_fp8(a, other, w, ws, out_dtype=odt), want)
         one = torch.full((1, 1), 0.25, device=dev()).expand(M, s.shape[1])
         assert torch.equal(FS.mm_fp8(a, one, w, ws, out_dtype=odt), FS.mm_fp8(a, one.contiguous(), w, ws, out_dtype=odt))
+        # one row, and one block, of a tensor whose strides no product could step by
+        far = s[:1].contiguous().as_strided((1, s.shape[1]), (1 << 40, 1))
+        assert torch.equal(FS.mm_fp8(a[:1], far, w, ws, out_dtype=odt), want[:1])
+        far = s[:, :1].as_strided((M, 1), (s.stride(0), 1 << 40))
+        assert torch.equal(FS.mm_fp8(a[:, :128].contiguous(), far, w[:, :128], ws[:, :1], out_dtype=odt),
+                           FS.mm_fp8(a[:, :128].contiguous(), s[:, :1], w[:, :128], ws[:, :1], out_dtype=odt))
         # codes and weight scales as views: copied
         big = torch.zeros((M, 2 * K), dtype=torch.uint8, device=dev()).view(F8)
         big.view(torch.uint8)[:, 8:8 + K] = a.view(torch.uint8)
@@ -445,3 +451,73 @@ def test_other_stream_and_graph():
             eager = FS.linear_fp8(xs, w, ws)
             torch.cuda.synchronize()
             assert torch.equal(y, eager)
+
+
+def test_offsets_beyond_32_bits():
+    """The last rows of tensors past 2^32 elements, as the same rows alone give them."""
+    from lockstep_amd import lockstep_fullstack as FS, moe_ref, t16n_ref
+    g = np.random.default_rng(15)
+    M, K, n = 2 ** 20 + 5, 4096, 7
+    x = torch.zeros((M, K), dtype=torch.bfloat16, device=dev())
+    x[-n:] = torch.from_numpy(_values(g, n, K)).to(torch.bfloat16)
+    few = x[-n:].clone()
+    say("quantise", M, K)
+    q, s = FS.quantize_rows_fp8(x)
+    qf, sf = FS.quantize_rows_fp8(few)
+    assert torch.equal(q[-n:].view(torch.uint8), qf.view(torch.uint8)) and torch.equal(s[-n:], sf)
+    w, ws = FS.quantize_weight_fp8(to_dev(_values(g, 40, K)))
+    say("products", M, K)
+    for odt in (torch.bfloat16, torch.float32):
+        assert torch.equal(FS.mm_fp8(q, s, w, ws, out_dtype=odt)[-n:], FS.mm_fp8(qf, sf, w, ws, out_dtype=odt))
+        assert torch.equal(FS.linear_fp8(x, w, ws, out_dtype=odt)[-n:], FS.linear_fp8(few, w, ws, out_dtype=odt))
+    say("by expert", M, K)
+    I = 32
+    tables = moe_ref.ExpertTablesFP8([tuple(FS.quantize_weight_fp8(to_dev(_values(g, *shape))) for shape in ((2 * I, K), (K, I)))
+                                      for _ in range(2)])
+    offs = torch.tensor([0, M - n - 1, M], dtype=torch.int32, device=dev())
+    last = torch.tensor([0, 0, n], dtype=torch.int32, device=dev())
+    y = moe_ref.grouped_linear_fp8(tables, "w13", q, s, offs)
+    assert torch.equal(y[-n:], moe_ref.grouped_linear_fp8(tables, "w13", qf, sf, last))
+    act, acts = FS.quantize_rows_fp8(y[:, :I].contiguous())
+    y = moe_ref.grouped_linear_fp8(tables, "w2", act, acts, offs)
+    assert torch.equal(y[-n:], moe_ref.grouped_linear_fp8(tables, "w2", act[-n:], acts[-n:], last))
+    del y
+    say("dequantise", M, K)
+    assert torch.equal(FS.dequant_fp8(q, s)[-n:], FS.dequant_fp8(qf, sf))
+    del q, s
+    say("norm", M, K)
+    gain = to_dev(_values(g, 1, K)[0])
+    for a, b in zip(t16n_ref.add_rmsnorm_fp8(x, x, gain, want_out=True), t16n_ref.add_rmsnorm_fp8(few, few, gain, want_out=True)):
+        assert np.array_equal(bits(a[-n:].contiguous().view(torch.uint8)) if a.dtype == F8 else bits(a[-n:].contiguous()),
+                              bits(b.contiguous().view(torch.uint8)) if b.dtype == F8 else bits(b.contiguous()))
+    del x
+    say("outputs", 70000, 65536)
+    a, s = FS.quantize_rows_fp8(to_dev(_values(g, 70000, 16)))
+    w, ws = FS.quantize_weight_fp8(to_dev(_values(g, 65536, 16)))
+    for odt in (torch.bfloat16, torch.float32):
+        out = FS.mm_fp8(a, s, w, ws, out_dtype=odt)
+        assert torch.equal(out[-n:], FS.mm_fp8(a[-n:], s[-n:], w, ws, out_dtype=odt))
+        del out
+    say("route", 2 ** 22 + 3, 1024)
+    z = torch.zeros((2 ** 22 + 3, 1024), device=dev())
+    z[-n:] = to_dev(_values(g, n, 1024))
+    for a, b in zip(moe_ref.route_experts(z, 8), moe_ref.route_experts(z[-n:].clone(), 8)):
+        assert torch.equal(a[-n:], b)
+
+
+def test_two_streams_at_once():
+    """Products of two streams side by side, each with a workspace of its own."""
+    from lockstep_amd import lockstep_fullstack as FS
+    g = np.random.default_rng(16)
+    w, ws = FS.quantize_weight_fp8(to_dev(_values(g, 2000, 2048)))
+    xs = [to_dev(_values(g, m, 2048)).to(torch.bfloat16) for m in (300, 300, 1, 40)]
+    want = [FS.linear_fp8(x, w, ws) for x in xs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(24):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((i % 4, FS.linear_fp8(xs[i % 4], w, ws)))
+    torch.cuda.synchronize()
+    for i, y in got:
+        assert torch.equal(y, want[i])

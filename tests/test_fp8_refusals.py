@@ -91,6 +91,16 @@ def test_grouped_refusals():
     assert grouped(R=0) == 0
 
 
+def test_products_beyond_a_grid_are_refused():
+    lib = L.load()
+    most = 2 ** 31 - 1
+    for odt in (L.LSK_F32, L.LSK_BF16):
+        for K in (0, 16, 4096):
+            _refused(lib.lsk_gemm_fp8(P, P, 1, 1, most, K, P, P, most, None, P, odt, most, None), b"grid too large")
+            _refused(lib.lsk_grouped_gemm_fp8(P, P, 1, 1, P, 8, most, P, K, P, (K + 127) // 128, None, most, K, P, odt, most, None),
+                     b"grid too large")
+
+
 def test_norm_refusals():
     lib = L.load()
 
