@@ -804,13 +804,13 @@ def quantize_rows_fp8(x: torch.Tensor):
         raise ValueError("quantize_rows_fp8: K=%d not a multiple of 16" % K)
     nb = (K + 127) // 128
     q = x.new_empty((M, K), dtype=FP8)
-    scale = x.new_empty((nb, M), dtype=torch.float32)
+    scale = x.new_empty_strided((M, nb), (1, M), dtype=torch.float32)
     if M and K:
         L.call_on(x, "lsk_quantize_rows_fp8", x.data_ptr(), code, M, K, ld, q.data_ptr(), scale.data_ptr(), 1, M,
                   L.stream_of(x))
     if len(lead) == 1:
-        return q, scale.t()
-    return q.view(*lead, K), scale.t().view(*lead, nb)
+        return q, scale
+    return q.view(*lead, K), scale.view(*lead, nb)
 
 
 def quantize_weight_fp8(w: torch.Tensor):

@@ -156,14 +156,14 @@ def add_rmsnorm_fp8(x, residual, weight, sN=None, eps=0.0, want_out=False):
     g = weight if weight.shape == (N,) and weight.dtype in _ODT and weight.device == x.device and weight.is_contiguous() \
         else _gain(weight, N, x.device)
     q = x.new_empty(shp, dtype=ops.FP8)
-    scale = x.new_empty((nb, R), dtype=torch.float32)
+    scale = x.new_empty_strided((R, nb), (1, R), dtype=torch.float32)
     out = x.new_empty(shp, dtype=torch.bfloat16) if want_out else None
     if R and N:
         # (sN 0: the C call computes fl32(sqrt(N)) itself)
         L.call_on(x, "lsk_add_rmsnorm_fp8", x2.data_ptr(), code, ldx, L.ptr(r2), ldr, R, N, g.data_ptr(), _ODT[g.dtype],
                   sN or 0.0, eps or 0.0, None if residual is None else h.data_ptr(), N, q.data_ptr(), scale.data_ptr(), 1, R,
                   L.ptr(out), L.stream_of(x))
-    return q, scale.t() if len(shp) == 2 else scale.t().view(*shp[:-1], nb), h, out
+    return q, scale if len(shp) == 2 else scale.view(*shp[:-1], nb), h, out
 
 
 def _rows_of(x, R, N):
