@@ -22,7 +22,8 @@ namespace lsk {
 // ---------------------------------------------------------------- the quantisers
 // 16 lanes per 128 values of a row (a lane holds eight), 16 of these to a thread block: `rows` rows of it by
 // 16 / rows blocks, kQuantDeep times along K with their loads in flight together.  With 16 rows a block its
-// scales are 64-byte runs of the block-by-block layout; few rows spread over K instead.  Bound by HBM.
+// scales are 64-byte runs of the block-by-block layout; few rows spread over K instead.  Bound by HBM: 8192 bf16 rows of
+// 4096, 102 MB, in 22.4 us on MI355X (25.4 with each load waited for), 4.5 TB/s.
 constexpr int kQuantDeep = 4;
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void quantize_rows_fp8_kernel(const void* __restrict__ x, int64_t ldx, int64_t M, int K,
@@ -33,20 +34,19 @@ __global__ __launch_bounds__(256) void quantize_rows_fp8_kernel(const void* __re
   const int64_t rb = blockIdx.x / across, row = rb * rows + g % rows;
   const int b0 = (int)(blockIdx.x - rb * across) * step + g / rows, c = 8 * (threadIdx.x & 15);
   if (row >= M) return;  // (16 lanes alike, as everywhere below)
-  float v[kQuantDeep][8];
+  Raw8<DT, VEC> raw[kQuantDeep];
 #pragma unroll
   for (int z = 0; z < kQuantDeep; ++z) {
     const int k = 128 * (b0 + per * z) + c;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) v[z][t] = 0.0f;
-    if (k < K) load8<DT, VEC>(x, row * ldx + k, v[z]);
+    raw[z] = raw8<DT, VEC>(x, row * ldx + k, k < K);
   }
 #pragma unroll
   for (int z = 0; z < kQuantDeep; ++z) {
     const int b = b0 + per * z, k = 128 * b + c;
     if (b >= nb) break;
-    float s;
-    const uint2 w = quantize_row_fp8(v[z], s);
+    float v[8], s;
+    raw8_values(raw[z], v);
+    const uint2 w = quantize_row_fp8(v, s);
     if (k < K) *(uint2*)(q + row * K + k) = w;
     if (c == 0) scale[row * sm + b * sb] = s;
   }
@@ -72,7 +72,7 @@ static int quantize_rows_launch(const void* x, int x_dtype, int64_t M, int64_t K
 }
 
 // A 128 x 128 block of a weight a thread block, 16 rows at a time, held in registers between its maximum and
-// its codes.  Bound by HBM.
+// its codes.  Bound by HBM: 28672 x 4096 in bf16, 352 MB, in 65 us on MI355X (72 with each load waited for), 5.4 TB/s.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void quantize_weight_fp8_kernel(const void* __restrict__ x, int64_t ldx, int64_t N,
                                                                   int K, uint8_t* __restrict__ q,
@@ -82,17 +82,15 @@ __global__ __launch_bounds__(256) void quantize_weight_fp8_kernel(const void* __
   const int64_t rb = blockIdx.x / nb;
   const int b = (int)(blockIdx.x - rb * nb), k = 128 * b + 8 * (threadIdx.x & 15);
   const int64_t row0 = 128 * rb + (threadIdx.x >> 4);
-  float v[8][8];
+  Raw8<DT, VEC> raw[8];
 #pragma unroll
-  for (int z = 0; z < 8; ++z) {
-#pragma unroll
-    for (int t = 0; t < 8; ++t) v[z][t] = 0.0f;
-    if (k < K && row0 + 16 * z < N) load8<DT, VEC>(x, (row0 + 16 * z) * ldx + k, v[z]);
-  }
+  for (int z = 0; z < 8; ++z) raw[z] = raw8<DT, VEC>(x, (row0 + 16 * z) * ldx + k, k < K && row0 + 16 * z < N);
   uint32_t top = 0;
+  float v[8];
 #pragma unroll
   for (int z = 0; z < 8; ++z) {
-    const uint32_t t = top8(v[z]);
+    raw8_values(raw[z], v);
+    const uint32_t t = top8(v);
     top = top > t ? top : t;
   }
   top = wave_max_u32(top);
@@ -103,34 +101,65 @@ __global__ __launch_bounds__(256) void quantize_weight_fp8_kernel(const void* __
   const Fp8Scale s = fp8_scale(top);
   if (threadIdx.x == 0) scale[blockIdx.x] = s.s;
 #pragma unroll
-  for (int z = 0; z < 8; ++z)
-    if (k < K && row0 + 16 * z < N) *(uint2*)(q + (row0 + 16 * z) * K + k) = quantize8_fp8(v[z], s.inv);
+  for (int z = 0; z < 8; ++z) {
+    raw8_values(raw[z], v);
+    if (k < K && row0 + 16 * z < N) *(uint2*)(q + (row0 + 16 * z) * K + k) = quantize8_fp8(v, s.inv);
+  }
 }
 
-// Codes times scales: eight values a thread, whole lines in and out.
+// Codes times scales, four times eight bytes of outputs a thread, so that a wave's stores are whole lines side by side
+// (MI355X, against eight consecutive values a thread: 28672 x 4096 to bf16 64 -> 54 us, to f32 466 -> 100; lines filled by
+// two stores past the caches reach HBM in parts).  Bound by HBM: 352 MB in 54 us are 6.5 TB/s.  `per` of these units to a row; part: 2^22 / per, rounded up.
 template <int ODT>
 __global__ __launch_bounds__(256) void dequant_fp8_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scale,
-                                                          int64_t sm, int64_t sb, int row_shift, int64_t total, int K8,
-                                                          void* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / K8;
-    const int c = (int)(i - row * K8);
-    const uint2 w = ((const uint2*)q)[i];
-    const float s = scale[(row >> row_shift) * sm + (c >> 4) * sb];
-    float v[8];
+                                                          int64_t sm, int64_t sb, int row_shift, int64_t total, uint32_t per,
+                                                          uint32_t part, void* __restrict__ out) {
+  constexpr int V = ODT == LSK_F32 ? 2 : 4, kStep = 4;
+  typedef std::conditional_t<V == 2, uint16_t, uint32_t> Codes;
+  for (int64_t base = (int64_t)blockIdx.x * (256 * kStep); base < total; base += (int64_t)gridDim.x * (256 * kStep)) {
+    const int64_t row0 = base >> 32 ? base / per : (int64_t)((uint32_t)base / per);
+    const uint32_t c0 = (uint32_t)(base - row0 * per) + threadIdx.x;
+    const bool wide = per >= 256 * kStep;  // (one row's end at most lies among a block's units)
+    int u[kStep];
+    float s[kStep];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int u = (int)(h ? w.y : w.x);
-      const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(u, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(u, true);
-      v[4 * h] = f32_mul(a[0], s), v[4 * h + 1] = f32_mul(a[1], s);
-      v[4 * h + 2] = f32_mul(b[0], s), v[4 * h + 3] = f32_mul(b[1], s);
+    for (int z = 0; z < kStep; ++z) {
+      // (short rows: t < 2^11, and 2^22 / per rounded up is off by less than per / 2^22)
+      const uint32_t t = c0 + 256 * z, down = wide ? t >= per : t * part >> 22, c = t - down * per;
+      u[z] = 0, s[z] = 0.0f;
+      if (base + 256 * z + threadIdx.x < total) {
+        u[z] = (int)((const Codes*)q)[base + 256 * z + threadIdx.x];
+        s[z] = scale[((row0 + down) >> row_shift) * sm + c / (128 / V) * sb];
+      }
     }
-    if constexpr (ODT == LSK_F16) {
-      // (the product is a binary32 number first: the compiler would round it to f16 in one instruction)
 #pragma unroll
-      for (int t = 0; t < 8; ++t) __asm__("" : "+v"(v[t]));
+    for (int z = 0; z < kStep; ++z) {
+      const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(u[z], false);
+      float v[4] = {f32_mul(a[0], s[z]), f32_mul(a[1], s[z]), 0.0f, 0.0f};
+      if constexpr (V == 4) {
+        const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(u[z], true);
+        v[2] = f32_mul(b[0], s[z]), v[3] = f32_mul(b[1], s[z]);
+      }
+      uint64_t w;
+      if constexpr (ODT == LSK_F32) {
+        w = (uint64_t)__float_as_uint(v[1]) << 32 | __float_as_uint(v[0]);
+      } else if constexpr (ODT == LSK_BF16) {
+        const float any = (v[0] + v[1]) + (v[2] + v[3]);  // (a NaN where one of them is)
+        uint32_t lo = pack_bf16x2_nonan(v[0], v[1]), hi = pack_bf16x2_nonan(v[2], v[3]);
+        if (__builtin_amdgcn_ballot_w64(any != any)) lo = pack_bf16x2(v[0], v[1]), hi = pack_bf16x2(v[2], v[3]);
+        w = (uint64_t)hi << 32 | lo;
+      } else {
+        uint16_t h[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          // (the product is a binary32 number first: the compiler would round it to f16 in one instruction)
+          __asm__("" : "+v"(v[t]));
+          h[t] = __builtin_bit_cast(uint16_t, (_Float16)v[t]);
+        }
+        w = (uint64_t)((uint32_t)h[2] | (uint32_t)h[3] << 16) << 32 | ((uint32_t)h[0] | (uint32_t)h[1] << 16);
+      }
+      if (base + 256 * z + threadIdx.x < total) __builtin_nontemporal_store(w, (uint64_t*)out + base + 256 * z + threadIdx.x);
     }
-    store_eight((char*)out + i * (ODT == LSK_F32 ? 32 : 16), ODT, v);
   }
 }
 
@@ -269,30 +298,31 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args p, const void* 
     // 16 lanes a block of 128 values, the rows end to end (zeros past K), kBatch loads of a thread in flight
     const int slots = 32 * parts, all = rows_a * slots;  // pieces of eight values
     constexpr int kBatch = 4;
-    for (int i0 = tid; i0 < all; i0 += 256 * kBatch) {
-      float v[kBatch][8];
-      int m[kBatch];
+    auto quantize = [&](auto aligned) {
+      for (int i0 = tid; i0 < all; i0 += 256 * kBatch) {
+        constexpr bool VEC = decltype(aligned)::value;
+        Raw8<DT, VEC> raw[kBatch];
+        int m[kBatch];
 #pragma unroll
-      for (int z = 0; z < kBatch; ++z) {
-        const int i = i0 + 256 * z;
-        m[z] = (int)((uint32_t)i / (uint32_t)slots);
-        const int k = 8 * (i - m[z] * slots);
+        for (int z = 0; z < kBatch; ++z) {
+          const int i = i0 + 256 * z;
+          m[z] = (int)((uint32_t)i / (uint32_t)slots);
+          const int k = 8 * (i - m[z] * slots);
+          raw[z] = raw8<DT, VEC>(x, (m0 + m[z]) * ldx + k, i < all && k < p.K);
+        }
 #pragma unroll
-        for (int t = 0; t < 8; ++t) v[z][t] = 0.0f;
-        if (i < all && k < p.K) {
-          if (vec) load8<DT, true>(x, (m0 + m[z]) * ldx + k, v[z]);
-          else load8<DT, false>(x, (m0 + m[z]) * ldx + k, v[z]);
+        for (int z = 0; z < kBatch; ++z) {
+          const int i = i0 + 256 * z, c = i - m[z] * slots;
+          if (i >= all) continue;  // (16 lanes alike: `slots` is a multiple of 32)
+          float v[8], s;
+          raw8_values(raw[z], v);
+          *(uint2*)(fused + m[z] * fp + 8 * c) = quantize_row_fp8(v, s);
+          if ((c & 15) == 0) scales[m[z] * sp + (c >> 4)] = (c >> 4) < nb ? f32_mul(s, sw[c >> 4]) : 0.0f;
         }
       }
-#pragma unroll
-      for (int z = 0; z < kBatch; ++z) {
-        const int i = i0 + 256 * z, c = i - m[z] * slots;
-        if (i >= all) continue;  // (16 lanes alike: `slots` is a multiple of 32)
-        float s;
-        *(uint2*)(fused + m[z] * fp + 8 * c) = quantize_row_fp8(v[z], s);
-        if ((c & 15) == 0) scales[m[z] * sp + (c >> 4)] = (c >> 4) < nb ? f32_mul(s, sw[c >> 4]) : 0.0f;
-      }
-    }
+    };
+    if (vec) quantize(std::true_type{});
+    else quantize(std::false_type{});
   }
 
   // wave w multiplies weight group w % NG with row tile w / NG
@@ -719,12 +749,13 @@ extern "C" int lsk_dequant_fp8(const uint8_t* q, const float* scale, int64_t sca
   if (M == 0 || K == 0) return LSK_OK;
   LSK_REQUIRE(q && scale && out, "lsk_dequant_fp8: null pointer");
   LSK_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0, "lsk_dequant_fp8: codes and out must be 16-byte aligned");
-  const int64_t total = M * (K / 8), blocks = (total + 255) / 256;
+  const int v = out_dtype == LSK_F32 ? 2 : 4;
+  const int64_t total = M * (K / v), blocks = (total + 1023) / 1024;
   const dim3 grid((unsigned)(blocks < (1 << 22) ? blocks : (1 << 22))), blk(256);
   const int shift = block_rows == 128 ? 7 : 0;
   auto run = [&](auto odt) {
     hipLaunchKernelGGL((lsk::dequant_fp8_kernel<decltype(odt)::value>), grid, blk, 0, (hipStream_t)stream, q, scale, scale_m,
-                       scale_b, shift, total, (int)(K / 8), out);
+                       scale_b, shift, total, (uint32_t)(K / v), (uint32_t)(((1 << 22) + K / v - 1) / (K / v)), out);
   };
   if (out_dtype == LSK_F32) run(std::integral_constant<int, LSK_F32>{});
   else if (out_dtype == LSK_BF16) run(std::integral_constant<int, LSK_BF16>{});

@@ -33,75 +33,135 @@ struct NormFp8Args {
   void* out;  // [R, N] bf16 or null
 };
 
-// Pairwise sum over the lanes of a wave, neighbours first, in every lane.
-LSK_DEV float wave_tree(float v) {
+// Pairwise sum over 16 lanes (a DPP row) or all of a wave, neighbours first, in every lane of them.
+LSK_DEV float row_tree(float v) {
   auto add = [&](int o) { v = f32_add(v, __int_as_float(o)); };
   add(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xb1, 0xf, 0xf, false));   // quad [1,0,3,2]
   add(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4e, 0xf, 0xf, false));   // quad [2,3,0,1]
   add(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, false));  // half-row mirror
   add(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xf, 0xf, false));  // row mirror
+  return v;
+}
+
+LSK_DEV float wave_tree(float v) {
+  v = row_tree(v);
   auto row = [&](int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); };
   return f32_add(f32_add(row(0), row(16)), f32_add(row(32), row(48)));
 }
 
-template <int DT, bool VEC>
-LSK_DEV void store8(void* o, int64_t i, const float (&v)[8]) {
-  if constexpr (VEC) {
-    store_eight((char*)o + i * (DT == LSK_F32 ? 4 : 2), DT, v);
-  } else {
+// A wave's groups first .. first + 63 of kWords / 2 times eight bytes each, those before G, to o + their bytes: through its
+// part of LDS, so that each store of eight bytes a lane fills whole lines.  (Stores past the caches at a lane's own
+// bytes fill parts of lines: 8192 rows of 4096 in binary32 113 -> 77 us on MI355X, in 16 bits level.)
+template <int kWords>
+LSK_DEV void store_groups(void* o, int first, int G, const uint32_t (&w)[kWords], char* strip) {
+  constexpr int kParts = kWords / 2;
+  const int lane = threadIdx.x & 63;
+  uint64_t* const mine = (uint64_t*)strip + kParts * lane;
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      store_out(o, DT, i + t, v[t]);
-      __asm__ volatile("" ::: "memory");  // (no 16-byte stores: store16_split)
-    }
+  for (int t = 0; t < kParts; ++t) mine[t] = (uint64_t)w[2 * t + 1] << 32 | w[2 * t];
+  // (a wave's own LDS operations run in order)
+#pragma unroll
+  for (int t = 0; t < kParts; ++t) {
+    const int u = 64 * t + lane;
+    if (first + u / kParts < G) __builtin_nontemporal_store(((const uint64_t*)strip)[u], (uint64_t*)o + kParts * first + u);
+    __asm__ volatile("" ::: "memory");  // (no 16-byte stores: store16_split)
+  }
+}
+
+// Eight values of type DT as they lie in memory.
+template <int DT>
+LSK_DEV void words_of(const float (&v)[8], uint32_t (&w)[DT == LSK_F32 ? 8 : 4], bool nan) {
+#pragma unroll
+  for (int t = 0; t < (DT == LSK_F32 ? 8 : 4); ++t) {
+    if constexpr (DT == LSK_F32) w[t] = __float_as_uint(v[t]);
+    else if constexpr (DT == LSK_BF16)
+      w[t] = nan ? pack_bf16x2(v[2 * t], v[2 * t + 1]) : pack_bf16x2_nonan(v[2 * t], v[2 * t + 1]);
+    else
+      w[t] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * t]) |
+             (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * t + 1]) << 16;
   }
 }
 
 template <int DT, bool VEC, int C>
 __global__ __launch_bounds__(1024) void add_rmsnorm_fp8_kernel(NormFp8Args p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[16];
   const int lane = threadIdx.x & 63, wave = wave_id(), W = blockDim.x >> 6;
   const int64_t m = blockIdx.x;
   const int G = p.N / 8, g0 = wave * C * 64 + lane;
-  // (one switch on the gain's type for all of a lane's loads)
-  auto gain = [&](auto& g, int first) {
-    auto load = [&](auto gdt) {
-#pragma unroll
-      for (int c = 0; c < (int)(sizeof(g) / sizeof(g[0])); ++c)
-        if (g0 + 64 * (first + c) < G) load8<decltype(gdt)::value, VEC>(p.g, 8 * (g0 + 64 * (first + c)), g[c]);
-    };
-    if (p.g_dtype == LSK_F32) load(std::integral_constant<int, LSK_F32>{});
-    else if (p.g_dtype == LSK_BF16) load(std::integral_constant<int, LSK_BF16>{});
-    else load(std::integral_constant<int, LSK_F16>{});
+  char* const strip = smem + wave * 64 * (DT == LSK_F32 ? 32 : 16);
+  // f(the gain's type, a compile-time value)
+  auto with_gain = [&](auto f) {
+    if (p.g_dtype == LSK_F32) f(std::integral_constant<int, LSK_F32>{});
+    else if (p.g_dtype == LSK_BF16) f(std::integral_constant<int, LSK_BF16>{});
+    else f(std::integral_constant<int, LSK_F16>{});
   };
   constexpr bool kEarly = C <= 4;  // (eight groups' residuals and gains beside the values would not fit the registers)
   constexpr int kE = kEarly ? C : 1;
-  float v[C][8], r[kE][8], g[kE][8];
-  auto residual = [&](int c, float (&w)[8]) {
-#pragma unroll
-    for (int t = 0; t < 8; ++t) w[t] = 0.0f;
-    if (p.r && g0 + 64 * c < G) load8<DT, VEC>(p.r, m * p.ldr + 8 * (g0 + 64 * c), w);
+  constexpr int kWords = DT == LSK_F32 ? 8 : 4;  // of a group in x's type
+  float v[C][8], y[8];
+  uint32_t gw[kE][8] = {};  // gains as they lie in memory
+  Raw8<DT, VEC> x[kE], r[kE];
+  auto load = [&](int c, int e) {
+    const bool in = g0 + 64 * c < G;
+    x[e] = raw8<DT, VEC>(p.x, m * p.ldx + 8 * (g0 + 64 * c), in);
+    r[e] = raw8<DT, VEC>(p.r ? p.r : p.x, m * p.ldr + 8 * (g0 + 64 * c), in && p.r);
   };
+  auto load_gain = [&](int c, int e) {
+    const bool in = g0 + 64 * c < G, wide = p.g_dtype == LSK_F32;
+    const int i = in ? 8 * (g0 + 64 * c) : 0;
+    if constexpr (VEC) {  // (without a branch; 16-bit gains twice)
+      const v4u32* const at = (const v4u32*)((const char*)p.g + i * (wide ? 4 : 2));
+      const v4u32 lo = at[0], hi = at[wide ? 1 : 0];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
+      for (int t = 0; t < 4; ++t) gw[e][t] = in ? lo[t] : 0, gw[e][4 + t] = in ? hi[t] : 0;
+    } else {
 #pragma unroll
-    for (int t = 0; t < 8; ++t) v[c][t] = 0.0f;
-    if (g0 + 64 * c < G) load8<DT, VEC>(p.x, m * p.ldx + 8 * (g0 + 64 * c), v[c]);
-    if constexpr (kEarly) residual(c, r[c]);
+      for (int t = 0; t < 8; ++t)
+        gw[e][t] = !in ? 0 : wide ? ((const uint32_t*)p.g)[i + t] : ((const uint16_t*)p.g)[i + t];
+    }
+  };
+  if constexpr (kEarly) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) load(c, c);
+#pragma unroll
+    for (int c = 0; c < C; ++c) load_gain(c, c);
+    __asm__ volatile("" ::: "memory");  // (the residual's loads stay ahead of the branch that uses them)
   }
-  if constexpr (kEarly) gain(g, 0);
   float S[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    if constexpr (!kEarly) residual(c, r[0]);
-    if (p.r)
+    const int e = kEarly ? c : 0;
+    if constexpr (!kEarly) load(c, e);
+    raw8_values(x[e], v[c]);
+    auto square = [&] {
+      float s = f32_mul(v[c][0], v[c][0]);
 #pragma unroll
-      for (int t = 0; t < 8; ++t) v[c][t] = round_out(DT, f32_add(v[c][t], r[kEarly ? c : 0][t]));
-    float s = f32_mul(v[c][0], v[c][0]);
+      for (int t = 1; t < 8; ++t) s = f32_add(s, f32_mul(v[c][t], v[c][t]));
+      return s;
+    };
+    float s;
+    uint32_t w[kWords];
+    if (p.r) {  // (uniform)
+      raw8_values(r[e], y);
 #pragma unroll
-    for (int t = 1; t < 8; ++t) s = f32_add(s, f32_mul(v[c][t], v[c][t]));
+      for (int t = 0; t < 8; ++t) y[t] = f32_add(v[c][t], y[t]);
+      auto rounded = [&](bool nan) {
+        words_of<DT>(y, w, nan);
+        Raw8<DT, true> h;
+#pragma unroll
+        for (int t = 0; t < kWords; ++t) h.w[t] = w[t];
+        raw8_values(h, v[c]);
+      };
+      rounded(false);
+      s = square();
+      if (DT == LSK_BF16 && __builtin_amdgcn_ballot_w64(s != s)) rounded(true);  // (a NaN makes the sum one)
+    } else {
+      if (p.h) words_of<DT>(v[c], w, true);
+      s = square();
+    }
+    if (p.h) store_groups((char*)p.h + m * p.ldh * (DT == LSK_F32 ? 4 : 2), g0 - lane + 64 * c, G, w, strip);
     S[c] = g0 + 64 * c < G ? s : -0.0f;
-    if (p.h && g0 + 64 * c < G) store8<DT, VEC>(p.h, m * p.ldh + 8 * (g0 + 64 * c), v[c]);
   }
 #pragma unroll
   for (int c = 0; c < C; ++c) S[c] = wave_tree(S[c]);
@@ -113,14 +173,7 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_fp8_kernel(NormFp8Args p) {
   if (W > 1) {
     if (lane == 0) red[wave] = sum;
     __syncthreads();
-    float w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = i < W ? red[i] : -0.0f;
-#pragma unroll
-    for (int h = 1; h < 16; h *= 2)
-#pragma unroll
-      for (int i = 0; i < 16; i += 2 * h) w[i] = f32_add(w[i], w[i + h]);
-    sum = w[0];
+    sum = row_tree((lane & 15) < W ? red[lane & 15] : -0.0f);
   }
   if (p.ne != 0.0f) sum = f32_add(sum, p.ne);
   sum = sum < 0x1p-126f ? 0x1p-126f : sum;  // (a NaN stays)
@@ -128,19 +181,28 @@ __global__ __launch_bounds__(1024) void add_rmsnorm_fp8_kernel(NormFp8Args p) {
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int grp = g0 + 64 * c;
-    if constexpr (!kEarly) gain(g, c);
-    float y[8];
+    const int e = kEarly ? c : 0;
+    if constexpr (!kEarly) load_gain(c, e);
+    // (beside a row's end v and the gain are 0, and so is y, unless the sum is a NaN, when all of the row's are)
+    with_gain([&](auto gdt) {
+      Raw8<decltype(gdt)::value, VEC> raw;
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      y[t] = f32_mul(f32_mul(v[c][t], rs), g[kEarly ? c : 0][t]);
-      if (grp >= G) y[t] = 0.0f;  // (beside a row's end: not to weigh in the block's maximum, a NaN sum's NaNs among them)
-    }
+      for (int t = 0; t < decltype(raw)::kWords; ++t) raw.w[t] = gw[e][t];
+      raw8_values(raw, y);
+    });
+#pragma unroll
+    for (int t = 0; t < 8; ++t) y[t] = f32_mul(f32_mul(v[c][t], rs), y[t]);
     float s;
     const uint2 code = quantize_row_fp8(y, s);
     if (grp < G) {
       *(uint2*)(p.q + m * p.N + 8 * grp) = code;
       if ((lane & 15) == 0) p.scale[m * p.sm + (grp >> 4) * p.sb] = s;
-      if (p.out) store8<LSK_BF16, true>(p.out, m * p.N + 8 * grp, y);
+    }
+    if (p.out) {
+      const float any = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));  // (a NaN where one of them is)
+      uint32_t w[4];
+      words_of<LSK_BF16>(y, w, __builtin_amdgcn_ballot_w64(any != any) != 0);
+      store_groups((uint16_t*)p.out + m * p.N, grp - lane, G, w, strip);
     }
   }
 }
@@ -157,25 +219,27 @@ extern "C" int lsk_add_rmsnorm_fp8(const void* x, int x_dtype, int64_t ldx, cons
   if (R == 0 || N == 0) return LSK_OK;
   LSK_REQUIRE(x && g && q && scale, "lsk_add_rmsnorm_fp8: null pointer");
   LSK_REQUIRE(R == 1 || (ldx >= N && (!residual || ldr >= N) && (!h || ldh >= N)), "lsk_add_rmsnorm_fp8: leading dimension below N");
-  LSK_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0, "lsk_add_rmsnorm_fp8: codes and out must be 16-byte aligned");
-  // One group a lane while 16 waves hold the row (MI355X, 1, 2, 4 and 8 groups a lane: 8192 rows of 4096 53.6, 58.5, 63.5,
-  // 64.3 us, 512 of them 6.6, 7.3, 10.4, 15.3, 16384 of 1024 27.3, 28.3, 28.2, 28.4; 235 MB in 53.6 us are 4.4 TB/s, a
-  // large copy reaches 5.0).
+  const int size = x_dtype == LSK_F32 ? 4 : 2;
+  auto even = [&](const void* a, int64_t ld) { return !a || ((uintptr_t)a % 16 == 0 && (R == 1 || ld * size % 16 == 0)); };
+  LSK_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && even(h, ldh),
+              "lsk_add_rmsnorm_fp8: codes, out and h must be 16-byte aligned, h's rows too");
+  // One group a lane while 16 waves hold the row, two for long 16-bit rows enough to fill the machine (MI355X, bf16, 1, 2, 4
+  // and 8 groups a lane: 8192 rows of 4096 49.0, 46.2, 48.8, 58.5 us, of 3584 44.0, 41.7, 44.3, 56.6, 512 of 4096 5.1, 5.5,
+  // 7.3, 11.3, 32 of them 3.9, 4.5, 5.8, 10.1, 16384 of 1024 21.8, 22.2, 27.0, 46.9; f32, 8192 of 4096 76.8, 77.7, 81.3, 95.4;
+  // 235 MB in 46.2 us are 5.1 TB/s, what a large copy reaches).
   int64_t P = 64;
   while (P < N / 8) P *= 2;
-  int C = 1;
+  int C = size == 2 && R >= 2048 && N >= 2048 ? 2 : 1;
   while (P / 64 > 16 * C) C *= 2;
   const int W = (int)(P / 64 / C);
   LSK_REQUIRE(R <= 0x7fffffff && grid_ok(R, 64 * W), "lsk_add_rmsnorm_fp8: grid too large");
   lsk::NormFp8Args p{x, residual, ldx, ldr, R, (int)N, g, g_dtype, sN, 0.0f, h, ldh, q, scale, scale_m, scale_b, out};
   if (!(sN > 0.0f)) p.sN = (float)__builtin_sqrt((double)N);  // the width constant fl32(sqrt(N))
   p.ne = (float)((double)N * eps);  // one binary64 product, one rounding
-  const int size = x_dtype == LSK_F32 ? 4 : 2;
-  auto even = [&](const void* a, int64_t ld) { return !a || ((uintptr_t)a % 16 == 0 && (R == 1 || ld * size % 16 == 0)); };
-  const bool vec = even(x, ldx) && even(residual, ldr) && even(h, ldh) && (uintptr_t)g % 16 == 0;
+  const bool vec = even(x, ldx) && even(residual, ldr) && (uintptr_t)g % 16 == 0;
   auto run = [&](auto dt, auto v, auto c) {
     hipLaunchKernelGGL((lsk::add_rmsnorm_fp8_kernel<decltype(dt)::value, decltype(v)::value, decltype(c)::value>),
-                       dim3((unsigned)R), dim3(64 * W), 0, (hipStream_t)stream, p);
+                       dim3((unsigned)R), dim3(64 * W), (size_t)(64 * W * 8 * size), (hipStream_t)stream, p);
   };
   auto with_c = [&](auto dt, auto v) {
     if (C == 1) run(dt, v, std::integral_constant<int, 1>{});

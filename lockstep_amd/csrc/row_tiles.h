@@ -18,6 +18,48 @@ LSK_DEV void load8(const void* x, int64_t i, float (&v)[8]) {
   }
 }
 
+// The same in two steps, so that the loads of many stand under one another's latency: raw8 loads, zeros where `in` does
+// not hold (x's first eight elements are read there and left), raw8_values converts.  (Under a condition each load was
+// waited for before the next went out: the norm of 8192 rows of 4096, fp8 rows out, 55 us, so 47.)
+template <int DT, bool VEC>
+struct Raw8 {
+  static constexpr int kWords = VEC && DT != LSK_F32 ? 4 : 8;
+  uint32_t w[kWords];
+};
+
+template <int DT, bool VEC>
+LSK_DEV Raw8<DT, VEC> raw8(const void* x, int64_t i, bool in) {
+  Raw8<DT, VEC> r;
+  i = in ? i : 0;
+  if constexpr (VEC) {
+    const v4u32* const p = (const v4u32*)((const char*)x + i * (DT == LSK_F32 ? 4 : 2));
+#pragma unroll
+    for (int h = 0; h < Raw8<DT, VEC>::kWords / 4; ++h) {
+      const v4u32 a = p[h];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) r.w[4 * h + t] = in ? a[t] : 0;
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const uint32_t a = DT == LSK_F32 ? ((const uint32_t*)x)[i + t] : ((const uint16_t*)x)[i + t];
+      r.w[t] = in ? a : 0;
+    }
+  }
+  return r;
+}
+
+template <int DT, bool VEC>
+LSK_DEV void raw8_values(const Raw8<DT, VEC>& r, float (&v)[8]) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const uint32_t w = VEC && DT != LSK_F32 ? (t & 1 ? r.w[t / 2] >> 16 : r.w[t / 2] & 0xffff) : r.w[t];
+    if constexpr (DT == LSK_F32) v[t] = __uint_as_float(w);
+    else if constexpr (DT == LSK_BF16) v[t] = __uint_as_float(w << 16);
+    else v[t] = (float)__builtin_bit_cast(_Float16, (uint16_t)w);
+  }
+}
+
 // f(dtype, vec) with the dtype and the alignment of x's rows as compile-time values.
 template <class F>
 inline void by_input(const void* x, int x_dtype, int64_t ldx, F f) {
@@ -118,18 +160,11 @@ LSK_DEV void store_quad(char* o, int dtype, v4f v) {
     uint32_t lo = pack_bf16x2_nonan(v[0], v[1]), hi = pack_bf16x2_nonan(v[2], v[3]);
     if (__builtin_amdgcn_ballot_w64(s != s)) lo = pack_bf16x2(v[0], v[1]), hi = pack_bf16x2(v[2], v[3]);
     put(o, lo, hi);
+    __asm__ volatile("" ::: "memory");  // (merged with the one below, a store is no longer a non-temporal one)
   } else {
     put(o, (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[0]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[1]) << 16),
         (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[3]) << 16));
   }
-}
-
-// Eight of them, in 8-byte stores too.
-LSK_DEV void store_eight(char* o, int dtype, const float (&v)[8]) {
-  store_quad(o, dtype, v4f{v[0], v[1], v[2], v[3]});
-  __asm__ volatile("" ::: "memory");
-  store_quad(o + (dtype == LSK_F32 ? 16 : 8), dtype, v4f{v[4], v[5], v[6], v[7]});
-  __asm__ volatile("" ::: "memory");
 }
 
 inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }

@@ -117,6 +117,8 @@ def test_norm_refusals():
     _refused(norm(q=None), b"null")
     _refused(norm(q=P + 8), b"aligned")
     _refused(norm(out=P + 8), b"aligned")
+    _refused(norm(h=P + 8), b"aligned")
+    _refused(norm(ldh=68), b"aligned")
     _refused(norm(R=1 << 31), b"grid too large")
     assert norm(R=0, x=None) == 0
 

@@ -117,3 +117,35 @@ def test_in_place_residual_through_c():
     L.call("lsk_add_rmsnorm_fp8", x.data_ptr(), L.LSK_BF16, 1040, r.data_ptr(), 1040, 20, 1040, gain.data_ptr(), L.LSK_F32, 0.0,
            1e-6, r.data_ptr(), 1040, q2.data_ptr(), s2.data_ptr(), 1, 20, None, L.stream_of(x))
     assert torch.equal(r, h) and torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2.t(), s)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,N", [(2050, 2064), (2048, 4096), (3000, 8208)])
+def test_a_row_is_the_same_in_every_batch(R, N, dtype):
+    """However many groups a lane holds; NaNs and infinities among the rows."""
+    from lockstep_amd import t16n_ref as T
+    say("norm", R, N, dtype)
+    g = torch.Generator(device="cuda").manual_seed(R)
+    x, r = ((3 * torch.randn((R, N), generator=g, device="cuda")).to(dtype) for _ in range(2))
+    x[5, 7], x[5, 9], x[R - 1, N - 1], r[9, 3], x[9, 3] = float("nan"), -float("nan"), float("nan"), -float("inf"), float("inf")
+    gain = (1 + 0.1 * torch.randn(N, generator=g, device="cuda")).to(dtype)
+    full = T.add_rmsnorm_fp8(x, r, gain, eps=1e-6, want_out=True)
+    for rows in (slice(0, 1), slice(4, 12), slice(R - 3, R)):
+        few = T.add_rmsnorm_fp8(x[rows], r[rows], gain, eps=1e-6, want_out=True)
+        for a, b in zip(full, few):
+            a, b = a[rows].contiguous(), b.contiguous()
+            if dtype == torch.float32 and a.dtype == torch.float32:
+                a, b = a.nan_to_num(nan=1e30, posinf=2e30), b.nan_to_num(nan=1e30, posinf=2e30)
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_h_without_a_residual_through_c():
+    """h is then x, a NaN of bf16 as every conversion to it gives one."""
+    from lockstep_amd import _lib as L
+    for dt, code in ((torch.bfloat16, L.LSK_BF16), (torch.float16, L.LSK_F16), (torch.float32, L.LSK_F32)):
+        x = torch.randn((7, 1040), device="cuda").to(dt)
+        gain = torch.ones(1040, device="cuda")
+        h, q, s = torch.zeros_like(x), torch.empty((7, 1040), dtype=torch.uint8, device="cuda"), torch.empty((9, 7), device="cuda")
+        L.call("lsk_add_rmsnorm_fp8", x.data_ptr(), code, 1040, None, 0, 7, 1040, gain.data_ptr(), L.LSK_F32, 0.0, 1e-6,
+               h.data_ptr(), 1040, q.data_ptr(), s.data_ptr(), 1, 7, None, L.stream_of(x))
+        assert torch.equal(h, x)
