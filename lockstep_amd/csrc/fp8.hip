@@ -462,7 +462,6 @@ LSK_DEV void fp8_tile_out(const Fp8Args& p, const typename C::Acc& acc, char* sm
 // of them, so the row tiles that share a weight tile run together on one L2.
 template <int BM, int BN, int WM, int WN, int RING, bool EXACT, bool GROUPED>
 __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8Args p, int64_t mtiles, int vec) {
-  using C = Fp8Cfg<BM, BN, WM, WN, RING>;
   constexpr int kGroupM = 4;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int ntiles = (int)((p.N + BN - 1) / BN);
@@ -494,33 +493,43 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8Args p, int64
   const int rows_a = m1 - m0 < BM ? m1 - m0 : BM, rows_w = (int)p.N - n0 < BN ? (int)p.N - n0 : BN;
   const int nb = (p.K + 127) / 128, blocks_w = (rows_w + 127) / 128;
 
-  Fp8Tile t;
-  t.ra = make_rsrc(p.a + (int64_t)m0 * p.lda, (int64_t)(rows_a - 1) * p.lda + p.K);
-  t.rb = make_rsrc(p.w + (int64_t)n0 * p.ldw, (int64_t)(rows_w - 1) * p.ldw + p.K);
-  t.rsa = make_rsrc(p.sa + m0 * p.sm, nb ? 4 * ((rows_a - 1) * p.sm + (nb - 1) * p.sb + 1) : 0);
-  t.rsb = make_rsrc(p.sw + (n0 >> 7) * p.ldsw, nb ? 4 * ((blocks_w - 1) * p.ldsw + nb) : 0);
-  t.lda = (int)p.lda, t.ldb = (int)p.ldw, t.rows_a = rows_a, t.rows_b = rows_w;
-  t.sta = (uint32_t)(4 * p.sb);
-  t.s = tid < BM ? (tid < rows_a ? (uint32_t)(4 * tid * p.sm) : kOob)
-                 : (tid - BM < blocks_w ? (uint32_t)(4 * (tid - BM) * p.ldsw) : kOob);
+  auto tile = [&](auto config) {
+    using C = decltype(config);
+    Fp8Tile t;
+    t.ra = make_rsrc(p.a + (int64_t)m0 * p.lda, (int64_t)(rows_a - 1) * p.lda + p.K);
+    t.rb = make_rsrc(p.w + (int64_t)n0 * p.ldw, (int64_t)(rows_w - 1) * p.ldw + p.K);
+    t.rsa = make_rsrc(p.sa + m0 * p.sm, nb ? 4 * ((rows_a - 1) * p.sm + (nb - 1) * p.sb + 1) : 0);
+    t.rsb = make_rsrc(p.sw + (n0 >> 7) * p.ldsw, nb ? 4 * ((blocks_w - 1) * p.ldsw + nb) : 0);
+    t.lda = (int)p.lda, t.ldb = (int)p.ldw, t.rows_a = rows_a, t.rows_b = rows_w;
+    t.sta = (uint32_t)(4 * p.sb);
+    t.s = tid < C::kBM ? (tid < rows_a ? (uint32_t)(4 * tid * p.sm) : kOob)
+                       : (tid - C::kBM < blocks_w ? (uint32_t)(4 * (tid - C::kBM) * p.ldsw) : kOob);
 
-  typename C::Acc acc;
+    typename C::Acc acc;
 #pragma unroll
-  for (int i = 0; i < C::TM; ++i)
+    for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-    for (int j = 0; j < C::TN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+      for (int j = 0; j < C::TN; ++j) acc[i][j] = v4f{0, 0, 0, 0};
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass does not instantiate the main loop twice)
-  fp8_mainloop<BM, BN, WM, WN, RING, EXACT>(acc, t, p.K, smem);
+    fp8_mainloop<C::kBM, C::kBN, C::kWM, C::kWN, C::kRing, EXACT>(acc, t, p.K, smem);
 #endif
-  __syncthreads();
+    __syncthreads();
 
-  auto out = [&](auto odt) {
-    if (vec == 2) fp8_tile_out<C, decltype(odt)::value, true>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
-    else fp8_tile_out<C, decltype(odt)::value, false>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
+    auto out = [&](auto odt) {
+      if (vec == 2) fp8_tile_out<C, decltype(odt)::value, true>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
+      else fp8_tile_out<C, decltype(odt)::value, false>(p, acc, smem, m0, n0, rows_a, rows_w, vec);
+    };
+    if constexpr (EXACT) out(std::integral_constant<int, LSK_F32>{});
+    else if (p.out_dtype == LSK_BF16) out(std::integral_constant<int, LSK_BF16>{});
+    else out(std::integral_constant<int, LSK_F16>{});
   };
-  if constexpr (EXACT) out(std::integral_constant<int, LSK_F32>{});
-  else if (p.out_dtype == LSK_BF16) out(std::integral_constant<int, LSK_BF16>{});
-  else out(std::integral_constant<int, LSK_F16>{});
+  // A half-empty tile's rows over all eight waves, 64 each, rather than over one group of four.  (MI355X: 16384 rows over 128
+  // experts of 1536 x 2048 150.8 -> 144.0 us, 32768 of them 200.8 -> 197.8, 16384 over 32 of 5760 x 2880 432 -> 428; the
+  // requests in flight bound such tiles as much as the products.)
+  if constexpr (BM == 256) {
+    if (rows_a <= 128) return tile(Fp8Cfg<128, BN, WM, WN, RING>{});
+  }
+  tile(Fp8Cfg<BM, BN, WM, WN, RING>{});
 }
 
 static int64_t fp8_row_tiles(const Fp8Args& p, int bm) {
