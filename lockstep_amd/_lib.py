@@ -145,6 +145,8 @@ class MoeArgs(ctypes.Structure):
 
 _lock = threading.Lock()
 _lib = None
+# (looked up once: a call of 10 us looks them up several times)
+_Tensor, _current_device, _current_stream = torch.Tensor, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 class LockstepError(RuntimeError):
@@ -184,7 +186,7 @@ def call(name: str, *args):
 def call_on(t: torch.Tensor, name: str, *args):
     """call() with t's device current: a launch goes to the current device, whose streams t's are not
     when t lives on another."""
-    if t.get_device() != torch._C._cuda_getDevice():
+    if t.get_device() != _current_device():
         with torch.cuda.device(t.device):
             return call(name, *args)
     rc = getattr(_lib or load(), name)(*args)
@@ -208,7 +210,7 @@ def ptr(t):
 def stream_of(t: torch.Tensor):
     """The raw handle of the tensor's device's current stream (torch.cuda.current_stream builds a
     stream object around it, 2 us of a 17 us call)."""
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+    return _current_stream(t.get_device())
 
 
 def require_cuda(*ts, what: str = "lockstep_amd"):
@@ -218,8 +220,8 @@ def require_cuda(*ts, what: str = "lockstep_amd"):
     for t in ts:
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise ValueError("%s: expected a GPU tensor, got %s" % (what, type(t).__name__ if not isinstance(t, torch.Tensor) else t.device))
+        if not isinstance(t, _Tensor) or not t.is_cuda:
+            raise ValueError("%s: expected a GPU tensor, got %s" % (what, type(t).__name__ if not isinstance(t, _Tensor) else t.device))
         if first is None:
             first, index = t, t.get_device()
         elif t.get_device() != index:

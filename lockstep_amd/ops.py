@@ -790,7 +790,7 @@ def linear_mxfp4(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=N
 
 # ---------------------------------------------------------------- fp8 rows and weights, a scale for each block of 128
 FP8 = torch.float8_e4m3fn
-FP8_BLOCK = 128
+_F32 = torch.float32
 
 
 def quantize_rows_fp8(x: torch.Tensor):
@@ -831,7 +831,7 @@ def quantize_weight_fp8(w: torch.Tensor):
 
 def _fp8_codes(q: torch.Tensor, what: str):
     """Codes [rows, K] as the kernels read them: contiguous, 16-byte aligned (a copy where they are not)."""
-    if q.dtype != FP8 or q.dim() != 2 or q.shape[1] % 16:
+    if q.dtype is not FP8 or q.dim() != 2 or q.size(1) % 16:
         raise ValueError("%s: float8_e4m3fn [rows, K] with K a multiple of 16 expected, got %s %s"
                          % (what, q.dtype, tuple(q.shape)))
     if not q.is_contiguous() or q.data_ptr() % 16:
@@ -840,7 +840,7 @@ def _fp8_codes(q: torch.Tensor, what: str):
 
 
 def _fp8_row_scales(scale: torch.Tensor, M: int, K: int, what: str):
-    if scale.dtype != torch.float32 or scale.shape != (M, (K + 127) // 128):
+    if scale.dtype is not _F32 or scale.shape != (M, (K + 127) // 128):
         raise ValueError("%s: scales f32 [%d, %d] expected for rows [%d, %d], got %s %s"
                          % (what, M, (K + 127) // 128, M, K, scale.dtype, tuple(scale.shape)))
     return scale
@@ -849,7 +849,7 @@ def _fp8_row_scales(scale: torch.Tensor, M: int, K: int, what: str):
 def _fp8_weight(w: torch.Tensor, scale: torch.Tensor, what: str):
     w = _fp8_codes(w, what)
     N, K = w.shape
-    if scale.dtype != torch.float32 or scale.shape != ((N + 127) // 128, (K + 127) // 128):
+    if scale.dtype is not _F32 or scale.shape != ((N + 127) // 128, (K + 127) // 128):
         raise ValueError("%s: scales f32 [%d, %d] expected for a weight [%d, %d], got %s %s"
                          % (what, (N + 127) // 128, (K + 127) // 128, N, K, scale.dtype, tuple(scale.shape)))
     return w, scale if scale.is_contiguous() else scale.contiguous(), N, K
@@ -863,19 +863,19 @@ def dequant_fp8(q: torch.Tensor, scale: torch.Tensor, out_dtype=torch.bfloat16) 
     shape = q.shape
     if not shape:
         raise ValueError("dequant_fp8: q must be [..., K], got a scalar")
-    K, nb = shape[-1], (shape[-1] + 127) // 128
-    if scale.dtype != torch.float32 or not (scale.shape == (*shape[:-1], nb) or len(shape) == 2
-                                            and scale.shape == ((shape[0] + 127) // 128, nb)):
+    *lead, K = shape
+    nb = (K + 127) // 128
+    rows = 1 if scale.shape == (*lead, nb) else 128
+    if scale.dtype is not _F32 or rows == 128 and (len(lead) != 1 or scale.shape != ((lead[0] + 127) // 128, nb)):
         raise ValueError("dequant_fp8: q %s with f32 scales of rows or of 128 x 128 blocks expected, got %s %s"
                          % (tuple(shape), scale.dtype, tuple(scale.shape)))
-    rows = 1 if scale.shape[:-1] == shape[:-1] else 128
-    if len(shape) != 2:
+    if len(lead) != 1:
         M = shape[:-1].numel()
         q, scale = q.reshape(M, K), scale.reshape(M, nb)
     q = _fp8_codes(q, "dequant_fp8")
     out = q.new_empty(shape, dtype=out_dtype)
     if out.numel():
-        L.call_on(q, "lsk_dequant_fp8", q.data_ptr(), scale.data_ptr(), scale.stride(0), scale.stride(1), rows, q.shape[0],
+        L.call_on(q, "lsk_dequant_fp8", q.data_ptr(), scale.data_ptr(), scale.stride(0), scale.stride(1), rows, q.size(0),
                   K, out.data_ptr(), code, L.stream_of(q))
     return out
 
