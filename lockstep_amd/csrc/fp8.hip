@@ -194,7 +194,7 @@ struct Fp8Args {
 // row's bits depend on its batch.  The products of the rows' scales with the weight's (a block's columns share
 // one weight scale) are put into LDS whole at the start; their loads go out before the ring's, which they would
 // wait for otherwise.
-// DT >= 0: the rows of x (at most 16; vec: 16-byte aligned) are quantised by every block into LDS
+// DT >= 0: the block's rows of x (at most 16; vec: 16-byte aligned) are quantised by every block into LDS
 // itself, which saves a launch and the wait for it; x comes from the L2.
 template <int NG, int MT, int KS, bool FUSE>
 struct Fp8StreamCfg {
@@ -690,11 +690,16 @@ static int fp8_product(const Fp8Args& p, hipStream_t s) {
   return fp8_launch(best, p, s);
 }
 
-// Whether a linear's few rows are quantised in the product's launch, by every block: while they hold few values.  (MI355X,
-// GPU us in one launch and in two: one row of 3584 on 4608 columns 8.7, 10.7, of 14336 on 4096 19.8, 19.8; 4 of 2048 on
-// 1024 7.4, 9.5, of 4096 on 4096 12.7, 12.5; 16 of 1024 on 2048 9.1, 9.3, on 12000 10.9, 10.3, of 2048 on 1024 13.7, 9.9.
-// A launch less is 3 us of a caller's time besides, but nothing in a replayed graph.)
-static bool fp8_fuses(int64_t M, int64_t K) { return K > 0 && M <= 16 && M * K <= 16384; }
+// Whether a linear's rows are quantised in the product's launch, by every block: up to 16 while they hold few values, more
+// while the blocks, of 16 rows each, are two a CU at most.  (MI355X, GPU us in one launch and in two: one row of 3584 on 4608
+// columns 8.7, 10.7, of 14336 on 4096 19.8, 19.8; 4 of 2048 on 1024 7.4, 9.5, of 4096 on 4096 12.7, 12.5; 16 of 1024 on 2048
+// 9.1, 9.3, on 12000 10.9, 10.3, of 2048 on 1024 13.7, 9.9; 64 of 512 on 2048 6.3, 8.8, 128 of 256 on 1024 6.2, 7.2, 200 of
+// 1024 on 512 8.4, 9.2, and with more blocks 128 of 256 on 2048 9.3, 7.3, 96 of 1024 on 2048 10.3, 9.0.  A launch and a workspace
+// less are 4 us of a caller's time besides, but nothing in a replayed graph.)
+static bool fp8_fuses(int64_t M, int64_t N, int64_t K) {
+  if (K == 0) return false;
+  return M <= 16 ? M * K <= 16384 : K <= 1024 && M <= 16 * 512 && (M + 15) / 16 * ((N + 15) / 16) <= 512;
+}
 
 // One group of 16 columns a block while a block a CU and a few more hold them, else two, then four.  (One row of 3584 on
 // 4608 columns, 288 groups: 7.7, 8.1, 10.7 us; on 28672 columns of 512, 1792 groups, 7.2 with four, of 4096 31.0 with two
@@ -808,7 +813,7 @@ extern "C" int lsk_gemm_fp8(const uint8_t* a, const float* a_scale, int64_t scal
 
 // The quantised rows come first in the workspace, then their scales, block by block.
 extern "C" int64_t lsk_linear_fp8_workspace(int64_t M, int64_t N, int64_t K) {
-  if (lsk::fp8_fuses(M, K)) return 0;
+  if (lsk::fp8_fuses(M, N, K)) return 0;
   return lsk::up256(M * K) + lsk::up256(4 * M * ((K + 127) / 128));
 }
 
@@ -833,7 +838,7 @@ extern "C" int lsk_linear_fp8(const void* x, int x_dtype, int64_t ldx, int64_t M
   p.lda = p.ldw = K, p.sm = 1, p.sb = M, p.ldsw = (K + 127) / 128;
   p.M = M, p.N = N, p.K = (int)K;
   p.bias = bias, p.out = out, p.out_dtype = out_dtype, p.ldo = ldo;
-  if (lsk::fp8_fuses(M, K)) {
+  if (lsk::fp8_fuses(M, N, K)) {
     LSK_REQUIRE(lsk::fp8_reach(p), "lsk_linear_fp8: N=%lld K=%lld beyond 31-bit offsets", (long long)N, (long long)K);
     return lsk::fp8_stream_fused(p, x, x_dtype, ldx, s);
   }

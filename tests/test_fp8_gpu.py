@@ -304,6 +304,24 @@ def test_linear_is_mm_of_the_quantised_rows(M, N, K, dtype):
     assert np.array_equal(bits(FS.linear_fp8(odd[:, 1:K + 1], w, ws)), bits(FS.linear_fp8(x, w, ws)))
 
 
+@pytest.mark.parametrize("M,N,K", [(17, 100, 512), (64, 2048, 512), (200, 500, 1024), (33, 17, 16), (130, 260, 656), (500, 16, 1024),
+                                   (8192, 16, 32), (8193, 16, 32), (129, 1024, 144), (128, 1025, 144)])
+def test_linear_of_rows_quantised_by_every_block(M, N, K):
+    """Sizes on both sides of where a linear quantises its rows in the product's launch; rows at any place."""
+    from lockstep_amd import lockstep_fullstack as FS
+    say("linear", M, N, K)
+    g = np.random.default_rng(M + N + K)
+    w, ws = FS.quantize_weight_fp8(to_dev(_values(g, N, K)))
+    bias = to_dev(g.standard_normal(N).astype(np.float32))
+    wide = to_dev(np.concatenate([_values(g, M, K), _values(g, M, 5)], 1))
+    for dtype in HALF:
+        x = wide.to(dtype)
+        for view in (x[:, :K].contiguous(), x[:, 3:3 + K]):
+            for odt in (torch.float32, torch.bfloat16):
+                want = FS.mm_fp8(*FS.quantize_rows_fp8(view), w, ws, bias, odt)
+                assert np.array_equal(bits(FS.linear_fp8(view, w, ws, bias, odt)), bits(want))
+
+
 def test_linear_shapes_and_empty():
     from lockstep_amd import lockstep_fullstack as FS
     g = np.random.default_rng(9)

@@ -65,14 +65,14 @@ def test_product_refusals():
     _refused(gemm(K=1280, sb=1 << 27), b"31-bit offsets")
     assert gemm(M=0, a=None, w=None, out=None) == 0
     assert gemm(N=0, ldo=0, a=None, w=None, out=None) == 0
-    need = lib.lsk_linear_fp8_workspace(17, 8, 64)
+    need = lib.lsk_linear_fp8_workspace(17, 8, 2048)
     assert need > 0
-    lin = lambda x=P, dt=L.LSK_F32, ldx=64, work=P, nbytes=need: lib.lsk_linear_fp8(x, dt, ldx, 17, 64, P, P, 8, None, P, L.LSK_F32, 8, work, nbytes, None)  # noqa: E731,E501
+    lin = lambda x=P, dt=L.LSK_F32, ldx=2048, work=P, nbytes=need: lib.lsk_linear_fp8(x, dt, ldx, 17, 2048, P, P, 8, None, P, L.LSK_F32, 8, work, nbytes, None)  # noqa: E731,E501
     _refused(lin(nbytes=need - 1), b"workspace")
     _refused(lin(work=P + 16), b"workspace")
     _refused(lin(work=None), b"workspace")
     _refused(lin(dt=L.LSK_I32), b"x_dtype")
-    _refused(lin(ldx=63), b"ldx")
+    _refused(lin(ldx=2047), b"ldx")
 
 
 def test_grouped_refusals():
