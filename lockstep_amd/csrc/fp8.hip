@@ -692,13 +692,14 @@ static int fp8_product(const Fp8Args& p, hipStream_t s) {
 
 // Whether a linear's rows are quantised in the product's launch, by every block: up to 16 while they hold few values, more
 // while the blocks, of 16 rows each, are two a CU at most.  (MI355X, GPU us in one launch and in two: one row of 3584 on 4608
-// columns 8.7, 10.7, of 14336 on 4096 19.8, 19.8; 4 of 2048 on 1024 7.4, 9.5, of 4096 on 4096 12.7, 12.5; 16 of 1024 on 2048
-// 9.1, 9.3, on 12000 10.9, 10.3, of 2048 on 1024 13.7, 9.9; 64 of 512 on 2048 6.3, 8.8, 128 of 256 on 1024 6.2, 7.2, 200 of
-// 1024 on 512 8.4, 9.2, and with more blocks 128 of 256 on 2048 9.3, 7.3, 96 of 1024 on 2048 10.3, 9.0.  A launch and a workspace
-// less are 4 us of a caller's time besides, but nothing in a replayed graph.)
+// columns 8.1, 10.7, of 18944 on 4096 20.1, 20.8, on 12000 50.1, 47.5; 4 of 2048 on 1024 6.4, 9.5, of 5120 on 4096 11.8, 12.3,
+// on 12000 17.9, 16.3, of 8192 on 4096 16.6, 14.1; 12 of 1536 on 2048 8.1, 9.0; 16 of 1024 on 2048 8.9, 9.0, of 2048 10.8, 9.4;
+// 64 of 512 on 2048 6.3, 8.8, 128 of 256 on 1024 6.2, 7.2, 200 of 1024 on 512 8.4, 9.2, and with more blocks 128 of 256 on 2048
+// 9.3, 7.3, 96 of 1024 on 2048 10.3, 9.0.  A launch and a workspace less are 4 us of a caller's time besides, but nothing in a
+// replayed graph.)
 static bool fp8_fuses(int64_t M, int64_t N, int64_t K) {
   if (K == 0) return false;
-  return M <= 16 ? M * K <= 16384 : K <= 1024 && M <= 16 * 512 && (M + 15) / 16 * ((N + 15) / 16) <= 512;
+  return M <= 16 ? M * K <= (N <= 4096 ? 20480 : 16384) : K <= 1024 && M <= 16 * 512 && (M + 15) / 16 * ((N + 15) / 16) <= 512;
 }
 
 // One group of 16 columns a block while a block a CU and a few more hold them, else two, then four.  (One row of 3584 on

@@ -305,7 +305,8 @@ def test_linear_is_mm_of_the_quantised_rows(M, N, K, dtype):
 
 
 @pytest.mark.parametrize("M,N,K", [(17, 100, 512), (64, 2048, 512), (200, 500, 1024), (33, 17, 16), (130, 260, 656), (500, 16, 1024),
-                                   (8192, 16, 32), (8193, 16, 32), (129, 1024, 144), (128, 1025, 144)])
+                                   (8192, 16, 32), (8193, 16, 32), (129, 1024, 144), (128, 1025, 144),
+                                   (1, 4096, 20480), (1, 4097, 16400), (16, 4096, 1280), (16, 130, 1296), (13, 4097, 1264)])
 def test_linear_of_rows_quantised_by_every_block(M, N, K):
     """Sizes on both sides of where a linear quantises its rows in the product's launch; rows at any place."""
     from lockstep_amd import lockstep_fullstack as FS
