@@ -684,6 +684,8 @@ static int fp8_product(const Fp8Args& p, hipStream_t s) {
   for (int c = 0; c < kLaunches; ++c) {
     if (p.K == 0 && c >= kStream1) break;
     if (c == kTile256 && p.out_dtype == LSK_F32) continue;  // (products kept whole need more registers than it has)
+    const Fp8Cost& f = kFp8Costs[c];
+    if (!grid_ok(fp8_row_tiles(p, f.bm) * ((p.N + f.bn - 1) / f.bn), c == kTile256 ? 512 : 256)) continue;
     const double t = fp8_us(c, p.M, p.N, p.K, E);
     if (t < us) us = t, best = c;
   }
