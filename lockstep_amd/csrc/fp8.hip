@@ -194,6 +194,8 @@ struct Fp8Args {
 // row's bits depend on its batch.  The products of the rows' scales with the weight's (a block's columns share
 // one weight scale) are put into LDS whole at the start; their loads go out before the ring's, which they would
 // wait for otherwise.
+// (MI355X: 32 rows on 4096 x 14336 17.2 us, 688 KB a CU, rows and weights, at 40 B/ns: a CU has some 32 KB of requests on
+// their way; 128 rows over 32 experts of 2880 x 2880 49 us, 4.9 TB/s; one row on 28672 x 4096 27, 4.4 TB/s.)
 // DT >= 0: the block's rows of x (at most 16; vec: 16-byte aligned) are quantised by every block into LDS
 // itself, which saves a launch and the wait for it; x comes from the L2.
 template <int NG, int MT, int KS, bool FUSE>
