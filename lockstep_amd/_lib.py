@@ -145,8 +145,7 @@ class MoeArgs(ctypes.Structure):
 
 _lock = threading.Lock()
 _lib = None
-# (looked up once: a call of 10 us looks them up several times)
-_Tensor, _current_device, _current_stream = torch.Tensor, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_Tensor = torch.Tensor   # (looked up once: a call of 10 us looks it up several times)
 
 
 class LockstepError(RuntimeError):
@@ -181,6 +180,20 @@ def call(name: str, *args):
     if rc != 0:
         raise LockstepError("%s failed (code %d): %s" % (name, rc, last_error()))
     return rc
+
+
+# torch's current device and the raw stream of a device, each looked up by the first call of its kind, which puts torch's
+# function in its own place: a torch build without them still imports this package, for its host-only parts.
+def _current_device():
+    global _current_device
+    _current_device = torch._C._cuda_getDevice
+    return _current_device()
+
+
+def _current_stream(device: int):
+    global _current_stream
+    _current_stream = torch._C._cuda_getCurrentRawStream
+    return _current_stream(device)
 
 
 def call_on(t: torch.Tensor, name: str, *args):
