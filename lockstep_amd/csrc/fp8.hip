@@ -694,6 +694,14 @@ static int fp8_product(const Fp8Args& p, hipStream_t s) {
   return fp8_launch(best, p, s);
 }
 
+// The columns of a block that quantises its rows itself: one group of 16 while a block a CU and a few more hold them,
+// else two, then four.  (One row of 3584 on 4608 columns, 288 groups: 7.7, 8.1, 10.7 us; on 28672 columns of 512, 1792
+// groups, 7.2 with four, of 4096 31.0 with two and 31.5 with four.)
+static int fp8_fused_columns(int64_t N) {
+  const int64_t groups = (N + 15) / 16;
+  return groups <= 300 ? 16 : groups <= 1600 ? 32 : 64;
+}
+
 // Whether a linear's rows are quantised in the product's launch, by every block: up to 16 while they hold few values, more
 // while the blocks, of 16 rows each, are two a CU at most.  (MI355X, GPU us in one launch and in two: one row of 3584 on 4608
 // columns 8.1, 10.7, of 18944 on 4096 20.1, 20.8, on 12000 50.1, 47.5; 4 of 2048 on 1024 6.4, 9.5, of 5120 on 4096 11.8, 12.3,
@@ -702,19 +710,17 @@ static int fp8_product(const Fp8Args& p, hipStream_t s) {
 // 9.3, 7.3, 96 of 1024 on 2048 10.3, 9.0.  A launch and a workspace less are 4 us of a caller's time besides, but nothing in a
 // replayed graph.)
 static bool fp8_fuses(int64_t M, int64_t N, int64_t K) {
-  if (K == 0) return false;
+  const int columns = fp8_fused_columns(N);
+  if (K == 0 || !grid_ok((M + 15) / 16 * ((N + columns - 1) / columns), 256)) return false;
   return M <= 16 ? M * K <= (N <= 4096 ? 20480 : 16384) : K <= 1024 && M <= 16 * 512 && (M + 15) / 16 * ((N + 15) / 16) <= 512;
 }
 
-// One group of 16 columns a block while a block a CU and a few more hold them, else two, then four.  (One row of 3584 on
-// 4608 columns, 288 groups: 7.7, 8.1, 10.7 us; on 28672 columns of 512, 1792 groups, 7.2 with four, of 4096 31.0 with two
-// and 31.5 with four.)
 static int fp8_stream_fused(const Fp8Args& p, const void* x, int x_dtype, int64_t ldx, hipStream_t s) {
-  const int64_t groups = (p.N + 15) / 16;
+  const int columns = fp8_fused_columns(p.N);
   auto run = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (groups <= 300) return fp8_stream_launch<1, 1, 2, 4, DT>(p, x, ldx, s);
-    if (groups <= 1600) return fp8_stream_launch<2, 1, 1, 3, DT>(p, x, ldx, s);
+    if (columns == 16) return fp8_stream_launch<1, 1, 2, 4, DT>(p, x, ldx, s);
+    if (columns == 32) return fp8_stream_launch<2, 1, 1, 3, DT>(p, x, ldx, s);
     return fp8_stream_launch<4, 1, 1, 2, DT>(p, x, ldx, s);
   };
   if (x_dtype == LSK_F32) return run(std::integral_constant<int, LSK_F32>{});
