@@ -534,14 +534,13 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8Args p, int64
   tile(Fp8Cfg<BM, BN, WM, WN, RING>{});
 }
 
-static int64_t fp8_row_tiles(const Fp8Args& p, int bm) {
-  return p.offs ? expert_tiles_max(p.M, p.E, bm) : (p.M + bm - 1) / bm;
-}
+// E: the experts, 0 for a dense product.
+static int64_t fp8_row_tiles(int64_t M, int64_t E, int bm) { return E ? expert_tiles_max(M, E, bm) : (M + bm - 1) / bm; }
 
 template <int BM, int BN, int WM, int WN, int RING>
 static int fp8_tile_launch(const Fp8Args& p, hipStream_t s) {
   using C = Fp8Cfg<BM, BN, WM, WN, RING>;
-  const int64_t mtiles = fp8_row_tiles(p, BM), blocks = mtiles * ((p.N + BN - 1) / BN);
+  const int64_t mtiles = fp8_row_tiles(p.M, p.E, BM), blocks = mtiles * ((p.N + BN - 1) / BN);
   LSK_REQUIRE(grid_ok(blocks, C::kThreads) && blocks <= 0x7fffffff, "fp8 product: grid too large");
   const int64_t pitch = p.ldo * (p.out_dtype == LSK_F32 ? 4 : 2);
   const int vec = !out_vec_ok(p.out, p.out_dtype, p.ldo) ? 0 : (uintptr_t)p.out % 128 == 0 && pitch % 128 == 0 ? 2 : 1;
@@ -569,7 +568,7 @@ static bool fp8_reach(const Fp8Args& p) {
 
 template <int NG, int MT, int KS, int RING, int DT>
 static int fp8_stream_launch(const Fp8Args& p, const void* x, int64_t ldx, hipStream_t s) {
-  const int64_t tiles = p.offs ? expert_tiles_max(p.M, p.E, 16 * MT) : (p.M + 16 * MT - 1) / (16 * MT);
+  const int64_t tiles = fp8_row_tiles(p.M, p.E, 16 * MT);
   const int64_t blocks = tiles * ((p.N + 16 * NG - 1) / (16 * NG));
   LSK_REQUIRE(grid_ok(blocks, 256) && blocks <= 0x7fffffff, "fp8 product: grid too large");
   const int64_t lds = fp8_stream_lds<NG, MT, KS, RING, (DT >= 0)>(p.K, (int)(p.M < 16 ? p.M : 16));
@@ -678,20 +677,30 @@ static double fp8_us(int which, int64_t M, int64_t N, int64_t K, int64_t E) {
          (rest ? c.round[rest - 1] + c.k[rest - 1] * nk : 0);
 }
 
-static int fp8_product(const Fp8Args& p, hipStream_t s) {
-  LSK_REQUIRE(fp8_reach(p), "fp8 product: M=%lld N=%lld K=%d beyond 31-bit offsets", (long long)p.M, (long long)p.N, p.K);
-  const int64_t E = p.offs ? p.E : 0;
-  int best = kTile128;
+// The launch of a product: of those whose grid holds it the one that is likely to take the shortest; -1 where none holds it.
+static int fp8_choice(int64_t M, int64_t N, int64_t K, int64_t E, int out_dtype) {
+  int best = -1;
   double us = 1e30;
   for (int c = 0; c < kLaunches; ++c) {
-    if (p.K == 0 && c >= kStream1) break;
-    if (c == kTile256 && p.out_dtype == LSK_F32) continue;  // (products kept whole need more registers than it has)
+    if (K == 0 && c >= kStream1) break;
+    if (c == kTile256 && out_dtype == LSK_F32) continue;  // (products kept whole need more registers than it has)
     const Fp8Cost& f = kFp8Costs[c];
-    if (!grid_ok(fp8_row_tiles(p, f.bm) * ((p.N + f.bn - 1) / f.bn), c == kTile256 ? 512 : 256)) continue;
-    const double t = fp8_us(c, p.M, p.N, p.K, E);
+    if (!grid_ok(fp8_row_tiles(M, E, f.bm) * ((N + f.bn - 1) / f.bn), c == kTile256 ? 512 : 256)) continue;
+    const double t = fp8_us(c, M, N, K, E);
     if (t < us) us = t, best = c;
   }
-  return fp8_launch(best, p, s);
+  return best;
+}
+
+static int fp8_check_launch(const Fp8Args& p, int which) {
+  LSK_REQUIRE(fp8_reach(p), "fp8 product: M=%lld N=%lld K=%d beyond 31-bit offsets", (long long)p.M, (long long)p.N, p.K);
+  LSK_REQUIRE(which >= 0, "fp8 product: grid too large");
+  return LSK_OK;
+}
+
+static int fp8_product(const Fp8Args& p, hipStream_t s) {
+  const int which = fp8_choice(p.M, p.N, p.K, p.E, p.out_dtype), rc = fp8_check_launch(p, which);
+  return rc ? rc : fp8_launch(which, p, s);
 }
 
 // The columns of a block that quantises its rows itself: one group of 16 while a block a CU and a few more hold them,
@@ -855,8 +864,10 @@ extern "C" int lsk_linear_fp8(const void* x, int x_dtype, int64_t ldx, int64_t M
   }
   int rows;
   LSK_REQUIRE(K == 0 || grid_ok(lsk::quantize_rows_blocks(M, K, rows), 256), "lsk_linear_fp8: grid too large");
+  const int which = lsk::fp8_choice(M, N, K, 0, out_dtype);
+  if ((rc = lsk::fp8_check_launch(p, which))) return rc;  // (before anything is launched)
   if (K > 0 && (rc = lsk::quantize_rows_launch(x, x_dtype, M, K, ldx, q, qs, 1, M, s))) return rc;
-  return lsk::fp8_product(p, s);
+  return lsk::fp8_launch(which, p, s);
 }
 
 extern "C" int lsk_grouped_gemm_fp8(const uint8_t* a, const float* a_scale, int64_t scale_m, int64_t scale_b,
