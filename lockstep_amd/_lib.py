@@ -125,6 +125,7 @@ SIGNATURES = {
     "lsk_linear_fp8": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I, _I64, _P, _I64, _P]),
     "lsk_grouped_gemm_fp8": (_I, [_P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I, _I64,
                                   _P]),
+    "lsk_fp8_launch": (_I, [_I64, _I64, _I64, _I64, _I]),
     "lsk_add_rmsnorm_fp8": (_I, [_P, _I, _I64, _P, _I64, _I64, _I64, _P, _I, ctypes.c_float, ctypes.c_double, _P, _I64, _P,
                                  _P, _I64, _I64, _P, _P]),
     "lsk_route_experts": (_I, [_P, _I, _I64, _I64, _I64, _I, _I, _P, _I, _I, _I, _I, ctypes.c_double, _P, _P, _I, _P]),
