@@ -585,7 +585,7 @@ __global__ __launch_bounds__(WM * WN * 64) void fp4_tile_kernel(Fp4Args p, const
       for (int h = 0; h < 4; ++h)
         *(v4f*)(strip + (lane & 31) * C::kLdc + j * 32 + 8 * h + 4 * (lane >> 5)) =
             v4f{acc[i][j][4 * h], acc[i][j][4 * h + 1], acc[i][j][4 * h + 2], acc[i][j][4 * h + 3]};
-    // (a wave's own LDS operations run in order)
+    wave_lds_fence();
 #pragma unroll
     for (int r0 = 0; r0 < 32; r0 += kRows, row += kRows, o += step) {
       v4f v = *(const v4f*)(strip + (r0 + lane / kLanes) * C::kLdc + lane % kLanes * 4);
@@ -599,6 +599,7 @@ __global__ __launch_bounds__(WM * WN * 64) void fp4_tile_kernel(Fp4Args p, const
         for (int z = 0; z < 4 && col + z < rows_w; ++z) store_out(o, p.out_dtype, z, v[z]);
       }
     }
+    wave_lds_fence();
   }
 }
 

@@ -442,7 +442,7 @@ LSK_DEV void fp8_tile_out(const Fp8Args& p, const typename C::Acc& acc, char* sm
   for (int i = 0; i < C::TM; ++i) {
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) *(v4f*)(strip + (lane & 15) * C::kLdc + j * 16 + 4 * (lane >> 4)) = acc[i][j];
-    // (a wave's own LDS operations run in order)
+    wave_lds_fence();
 #pragma unroll
     for (int r0 = 0; r0 < 16; r0 += kRows, row += kRows, o += step) {
       v4f v = *(const v4f*)(strip + (r0 + lane / kLanes) * C::kLdc + lane % kLanes * 4);
@@ -457,6 +457,7 @@ LSK_DEV void fp8_tile_out(const Fp8Args& p, const typename C::Acc& acc, char* sm
         for (int z = 0; z < 4 && col + z < rows_w; ++z) store_out(o, ODT, z, v[z]);
       }
     }
+    wave_lds_fence();
   }
 }
 

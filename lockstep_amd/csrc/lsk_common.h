@@ -24,6 +24,11 @@ typedef unsigned int v4u32 __attribute__((ext_vector_type(4)));
 // prove threadIdx.x / 64 uniform by itself, and treats code that depends on it as divergent.
 LSK_DEV int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
+// Between what a wave's lanes write to LDS and other lanes of it read there, and before the next writes.  The hardware
+// runs a wave's own LDS operations in order; the compiler, which sees the addresses of one lane, may find the two apart
+// and change their order.  No instruction.
+LSK_DEV void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
 // A 64-bit value the caller knows to be equal in every lane (an entry of a per-block table, say)
 // moved to scalar registers.  Without it a buffer resource built from such a pointer can end up
 // in vector registers, and every load through it is wrapped in a loop over distinct resources.

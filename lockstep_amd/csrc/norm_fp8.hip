@@ -59,13 +59,14 @@ LSK_DEV void store_groups(void* o, int first, int G, const uint32_t (&w)[kWords]
   uint64_t* const mine = (uint64_t*)strip + kParts * lane;
 #pragma unroll
   for (int t = 0; t < kParts; ++t) mine[t] = (uint64_t)w[2 * t + 1] << 32 | w[2 * t];
-  // (a wave's own LDS operations run in order)
+  wave_lds_fence();
 #pragma unroll
   for (int t = 0; t < kParts; ++t) {
     const int u = 64 * t + lane;
     if (first + u / kParts < G) __builtin_nontemporal_store(((const uint64_t*)strip)[u], (uint64_t*)o + kParts * first + u);
     __asm__ volatile("" ::: "memory");  // (no 16-byte stores: store16_split)
   }
+  wave_lds_fence();
 }
 
 // Eight values of type DT as they lie in memory.

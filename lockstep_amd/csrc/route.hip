@@ -287,7 +287,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
     if constexpr (GROUPS) {
 #pragma unroll
       for (int j = 0; j < EPL; ++j) values[wave][lane + 64 * j] = c[j];
-      // (a wave's own LDS operations run in order)
+      wave_lds_fence();
       const uint64_t kept = kept_groups(p, values[wave]);
       const uint32_t recip = (1u << 20) / (uint32_t)(p.E / p.groups) + 1;  // e / size for e < 1024, size < 1024
 #pragma unroll
