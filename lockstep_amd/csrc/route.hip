@@ -230,27 +230,31 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs p) {
   if (t >= p.T) return;
   double s[EPL], c[EPL];
   double top = -__builtin_inf();
-  // All of a lane's loads go out together: none under a condition, 32-bit logits by halves, 16-bit ones twice, and
-  // what lies past E or is not there from a place that is.  (MI355X, waited for one by one and so:
-  // 4096 tokens of 384 experts 14.2, 12.8 us, 32 of 256 in groups 7.5, 6.9, 8192 of them 18.1, 17.6, 32 of 128 4.9, 4.9.)
+  // All of a lane's loads go out together: conversions wait until they are on their way, and what lies past E comes from
+  // E's last place.  (MI355X, each waited for before the next, and so: 4096 tokens of 384 experts 14.2, 11.8 us, 8192 of
+  // 256 in groups 18.1, 16.7, 32 of 256 in groups 7.5, 6.9, 32 of 128 4.9, 4.9.)
   const bool wide = p.g_dtype == LSK_F32;
-  const uint16_t* const row = (const uint16_t*)p.g + t * p.ldg * (wide ? 2 : 1);
-  const float* const from = p.bias ? p.bias : (const float*)p.idx;
-  uint32_t lo[EPL], hi[EPL];
-  float bias[EPL];
+  uint32_t raw[EPL];
+  float bias[EPL] = {};
+  if (wide) {  // (uniform, as the others)
+    const uint32_t* const row = (const uint32_t*)p.g + t * p.ldg;
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int e = min(lane + 64 * j, p.E - 1);
-    lo[j] = row[wide ? 2 * e : e], hi[j] = row[wide ? 2 * e + 1 : e];
-    bias[j] = from[p.bias ? e : 0];
+    for (int j = 0; j < EPL; ++j) raw[j] = row[min(lane + 64 * j, p.E - 1)];
+  } else {
+    const uint16_t* const row = (const uint16_t*)p.g + t * p.ldg;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) raw[j] = row[min(lane + 64 * j, p.E - 1)];
+  }
+  if (p.bias) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) bias[j] = p.bias[min(lane + 64 * j, p.E - 1)];
   }
   __asm__ volatile("" ::: "memory");  // (none behind the branches below)
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
-    const float v = wide ? __uint_as_float(hi[j] << 16 | lo[j])
-                         : p.g_dtype == LSK_BF16 ? __uint_as_float(lo[j] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)lo[j]);
+    const float v = wide ? __uint_as_float(raw[j])
+                         : p.g_dtype == LSK_BF16 ? __uint_as_float(raw[j] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)raw[j]);
     s[j] = lane + 64 * j < p.E ? (double)v : -__builtin_inf();
-    bias[j] = p.bias ? bias[j] : 0.0f;
   }
 #pragma unroll
   for (int j = 0; j < EPL; ++j) top = larger(top, s[j]);
