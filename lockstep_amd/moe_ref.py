@@ -694,7 +694,9 @@ def grouped_linear_fp8(tables, which: str, a, a_scale, offs, out_dtype=BF):
     lockstep_fullstack.mm_fp8(a[rows], a_scale[rows], w_e, scale_e[, b_e]) over expert-sorted rows, the same bits.
     tables: ExpertTablesFP8; a float8_e4m3fn [R, K], a_scale f32 [R, ceil(K / 128)] (any strides) as
     lockstep_fullstack.quantize_rows_fp8 gives them; offs int32 [E + 1] on the device; out [R, N] of out_dtype.  Rows past
-    offs[E] belong to no expert and are not written."""
+    offs[E] belong to no expert and are not written.  16-bit outputs, the default among them, come from the fp8
+    instruction, which drops what lies below 2^-13 of the largest of eight products (1.4e-5 of the result on normal data, at
+    most 2^-10 of the sum of magnitudes); float32 ones from whole products."""
     what = "grouped_linear_fp8"
     if which not in ("w13", "w2"):
         raise ValueError("%s: which must be 'w13' or 'w2'" % what)

@@ -886,7 +886,8 @@ def mm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: tor
     [ceil(N / 128), ceil(K / 128)] (+ bias [N]) -> [M, N] of out_dtype.  The blocks' sums are added in binary32 over
     ascending K, one rounding at the end.  A row's result is the same bits whatever the other rows are and
     however many.  Products are whole for float32; for 16-bit outputs the matrix core's fp8 instruction drops what lies
-    below 2^-13 of the largest of eight (1.4e-5 of the result on normal data)."""
+    below 2^-13 of the largest of eight (1.4e-5 of the result on normal data, at most 2^-10 of the sum of magnitudes).
+    The product of a row's and the weight's scale of a block has to be a normal binary32 number."""
     L.require_cuda(a, a_scale, w, w_scale, bias, what="mm_fp8")
     a = _fp8_codes(a, "mm_fp8")
     w, w_scale, N, K = _fp8_weight(w, w_scale, "mm_fp8")
@@ -906,7 +907,10 @@ def mm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: tor
 def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=None, out_dtype=None) -> torch.Tensor:
     """x [..., K] (f32 / bf16 / f16) quantised to fp8 (quantize_rows_fp8) and multiplied with fp8 weight rows w [N, K],
     w_scale [ceil(N / 128), ceil(K / 128)] (+ bias [N]) -> [..., N] of out_dtype (x's by default): mm_fp8 of the
-    quantised rows, the same bits, in one call."""
+    quantised rows, the same bits, in one call.  As there, float32 outputs come from whole products; 16-bit ones, so those
+    of 16-bit rows by default, from the fp8 instruction, which drops what lies below 2^-13 of the largest of eight
+    (1.4e-5 of the result on normal data, at most 2^-10 of the sum of magnitudes): ask for float32 where large products
+    cancel."""
     L.require_cuda(x, w, w_scale, bias, what="linear_fp8")
     w, w_scale, N, K = _fp8_weight(w, w_scale, "linear_fp8")
     lead = x.shape[:-1]
