@@ -804,10 +804,11 @@ int lsk_grouped_gemm_fp8(const uint8_t* a, const float* a_scale, int64_t scale_m
                          const int64_t* b_ptrs, int64_t N, int64_t K, void* out, int out_dtype, int64_t ldo, void* stream);
 
 /* The residual's addition, the contract's float RMS norm (lsk_rmsnorm_float) and fp8 rows of its output in one pass:
- * h = round(x + residual) to x's type (h = x without a residual; a NaN stays one, of bf16 0x7fc0), y = the norm's binary32 value before its rounding to
- * bf16, q and scale = lsk_quantize_rows_fp8 of y.  x and residual [R, N] of x_dtype; g [N]; sN, eps as
- * lsk_rmsnorm_float takes them; h [R, N] (rows ldh apart, each 16-byte aligned; may be the residual's own memory, row for
- * row) or NULL; out [R, N] bf16 (= lsk_rmsnorm_float of h) or NULL, contiguous, 16-byte aligned.  N % 16 == 0, N <= 65536. */
+ * h = round(x + residual) to x's type (h = x without a residual; a NaN stays one, of bf16 0x7fc0), y = the norm's binary32
+ * value before its rounding to bf16, q and scale = lsk_quantize_rows_fp8 of y.  x and residual [R, N] of x_dtype; g [N];
+ * sN, eps as lsk_rmsnorm_float takes them; h [R, N] (rows ldh apart, each 16-byte aligned; may be the residual's own memory,
+ * row for row) or NULL; out [R, N] bf16 (= lsk_rmsnorm_float of h) or NULL, contiguous, 16-byte aligned.  N % 16 == 0,
+ * N <= 65536. */
 int lsk_add_rmsnorm_fp8(const void* x, int x_dtype, int64_t ldx, const void* residual, int64_t ldr, int64_t R, int64_t N,
                         const void* g, int g_dtype, float sN, double eps, void* h, int64_t ldh, uint8_t* q, float* scale,
                         int64_t scale_m, int64_t scale_b, void* out, void* stream);

@@ -109,7 +109,8 @@ __global__ __launch_bounds__(256) void quantize_weight_fp8_kernel(const void* __
 
 // Codes times scales, four times eight bytes of outputs a thread, so that a wave's stores are whole lines side by side
 // (MI355X, against eight consecutive values a thread: 28672 x 4096 to bf16 64 -> 54 us, to f32 466 -> 100; lines filled by
-// two stores past the caches reach HBM in parts).  Bound by HBM: 352 MB in 54 us are 6.5 TB/s.  `per` of these units to a row; part: 2^22 / per, rounded up.
+// two stores past the caches reach HBM in parts).  Bound by HBM: 352 MB in 54 us are 6.5 TB/s.  `per` of these units to a
+// row; part: 2^22 / per, rounded up.
 template <int ODT>
 __global__ __launch_bounds__(256) void dequant_fp8_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scale,
                                                           int64_t sm, int64_t sb, int row_shift, int64_t total, uint32_t per,
@@ -194,8 +195,9 @@ struct Fp8Args {
 // row's bits depend on its batch.  The products of the rows' scales with the weight's (a block's columns share
 // one weight scale) are put into LDS whole at the start; their loads go out before the ring's, which they would
 // wait for otherwise.
-// (MI355X: 32 rows on 4096 x 14336 17.2 us, 688 KB a CU, rows and weights, at 40 B/ns: a CU has some 32 KB of requests on
-// their way; 128 rows over 32 experts of 2880 x 2880 49 us, 4.9 TB/s; one row on 28672 x 4096 27, 4.4 TB/s.)
+// (MI355X: 32 rows on 4096 x 14336 17.2 us, 688 KB a CU, rows and weights, at 40 B/ns; 128 rows over 32 experts of
+// 2880 x 2880 49 us, 4.9 TB/s; one row on 28672 x 4096 26, 4.5 TB/s.  With one block of 16 weight rows a CU the depth of the
+// ring counts: the product of one row of 18944 with 3584 columns takes 22.3 us with four stages in the ring, 17.8 with six.)
 // DT >= 0: the block's rows of x (at most 16; vec: 16-byte aligned) are quantised by every block into LDS
 // itself, which saves a launch and the wait for it; x comes from the L2.
 template <int NG, int MT, int KS, bool FUSE>
@@ -418,9 +420,10 @@ __global__ __launch_bounds__(256) void fp8_stream_kernel(Fp8Args p, const void* 
 
 // ---------------------------------------------------------------- tiles
 // The tile's outputs: a 16-row strip at a time through the wave's part of LDS, out of it four consecutive columns a lane.
-// LINES: rows begin on lines of 128 bytes, and whole lines go past the caches (store_quad; MI355X, past them and not:
-// 4096 rows of 28672 x 4096 426 us, 456; 4096 of 4096 x 2048 39.4, 41.5); lines that two rows share are put together in
-// the L2 (3102 rows of 13016 x 128 47.9, 41.7).
+// LINES: rows begin on lines of 128 bytes, and whole lines go past the caches (store_quad; MI355X, builds in turn, past them
+// and not: 4096 rows of 28672 x 4096 422 us, 434; 4096 of 4096 x 2048 34.6, 36.8; 32768 over 128 experts of 1536 x 2048 186,
+// 196); lines that two rows share are put together in the L2 (3102 rows of 13016 x 128 40.6, 34.5; 4000 of 4600 x 2880
+// 82.4, 84.0).
 template <class C, int ODT, bool LINES>
 LSK_DEV void fp8_tile_out(const Fp8Args& p, const typename C::Acc& acc, char* smem, int m0, int n0, int rows_a, int rows_w,
                           int vec) {
@@ -526,9 +529,9 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_tile_kernel(Fp8Args p, int64
     else if (p.out_dtype == LSK_BF16) out(std::integral_constant<int, LSK_BF16>{});
     else out(std::integral_constant<int, LSK_F16>{});
   };
-  // A half-empty tile's rows over all eight waves, 64 each, rather than over one group of four.  (MI355X: 16384 rows over 128
-  // experts of 1536 x 2048 150.8 -> 144.0 us, 32768 of them 200.8 -> 197.8, 16384 over 32 of 5760 x 2880 432 -> 428; the
-  // requests in flight bound such tiles as much as the products.)
+  // A half-empty tile's rows over all eight waves, 64 each, rather than over one group of four.  (MI355X, builds in turn:
+  // 16384 rows over 128 experts of 1536 x 2048 145.1 -> 141.2 us, 32768 of them 188.8 -> 185.8, 16384 over 32 of 5760 x 2880
+  // 421 -> 416; the requests in flight bound such tiles as much as the products.)
   if constexpr (BM == 256) {
     if (rows_a <= 128) return tile(Fp8Cfg<128, BN, WM, WN, RING>{});
   }
@@ -597,9 +600,15 @@ static int fp8_stream_launch(const Fp8Args& p, const void* x, int64_t ldx, hipSt
 // them, works through them `resident` at a time, a round of o blocks at once in round[o - 1] + k[o - 1] a block of 128
 // values of K; every million outputs cost `out` and `area` a block of K, every 10^9 weights read `weights`, and every
 // 10^9 bytes of a block's operands `spill` where the rows (of an expert) outgrow an XCD's 4 MB of L2.  Fitted to 902
-// products on MI355X (1 to 4096 rows of 17 to 37888 columns, K = 16 to 18944; 1 to 32768 rows over 2 to 128 experts):
-// what it picks is 1.3 % slower than the best of these on average and 27 % at most (50 rows of 19 x 736, 6.5 and 5.1 us;
-// among those over 10 us 18 %, 256 rows over 8 experts of 4096 x 4096).  All of them give the same bits.
+// products with bf16 outputs on MI355X (1 to 4096 rows of 17 to 37888 columns, K = 16 to 18944; 1 to 32768 rows over 2 to
+// 128 experts), 256 x 256 tiles of at most 128 rows then still computed as full ones; binary32 outputs, which are other
+// instructions and twice the bytes, choose by the same constants.  On products that it was not fitted to, what it picks is
+// slower than the best of these launches by (755 dense, 380 by expert of each):
+//   bf16 outputs      2.6 % on average, dense, and 2.4 % by expert; nine of ten within 9.3 and 8.3 %; at most 45 % (221 rows of
+//                     3136 x 4864, 23.7 us on 32 x 32 blocks, 16.4 on 64 x 64 tiles) and 26 % (2 rows over 44 experts)
+//   binary32 outputs  2.5 and 2.9 %; nine of ten within 7.1 and 9.8 %; at most 28 % (348 rows of 125 x 736, 8.1 and 6.3 us)
+//                     and 25 % (2405 rows over 23 experts of 2091 x 3904, 104 and 83 us)
+// All of them give the same bits.
 struct Fp8Cost {
   int bm, bn, resident;  // resident 0: as many as the LDS holds at this K, to four
   double base, out, area, weights, spill, round[4], k[4];
@@ -705,20 +714,24 @@ static int fp8_product(const Fp8Args& p, hipStream_t s) {
 }
 
 // The columns of a block that quantises its rows itself: one group of 16 while a block a CU and a few more hold them,
-// else two, then four.  (One row of 3584 on 4608 columns, 288 groups: 7.7, 8.1, 10.7 us; on 28672 columns of 512, 1792
-// groups, 7.2 with four, of 4096 31.0 with two and 31.5 with four.)
+// else two, then four; the borders, 300 and 1600 groups, are thresholds.  (MI355X, in a graph, us with 16, 32 and 64:
+// one row of 3584 on 4608 columns, 288 groups, 7.7, 8.3, 10.7, four rows 10.5, 10.0, 12.5, one of 768 4.7, 4.4, 4.5; one of
+// 2048 on 4800, 300 groups, 6.4, 6.3, 7.6, on 5120 6.5, 6.3, 7.7, on 16384 11.0, 8.8, 8.8; one of 4096 on 25600, 1600
+// groups, 28.0, 27.4, 24.5, on 28672 30.2, 28.8, 26.2; one of 3584 on 37888 29.0, 24.7, 25.0; sixteen of 1024 on 28672
+// 21.3, 15.6, 11.1; 64 of 512 on 2048 5.7, 5.3, 5.3, 128 of 256 on 1024 5.7, 4.4, 4.6.  So up to 12 % from the best of
+// the three for up to 16 rows, and 30 % for more, which always take 16.)
 static int fp8_fused_columns(int64_t N) {
   const int64_t groups = (N + 15) / 16;
   return groups <= 300 ? 16 : groups <= 1600 ? 32 : 64;
 }
 
 // Whether a linear's rows are quantised in the product's launch, by every block: up to 16 while they hold few values, more
-// while the blocks, of 16 rows each, are two a CU at most.  (MI355X, GPU us in one launch and in two: one row of 3584 on 4608
-// columns 8.1, 10.7, of 18944 on 4096 20.1, 20.8, on 12000 50.1, 47.5; 4 of 2048 on 1024 6.4, 9.5, of 5120 on 4096 11.8, 12.3,
-// on 12000 17.9, 16.3, of 8192 on 4096 16.6, 14.1; 12 of 1536 on 2048 8.1, 9.0; 16 of 1024 on 2048 8.9, 9.0, of 2048 10.8, 9.4;
-// 64 of 512 on 2048 6.3, 8.8, 128 of 256 on 1024 6.2, 7.2, 200 of 1024 on 512 8.4, 9.2, and with more blocks 128 of 256 on 2048
-// 9.3, 7.3, 96 of 1024 on 2048 10.3, 9.0.  A launch and a workspace less are 4 us of a caller's time besides, but nothing in a
-// replayed graph.)
+// while the blocks, of 16 rows each, are two a CU at most.  (MI355X, in a graph, us in one launch and in two: one row of 3584
+// on 4608 columns 7.7, 9.8, of 14336 on 4096 19.7, 18.2, of 18944 on 3584 25.1, 21.1; 4 of 2048 on 1024 5.8, 8.3, of 5120 on
+// 4096 11.1, 11.4, of 8192 on 4096 16.0, 13.5, of 4096 on 12000 17.3, 16.3; 12 of 1536 on 2048 7.7, 8.4; 16 of 1024 on 2048
+// 6.8, 8.1, of 2048 10.2, 8.9; 64 of 512 on 2048 5.7, 8.3, 128 of 256 on 1024 5.7, 6.8, 200 of 1024 on 512 8.0, 8.6, and with
+// more blocks 128 of 256 on 2048 8.8, 6.7, 96 of 1024 on 2048 10.0, 8.6.  A launch and a workspace less are 4 us of a
+// caller's time besides, which is why one long row stays in one launch; in a replayed graph it is up to 19 % slower there.)
 static bool fp8_fuses(int64_t M, int64_t N, int64_t K) {
   const int columns = fp8_fused_columns(N);
   if (K == 0 || !grid_ok((M + 15) / 16 * ((N + columns - 1) / columns), 256)) return false;

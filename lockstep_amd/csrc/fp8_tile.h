@@ -151,14 +151,16 @@ LSK_DEV void fp8_mainloop(typename Fp8Cfg<BM, BN, WM, WN, RING>::Acc& acc, const
       f.a[i] = fp8_operand(*(const v4i*)(base + offA + i * 2048 + lo), *(const v4i*)(base + offA + i * 2048 + hi));
   };
   // Three products ahead of the FMAs that use them: a result takes the matrix core's eight passes and three more to
-  // come back, and a wave that waited for each would leave the core idle as long (256 x 256 tiles, 4096 rows of 28672
-  // x 4096: 577 us as the compiler ordered it, 452 two ahead, 439 three).
+  // come back, and a wave that waited for each would leave the core idle as long (MI355X, builds in turn, in the compiler's
+  // order, two and three ahead: 256 x 256 tiles, 4096 rows of 28672 x 4096, 436, 442, 422 us; 128 x 128, 2048 of 4096 x 4096,
+  // 39.7, 38.9, 37.8; by expert, where loads bound the tiles, 16384 over 32 of 5760 x 2880 398, 422, 416).
   constexpr int kTiles = C::TM * C::TN, kDepth = kTiles < 3 ? kTiles : 3;
   constexpr int kEvery = kTiles / C::kPer > 0 ? kTiles / C::kPer : 1;  // products to a load
   static_assert(C::kThreads == 256 || kTiles >= C::kPer, "a stage's loads fit among its products");
   // with: the loads of stage s among the products.  (Every caller raises the wave's priority for them: the SIMD's other
-  // waves read and issue loads meanwhile, and take their slots otherwise; 256 x 256 tiles on 4096 rows of 28672 x 4096
-  // 477 -> 460 us, 128 x 128 on 2048 of 4096 x 4096 45.0 -> 41.6.)
+  // waves read and issue loads meanwhile, and take their slots otherwise; without and with, builds in turn: 256 x 256 tiles
+  // on 4096 rows of 28672 x 4096 429, 422 us, 128 x 128 on 2048 of 4096 x 4096 41.6, 37.8; by expert 16384 rows over 32 of
+  // 5760 x 2880 410, 416.)
   auto multiply = [&](const Frag& f, auto with, int s) {
     constexpr bool kWith = decltype(with)::value;
     if constexpr (EXACT) {
@@ -231,9 +233,9 @@ LSK_DEV void fp8_mainloop(typename Fp8Cfg<BM, BN, WM, WN, RING>::Acc& acc, const
     // Two groups of four waves, half a period apart: while one multiplies stage kt the other reads its fragments
     // (group 0 reads in period 2 kt and multiplies in 2 kt + 1, group 1 a period later).  Both request stage kt + 1 in
     // period 2 kt, into the slot of stage kt - 1, which group 1 has read by the end of 2 kt - 1, and wait for it at the
-    // end of 2 kt + 1.  A CU has about 32 KB of requests on their way, half a stage, and a wave that issues more
-    // waits: so group 0 issues behind its reads and group 1 one request to every three products (all of them ahead of
-    // the products 495 us for the case above, so 452).
+    // end of 2 kt + 1.  Group 0 issues behind its reads and group 1 one request to every three products.  (All of
+    // group 1's ahead of its products is no worse, builds in turn: so and ahead, 4096 rows of 28672 x 4096 422, 416 us, 32768
+    // over 128 experts of 1536 x 2048 186, 181.)
     issue(0);
     wait_vm<0>();
     phase_barrier();
