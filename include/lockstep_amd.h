@@ -781,8 +781,8 @@ int lsk_dequant_fp8(const uint8_t* q, const float* scale, int64_t scale_m, int64
  * is added in binary32; one rounding to out_dtype.  For binary32 outputs a block's products are summed whole in
  * binary32; for 16-bit outputs on the fp8 instruction, which sums eight products at a time and drops what lies below
  * 2^-13 of the largest (1.4e-5 of the result on normal data, and at most 2^-10 of the sum of magnitudes).  The two
- * scales' product has to be a normal binary32 number.  A row's results are the same bits whatever the other rows are
- * and however many, and on every launch.  K = 0: the bias alone. */
+ * scales' product has to be a normal binary32 number (below only where the codes are zeros).  A row's results are the same
+ * bits whatever the other rows are and however many, and on every launch.  K = 0: the bias alone. */
 int lsk_gemm_fp8(const uint8_t* a, const float* a_scale, int64_t scale_m, int64_t scale_b, int64_t M, int64_t K,
                  const uint8_t* w, const float* w_scale, int64_t N, const float* bias, void* out, int out_dtype, int64_t ldo,
                  void* stream);

@@ -55,3 +55,21 @@ def test_at_its_worst(M):
         # a block's whole products add up to a whole number below 2^24; the nine blocks' chain rounds nine times at most
         got = FS.mm_fp8(a, sa, w, sw).double()
         assert ((got - y).abs() <= 9 * 2.0 ** -24 * abs(y)).all()
+
+
+@pytest.mark.parametrize("M", [1, 30, 300])
+def test_blocks_of_zeros(M):
+    """A block of zeros has the scale 2^-126, whose product with a weight's is below the normal numbers: it adds nothing."""
+    from lockstep_amd import lockstep_fullstack as FS
+    N, K = 300, 656
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = torch.randn((M, K), generator=g, device="cuda")
+    x[:, 128:256], x[:, 640:], x[::3] = 0, 0, 0
+    w, sw = FS.quantize_weight_fp8(1e-3 * torch.randn((N, K), generator=g, device="cuda"))
+    a, sa = FS.quantize_rows_fp8(x)
+    assert (sa[:, 1] == 2.0 ** -126).all() and float(sw.max()) < 1
+    one = torch.where(sa == 2.0 ** -126, torch.ones_like(sa), sa)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        got = FS.mm_fp8(a, sa, w, sw, out_dtype=dtype)
+        assert torch.equal(got, FS.mm_fp8(a, one, w, sw, out_dtype=dtype)) and (got[::3] == 0).all()
+        assert torch.equal(got, FS.linear_fp8(x, w, sw, out_dtype=dtype))
