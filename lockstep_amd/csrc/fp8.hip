@@ -905,6 +905,8 @@ extern "C" int lsk_grouped_gemm_fp8(const uint8_t* a, const float* a_scale, int6
 }
 
 extern "C" int lsk_fp8_launch(int64_t M, int64_t N, int64_t K, int64_t E, int out_dtype) {
-  if (M < 1 || N < 1 || K < 0 || E < 0 || M > 0x7fffffff || N > 0x7fffffff || K >= (1 << 22) || E > (1 << 20)) return -1;
+  if (M < 1 || N < 1 || K < 0 || K % 16 || E < 0 || M > 0x7fffffff || N > 0x7fffffff || K >= (1 << 22) || E > (1 << 20) ||
+      !lsk::is_float_dtype(out_dtype))
+    return -1;
   return lsk::fp8_choice(M, N, K, E, out_dtype);
 }

@@ -77,6 +77,7 @@ def test_the_query_itself():
     fn = L.load().lsk_fp8_launch
     for bad in ((0, 16, 16, 0), (1, 0, 16, 0), (1, 16, -1, 0), (1, 16, 1 << 22, 0), (1, 16, 16, -1), (1 << 31, 16, 16, 0)):
         assert fn(*bad, L.LSK_BF16) == -1
+    assert fn(1, 16, 24, 0, L.LSK_BF16) == fn(1, 16, 16, 0, L.LSK_I8) == -1
     assert fn((1 << 31) - 1, (1 << 31) - 1, 16, 0, L.LSK_BF16) == -1
     assert fn(5, 16, 0, 0, L.LSK_BF16) in range(6) and fn(1, 1, 16, 1 << 20, L.LSK_F32) in LAUNCHES
 
