@@ -853,8 +853,8 @@ int lsk_bf16_cvt_check(uint64_t start, uint64_t count, uint32_t* mismatches, uin
  * reference, computed on the host.  Tiles of rows x columns: 0 256 x 256, 1 128 x 128, 2 64 x 128, 3 64 x 64, 4 64 x 64
  * with four stages in flight, 5 128 x 64; streaming blocks: 6 16 x 16, 7 16 x 32, 8 16 x 64, 9 16 x 16 with six
  * stages, 10 32 x 16, 11 32 x 32, 12 32 x 32 with four stages of 512 values; -1: none holds them, or sizes or an
- * out_dtype that the products refuse.  (lsk_linear_fp8 takes
- * the same where its workspace is not 0.)  The results' bits do not depend on it. */
+ * out_dtype that the products refuse.  (lsk_linear_fp8 takes the same where its workspace is not 0.)  The results' bits
+ * do not depend on it. */
 int lsk_fp8_launch(int64_t M, int64_t N, int64_t K, int64_t E, int out_dtype);
 
 #ifdef __cplusplus
